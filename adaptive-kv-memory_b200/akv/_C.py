@@ -18,6 +18,7 @@ BLOCK_TOKENS = 32
 ERRORS = {
     -1: "AKV_ERR_SHAPE", -2: "AKV_ERR_BITS", -3: "AKV_ERR_ALIGN", -4: "AKV_ERR_UNSUPPORTED",
     -5: "AKV_ERR_LAUNCH", -6: "AKV_ERR_TIMEOUT", -7: "AKV_ERR_NULL", -8: "AKV_ERR_WORKSPACE",
+    -9: "AKV_ERR_EXHAUSTED",
 }
 
 
@@ -65,6 +66,24 @@ class LayerStep(ctypes.Structure):
                 ("protect_recent", c_int32), ("decay", c_float), ("total_len", c_int64), ("step", c_int64),
                 ("warm_len", c_int64), ("warm_bytes_packed", c_int64), ("bytes_per_event", c_int64),
                 ("status", c_void_p)]
+
+
+class Int4Layout(ctypes.Structure):
+    """akv_int4_layout: byte offsets inside one 32-token record of the 4-bit cache."""
+    _fields_ = [(n, c_int32) for n in ("head_dim", "group", "n_groups", "kc", "vc", "kp", "vp", "bytes")]
+
+
+class Int4Cache(ctypes.Structure):
+    """akv_int4_cache (include/akv_b200.h): one layer of a 4-bit paged cache."""
+    _fields_ = [("pool", c_void_p), ("page_stride", c_int64), ("head_stride", c_int64), ("n_pages", c_int32),
+                ("table", c_void_p), ("table_stride", c_int64), ("lens", c_void_p), ("max_seqs", c_int32),
+                ("max_blocks", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("group", c_int32)]
+
+
+class PageTable(ctypes.Structure):
+    """akv_page_table (include/akv_b200.h): device-side page ownership."""
+    _fields_ = [("table", c_void_p), ("table_stride", c_int64), ("lens", c_void_p), ("refs", c_void_p),
+                ("free_bits", c_void_p), ("max_seqs", c_int32), ("max_blocks", c_int32), ("n_pages", c_int32)]
 
 
 # name -> (restype, argtypes); must list every function declared in akv_b200.h
@@ -157,6 +176,27 @@ SIGNATURES = {
                                 c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
     "akv_scatter_rows": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int,
                                  c_int, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
+    "akv_int4_layout_init": (c_int, [c_int, c_int, POINTER(Int4Layout)]),
+    "akv_int4_append": (c_int, [POINTER(Int4Cache), c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int64,
+                                c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "akv_int4_read": (c_int, [POINTER(Int4Cache), c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64,
+                              c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "akv_int4_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "akv_int4_attention": (c_int, [POINTER(Int4Cache), c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int64,
+                                   c_int64, c_int64, c_float, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int,
+                                   c_void_p, c_size_t, c_void_p, c_void_p]),
+    "akv_pages_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "akv_pages_fork": (c_int, [POINTER(PageTable), c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "akv_pages_reserve": (c_int, [POINTER(PageTable), c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
+                                  c_int64, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "akv_pages_truncate": (c_int, [POINTER(PageTable), c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "akv_pages_compact": (c_int, [POINTER(PageTable), c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p,
+                                  c_size_t, c_void_p, c_void_p]),
+    "akv_pages_copy": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                               c_void_p]),
+    "akv_verify_draft": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                 c_void_p]),
     "akv_selftest_wait": (c_int, [c_int, c_int64, c_void_p, c_void_p, c_void_p]),
     "akv_cold_copy": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
 }
@@ -241,6 +281,12 @@ def warm_layout(head_dim: int, key_bits: int, value_bits: int, n_outlier: int) -
     L = WarmLayout()
     check(load().akv_warm_layout_init(head_dim, key_bits, value_bits, n_outlier, ctypes.byref(L)),
           "akv_warm_layout_init")
+    return L
+
+
+def int4_layout(head_dim: int, group: int) -> Int4Layout:
+    L = Int4Layout()
+    check(load().akv_int4_layout_init(head_dim, group, ctypes.byref(L)), "akv_int4_layout_init")
     return L
 
 

@@ -14,6 +14,8 @@ from .fused_attention import (fused_int4_decode_attention, int4_group_dequant, m
 from .packed_layout import WarmArena, measure_packed_bytes
 from .drop_in import AKVCache, AKVLayer, recommend_preset
 from .graphs import DecodeGraph
+from .int4_cache import Int4PagedCache
+from .speculative import verify_draft
 from .tiering import fused_importance_update
 from .triton_ops import HAS_TRITON, fused_mixed_precision_attention, fused_quantized_attention
 from .triton_kernels import fused_decode_attention, fused_quantize_evict
@@ -27,5 +29,6 @@ __all__ = [
     "int4_group_dequant", "prefill_attention",
     "HAS_TRITON", "fused_quantized_attention", "fused_mixed_precision_attention", "fused_importance_update",
     "fused_decode_attention", "fused_quantize_evict",
+    "Int4PagedCache", "verify_draft",
     "pack", "unpack", "packed_bytes",
 ]

@@ -639,6 +639,7 @@ extern "C" const char* akv_strerror(int status) {
     case AKV_ERR_TIMEOUT: return "device-side wait timed out";
     case AKV_ERR_NULL: return "required pointer is NULL";
     case AKV_ERR_WORKSPACE: return "workspace too small";
+    case AKV_ERR_EXHAUSTED: return "page pool exhausted";
     default: return "unknown status";
   }
 }

@@ -44,8 +44,12 @@ enum {
   AKV_ERR_LAUNCH = -5,      /* kernel launch / CUDA runtime error */
   AKV_ERR_TIMEOUT = -6,     /* a bounded device-side wait ran out */
   AKV_ERR_NULL = -7,        /* required pointer is NULL */
-  AKV_ERR_WORKSPACE = -8    /* workspace too small */
+  AKV_ERR_WORKSPACE = -8,   /* workspace too small */
+  AKV_ERR_EXHAUSTED = -9    /* the page pool has no free page left (status word only) */
 };
+
+/* Element types of the entries that take more than fp16. */
+enum { AKV_FP16 = 0, AKV_BF16 = 1, AKV_FP32 = 2 };
 
 const char* akv_strerror(int status);
 int akv_abi_version(void);
@@ -620,6 +624,148 @@ int akv_peer_combine(const float* gather, const int* flags, int rows, int D, int
  * ---------------------------------------------------------------------- */
 int akv_cold_copy(void* dst, int64_t dst_stride, const void* src, int64_t src_stride,
                   int64_t chunk_bytes, int64_t count, int dir, void* stream, void* event);
+
+/* ------------------------------------------------------------------------
+ * 4-bit paged cache: every token is held in 4 bits from the moment it
+ * arrives.  No counterpart in the reference, whose INT4 tier is quantised in
+ * bulk and read through an FP16 copy (akv/fused_attention.py:213-290); codes
+ * keep that tier's byte order (even channel in the high nibble).
+ *
+ * A page holds 32 consecutive tokens of one sequence for every KV head; the
+ * record of one head is
+ *   kc  K codes [32][D/2] u8   vc  V codes [32][D/2] u8
+ *   kp  K (scale, zero) fp16 pairs [32][G]   vp  the same for V [32][G]
+ * with G = D / group.  A code c stands for c * scale + zero.  Record and page
+ * sizes are multiples of 16 bytes.  head_dim 64, 128 or 256; group = D, D/2
+ * or D/4.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  int32_t head_dim, group, n_groups, kc, vc, kp, vp, bytes;
+} akv_int4_layout;
+int akv_int4_layout_init(int head_dim, int group, akv_int4_layout* out);
+
+/* One layer of a 4-bit paged cache, as the entries below read and write it.
+ * Record of (page p, KV head h): pool + p*page_stride + h*head_stride; row s
+ * holds lens[s] tokens, token t on page table[s*table_stride + t/32].  A page
+ * or row number out of range records AKV_ERR_SHAPE in *status; nothing is
+ * written then, and a read takes page 0. */
+typedef struct {
+  uint8_t* pool; /* 16-byte aligned; strides in bytes, multiples of 16 */
+  int64_t page_stride, head_stride;
+  int32_t n_pages;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lens;
+  int32_t max_seqs, max_blocks, kv_heads, head_dim, group;
+} akv_int4_cache;
+
+/* Quantise new K / V rows into the pages.  Call row i is sequence rows[i]
+ * (NULL: i) whose last n_new[i] (NULL: M; clamped to [0, M]) tokens are rows
+ * m = 0..n_new-1 of k / v: element (i, h, m, d) at k + i*k_sr + h*k_sh +
+ * m*k_sm + d (element strides), dtype AKV_FP16 or AKV_BF16, any alignment.
+ * NaN counts as 0, infinities as +-65504; per group, in fp32:
+ *   zero = fp16(min), scale = fp16((max - zero) / 15),
+ *   code = clamp(rint((x - zero) / scale), 0, 15), 0 where scale is 0. */
+int akv_int4_append(const akv_int4_cache* c, const int32_t* rows, const int32_t* n_new, int R, int M,
+                    const void* k, int64_t k_sr, int64_t k_sh, int64_t k_sm,
+                    const void* v, int64_t v_sr, int64_t v_sh, int64_t v_sm, int dtype, int* status, void* stream);
+
+/* The values the cache stands for: out (i, h, t, d), t < N, is token
+ * start[i] + t of sequence rows[i] (start NULL: its last n_new[i] tokens,
+ * n_new NULL: N), 0 where there is no such token; fp16 results are held to
+ * +-65504. */
+int akv_int4_read(const akv_int4_cache* c, const int32_t* rows, const int32_t* start, const int32_t* n_new, int R,
+                  int N, void* k, int64_t k_sr, int64_t k_sh, int64_t k_sm,
+                  void* v, int64_t v_sr, int64_t v_sh, int64_t v_sm, int dtype, int* status, void* stream);
+
+/* Attention of M query tokens per call row over its sequence.  Query m <
+ * n_new[i] stands at position lens - n_new + m and sees every token up to its
+ * own; a query with m >= n_new[i], or that sees no token, gets a zero row and
+ * lse -inf.  q element (i, hq, m, d) at q + i*q_sr + hq*q_sh + m*q_sm + d, out
+ * alike, both dtype AKV_FP16 or AKV_BF16; lse fp32 [R][Hq][M] (nullable,
+ * natural log).  Query head hq reads KV head hq / (Hq / kv_heads).
+ * Workspace: akv_int4_attention_workspace_bytes(...), 16-byte aligned. */
+size_t akv_int4_attention_workspace_bytes(int R, int M, int Hq, int kv_heads, int head_dim, int max_blocks);
+int akv_int4_attention(const akv_int4_cache* c, const int32_t* rows, const int32_t* n_new, int R, int M, int Hq,
+                       const void* q, int64_t q_sr, int64_t q_sh, int64_t q_sm, float sm_scale,
+                       void* out, int64_t o_sr, int64_t o_sh, int64_t o_sm, float* lse, int dtype,
+                       void* workspace, size_t workspace_bytes, int* status, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Ownership of the pages, kept on the device so that no step of a serving
+ * loop waits for the host.  refs[p] sequences hold page p; bit p of free_bits
+ * is set when none does (bits from n_pages up are 0).  Table entries past a
+ * row's pages are -1.  Results do not depend on timing: the lowest free pages
+ * are handed out in the order of the request.  A request with a bad or
+ * repeated row, or a bad length, is refused alone (AKV_ERR_SHAPE in *status).
+ *
+ * Workspace of reserve and compact: akv_pages_workspace_bytes(n_pages, n).
+ * pool: page p of layer l at pool + l*layer_stride + p*page_bytes (16-byte
+ * aligned, sizes multiples of 16).
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  int32_t* table;
+  int64_t table_stride;
+  int32_t* lens;
+  int32_t* refs;
+  uint32_t* free_bits;
+  int32_t max_seqs, max_blocks, n_pages;
+} akv_page_table;
+
+size_t akv_pages_workspace_bytes(int n_pages, int n);
+
+/* Row children[i] (empty) becomes a second holder of every page of row
+ * parents[i] and takes its length.  No row may be both parent and child. */
+int akv_pages_fork(const akv_page_table* t, const int32_t* parents, const int32_t* children, int n, int* status,
+                   void* stream);
+
+/* Room for n_new[i] (NULL: n_new_all) more tokens in row rows[i] (NULL: i),
+ * i < n <= 1024, and the lengths advanced.  A row whose partly filled last
+ * page has other holders gets a copy of it in every layer first (requests
+ * count in order, so the last holder keeps the page).  granted[i] = n_new, or
+ * 0 for a refused request; when the pool runs out, that request and all after
+ * it are refused (AKV_ERR_EXHAUSTED). */
+int akv_pages_reserve(const akv_page_table* t, const int32_t* rows, const int32_t* n_new, int n_new_all, int n,
+                      int32_t* granted, uint8_t* pool, int n_layers, int64_t layer_stride, int64_t page_bytes,
+                      void* workspace, size_t workspace_bytes, int* status, void* stream);
+
+/* Row rows[i] (NULL: i) shortened to new_lens[i] (NULL: 0) tokens; pages
+ * beyond it lose this holder and, with the last one gone, become free. */
+int akv_pages_truncate(const akv_page_table* t, const int32_t* rows, const int32_t* new_lens, int n, int* status,
+                       void* stream);
+
+/* The live pages moved to [0, n_live): the live page of rank i above n_live
+ * goes to the free page of rank i below it, in every layer, table and refs
+ * following.  *n_live (device) receives the count. */
+int akv_pages_compact(const akv_page_table* t, uint8_t* pool, int n_layers, int64_t layer_stride, int64_t page_bytes,
+                      int32_t* n_live, void* workspace, size_t workspace_bytes, int* status, void* stream);
+
+/* Page src[i] copied to page dst[i] in every layer, i < n (no page may be in
+ * both lists, nor twice in dst). */
+int akv_pages_copy(uint8_t* pool, int n_layers, int64_t layer_stride, int64_t page_bytes, int n_pages,
+                   const int32_t* src, const int32_t* dst, int n, int* status, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Verification of drafted tokens (speculative decoding).  target (b, j, x) at
+ * target + b*t_sb + j*t_sj + x, j <= K: the target model's probabilities
+ * after j accepted drafts; draft (b, j, x), j < K, the draft model's (NULL:
+ * drafts without a distribution, q = 1 on the drafted token); dtype AKV_FP32,
+ * AKV_FP16 or AKV_BF16; element strides, x contiguous, any alignment.
+ * tokens int64 (b, j) at tokens + b*K + j; accept_u fp32 [B][K], sample_u
+ * fp32 [B], uniform in [0, 1).  Sequence b offers n_draft[b] (NULL: K;
+ * clamped to [0, K]) drafts: draft j is accepted while accept_u * q < p holds
+ * (the product exact); the first rejected one ends it.  The next token is
+ * drawn from max(P - Q, 0) at the rejected position, or from P after the last
+ * draft, where P, Q count whole units of 2^-40 (negative and NaN count as 0,
+ * more than 1 as 1): the lowest x whose cumulative count exceeds
+ * floor(floor(2^24 sample_u) * total / 2^24); P itself where the difference
+ * is empty, and -1 where P is.  accepted[b] = drafts kept; out int64
+ * [B][K+1] = them, the drawn token, then -1.  A token outside [0, vocab) is
+ * rejected (AKV_ERR_SHAPE in *status).
+ * ---------------------------------------------------------------------- */
+int akv_verify_draft(const void* target, int64_t t_sb, int64_t t_sj, const void* draft, int64_t d_sb, int64_t d_sj,
+                     const int64_t* tokens, const int32_t* n_draft, const float* accept_u, const float* sample_u,
+                     int B, int K, int vocab, int dtype, int32_t* accepted, int64_t* out, int* status, void* stream);
 
 #ifdef __cplusplus
 }
