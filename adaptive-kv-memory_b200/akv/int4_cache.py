@@ -70,6 +70,7 @@ class Int4PagedCache:
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self._pt = _C.PageTable(self.table.data_ptr(), max_blocks, self.lens.data_ptr(), self.refs.data_ptr(),
                                 self.free_bits.data_ptr(), max_seqs, max_blocks, n_pages)
+        self._ws: dict = {}
         self._views = [self._view(layer) for layer in range(n_layers)]
 
     # ------------------------------------------------------------------ state
@@ -151,6 +152,16 @@ class Int4PagedCache:
     def _count(self, rows, n: int) -> None:
         if rows is None and n > self.max_seqs:
             raise ValueError(f"{n} rows, but the cache holds {self.max_seqs} sequences")
+
+    def _workspace(self, need: int, stream: int) -> torch.Tensor:
+        """Zeroed scratch for attention on a stream: kept per stream (calls on two streams may overlap), its own
+        for each call of a captured graph (replays may overlap eager calls)."""
+        if torch.cuda.is_current_stream_capturing():
+            return torch.zeros(need, dtype=torch.uint8, device=self.device)
+        ws = self._ws.get(stream)
+        if ws is None or ws.numel() < need:
+            ws = self._ws[stream] = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=self.device)
+        return ws
 
     # ------------------------------------------------------------------ pages
     def reserve(self, rows, n_new) -> torch.Tensor:
@@ -294,12 +305,13 @@ class Int4PagedCache:
         lse = torch.empty(R, Hq, M, dtype=torch.float32, device=q.device) if return_lse else None
         lib = _C.load()
         need = _C.workspace_bytes("akv_int4_attention_workspace_bytes", R, M, Hq, self.H, D, self.max_blocks)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        stream = _C.stream_of(q)
+        ws = self._workspace(need, stream)
         rc = lib.akv_int4_attention(ctypes.byref(view), _C.ptr(rows), _C.ptr(n_new), R, M, Hq,
                                     q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
                                     1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
                                     o.data_ptr(), o.stride(0), o.stride(1), o.stride(2), _C.ptr(lse), dt,
-                                    ws.data_ptr(), need, self.status.data_ptr(), _C.stream_of(q))
+                                    ws.data_ptr(), need, self.status.data_ptr(), stream)
         _C.check(rc, "akv_int4_attention")
         res = o.squeeze(2) if query.dim() == 3 else o
         return (res, lse) if return_lse else res

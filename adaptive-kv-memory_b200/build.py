@@ -21,7 +21,8 @@ INCLUDE = os.path.join(ROOT, "include")
 OUT_DIR = os.path.join(HERE, "akv", "_lib")
 LIB = os.path.join(OUT_DIR, "libakv_sm100.so")
 SOURCES = ["quant_pack.cu", "decode_attn.cu", "tiering.cu", "prefill_attn.cu", "group_format.cu", "layer_step.cu", "peer_exchange.cu",
-           "int4_cache.cu", "int4_attn.cu", "page_table.cu", "verify_draft.cu"]
+           "int4_cache.cu", "int4_attn.cu", "int4_attn_64.cu", "int4_attn_128.cu", "int4_attn_256.cu",
+           "page_table.cu", "verify_draft.cu"]
 
 
 def nvcc() -> str:
@@ -42,7 +43,7 @@ def flags(verbose: bool = False) -> list:
 def build(verbose: bool = False, force: bool = False) -> str:
     os.makedirs(OUT_DIR, exist_ok=True)
     srcs = [os.path.join(CSRC, s) for s in SOURCES]
-    deps = srcs + [os.path.join(CSRC, h) for h in ("common.cuh", "int4.cuh")] + [os.path.join(INCLUDE, "akv_b200.h")]
+    deps = srcs + [os.path.join(CSRC, h) for h in ("common.cuh", "int4.cuh", "int4_attn.cuh")] + [os.path.join(INCLUDE, "akv_b200.h")]
     if not force and os.path.exists(LIB):
         lib_t = os.path.getmtime(LIB)
         if all(os.path.getmtime(d) <= lib_t for d in deps):

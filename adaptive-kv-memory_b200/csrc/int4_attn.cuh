@@ -1,0 +1,864 @@
+// Attention over the 4-bit paged cache, straight from the packed pages
+// (kernel templates; one translation unit per head dim instantiates them).
+//
+// Mathematics.  With token t's value c*s_tg + z_tg in channel group g,
+//   q.K_t = sum_g  s_tg (q_g . c_tg) + z_tg sum(q_g)
+//   O     = sum_t p_t V_t
+//         = sum_t (p_t s_tg)(c - 8) + sum_t p_t (z_tg + 8 s_tg)
+// so both contractions run on codes.  For K a code needs no conversion: alone
+// in bits 4..7 of a half it is the fp16 subnormal c * 2^-20, one shift and one
+// AND for two codes of a word.  (The MMA aligns its products by the operands'
+// nominal exponents and cuts them off, so bits 0..3 would lose 4 bits more of
+// the sum.)  Over the thousands of additions of P.V that cutting off is a
+// drift of the growing sum; there the codes are centred, exactly, by one fp16
+// operation more, and the sums stay as small as the output.  Online softmax,
+// maximum and sums in fp32.
+//
+// Roundings: q is scaled per row by a power of two into fp16's middle range
+// (exact unless 2^-24 of the row's largest).  p_t s_tg enters the MMA as one
+// fp16 term for a bf16 output (an eighth of that output's own rounding), as
+// two, the second holding the first's error, for an fp16 output (LO).  The
+// zero-point sum, l and the partial results are fp32.
+#pragma once
+
+#include "int4.cuh"
+
+namespace akv {
+
+constexpr int kAttnWarps = 4;
+constexpr int kAttnThreads = kAttnWarps * 32;
+constexpr int kAttnEntries = 1024;  // (row, row tile) pairs of one launch
+constexpr int kAttnMinPages = 4;    // pages of a CTA's share, at least (one per warp)
+constexpr int kAttnFused = 1024;    // partial rows of a unit that its last CTA merges by itself
+constexpr float kLazyLog2 = 6.f;    // weights may reach 2^6 before the maximum moves
+
+struct Int4AttnParams {
+  akv_int4_cache c;
+  const int32_t* rows;
+  const int32_t* n_new;
+  int row0, R;  // call rows [row0, row0 + R) of this launch
+  int M, Hq, tiles;
+  const uint16_t* q;
+  int64_t q_sr, q_sh, q_sm;
+  float scale;
+  uint16_t* out;
+  int64_t o_sr, o_sh, o_sm;
+  float* lse;
+  int bf16;
+  float* part;         // [slot][8 NT][D + 2]
+  unsigned* arrived;   // per unit: CTAs that have stored their part; 0 between calls
+  int2* meta;          // per unit: first and last CTA, for the combine kernel (NULL: the last CTA merges)
+  int* status;
+};
+
+template <int D, int G, int NT>
+struct AttnShape {
+  static constexpr int GS = D / G;              // channels of a group
+  static constexpr int BK = GS / 8;             // K bytes of a thread per token and group
+  static constexpr int BV = GS / 16;            // V bytes of a thread per token and group
+  static constexpr int REC = int4_layout(D, G).bytes;
+  static constexpr int ROWS = 8 * NT;           // query rows of a CTA
+  static constexpr int STAGES = D == 64 ? 4 : (D == 128 && (NT > 1 || G == 1) ? 3 : 2);
+  static constexpr int RING = kAttnWarps * STAGES * REC;
+  static constexpr int PITCH = D + 4;
+  static constexpr int MERGE = kAttnWarps * ROWS * PITCH * 4;
+  static constexpr int BUF = RING > MERGE ? RING : MERGE;
+  static constexpr int FRAG = D / 16 * NT * 32 * 8;
+  // ring / merge buffer, fragments, then: group sums of q, exponent factors,
+  // visible lengths, (y, l) per warp and row, barriers; per entry: prefix sums
+  // of pages, lengths, new tokens
+  static constexpr int OFF_FRAG = (BUF + 127) / 128 * 128;
+  static constexpr int OFF_QS = OFF_FRAG + FRAG;
+  static constexpr int OFF_CQ = OFF_QS + ROWS * G * 4;
+  static constexpr int OFF_SEE = OFF_CQ + ROWS * 4;
+  static constexpr int OFF_ML = OFF_SEE + ROWS * 4;
+  static constexpr int OFF_BAR = OFF_ML + kAttnWarps * ROWS * 8;
+  static constexpr int OFF_PREF = OFF_BAR + kAttnWarps * STAGES * 8;
+  static constexpr int OCC = NT == 1 ? (D == 256 ? 2 : 4) : (NT == 2 ? (D == 256 ? 2 : 3) : 2);
+  static constexpr int smem(int entries) { return OFF_PREF + (3 * entries + 1) * 4; }
+  static_assert(OCC * (smem(64) + 1024) <= 228 * 1024, "resident CTAs do not fit");
+};
+
+// token of tile row g: a permutation within 8 that spreads the V loads of the
+// four thread columns over the banks (rows of both parities in every load)
+AKV_DEV int tile_token(int g) { return g ^ ((g >> 2) & 1); }
+
+// the codes in bits 0..3 (4..7) of both halves, as the fp16 pair c - 8
+AKV_DEV uint32_t low_code(uint32_t y) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(lop_magic<0x000F000Fu>(y)), "r"(0xE408E408u));  // 1024 + c - 1032
+  return r;
+}
+AKV_DEV uint32_t high_code(uint32_t y) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;"  // (1024 + 16 c) / 16 - 72
+      : "=r"(r)
+      : "r"(lop_magic<0x00F000F0u>(y)), "r"(0x2C002C00u), "r"(0xD480D480u));
+  return r;
+}
+
+template <int BYTES>
+AKV_DEV void lds_bytes(const uint8_t* p, uint32_t (&w)[BYTES < 4 ? 1 : BYTES / 4]) {
+  if constexpr (BYTES >= 16) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + 16 * i);
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (BYTES == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else if constexpr (BYTES == 4) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (BYTES == 2) {
+    w[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else {
+    w[0] = *p;
+  }
+}
+
+// tokens that query tokens [0, m_last] of call row i see, in pages
+AKV_DEV int visible_pages(const Int4Row& r, int m_last) {
+  const int see = r.len - r.n_new + m_last + 1;
+  return see > 0 ? (see + kBlockTokens - 1) / kBlockTokens : 0;
+}
+
+// Output channels of accumulator pair p (order of the merge buffer) of query
+// row rr of (call row i, KV head h); its lse with pair 0.
+template <int D, int G>
+AKV_DEV void store_pair(const Int4AttnParams& P, int i, int h, int rep, int rr, int n_new, int p, float2 v, float top,
+                        float L) {
+  constexpr int GS = D / G, BV = GS / 16;
+  const int j = p / 8, g = p % 8;
+  const int ch = j / BV * GS + g * 2 * BV + 2 * (j % BV);
+  const int m = rr / rep, hq = h * rep + rr % rep;
+  const bool on = m < n_new && L > 0.f;
+  const float inv = on ? 1.f / L : 0.f;
+  v.x = on ? v.x * inv : 0.f;
+  v.y = on ? v.y * inv : 0.f;
+  uint16_t* o = P.out + i * P.o_sr + hq * P.o_sh + m * P.o_sm + ch;
+  const uint32_t w = P.bf16 ? pack_elems<true>(v.x, v.y) : pack_elems<false>(v.x, v.y);
+  o[0] = static_cast<uint16_t>(w);
+  o[1] = static_cast<uint16_t>(w >> 16);
+  if (P.lse && p == 0)
+    P.lse[(static_cast<int64_t>(i) * P.Hq + hq) * P.M + m] = on ? (top + log2f(L)) * 0.6931471805599453f : -INFINITY;
+}
+
+// One CTA merges the parts of a unit (segs * 8 NT <= kAttnFused, so their
+// weights fit the buffer w).
+template <int D, int G, int NT>
+AKV_DEV void merge_parts(const Int4AttnParams& P, const float* part, int segs, int i, int h, int rep, int tile,
+                         int valid, int n_new, float* w) {
+  constexpr int ROWS = 8 * NT;
+  constexpr int64_t STEP = static_cast<int64_t>(ROWS) * (D + 2);
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  float2* s_tl = reinterpret_cast<float2*>(w + kAttnFused);  // per row: maximum, sum
+  for (int n = warp; n < valid; n += kAttnWarps) {
+    const float* ml = part + n * (D + 2) + D;
+    float top = -INFINITY, L = 0.f;
+    for (int s = lane; s < segs; s += 32) top = fmaxf(top, __ldcg(ml + s * STEP));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    for (int s = lane; s < segs; s += 32) {
+      const float2 yl = __ldcg(reinterpret_cast<const float2*>(ml + s * STEP));
+      const float x = yl.x == -INFINITY ? 0.f : exp2f(yl.x - top);
+      w[n * segs + s] = x;
+      L = fmaf(x, yl.y, L);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
+    if (lane == 0) s_tl[n] = make_float2(top, L);
+  }
+  __syncthreads();
+  for (int k = t; k < valid * (D / 2); k += kAttnThreads) {
+    const int n = k / (D / 2), p = k % (D / 2);
+    const float* at = part + n * (D + 2) + 2 * p;
+    float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 8
+    for (int s = 0; s < segs; ++s) {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(at + s * STEP));
+      const float x = w[n * segs + s];
+      acc.x = fmaf(x, v.x, acc.x);
+      acc.y = fmaf(x, v.y, acc.y);
+    }
+    store_pair<D, G>(P, i, h, rep, tile * ROWS + n, n_new, p, acc, s_tl[n].x, s_tl[n].y);
+  }
+}
+
+template <int D, int G, int NT, bool LO>
+__global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_attn_kernel(const Int4AttnParams P) {
+  using S = AttnShape<D, G, NT>;
+  constexpr int KS = D / 16;  // MMA steps of q.K
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* s_qs = reinterpret_cast<float*>(smem + S::OFF_QS);
+  float* s_cq = reinterpret_cast<float*>(smem + S::OFF_CQ);
+  int* s_see = reinterpret_cast<int*>(smem + S::OFF_SEE);
+  float2* s_ml = reinterpret_cast<float2*>(smem + S::OFF_ML);
+  uint64_t* s_bar = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
+  int* s_pref = reinterpret_cast<int*>(smem + S::OFF_PREF);
+  __shared__ int s_scan[kAttnWarps], s_max[kAttnWarps], s_last;
+
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int g = lane >> 2, q4 = lane & 3;
+  const int H = P.c.kv_heads, rep = P.Hq / H;
+  const int entries = P.R * P.tiles;
+  int* s_len = s_pref + entries + 1;
+  int* s_new = s_len + entries;
+
+  if (lane < S::STAGES) mbar_init(s_bar + warp * S::STAGES + lane, 1);
+  fence_mbar_init();
+
+  // Pages of every (row, row tile), as a prefix sum; all heads of a row alike.
+  {
+    int base = 0, most = 0;
+    for (int e0 = 0; e0 < entries; e0 += kAttnThreads) {
+      const int e = e0 + t;
+      int n = 0;
+      if (e < entries) {
+        const int i = P.row0 + e / P.tiles, tile = e % P.tiles;
+        const Int4Row r = int4_row(P.c, P.rows, P.n_new, i, P.M, P.status);
+        const int first = tile * S::ROWS / rep;  // its first query token
+        int last = (tile * S::ROWS + S::ROWS - 1) / rep;
+        if (last >= r.n_new) last = r.n_new - 1;
+        if (first <= last) n = visible_pages(r, last);
+        s_len[e] = r.len;
+        s_new[e] = r.n_new;
+      }
+      most = n > most ? n : most;
+      int x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(~0u, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == 31) s_scan[warp] = x;
+      __syncthreads();
+      int before = base, sum = base;
+#pragma unroll
+      for (int w = 0; w < kAttnWarps; ++w) {
+        if (w < warp) before += s_scan[w];
+        sum += s_scan[w];
+      }
+      if (e < entries) s_pref[e + 1] = before + x;
+      base = sum;
+      __syncthreads();
+    }
+    most = __reduce_max_sync(~0u, most);
+    if (lane == 0) s_max[warp] = most;
+    if (t == 0) s_pref[0] = 0;
+    __syncthreads();
+  }
+
+  // rows without any visible token: zero output
+  for (int u = blockIdx.x; u < entries * H; u += gridDim.x) {
+    const int e = u / H, h = u % H;
+    if (s_pref[e + 1] != s_pref[e]) continue;
+    const int i = P.row0 + e / P.tiles;
+    if (t == 0 && P.meta) P.meta[u] = make_int2(0, 0);
+    for (int k = t; k < S::ROWS * D; k += kAttnThreads) {
+      const int rr = e % P.tiles * S::ROWS + k / D, m = rr / rep;
+      if (m >= P.M) break;
+      const int hq = h * rep + rr % rep;
+      P.out[i * P.o_sr + hq * P.o_sh + m * P.o_sm + k % D] = 0;
+      if (P.lse && k % D == 0) P.lse[(static_cast<int64_t>(i) * P.Hq + hq) * P.M + m] = -INFINITY;
+    }
+  }
+
+  // This CTA's share of all pages, a contiguous run over (row, tile, head, page).
+  const int64_t total = static_cast<int64_t>(s_pref[entries]) * H;
+  int64_t share = (total + gridDim.x - 1) / gridDim.x;
+  {
+    int least = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+    if (least > kAttnMinPages) least = kAttnMinPages;
+    if (share < least) share = least;
+  }
+  int64_t pos = share * blockIdx.x;
+  const int64_t end = pos + share < total ? pos + share : total;
+  if (pos >= end) return;
+  int e = 0;
+  {
+    int hi = entries;  // the last entry that starts at or before pos
+    while (hi - e > 1) {
+      const int mid = (e + hi) / 2;
+      if (static_cast<int64_t>(s_pref[mid]) * H <= pos) e = mid; else hi = mid;
+    }
+  }
+  uint32_t stage = 0, phase = 0;
+  bool alive = true;
+  uint8_t* ring = smem + warp * S::STAGES * S::REC;
+  uint64_t* bars = s_bar + warp * S::STAGES;
+
+  while (pos < end) {
+    while (s_pref[e + 1] == s_pref[e]) ++e;
+    const int64_t e_start = static_cast<int64_t>(s_pref[e]) * H;
+    const int pages = s_pref[e + 1] - s_pref[e];
+    const int h = static_cast<int>((pos - e_start) / pages);
+    const int page0 = static_cast<int>((pos - e_start) % pages);
+    int n_pages = pages - page0;
+    if (n_pages > end - pos) n_pages = static_cast<int>(end - pos);
+    const int unit = e * H + h;
+    const int64_t u_start = e_start + static_cast<int64_t>(h) * pages;
+    const int cta0 = static_cast<int>(u_start / share), cta1 = static_cast<int>((u_start + pages - 1) / share);
+    const int i = P.row0 + e / P.tiles, tile = e % P.tiles;
+    const int len = s_len[e], n_new = s_new[e];
+    const int seq = P.rows ? __ldg(P.rows + i) : i;  // in range: its pages are not 0
+    const int32_t* table = P.c.table + seq * P.c.table_stride + page0;
+    const uint8_t* pool = P.c.pool + h * P.c.head_stride;
+    const int mine = (n_pages - warp + kAttnWarps - 1) / kAttnWarps;  // pages warp, warp + 4, ...
+
+    // page numbers of this warp's next 32 pages, one per lane
+    auto page_ids = [&](int k0) -> int {
+      const int k = k0 + lane;
+      int p = 0;
+      if (k < mine) {
+        p = __ldg(table + warp + k * kAttnWarps);
+        if (p < 0 || p >= P.c.n_pages) {
+          set_status(P.status, AKV_ERR_SHAPE);
+          p = 0;
+        }
+      }
+      return p;
+    };
+    auto issue = [&](int p, uint32_t st) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bars + st, S::REC);
+        tma_load_1d(ring + st * S::REC, pool + p * P.c.page_stride, S::REC, bars + st);
+      }
+    };
+    int ids = page_ids(0);
+#pragma unroll
+    for (int k = 0; k < S::STAGES; ++k) {
+      const int p = __shfl_sync(~0u, ids, k);
+      if (k < mine && alive) issue(p, (stage + k) % S::STAGES);
+    }
+
+    // Queries of the tile: scaled to fp16, placed as MMA operands; sums per group.
+    {
+      uint16_t* frag = reinterpret_cast<uint16_t*>(smem + S::OFF_FRAG);
+      constexpr int PER = D / 32;
+      constexpr int RW = S::ROWS / kAttnWarps;  // rows of a warp, all loads in flight at once
+      uint16_t raw[RW][PER];
+#pragma unroll
+      for (int k2 = 0; k2 < RW; ++k2) {
+        const int rr = tile * S::ROWS + k2 * kAttnWarps + warp, m = rr / rep;
+        const uint16_t* src = P.q + i * P.q_sr + (h * rep + rr % rep) * P.q_sh + m * P.q_sm + lane * PER;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) raw[k2][k] = m < n_new ? src[k] : 0;
+      }
+#pragma unroll
+      for (int k2 = 0; k2 < RW; ++k2) {
+        const int n = k2 * kAttnWarps + warp;
+        const int m = (tile * S::ROWS + n) / rep;
+        float x[PER];
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          x[k] = P.bf16 ? elem_to_float<true>(raw[k2][k]) : elem_to_float<false>(raw[k2][k]);
+          top = fmaxf(top, fabsf(x[k]));
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        int ex = 0;  // 2^ex brings the largest into [2^9, 2^10)
+        if (top > 0.f) ex = 9 - (static_cast<int>(__float_as_uint(top) >> 23) - 127);
+        ex = ex > 120 ? 120 : (ex < -120 ? -120 : ex);
+        const float up = exp2f(static_cast<float>(ex)) * (P.scale < 0.f ? -1.f : 1.f);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const int c = lane * PER + k;
+          const __half hv = __float2half_rn(x[k] * up);
+          sum += __half2float(hv);
+          const int gi = c / S::GS, r = c % S::GS, col = r / (S::GS / 4), r2 = r % (S::GS / 4);
+          int ks, reg, half;
+          if constexpr (S::BK >= 4) {
+            ks = gi * (S::GS / 16) + (r2 / 8) * 2 + ((r2 >> 1) & 1);
+            half = (r2 >> 2) & 1;
+          } else {
+            ks = gi;
+            half = r2 >> 1;
+          }
+          reg = c & 1 ? 0 : 1;
+          frag[(((ks * NT + n / 8) * 32 + (n % 8) * 4 + col) * 2 + reg) * 2 + half] = __half_as_ushort(hv);
+        }
+        constexpr int GL = 32 / G;  // lanes of a group
+#pragma unroll
+        for (int o = 1; o < GL; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (lane % GL == 0) s_qs[n * G + lane / GL] = sum * 9.5367431640625e-7f;  // 2^-20, the codes' unit
+        if (lane == 0) {
+          // log2 e * scale in units of the MMA result; never 0, so that -inf stays -inf
+          s_cq[n] = fmaxf(ldexpf(fabsf(P.scale) * 1.4426950408889634f, 20 - ex), 1e-37f);
+          s_see[n] = len - n_new + (m < n_new ? m : n_new - 1) + 1;
+        }
+      }
+    }
+    __syncthreads();
+
+    uint2 qf[NT == 1 ? KS : 1];
+    const uint2* frag2 = reinterpret_cast<const uint2*>(smem + S::OFF_FRAG) + lane;
+    if constexpr (NT == 1) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[ks] = frag2[ks * 32];
+    }
+    float qs[NT][2][G], cq[NT][2];
+    float mx[NT][2], mc[NT][2], lim[NT][2], l[NT][2], zs[NT][2][G];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int n = nt * 8 + q4 * 2 + c;
+        cq[nt][c] = s_cq[n];
+        mx[nt][c] = lim[nt][c] = -INFINITY;
+        mc[nt][c] = l[nt][c] = 0.f;
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) {
+          qs[nt][c][gi] = s_qs[n * G + gi];
+          zs[nt][c][gi] = 0.f;
+        }
+      }
+    const int see_min = s_see[0];
+    float O[NT][D / 16][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) O[nt][j][k] = 0.f;
+    float vref = 0.f, vinv = 0.f, vunit = 0.f;  // power of two above the V scales seen so far, its inverse
+
+    for (int k = 0; k < mine; ++k) {
+      if (!alive || !__all_sync(~0u, mbar_wait(bars + stage, phase, P.status))) {
+        // a copy never came: take no more, but see the ones in flight land
+        if (alive)
+          for (int r = 1; r < S::STAGES && k + r < mine; ++r) {
+            const uint32_t st = (stage + r) % S::STAGES;
+            mbar_wait(bars + st, stage + r >= S::STAGES ? phase ^ 1 : phase, P.status);
+          }
+        alive = false;
+        break;
+      }
+      const uint8_t* rec = ring + stage * S::REC;
+      const int tok0 = (page0 + warp + k * kAttnWarps) * kBlockTokens;
+
+      // ---- scores: tokens are the MMA's rows, queries its columns
+      float x[2][NT][4];
+      const __half2* kp = reinterpret_cast<const __half2*>(rec + int4_layout(D, G).kp);
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) {
+        uint32_t kw[4][S::BK < 4 ? 1 : S::BK / 4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          lds_bytes<S::BK>(rec + (r * 8 + tile_token(g)) * (D / 2) + gi * (S::GS / 2) + q4 * S::BK, kw[r]);
+        float acc[2][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[mt][nt][c] = 0.f;
+#pragma unroll
+        for (int s = 0; s < S::GS / 16; ++s) {
+          const int ks = gi * (S::GS / 16) + s;
+          uint2 b[NT];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) b[nt] = NT == 1 ? qf[NT == 1 ? ks : 0] : frag2[(ks * NT + nt) * 32];
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            // codes of the step's two channel pairs, at bits 4..7 of each half
+            uint32_t a[4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              if constexpr (S::BK >= 4) {
+                const uint32_t w = kw[2 * mt + r][s / 2];
+                a[r] = (s & 1 ? w >> 4 : w << 4) & 0x00F000F0u;
+                a[2 + r] = (s & 1 ? w >> 8 : w) & 0x00F000F0u;
+              } else {
+                const uint32_t w = prmt(kw[2 * mt + r][0], 0u, 0x4140);
+                a[r] = (w << 4) & 0x00F000F0u;
+                a[2 + r] = w & 0x00F000F0u;
+              }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816(acc[mt][nt], a[0], a[1], a[2], a[3], b[nt].x, b[nt].y);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float2 sz = __half22float2(kp[(r * 8 + tile_token(g)) * G + gi]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float& v = x[r >> 1][nt][(r & 1) * 2 + c];
+              const float zq = gi == 0 ? sz.y * qs[nt][c][gi] : fmaf(sz.y, qs[nt][c][gi], v);
+              v = fmaf(acc[r >> 1][nt][(r & 1) * 2 + c], sz.x, zq);
+            }
+        }
+      }
+      const bool tail = tok0 + kBlockTokens > see_min;
+      if (tail) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int see = s_see[nt * 8 + q4 * 2 + c] - tok0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (r * 8 + tile_token(g) >= see) x[r >> 1][nt][(r & 1) * 2 + c] = -INFINITY;
+          }
+      }
+      // ---- V scales and zeros of this thread's tokens
+      float vs[4][G], vz[4][G];
+      {
+        const __half2* vp = reinterpret_cast<const __half2*>(rec + int4_layout(D, G).vp);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int gi = 0; gi < G; ++gi) {
+            float2 sz = __half22float2(vp[(r * 8 + tile_token(g)) * G + gi]);
+            // slots past the row's end hold anything: nothing of them may reach a sum
+            if (tail && tok0 + r * 8 + tile_token(g) >= len) sz = make_float2(0.f, 0.f);
+            vs[r][gi] = sz.x;
+            vz[r][gi] = fmaf(8.f, sz.x, sz.y);
+          }
+      }
+      // ---- running maximum and V unit move together, rarely
+      bool move = false;
+      float top[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          top[nt][c] = fmaxf(fmaxf(x[0][nt][c], x[0][nt][2 + c]), fmaxf(x[1][nt][c], x[1][nt][2 + c]));
+          move |= top[nt][c] > lim[nt][c];
+        }
+      float vtop = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) vtop = fmaxf(vtop, fabsf(vs[r][gi]));
+      move |= vtop > vref;
+      if (__any_sync(~0u, move)) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(~0u, vtop, o));
+        float fv = 1.f;
+        if (vtop > vref) {
+          // the power of two above vtop (scales are finite fp16 values)
+          const float ref = __uint_as_float((__float_as_uint(vtop) & 0x7F800000u) + 0x00800000u);
+          fv = vref > 0.f ? vref / ref : 1.f;
+          vref = ref;
+          vinv = 1.f / ref;
+          vunit = ref;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float f[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float m = top[nt][c];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+            m = fmaxf(m, mx[nt][c]);
+            const float y = m == -INFINITY ? 0.f : m * cq[nt][c];
+            f[c] = mx[nt][c] == -INFINITY ? 0.f : exp2f(mc[nt][c] - y);
+            mx[nt][c] = m;
+            mc[nt][c] = y;
+            lim[nt][c] = m + kLazyLog2 / cq[nt][c];
+            l[nt][c] *= f[c];
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) zs[nt][c][gi] *= f[c];
+          }
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) O[nt][j][c] *= f[c & 1] * fv;
+        }
+      }
+      // ---- weights
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float& v = x[r >> 1][nt][(r & 1) * 2 + c];
+            v = fast_exp2(fmaf(v, cq[nt][c], -mc[nt][c]));
+            l[nt][c] += v;
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) zs[nt][c][gi] = fmaf(v, vz[r][gi], zs[nt][c][gi]);
+          }
+      // ---- values: channels are the MMA's rows, tokens its depth
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) {
+        uint32_t pb[4][NT], pl[LO ? 4 : 1][LO ? NT : 1];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float sn = vs[r][gi] * vinv;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float w0 = x[r >> 1][nt][(r & 1) * 2] * sn, w1 = x[r >> 1][nt][(r & 1) * 2 + 1] * sn;
+            const uint32_t hi = pack_h2(w0, w1);
+            pb[r][nt] = movmatrix_trans(hi);
+            if constexpr (LO) {
+              const float2 back = __half22float2(u32_as_h2(hi));
+              pl[r][nt] = movmatrix_trans(pack_h2(w0 - back.x, w1 - back.y));
+            }
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          constexpr int NW = S::BV < 4 ? 1 : S::BV / 4;
+          uint32_t va[2][NW], vb[2][NW];  // the two tokens of each 8-token tile
+#pragma unroll
+          for (int T = 0; T < 2; ++T) {
+            const uint8_t* vr = rec + int4_layout(D, G).vc + ((2 * kk + T) * 8) * (D / 2) + gi * (S::GS / 2) + g * S::BV;
+            lds_bytes<S::BV>(vr + tile_token(2 * q4) * (D / 2), va[T]);
+            lds_bytes<S::BV>(vr + tile_token(2 * q4 + 1) * (D / 2), vb[T]);
+          }
+#pragma unroll
+          for (int b = 0; b < S::BV; ++b) {
+            // bytes b of both tokens, the first in the low half
+            const uint32_t y0 = prmt(va[0][b / 4], vb[0][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
+            const uint32_t y1 = prmt(va[1][b / 4], vb[1][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint32_t a0 = low_code(y0), a1 = high_code(y0), a2 = low_code(y1), a3 = high_code(y1);
+              mma_16816(O[nt][gi * S::BV + b], a0, a1, a2, a3, pb[2 * kk][nt], pb[2 * kk + 1][nt]);
+              if constexpr (LO)
+                mma_16816(O[nt][gi * S::BV + b], a0, a1, a2, a3, pl[2 * kk][nt], pl[2 * kk + 1][nt]);
+            }
+          }
+        }
+      }
+      // ---- the stage is free: the page STAGES ahead
+      __syncwarp();
+      const int next = k + S::STAGES;
+      if (next < mine) {
+        if ((next & 31) == 0) ids = page_ids(next);
+        const int p = __shfl_sync(~0u, ids, next & 31);
+        issue(p, stage);
+      }
+      if (++stage == S::STAGES) stage = 0, phase ^= 1;
+    }
+
+    // ---- the warps' results meet
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          l[nt][c] += __shfl_xor_sync(~0u, l[nt][c], o);
+#pragma unroll
+          for (int gi = 0; gi < G; ++gi) zs[nt][c][gi] += __shfl_xor_sync(~0u, zs[nt][c][gi], o);
+        }
+        if (g == 0)
+          s_ml[warp * S::ROWS + nt * 8 + q4 * 2 + c] = make_float2(mx[nt][c] == -INFINITY ? -INFINITY : mc[nt][c], l[nt][c]);
+      }
+    __syncthreads();  // every warp is done with its ring
+    float* merge = reinterpret_cast<float*>(smem);
+    float f[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int n = nt * 8 + q4 * 2 + c;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) m = fmaxf(m, s_ml[w * S::ROWS + n].x);
+        f[nt][c] = mx[nt][c] == -INFINITY ? 0.f : exp2f(mc[nt][c] - m);
+      }
+    // each warp's share, scaled to the common maximum; within a row the
+    // channels stand in the accumulators' order, 16 (j, g, parity) at a time
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi)
+#pragma unroll
+        for (int b = 0; b < S::BV; ++b) {
+          const int j = gi * S::BV + b;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float2 v;  // even channel (high nibble), odd channel
+            v.x = f[nt][c] * fmaf(O[nt][j][2 + c], vunit, zs[nt][c][gi]);
+            v.y = f[nt][c] * fmaf(O[nt][j][c], vunit, zs[nt][c][gi]);
+            *reinterpret_cast<float2*>(merge + (warp * S::ROWS + nt * 8 + q4 * 2 + c) * S::PITCH + j * 16 + g * 2) = v;
+          }
+        }
+    __syncthreads();
+    const int valid = min(S::ROWS, P.M * rep - tile * S::ROWS);  // query rows of this tile
+    const bool whole = cta0 == cta1;
+    constexpr int64_t STEP = static_cast<int64_t>(S::ROWS) * (D + 2);
+    float* part = P.part + (static_cast<int64_t>(blockIdx.x) + unit) * STEP;
+    for (int k = t; k < valid * (D / 2); k += kAttnThreads) {
+      const int n = k / (D / 2), p = k % (D / 2);
+      float top = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, s_ml[w * S::ROWS + n].x);
+      float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kAttnWarps; ++w) {
+        const float2 a = s_ml[w * S::ROWS + n];
+        if (a.x != -INFINITY) L = fmaf(a.y, exp2f(a.x - top), L);
+        const float2 o = *reinterpret_cast<const float2*>(merge + (w * S::ROWS + n) * S::PITCH + 2 * p);
+        v.x += o.x, v.y += o.y;
+      }
+      if (whole) {
+        store_pair<D, G>(P, i, h, rep, tile * S::ROWS + n, n_new, p, v, top, L);
+      } else {
+        *reinterpret_cast<float2*>(part + n * (D + 2) + 2 * p) = v;
+        if (p == 0) *reinterpret_cast<float2*>(part + n * (D + 2) + D) = make_float2(top, L);
+      }
+    }
+    if (!whole) {
+      if (P.meta) {
+        if (t == 0 && cta0 == static_cast<int>(blockIdx.x)) P.meta[unit] = make_int2(cta0, cta1);
+      } else {
+        // the last of the unit's CTAs to arrive merges their parts
+        __threadfence();
+        __syncthreads();
+        if (t == 0) {
+          const unsigned segs = cta1 - cta0 + 1;
+          s_last = atomicInc(P.arrived + unit, segs - 1) == segs - 1;  // wraps to 0 for the next call
+        }
+        __syncthreads();
+        if (s_last) {
+          __threadfence();
+          merge_parts<D, G, NT>(P, P.part + (static_cast<int64_t>(cta0) + unit) * STEP, cta1 - cta0 + 1, i, h, rep, tile,
+                                valid, n_new, reinterpret_cast<float*>(smem));
+        }
+      }
+    }
+    // the merge buffer goes back to the copies
+    fence_proxy_async_shared();
+    __syncthreads();
+    pos += n_pages;
+    if (pos - e_start >= static_cast<int64_t>(pages) * H) ++e;
+  }
+}
+
+// Partial results of the units that several CTAs shared, one query row per CTA.
+template <int D, int G, int NT>
+__global__ void __launch_bounds__(128) int4_combine_kernel(const Int4AttnParams P) {
+  constexpr int ROWS = 8 * NT;
+  constexpr int64_t STEP = static_cast<int64_t>(ROWS) * (D + 2);
+  __shared__ float s_w[128], s_red[8];
+  __shared__ float2 s_acc[128];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int unit = blockIdx.x, n = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int2 cta = P.meta[unit];
+  const int segs = cta.y - cta.x + 1;
+  if (segs <= 1) return;
+  const int H = P.c.kv_heads, rep = P.Hq / H;
+  const int e = unit / H, h = unit % H, i = P.row0 + e / P.tiles;
+  const int rr = e % P.tiles * ROWS + n;
+  if (rr / rep >= P.M) return;
+  const Int4Row row = int4_row(P.c, P.rows, P.n_new, i, P.M, nullptr);
+  const float* part = P.part + (static_cast<int64_t>(cta.x) + unit) * STEP + n * (D + 2);
+  float top = -INFINITY;
+  for (int s = t; s < segs; s += 128) top = fmaxf(top, part[s * STEP + D]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  if (lane == 0) s_red[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  // channel pairs across, the rest of the threads take every other part
+  constexpr int PAIRS = D / 2, WAYS = 128 / PAIRS;
+  const int p = t % PAIRS, way = t / PAIRS;
+  float L = 0.f;
+  float2 acc = make_float2(0.f, 0.f);
+  for (int s0 = 0; s0 < segs; s0 += 128) {
+    __syncthreads();
+    if (s0 + t < segs) {
+      const float2 yl = *reinterpret_cast<const float2*>(part + (s0 + t) * STEP + D);
+      const float w = yl.x == -INFINITY ? 0.f : exp2f(yl.x - top);
+      s_w[t] = w;
+      L += w * yl.y;
+    }
+    __syncthreads();
+    const int cnt = segs - s0 < 128 ? segs - s0 : 128;
+#pragma unroll 8
+    for (int s = way; s < cnt; s += WAYS) {
+      const float2 v = *reinterpret_cast<const float2*>(part + (s0 + s) * STEP + 2 * p);
+      acc.x = fmaf(s_w[s], v.x, acc.x);
+      acc.y = fmaf(s_w[s], v.y, acc.y);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
+  if (lane == 0) s_red[4 + warp] = L;
+  if (way) s_acc[(way - 1) * PAIRS + p] = acc;
+  __syncthreads();
+  if (way) return;
+  L = s_red[4] + s_red[5] + s_red[6] + s_red[7];
+#pragma unroll
+  for (int w = 1; w < WAYS; ++w) {
+    acc.x += s_acc[(w - 1) * PAIRS + p].x;
+    acc.y += s_acc[(w - 1) * PAIRS + p].y;
+  }
+  store_pair<D, G>(P, i, h, rep, rr, row.n_new, p, acc, top, L);
+}
+
+// ---------------------------------------------------------------- host
+constexpr int kSMs = 148;
+
+// column tiles of 8 query rows for `rows` rows of a (sequence, KV head)
+inline int attn_nt(int D, int rows) {
+  const int most = D == 256 ? 2 : 4;
+  const int nt = (rows + 7) / 8;
+  return nt < most ? nt : most;
+}
+
+inline int attn_occ(int D, int nt) { return nt == 1 ? (D == 256 ? 2 : 4) : (nt == 2 ? (D == 256 ? 2 : 3) : 2); }
+
+template <int D, int G, int NT, bool LO>
+int attn_launch(const Int4AttnParams& p, cudaStream_t st) {
+  using S = AttnShape<D, G, NT>;
+  const int entries = p.R * p.tiles;
+  const int smem = S::smem(entries);
+  if (!ensure_dynamic_smem<int4_attn_kernel<D, G, NT, LO>>(S::smem(kAttnEntries))) return AKV_ERR_LAUNCH;
+  const int grid = kSMs * S::OCC;
+  int4_attn_kernel<D, G, NT, LO><<<grid, kAttnThreads, smem, st>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return AKV_ERR_LAUNCH;
+  if (!p.meta) return AKV_OK;
+  cudaLaunchConfig_t cfg{};
+  const int q_rows = p.M * (p.Hq / p.c.kv_heads);
+  cfg.gridDim = dim3(entries * p.c.kv_heads, q_rows < S::ROWS ? q_rows : S::ROWS);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, int4_combine_kernel<D, G, NT>, p) == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH;
+}
+
+template <int D, int G, int NT>
+int attn_dispatch_lo(const Int4AttnParams& p, cudaStream_t st) {
+  return p.bf16 ? attn_launch<D, G, NT, false>(p, st) : attn_launch<D, G, NT, true>(p, st);
+}
+
+template <int D, int G>
+int attn_dispatch_nt(const Int4AttnParams& p, int nt, cudaStream_t st) {
+  if (nt == 1) return attn_dispatch_lo<D, G, 1>(p, st);
+  if (nt == 2) return attn_dispatch_lo<D, G, 2>(p, st);
+  if constexpr (D != 256) {
+    if (nt == 3) return attn_dispatch_lo<D, G, 3>(p, st);
+    if (nt == 4) return attn_dispatch_lo<D, G, 4>(p, st);
+  }
+  return AKV_ERR_UNSUPPORTED;
+}
+
+template <int D>
+int attn_dispatch(const Int4AttnParams& p, int nt, cudaStream_t st) {
+  const int G = D / p.c.group;
+  if (G == 1) return attn_dispatch_nt<D, 1>(p, nt, st);
+  if (G == 2) return attn_dispatch_nt<D, 2>(p, nt, st);
+  return attn_dispatch_nt<D, 4>(p, nt, st);
+}
+
+int int4_attn_64(const Int4AttnParams& p, int nt, cudaStream_t st);
+int int4_attn_128(const Int4AttnParams& p, int nt, cudaStream_t st);
+int int4_attn_256(const Int4AttnParams& p, int nt, cudaStream_t st);
+
+}  // namespace akv

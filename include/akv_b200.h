@@ -684,7 +684,9 @@ int akv_int4_read(const akv_int4_cache* c, const int32_t* rows, const int32_t* s
  * lse -inf.  q element (i, hq, m, d) at q + i*q_sr + hq*q_sh + m*q_sm + d, out
  * alike, both dtype AKV_FP16 or AKV_BF16; lse fp32 [R][Hq][M] (nullable,
  * natural log).  Query head hq reads KV head hq / (Hq / kv_heads).
- * Workspace: akv_int4_attention_workspace_bytes(...), 16-byte aligned. */
+ * Workspace: akv_int4_attention_workspace_bytes(...), 16-byte aligned, zeroed
+ * once before its first use (its counters are 0 again after every call, so
+ * calls in order on one stream may share it, whatever their shapes). */
 size_t akv_int4_attention_workspace_bytes(int R, int M, int Hq, int kv_heads, int head_dim, int max_blocks);
 int akv_int4_attention(const akv_int4_cache* c, const int32_t* rows, const int32_t* n_new, int R, int M, int Hq,
                        const void* q, int64_t q_sr, int64_t q_sh, int64_t q_sm, float sm_scale,
