@@ -8,8 +8,10 @@
 // Bound by memory: 2*D*2 bytes in and D + 8*G bytes out per token and head.
 // One thread holds 8 channels (one 16-byte load, one 4-byte store of codes),
 // D/8 threads a row, four rows in flight; a group's min and max meet as one
-// 16-bit pair in log2(g/8) shuffles.  A CTA takes 64 tokens of one sequence,
-// so the row and page lookups are paid once.
+// 16-bit pair in log2(g/8) shuffles.  A CTA takes one page of one sequence, so
+// the row and page lookups are paid once.
+#include <type_traits>
+
 #include "int4.cuh"
 
 namespace akv {
@@ -29,60 +31,44 @@ struct Int4Io {
 };
 
 constexpr int kIoThreads = 256;
-constexpr int kIoTokens = 64;  // tokens of a CTA: at most three pages
-constexpr int kIoUnroll = 4;   // rows a thread has in flight
+constexpr int kIoWarps = kIoThreads / 32;
+constexpr int kIoUnroll = 4;  // rows a thread has in flight
 
-// The CTA's tokens [m0, m0 + count) of call row i: their first position and the
-// pages they lie on (-1: none), read once.
-struct IoTile {
-  int seq, count, page0;
-  int64_t pos0;
-  int pages[3];
+// The call tokens of row i that lie on one page: block `blk` of the pages that
+// its tokens start on.  Token m of the call is at position pos0 + m.
+struct IoPage {
+  int seq, page;
+  int m0, m1;   // call tokens on it
+  int end;      // those from here on do not exist (yet)
+  int slot0;    // slot of token m0
 };
 
-AKV_DEV bool io_tile(const Int4Io& a, int i, int m0, bool write, IoTile& t, int* s_pages) {
-  const Int4Row row = int4_row(a.c, a.rows, a.n_new, i, a.M, threadIdx.x == 0 ? a.status : nullptr);
+AKV_DEV IoPage io_page(const Int4Io& a, int i, int blk, bool write) {
+  int* status = threadIdx.x == 0 ? a.status : nullptr;
+  const Int4Row row = int4_row(a.c, a.rows, a.n_new, i, a.M, status);
+  IoPage t;
   t.seq = row.seq;
-  int n = a.M - m0;  // tokens of the call here
-  if (write && n > row.n_new - m0) n = row.n_new - m0;
-  t.count = n < kIoTokens ? n : kIoTokens;
-  const int64_t first = a.start ? static_cast<int64_t>(a.start[i]) : static_cast<int64_t>(row.len) - row.n_new;
-  t.pos0 = first + m0;
-  // a page is looked up where it holds one of these tokens
-  const int64_t lo = t.pos0 > 0 ? t.pos0 : 0;
-  t.page0 = lo < row.len ? static_cast<int>(lo / kBlockTokens) : 0;
-  if (threadIdx.x < 3) {
-    const int j = t.page0 + threadIdx.x;
-    int p = -1;
-    if (row.seq >= 0 && static_cast<int64_t>(j) * kBlockTokens < row.len &&
-        static_cast<int64_t>(j) * kBlockTokens < t.pos0 + t.count) {
-      p = a.c.table[row.seq * a.c.table_stride + j];
-      if (p < 0 || p >= a.c.n_pages) {
-        set_status(a.status, AKV_ERR_SHAPE);
-        p = write ? -1 : 0;
-      }
+  t.page = -1;
+  const int64_t pos0 = a.start ? static_cast<int64_t>(a.start[i]) : static_cast<int64_t>(row.len) - row.n_new;
+  const int64_t b0 = pos0 >= 0 ? pos0 / kBlockTokens : -((kBlockTokens - 1 - pos0) / kBlockTokens);  // floor
+  const int64_t first = (b0 + blk) * kBlockTokens - pos0;  // call token at the page's first slot
+  const int n = write ? row.n_new : a.M;
+  t.m0 = first > 0 ? static_cast<int>(first < n ? first : n) : 0;
+  t.m1 = first + kBlockTokens < n ? static_cast<int>(first + kBlockTokens) : n;
+  t.slot0 = first > 0 ? 0 : static_cast<int>(-first);
+  const int64_t pos = (b0 + blk) * kBlockTokens;
+  if (row.seq >= 0 && b0 + blk >= 0 && pos < row.len && t.m0 < t.m1) {
+    t.page = a.c.table[row.seq * a.c.table_stride + b0 + blk];
+    if (t.page < 0 || t.page >= a.c.n_pages) {
+      set_status(status, AKV_ERR_SHAPE);
+      t.page = write ? -1 : 0;
     }
-    s_pages[threadIdx.x] = p;
   }
-  __syncthreads();
-  return t.count > 0;
+  const int64_t end = row.len - pos0;
+  t.end = t.page < 0 || end < t.m0 ? t.m0 : (end < t.m1 ? static_cast<int>(end) : t.m1);
+  if (write) t.m1 = t.end;
+  return t;
 }
-
-// Walk of the (token, head, K / V) rows of a tile by groups of L threads,
-// without a division per row.
-struct IoWalk {
-  int m, hk, dm, dhk, rows2;
-  AKV_DEV void init(int first, int step, int h2) {
-    rows2 = h2;
-    m = first / h2, hk = first % h2;
-    dm = step / h2, dhk = step % h2;
-  }
-  AKV_DEV void next() {
-    m += dm;
-    hk += dhk;
-    if (hk >= rows2) hk -= rows2, ++m;
-  }
-};
 
 // x / s to the nearest float, for r the float nearest 1/s: one Newton step on
 // the quotient leaves the correctly rounded result (Markstein), so ties in
@@ -99,7 +85,12 @@ AKV_DEV float recip(float s) {
   return __fmaf_rn(__fmaf_rn(-s, r, 1.f), r, r);
 }
 
-// minimum of both halves
+AKV_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 template <bool BF>
 AKV_DEV uint32_t min2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -107,171 +98,223 @@ AKV_DEV uint32_t min2(uint32_t a, uint32_t b) {
   else asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-
 template <bool BF>
-__global__ void __launch_bounds__(kIoThreads) int4_append_kernel(const Int4Io a) {
-  __shared__ int s_pages[3];
-  IoTile tile;
-  const int i = blockIdx.y, m0 = blockIdx.x * kIoTokens;
-  if (!io_tile(a, i, m0, true, tile, s_pages)) return;
-  const int D = a.c.head_dim, L = D / 8, group = a.c.group;
-  const int part = threadIdx.x % L;  // 8 channels of a row
-  const int gl = group / 8;          // threads of a group
-  const int G = D / group, gi = part / gl;
-  const int vc = kBlockTokens * D / 2, vp = kBlockTokens * G * 4;
-  const uint16_t* k = a.k + i * a.k_sr + m0 * a.k_sm + part * 8;
-  const uint16_t* v = a.v + i * a.v_sr + m0 * a.v_sm + part * 8;
-  IoWalk w;
-  w.init(threadIdx.x / L, kIoThreads / L, 2 * a.c.kv_heads);
-  // all threads of a warp stay together (the shuffles): rows past the end idle
-  const int rows = tile.count * w.rows2, rounds = (rows + kIoThreads / L - 1) / (kIoThreads / L);
-  for (int it = 0; it < rounds; it += kIoUnroll) {
-    uint4 raw[kIoUnroll];
-    int m[kIoUnroll], hk[kIoUnroll];
+AKV_DEV uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (BF) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Eight channels of a group spread over gl threads: codes (word in the
+// record's byte order), scale and zero.  All lanes of the warp take part.
+template <bool BF>
+AKV_DEV uint32_t quantise8(uint4 raw, int gl, __half2& sz) {
+  const uint32_t e[4] = {raw.x, raw.y, raw.z, raw.w};
+  // a bit 15 / 31 where an element is NaN, infinite or past 65504
+  constexpr uint32_t PAST = BF ? 0x38803880u : 0x04000400u;
+  uint32_t odd = 0;
 #pragma unroll
-    for (int u = 0; u < kIoUnroll; ++u) {
-      m[u] = w.m, hk[u] = w.hk;
-      w.next();
-      raw[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (m[u] < tile.count) {
-        const int h = hk[u] >> 1;
-        const uint16_t* src = hk[u] & 1 ? v + h * a.v_sh + m[u] * a.v_sm : k + h * a.k_sh + m[u] * a.k_sm;
-        if (a.aligned) {
-          raw[u] = ldg_nc_v4(src);
-        } else {
-          uint16_t e[8];
+  for (int j = 0; j < 4; ++j) odd |= (e[j] & 0x7FFF7FFFu) + PAST;
+  float x[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) e[j] = src[j];
-          raw[u] = *reinterpret_cast<const uint4*>(e);
-        }
-      }
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = elem_to_float<BF>(static_cast<uint16_t>(e[j]));
+    x[2 * j + 1] = BF ? __uint_as_float(e[j] & 0xFFFF0000u) : elem_to_float<BF>(static_cast<uint16_t>(e[j] >> 16));
+  }
+  float lo, hi;
+  if (__any_sync(~0u, (odd & 0x80008000u) != 0)) {
+    // NaN counts as 0, anything past fp16's range as its end
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = x[j] == x[j] ? fminf(fmaxf(x[j], -65504.f), 65504.f) : 0.f;
+    lo = hi = x[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]);
+    for (int o = 1; o < gl; o <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
     }
+  } else {
+    // (minimum, negated maximum) of the group as one 16-bit pair
+    const uint32_t a2 = min2<BF>(min2<BF>(e[0], e[1]), min2<BF>(e[2], e[3]));
+    const uint32_t b2 = max2<BF>(max2<BF>(e[0], e[1]), max2<BF>(e[2], e[3])) ^ 0x80008000u;
+    uint32_t p = min2<BF>(prmt(a2, b2, 0x5410), prmt(a2, b2, 0x7632));
+    for (int o = 1; o < gl; o <<= 1) p = min2<BF>(p, __shfl_xor_sync(~0u, p, o));
+    lo = elem_to_float<BF>(static_cast<uint16_t>(p));
+    hi = -elem_to_float<BF>(static_cast<uint16_t>(p >> 16));
+  }
+  const __half zh = __float2half_rn(lo);
+  const float z = __half2float(zh);
+  const __half sh = __float2half_rn(div_by(__fsub_rn(hi, z), 15.f, 1.f / 15.f));
+  const float s = __half2float(sh);
+  const float r = s > 0.f ? recip(s) : 0.f;  // scale 0: every quotient 0
+  sz = __halves2half2(sh, zh);
+  // 1.5 * 2^23 + quotient: the sum rounds half to even and holds the code in its low bits
+  const uint64_t nz = f2_make(-z, -z), r2 = f2_make(r, r), ns = f2_make(-s, -s), magic = f2_make(12582912.f, 12582912.f);
+  float c[8];
 #pragma unroll
-    for (int u = 0; u < kIoUnroll; ++u) {
-      uint32_t e[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-      // NaN counts as 0, anything past fp16's range as its end
-      bool odd = false;
+  for (int j = 0; j < 4; ++j) {
+    const uint64_t d = f2_add(f2_make(x[2 * j], x[2 * j + 1]), nz);
+    const uint64_t q0 = f2_mul(d, r2);
+    const uint64_t q = f2_fma(f2_fma(ns, q0, d), r2, q0);
+    const float2 v = f2_split(f2_add(q, magic));
+    c[2 * j] = v.x, c[2 * j + 1] = v.y;
+  }
+  // Quotients leave [0, 15.5) only where the zero was rounded up or the scale
+  // has lost bits (below fp16's normal range).
+  if (__any_sync(~0u, z > lo || s < 6.103515625e-5f)) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (BF) {
-          odd |= !(fabsf(__uint_as_float(e[j] << 16)) <= 65504.f) | !(fabsf(__uint_as_float(e[j] & 0xFFFF0000u)) <= 65504.f);
-        } else {
-          odd |= (e[j] & 0x7C00u) == 0x7C00u || (e[j] & 0x7C000000u) == 0x7C000000u;
+    for (int j = 0; j < 8; ++j) c[j] = fminf(fmaxf(c[j], 12582912.f), 12582927.f);
+  }
+  // nibbles from the top: channels 6 7 4 5 2 3 0 1; the exponents' share of the sum taken off at the end
+  uint32_t w = __float_as_uint(c[6]);
+  w = w * 16u + __float_as_uint(c[7]);
+  w = w * 16u + __float_as_uint(c[4]);
+  w = w * 16u + __float_as_uint(c[5]);
+  w = w * 16u + __float_as_uint(c[2]);
+  w = w * 16u + __float_as_uint(c[3]);
+  w = w * 16u + __float_as_uint(c[0]);
+  w = w * 16u + __float_as_uint(c[1]);
+  return w - 0x4B400000u * 0x11111111u;
+}
+
+// A CTA takes one page of one call row, a warp one (head, K / V) of it at a
+// time: D/8 threads a token, so 32 / (D/8) tokens a step.
+template <bool BF, int D>
+__global__ void __launch_bounds__(kIoThreads) int4_append_kernel(const Int4Io a) {
+  constexpr int L = D / 8, TW = 32 / L;
+  const int i = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const IoPage t = io_page(a, i, blockIdx.x, true);
+  const int n = t.m1 - t.m0;
+  if (n <= 0) return;
+  const int part = lane % L, tw = lane / L, gl = a.c.group / 8, G = D / a.c.group;
+  for (int hk = warp; hk < 2 * a.c.kv_heads; hk += kIoWarps) {
+    const int h = hk >> 1, is_v = hk & 1;
+    const int64_t sm = is_v ? a.v_sm : a.k_sm;
+    const uint16_t* src = (is_v ? a.v + i * a.v_sr + h * a.v_sh : a.k + i * a.k_sr + h * a.k_sh) +
+                          (t.m0 + tw) * sm + part * 8;
+    uint8_t* rec = a.c.pool + t.page * a.c.page_stride + h * a.c.head_stride;
+    uint8_t* codes = rec + is_v * (kBlockTokens * D / 2) + (t.slot0 + tw) * (D / 2) + part * 4;
+    uint8_t* pairs = rec + kBlockTokens * D + is_v * (kBlockTokens * G * 4) + ((t.slot0 + tw) * G + part / gl) * 4;
+    const bool lead = part % gl == 0;
+    for (int m = 0; m < n; m += TW * kIoUnroll) {
+      uint4 raw[kIoUnroll];
+#pragma unroll
+      for (int u = 0; u < kIoUnroll; ++u) {
+        raw[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (m + u * TW + tw < n) {
+          const uint16_t* p = src + (m + u * TW) * sm;
+          if (a.aligned) {
+            raw[u] = ldg_nc_v4(p);
+          } else {
+            raw[u].x = p[0] | static_cast<uint32_t>(p[1]) << 16;
+            raw[u].y = p[2] | static_cast<uint32_t>(p[3]) << 16;
+            raw[u].z = p[4] | static_cast<uint32_t>(p[5]) << 16;
+            raw[u].w = p[6] | static_cast<uint32_t>(p[7]) << 16;
+          }
         }
       }
-      float x[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[2 * j] = elem_to_float<BF>(static_cast<uint16_t>(e[j]));
-        x[2 * j + 1] = elem_to_float<BF>(static_cast<uint16_t>(e[j] >> 16));
-      }
-      float lo, hi;
-      if (__any_sync(~0u, odd)) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = x[j] == x[j] ? fminf(fmaxf(x[j], -65504.f), 65504.f) : 0.f;
-        lo = hi = x[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]);
-        for (int o = 1; o < gl; o <<= 1) {
-          lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
-          hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
+      for (int u = 0; u < kIoUnroll; ++u) {
+        if (m + u * TW >= n) break;  // the whole warp
+        __half2 sz;
+        const uint32_t w = quantise8<BF>(raw[u], gl, sz);
+        if (m + u * TW + tw < n) {
+          *reinterpret_cast<uint32_t*>(codes + (m + u * TW) * (D / 2)) = w;
+          if (lead) *reinterpret_cast<__half2*>(pairs + (m + u * TW) * G * 4) = sz;
         }
-      } else {
-        // (minimum, minimum of the negated) of the group in one 16-bit pair
-        uint32_t a2 = min2<BF>(min2<BF>(e[0], e[1]), min2<BF>(e[2], e[3]));
-        uint32_t b2 = min2<BF>(min2<BF>(e[0] ^ 0x80008000u, e[1] ^ 0x80008000u),
-                               min2<BF>(e[2] ^ 0x80008000u, e[3] ^ 0x80008000u));
-        uint32_t p = min2<BF>(prmt(a2, b2, 0x5410), prmt(a2, b2, 0x7632));
-        for (int o = 1; o < gl; o <<= 1) p = min2<BF>(p, __shfl_xor_sync(~0u, p, o));
-        lo = elem_to_float<BF>(static_cast<uint16_t>(p));
-        hi = -elem_to_float<BF>(static_cast<uint16_t>(p >> 16));
       }
-      if (m[u] >= tile.count) continue;
-      const __half zh = __float2half_rn(lo);
-      const float z = __half2float(zh);
-      const __half sh = __float2half_rn(div_by(__fsub_rn(hi, z), 15.f, 1.f / 15.f));
-      const float s = __half2float(sh);
-      const float r = s > 0.f ? recip(s) : 0.f;  // scale 0: every quotient 0
-      // the float 1.5 * 2^23 + c holds the code in its low bits (rounded half to even by the addition)
-      uint32_t word = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float q = div_by(__fsub_rn(x[j], z), s, r);
-        const float c = fminf(fmaxf(__fadd_rn(q, 12582912.f), 12582912.f), 12582927.f);
-        word += __float_as_uint(c) << ((j & 1 ? 0 : 4) + 8 * (j >> 1));
-      }
-      word -= 0x4B400000u * 0x11111111u;  // the eight exponents' share of the sum
-      const int64_t pos = tile.pos0 + m[u];
-      const int page = pos >= 0 ? s_pages[static_cast<int>(pos / kBlockTokens) - tile.page0] : -1;
-      if (page < 0) continue;
-      const int slot = static_cast<int>(pos) % kBlockTokens;
-      uint8_t* rec = a.c.pool + page * a.c.page_stride + (hk[u] >> 1) * a.c.head_stride;
-      *reinterpret_cast<uint32_t*>(rec + (hk[u] & 1) * vc + slot * (D / 2) + part * 4) = word;
-      if (part % gl == 0)
-        *reinterpret_cast<__half2*>(rec + 2 * vc + (hk[u] & 1) * vp + (slot * G + gi) * 4) = __halves2half2(sh, zh);
     }
   }
 }
 
+// Values of eight channels: four output words.
 template <bool BF>
-__global__ void __launch_bounds__(kIoThreads) int4_read_kernel(const Int4Io a) {
-  __shared__ int s_pages[3];
-  IoTile tile;
-  const int i = blockIdx.y, m0 = blockIdx.x * kIoTokens;
-  if (!io_tile(a, i, m0, false, tile, s_pages)) return;
-  const int D = a.c.head_dim, L = D / 8, group = a.c.group;
-  const int part = threadIdx.x % L;
-  const int G = D / group, gi = part * 8 / group;
-  const int vc = kBlockTokens * D / 2, vp = kBlockTokens * G * 4;
-  const int len = tile.seq >= 0 ? a.c.lens[tile.seq] : 0;
-  uint16_t* k = a.k + i * a.k_sr + m0 * a.k_sm + part * 8;
-  uint16_t* v = a.v + i * a.v_sr + m0 * a.v_sm + part * 8;
-  IoWalk w;
-  w.init(threadIdx.x / L, kIoThreads / L, 2 * a.c.kv_heads);
-  while (w.m < tile.count) {
-    uint32_t word[kIoUnroll];
-    __half2 sz[kIoUnroll];
-    int m[kIoUnroll], hk[kIoUnroll];
+AKV_DEV uint4 dequantise8(uint32_t word, __half2 sz) {
+  // fp16 pairs of codes: channels (1, 5), (0, 4), (3, 7), (2, 6)
+  uint32_t c[4];
+  c[0] = h2_as_u32(__hadd2(u32_as_h2(lop_magic<0x000F000Fu>(word)), u32_as_h2(0xE400E400u)));  // 1024 + c - 1024
+  c[1] = fix_magic<16>(lop_magic<0x00F000F0u>(word));
+  c[2] = h2_as_u32(__hadd2(u32_as_h2(lop_magic<0x000F000Fu>(word >> 8)), u32_as_h2(0xE400E400u)));
+  c[3] = fix_magic<16>(lop_magic<0x00F000F0u>(word >> 8));
+  if constexpr (BF) {
+    const float s = __low2float(sz), z = __high2float(sz);
+    float2 f[4];
 #pragma unroll
-    for (int u = 0; u < kIoUnroll; ++u) {
-      m[u] = w.m, hk[u] = w.hk;
-      w.next();
-      word[u] = 0u;
-      sz[u] = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-      const int64_t pos = tile.pos0 + m[u];
-      if (m[u] < tile.count && pos >= 0 && pos < len) {
-        const int page = s_pages[static_cast<int>(pos / kBlockTokens) - tile.page0];
-        const int slot = static_cast<int>(pos) % kBlockTokens;
-        const uint8_t* rec = a.c.pool + page * a.c.page_stride + (hk[u] >> 1) * a.c.head_stride;
-        word[u] = __ldg(reinterpret_cast<const uint32_t*>(rec + (hk[u] & 1) * vc + slot * (D / 2) + part * 4));
-        sz[u] = __ldg(reinterpret_cast<const __half2*>(rec + 2 * vc + (hk[u] & 1) * vp + (slot * G + gi) * 4));
-      }
+    for (int j = 0; j < 4; ++j) {
+      f[j] = __half22float2(u32_as_h2(c[j]));
+      f[j].x = fmaf(f[j].x, s, z);
+      f[j].y = fmaf(f[j].y, s, z);
     }
+    return make_uint4(pack_elems<true>(f[1].x, f[0].x), pack_elems<true>(f[3].x, f[2].x),
+                      pack_elems<true>(f[1].y, f[0].y), pack_elems<true>(f[3].y, f[2].y));
+  } else {
+    // c*s + z in one rounding; 15 steps of a rounded-up scale can pass the largest fp16
+    const __half2 s2 = __low2half2(sz), z2 = __high2half2(sz);
 #pragma unroll
-    for (int u = 0; u < kIoUnroll; ++u) {
-      if (m[u] >= tile.count) continue;
-      const float s = __low2float(sz[u]), z = __high2float(sz[u]);
-      uint32_t out[4];
+    for (int j = 0; j < 4; ++j)
+      c[j] = max2<false>(min2<false>(h2_as_u32(__hfma2(u32_as_h2(c[j]), s2, z2)), 0x7BFF7BFFu), 0xFBFFFBFFu);
+    return make_uint4(prmt(c[1], c[0], 0x5410), prmt(c[3], c[2], 0x5410), prmt(c[1], c[0], 0x7632),
+                      prmt(c[3], c[2], 0x7632));
+  }
+}
+
+template <bool BF, int D>
+__global__ void __launch_bounds__(kIoThreads) int4_read_kernel(const Int4Io a) {
+  constexpr int L = D / 8, TW = 32 / L;
+  const int i = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const IoPage t = io_page(a, i, blockIdx.x, false);
+  const int n = t.m1 - t.m0;
+  if (n <= 0) return;
+  const int have = t.end - t.m0;  // the rest are zeros
+  const int part = lane % L, tw = lane / L, gl = a.c.group / 8, G = D / a.c.group;
+  for (int hk = warp; hk < 2 * a.c.kv_heads; hk += kIoWarps) {
+    const int h = hk >> 1, is_v = hk & 1;
+    const int64_t sm = is_v ? a.v_sm : a.k_sm;
+    uint16_t* dst = (is_v ? a.v + i * a.v_sr + h * a.v_sh : a.k + i * a.k_sr + h * a.k_sh) + (t.m0 + tw) * sm + part * 8;
+    const uint8_t* rec = a.c.pool + (t.page < 0 ? 0 : t.page) * a.c.page_stride + h * a.c.head_stride;
+    const uint8_t* codes = rec + is_v * (kBlockTokens * D / 2) + (t.slot0 + tw) * (D / 2) + part * 4;
+    const uint8_t* pairs = rec + kBlockTokens * D + is_v * (kBlockTokens * G * 4) + ((t.slot0 + tw) * G + part / gl) * 4;
+    for (int m = 0; m < n; m += TW * kIoUnroll) {
+      uint32_t word[kIoUnroll];
+      __half2 sz[kIoUnroll];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float e = fmaf(static_cast<float>((word[u] >> (8 * j + 4)) & 15u), s, z);
-        float o = fmaf(static_cast<float>((word[u] >> (8 * j)) & 15u), s, z);
-        if constexpr (!BF) {  // 15 steps of a rounded-up scale can pass the largest fp16
-          e = fminf(fmaxf(e, -65504.f), 65504.f);
-          o = fminf(fmaxf(o, -65504.f), 65504.f);
+      for (int u = 0; u < kIoUnroll; ++u) {
+        word[u] = 0u;
+        sz[u] = u32_as_h2(0u);
+        if (m + u * TW + tw < have) {
+          word[u] = __ldg(reinterpret_cast<const uint32_t*>(codes + (m + u * TW) * (D / 2)));
+          sz[u] = __ldg(reinterpret_cast<const __half2*>(pairs + (m + u * TW) * G * 4));
         }
-        out[j] = pack_elems<BF>(e, o);
       }
-      const int h = hk[u] >> 1;
-      uint16_t* dst = hk[u] & 1 ? v + h * a.v_sh + m[u] * a.v_sm : k + h * a.k_sh + m[u] * a.k_sm;
-      if (a.aligned) {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
-      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dst[j] = static_cast<uint16_t>(out[j / 2] >> (16 * (j & 1)));
+      for (int u = 0; u < kIoUnroll; ++u) {
+        if (m + u * TW + tw >= n) continue;
+        const uint4 v = dequantise8<BF>(word[u], sz[u]);
+        uint16_t* p = dst + (m + u * TW) * sm;
+        if (a.aligned) {
+          *reinterpret_cast<uint4*>(p) = v;
+        } else {
+          const uint32_t o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[j] = static_cast<uint16_t>(o[j / 2] >> (16 * (j & 1)));
+        }
       }
     }
   }
+}
+
+template <bool WRITE>
+void io_launch(const Int4Io& p, dim3 grid, int dtype, cudaStream_t st) {
+  auto go = [&](auto bf) {
+    constexpr bool BF = decltype(bf)::value;
+    auto one = [&](auto kern) { kern<<<grid, kIoThreads, 0, st>>>(p); };
+    if (p.c.head_dim == 64) WRITE ? one(int4_append_kernel<BF, 64>) : one(int4_read_kernel<BF, 64>);
+    else if (p.c.head_dim == 128) WRITE ? one(int4_append_kernel<BF, 128>) : one(int4_read_kernel<BF, 128>);
+    else WRITE ? one(int4_append_kernel<BF, 256>) : one(int4_read_kernel<BF, 256>);
+  };
+  if (dtype == AKV_BF16) go(std::true_type{});
+  else go(std::false_type{});
 }
 
 }  // namespace akv
@@ -286,10 +329,11 @@ extern "C" int akv_int4_layout_init(int head_dim, int group, akv_int4_layout* ou
   return AKV_OK;
 }
 
-// shared argument checks and launch of append and read
-template <class Launch>
-static int int4_io(const akv_int4_cache* c, int R, int M, const void* k, int64_t k_sr, int64_t k_sh, int64_t k_sm,
-                   const void* v, int64_t v_sr, int64_t v_sh, int64_t v_sm, int dtype, Int4Io& a, Launch launch) {
+// argument checks and launch of append and read
+template <bool WRITE>
+static int int4_io(const akv_int4_cache* c, const int32_t* rows, const int32_t* start, const int32_t* n_new, int R, int M,
+                   const void* k, int64_t k_sr, int64_t k_sh, int64_t k_sm, const void* v, int64_t v_sr, int64_t v_sh,
+                   int64_t v_sm, int dtype, int* status, void* stream) {
   const int rc = int4_check(c);
   if (rc) return rc;
   if (dtype != AKV_FP16 && dtype != AKV_BF16) return AKV_ERR_UNSUPPORTED;
@@ -297,16 +341,22 @@ static int int4_io(const akv_int4_cache* c, int R, int M, const void* k, int64_t
   if (R == 0 || M == 0) return AKV_OK;
   if (!k || !v) return AKV_ERR_NULL;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 1) return AKV_ERR_ALIGN;
-  const int blocks = (M + kIoTokens - 1) / kIoTokens;
-  if (R > 65535 || c->kv_heads > (1 << 20)) return AKV_ERR_UNSUPPORTED;
+  if (R > 65535 || c->kv_heads > (1 << 20) || M > INT32_MAX - 64) return AKV_ERR_UNSUPPORTED;
+  Int4Io a{};
   a.c = *c;
+  a.rows = rows;
+  a.n_new = n_new;
+  a.start = start;
   a.M = M;
   a.k = static_cast<uint16_t*>(const_cast<void*>(k));
   a.k_sr = k_sr; a.k_sh = k_sh; a.k_sm = k_sm;
   a.v = static_cast<uint16_t*>(const_cast<void*>(v));
   a.v_sr = v_sr; a.v_sh = v_sh; a.v_sm = v_sm;
   a.aligned = rows_aligned16(k, k_sr, k_sh, k_sm) && rows_aligned16(v, v_sr, v_sh, v_sm);
-  launch(dim3(blocks, R), a);
+  a.status = status;
+  // M tokens from any slot on touch at most this many pages
+  const int blocks = (M + 2 * kBlockTokens - 2) / kBlockTokens;
+  io_launch<WRITE>(a, dim3(blocks, R), dtype, static_cast<cudaStream_t>(stream));
   return cudaGetLastError() == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH;
 }
 
@@ -314,30 +364,11 @@ extern "C" int akv_int4_append(const akv_int4_cache* c, const int32_t* rows, con
                                const void* k, int64_t k_sr, int64_t k_sh, int64_t k_sm,
                                const void* v, int64_t v_sr, int64_t v_sh, int64_t v_sm, int dtype, int* status,
                                void* stream) {
-  Int4Io a{};
-  a.rows = rows;
-  a.n_new = n_new;
-  a.status = status;
-  return int4_io(c, R, M, k, k_sr, k_sh, k_sm, v, v_sr, v_sh, v_sm, dtype, a, [&](dim3 grid, const Int4Io& p) {
-    if (dtype == AKV_BF16)
-      int4_append_kernel<true><<<grid, kIoThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    else
-      int4_append_kernel<false><<<grid, kIoThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  });
+  return int4_io<true>(c, rows, nullptr, n_new, R, M, k, k_sr, k_sh, k_sm, v, v_sr, v_sh, v_sm, dtype, status, stream);
 }
 
 extern "C" int akv_int4_read(const akv_int4_cache* c, const int32_t* rows, const int32_t* start, const int32_t* n_new,
                              int R, int N, void* k, int64_t k_sr, int64_t k_sh, int64_t k_sm,
                              void* v, int64_t v_sr, int64_t v_sh, int64_t v_sm, int dtype, int* status, void* stream) {
-  Int4Io a{};
-  a.rows = rows;
-  a.n_new = n_new;
-  a.start = start;
-  a.status = status;
-  return int4_io(c, R, N, k, k_sr, k_sh, k_sm, v, v_sr, v_sh, v_sm, dtype, a, [&](dim3 grid, const Int4Io& p) {
-    if (dtype == AKV_BF16)
-      int4_read_kernel<true><<<grid, kIoThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    else
-      int4_read_kernel<false><<<grid, kIoThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  });
+  return int4_io<false>(c, rows, start, n_new, R, N, k, k_sr, k_sh, k_sm, v, v_sr, v_sh, v_sm, dtype, status, stream);
 }
