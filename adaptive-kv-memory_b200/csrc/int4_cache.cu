@@ -26,13 +26,13 @@ struct Int4Io {
   int64_t k_sr, k_sh, k_sm;
   uint16_t* v;
   int64_t v_sr, v_sh, v_sm;
-  int aligned;  // rows on 16-byte boundaries: vector accesses
   int* status;
 };
 
 constexpr int kIoThreads = 256;
 constexpr int kIoWarps = kIoThreads / 32;
-constexpr int kIoUnroll = 4;  // rows a thread has in flight
+constexpr int kIoUnroll = 4;    // token steps in flight per warp: append,
+constexpr int kReadUnroll = 8;  // read (a quarter of the bytes a step)
 
 // The call tokens of row i that lie on one page: block `blk` of the pages that
 // its tokens start on.  Token m of the call is at position pos0 + m.
@@ -108,8 +108,8 @@ AKV_DEV uint32_t max2(uint32_t a, uint32_t b) {
 
 // Eight channels of a group spread over gl threads: codes (word in the
 // record's byte order), scale and zero.  All lanes of the warp take part.
-template <bool BF>
-AKV_DEV uint32_t quantise8(uint4 raw, int gl, __half2& sz) {
+template <bool BF, int gl>
+AKV_DEV uint32_t quantise8(uint4 raw, __half2& sz) {
   const uint32_t e[4] = {raw.x, raw.y, raw.z, raw.w};
   // a bit 15 / 31 where an element is NaN, infinite or past 65504
   constexpr uint32_t PAST = BF ? 0x38803880u : 0x04000400u;
@@ -130,6 +130,7 @@ AKV_DEV uint32_t quantise8(uint4 raw, int gl, __half2& sz) {
     lo = hi = x[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]);
+#pragma unroll
     for (int o = 1; o < gl; o <<= 1) {
       lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
       hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
@@ -139,6 +140,7 @@ AKV_DEV uint32_t quantise8(uint4 raw, int gl, __half2& sz) {
     const uint32_t a2 = min2<BF>(min2<BF>(e[0], e[1]), min2<BF>(e[2], e[3]));
     const uint32_t b2 = max2<BF>(max2<BF>(e[0], e[1]), max2<BF>(e[2], e[3])) ^ 0x80008000u;
     uint32_t p = min2<BF>(prmt(a2, b2, 0x5410), prmt(a2, b2, 0x7632));
+#pragma unroll
     for (int o = 1; o < gl; o <<= 1) p = min2<BF>(p, __shfl_xor_sync(~0u, p, o));
     lo = elem_to_float<BF>(static_cast<uint16_t>(p));
     hi = -elem_to_float<BF>(static_cast<uint16_t>(p >> 16));
@@ -180,14 +182,15 @@ AKV_DEV uint32_t quantise8(uint4 raw, int gl, __half2& sz) {
 
 // A CTA takes one page of one call row, a warp one (head, K / V) of it at a
 // time: D/8 threads a token, so 32 / (D/8) tokens a step.
-template <bool BF, int D>
-__global__ void __launch_bounds__(kIoThreads) int4_append_kernel(const Int4Io a) {
+template <bool BF, int D, int G, bool AL>
+__global__ void __launch_bounds__(kIoThreads, 4) int4_append_kernel(const Int4Io a) {
   constexpr int L = D / 8, TW = 32 / L;
   const int i = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const IoPage t = io_page(a, i, blockIdx.x, true);
   const int n = t.m1 - t.m0;
   if (n <= 0) return;
-  const int part = lane % L, tw = lane / L, gl = a.c.group / 8, G = D / a.c.group;
+  const int part = lane % L, tw = lane / L;
+  constexpr int gl = L / G;  // threads of a group
   for (int hk = warp; hk < 2 * a.c.kv_heads; hk += kIoWarps) {
     const int h = hk >> 1, is_v = hk & 1;
     const int64_t sm = is_v ? a.v_sm : a.k_sm;
@@ -197,14 +200,16 @@ __global__ void __launch_bounds__(kIoThreads) int4_append_kernel(const Int4Io a)
     uint8_t* codes = rec + is_v * (kBlockTokens * D / 2) + (t.slot0 + tw) * (D / 2) + part * 4;
     uint8_t* pairs = rec + kBlockTokens * D + is_v * (kBlockTokens * G * 4) + ((t.slot0 + tw) * G + part / gl) * 4;
     const bool lead = part % gl == 0;
-    for (int m = 0; m < n; m += TW * kIoUnroll) {
+    // kIoUnroll steps; only the last round of a page has to look at its end
+    auto round = [&](int m, auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
       uint4 raw[kIoUnroll];
 #pragma unroll
       for (int u = 0; u < kIoUnroll; ++u) {
-        raw[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (m + u * TW + tw < n) {
+        if (!WHOLE) raw[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (WHOLE || m + u * TW + tw < n) {
           const uint16_t* p = src + (m + u * TW) * sm;
-          if (a.aligned) {
+          if constexpr (AL) {
             raw[u] = ldg_nc_v4(p);
           } else {
             raw[u].x = p[0] | static_cast<uint32_t>(p[1]) << 16;
@@ -216,15 +221,18 @@ __global__ void __launch_bounds__(kIoThreads) int4_append_kernel(const Int4Io a)
       }
 #pragma unroll
       for (int u = 0; u < kIoUnroll; ++u) {
-        if (m + u * TW >= n) break;  // the whole warp
+        if (!WHOLE && m + u * TW >= n) break;  // the whole warp
         __half2 sz;
-        const uint32_t w = quantise8<BF>(raw[u], gl, sz);
-        if (m + u * TW + tw < n) {
+        const uint32_t w = quantise8<BF, gl>(raw[u], sz);
+        if (WHOLE || m + u * TW + tw < n) {
           *reinterpret_cast<uint32_t*>(codes + (m + u * TW) * (D / 2)) = w;
           if (lead) *reinterpret_cast<__half2*>(pairs + (m + u * TW) * G * 4) = sz;
         }
       }
-    }
+    };
+    int m = 0;
+    for (; m + TW * kIoUnroll <= n; m += TW * kIoUnroll) round(m, std::true_type{});
+    if (m < n) round(m, std::false_type{});
   }
 }
 
@@ -259,15 +267,16 @@ AKV_DEV uint4 dequantise8(uint32_t word, __half2 sz) {
   }
 }
 
-template <bool BF, int D>
-__global__ void __launch_bounds__(kIoThreads) int4_read_kernel(const Int4Io a) {
+template <bool BF, int D, int G, bool AL>
+__global__ void __launch_bounds__(kIoThreads, 4) int4_read_kernel(const Int4Io a) {
   constexpr int L = D / 8, TW = 32 / L;
   const int i = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const IoPage t = io_page(a, i, blockIdx.x, false);
   const int n = t.m1 - t.m0;
   if (n <= 0) return;
   const int have = t.end - t.m0;  // the rest are zeros
-  const int part = lane % L, tw = lane / L, gl = a.c.group / 8, G = D / a.c.group;
+  const int part = lane % L, tw = lane / L;
+  constexpr int gl = L / G;
   for (int hk = warp; hk < 2 * a.c.kv_heads; hk += kIoWarps) {
     const int h = hk >> 1, is_v = hk & 1;
     const int64_t sm = is_v ? a.v_sm : a.k_sm;
@@ -275,24 +284,24 @@ __global__ void __launch_bounds__(kIoThreads) int4_read_kernel(const Int4Io a) {
     const uint8_t* rec = a.c.pool + (t.page < 0 ? 0 : t.page) * a.c.page_stride + h * a.c.head_stride;
     const uint8_t* codes = rec + is_v * (kBlockTokens * D / 2) + (t.slot0 + tw) * (D / 2) + part * 4;
     const uint8_t* pairs = rec + kBlockTokens * D + is_v * (kBlockTokens * G * 4) + ((t.slot0 + tw) * G + part / gl) * 4;
-    for (int m = 0; m < n; m += TW * kIoUnroll) {
-      uint32_t word[kIoUnroll];
-      __half2 sz[kIoUnroll];
+    auto round = [&](int m, auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      uint32_t word[kReadUnroll];
+      __half2 sz[kReadUnroll];
 #pragma unroll
-      for (int u = 0; u < kIoUnroll; ++u) {
-        word[u] = 0u;
-        sz[u] = u32_as_h2(0u);
-        if (m + u * TW + tw < have) {
+      for (int u = 0; u < kReadUnroll; ++u) {
+        if (!WHOLE) word[u] = 0u, sz[u] = u32_as_h2(0u);
+        if (WHOLE || m + u * TW + tw < have) {
           word[u] = __ldg(reinterpret_cast<const uint32_t*>(codes + (m + u * TW) * (D / 2)));
           sz[u] = __ldg(reinterpret_cast<const __half2*>(pairs + (m + u * TW) * G * 4));
         }
       }
 #pragma unroll
-      for (int u = 0; u < kIoUnroll; ++u) {
-        if (m + u * TW + tw >= n) continue;
+      for (int u = 0; u < kReadUnroll; ++u) {
+        if (!WHOLE && m + u * TW + tw >= n) continue;
         const uint4 v = dequantise8<BF>(word[u], sz[u]);
         uint16_t* p = dst + (m + u * TW) * sm;
-        if (a.aligned) {
+        if constexpr (AL) {
           *reinterpret_cast<uint4*>(p) = v;
         } else {
           const uint32_t o[4] = {v.x, v.y, v.z, v.w};
@@ -300,21 +309,35 @@ __global__ void __launch_bounds__(kIoThreads) int4_read_kernel(const Int4Io a) {
           for (int j = 0; j < 8; ++j) p[j] = static_cast<uint16_t>(o[j / 2] >> (16 * (j & 1)));
         }
       }
-    }
+    };
+    int m = 0;
+    for (; m + TW * kReadUnroll <= have; m += TW * kReadUnroll) round(m, std::true_type{});
+    for (; m < n; m += TW * kReadUnroll) round(m, std::false_type{});
   }
 }
 
-template <bool WRITE>
-void io_launch(const Int4Io& p, dim3 grid, int dtype, cudaStream_t st) {
-  auto go = [&](auto bf) {
-    constexpr bool BF = decltype(bf)::value;
-    auto one = [&](auto kern) { kern<<<grid, kIoThreads, 0, st>>>(p); };
-    if (p.c.head_dim == 64) WRITE ? one(int4_append_kernel<BF, 64>) : one(int4_read_kernel<BF, 64>);
-    else if (p.c.head_dim == 128) WRITE ? one(int4_append_kernel<BF, 128>) : one(int4_read_kernel<BF, 128>);
-    else WRITE ? one(int4_append_kernel<BF, 256>) : one(int4_read_kernel<BF, 256>);
+template <bool WRITE, bool BF, bool AL>
+void io_launch_dim(const Int4Io& p, dim3 grid, cudaStream_t st) {
+  auto one = [&](auto dim, auto groups) {
+    constexpr int D = decltype(dim)::value, G = decltype(groups)::value;
+    if constexpr (WRITE) int4_append_kernel<BF, D, G, AL><<<grid, kIoThreads, 0, st>>>(p);
+    else int4_read_kernel<BF, D, G, AL><<<grid, kIoThreads, 0, st>>>(p);
   };
-  if (dtype == AKV_BF16) go(std::true_type{});
-  else go(std::false_type{});
+  auto by_group = [&](auto dim) {
+    const int G = p.c.head_dim / p.c.group;
+    if (G == 1) one(dim, std::integral_constant<int, 1>{});
+    else if (G == 2) one(dim, std::integral_constant<int, 2>{});
+    else one(dim, std::integral_constant<int, 4>{});
+  };
+  if (p.c.head_dim == 64) by_group(std::integral_constant<int, 64>{});
+  else if (p.c.head_dim == 128) by_group(std::integral_constant<int, 128>{});
+  else by_group(std::integral_constant<int, 256>{});
+}
+
+template <bool WRITE>
+void io_launch(const Int4Io& p, dim3 grid, bool bf16, bool aligned, cudaStream_t st) {
+  if (aligned) bf16 ? io_launch_dim<WRITE, true, true>(p, grid, st) : io_launch_dim<WRITE, false, true>(p, grid, st);
+  else bf16 ? io_launch_dim<WRITE, true, false>(p, grid, st) : io_launch_dim<WRITE, false, false>(p, grid, st);
 }
 
 }  // namespace akv
@@ -352,11 +375,11 @@ static int int4_io(const akv_int4_cache* c, const int32_t* rows, const int32_t* 
   a.k_sr = k_sr; a.k_sh = k_sh; a.k_sm = k_sm;
   a.v = static_cast<uint16_t*>(const_cast<void*>(v));
   a.v_sr = v_sr; a.v_sh = v_sh; a.v_sm = v_sm;
-  a.aligned = rows_aligned16(k, k_sr, k_sh, k_sm) && rows_aligned16(v, v_sr, v_sh, v_sm);
   a.status = status;
   // M tokens from any slot on touch at most this many pages
   const int blocks = (M + 2 * kBlockTokens - 2) / kBlockTokens;
-  io_launch<WRITE>(a, dim3(blocks, R), dtype, static_cast<cudaStream_t>(stream));
+  const bool aligned = rows_aligned16(k, k_sr, k_sh, k_sm) && rows_aligned16(v, v_sr, v_sh, v_sm);
+  io_launch<WRITE>(a, dim3(blocks, R), dtype == AKV_BF16, aligned, static_cast<cudaStream_t>(stream));
   return cudaGetLastError() == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH;
 }
 
