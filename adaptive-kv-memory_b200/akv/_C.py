@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import POINTER, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p, c_char_p
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libakv_sm100.so")
@@ -85,6 +86,12 @@ class PageTable(ctypes.Structure):
     _fields_ = [("table", c_void_p), ("table_stride", c_int64), ("lens", c_void_p), ("refs", c_void_p),
                 ("free_bits", c_void_p), ("max_seqs", c_int32), ("max_blocks", c_int32), ("n_pages", c_int32)]
 
+
+# Argument structs of the entries a serving loop calls every step, packed field by field (a struct.pack costs a
+# tenth of converting as many ctypes arguments): pointers and 64-bit fields first, then 32-bit ones.
+IO_ARGS = struct.Struct("13q4i")         # akv_int4_io_args
+ATTENTION_ARGS = struct.Struct("15q4ifi")  # akv_int4_attention_args
+VERIFY_ARGS = struct.Struct("13q4i")     # akv_verify_args
 
 # name -> (restype, argtypes); must list every function declared in akv_b200.h
 SIGNATURES = {
@@ -177,14 +184,10 @@ SIGNATURES = {
     "akv_scatter_rows": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int,
                                  c_int, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
     "akv_int4_layout_init": (c_int, [c_int, c_int, POINTER(Int4Layout)]),
-    "akv_int4_append": (c_int, [POINTER(Int4Cache), c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int64,
-                                c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
-    "akv_int4_read": (c_int, [POINTER(Int4Cache), c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64,
-                              c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "akv_int4_append": (c_int, [c_char_p, c_void_p]),
+    "akv_int4_read": (c_int, [c_char_p, c_void_p]),
     "akv_int4_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
-    "akv_int4_attention": (c_int, [POINTER(Int4Cache), c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int64,
-                                   c_int64, c_int64, c_float, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int,
-                                   c_void_p, c_size_t, c_void_p, c_void_p]),
+    "akv_int4_attention": (c_int, [c_char_p, c_void_p]),
     "akv_pages_workspace_bytes": (c_size_t, [c_int, c_int]),
     "akv_pages_fork": (c_int, [POINTER(PageTable), c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "akv_pages_reserve": (c_int, [POINTER(PageTable), c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
@@ -194,9 +197,7 @@ SIGNATURES = {
                                   c_size_t, c_void_p, c_void_p]),
     "akv_pages_copy": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p,
                                c_void_p]),
-    "akv_verify_draft": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
-                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
-                                 c_void_p]),
+    "akv_verify_draft": (c_int, [c_char_p, c_void_p]),
     "akv_selftest_wait": (c_int, [c_int, c_int64, c_void_p, c_void_p, c_void_p]),
     "akv_cold_copy": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
 }
@@ -255,6 +256,15 @@ def ptr(t) -> int | None:
 
 
 _raw_stream = None
+
+
+def raw_stream(device_index: int) -> int:
+    """The current torch stream handle of a device, by torch's raw accessor where it has one."""
+    global _raw_stream
+    import torch
+    if _raw_stream is None:
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", False)
+    return _raw_stream(device_index) if _raw_stream else torch.cuda.current_stream(device_index).cuda_stream
 
 
 def stream_of(t) -> int:

@@ -32,15 +32,17 @@ import torch
 from . import _C
 
 BLOCK = _C.BLOCK_TOKENS
-_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _ROWS_PER_CALL = 1024  # requests one reserve plan holds
 
 
-def _half_dtype(*tensors) -> int:
-    d = tensors[0].dtype
-    if d not in (torch.float16, torch.bfloat16) or any(t.dtype != d for t in tensors):
-        raise TypeError(f"fp16 or bf16 tensors of one type wanted (got {[str(t.dtype) for t in tensors]})")
-    return _DTYPES[d]
+_HALF = {torch.float16: 0, torch.bfloat16: 1}
+
+
+def _half_dtype(t: torch.Tensor) -> int:
+    d = _HALF.get(t.dtype)
+    if d is None:
+        raise TypeError(f"fp16 or bf16 wanted (got {t.dtype})")
+    return d
 
 
 class Int4PagedCache:
@@ -58,6 +60,7 @@ class Int4PagedCache:
         self.n_layers, self.n_pages, self.H, self.D, self.group = n_layers, n_pages, kv_heads, head_dim, group_size
         self.max_seqs, self.max_blocks = max_seqs, max_blocks
         self.rec = self.layout.bytes
+        self._lib = _C.load()
         self.buf = torch.zeros(n_layers, n_pages, kv_heads, self.rec, dtype=torch.uint8, device=device)
         # the bookkeeping in one buffer, so that it is saved and restored by one copy
         words = (n_pages + 31) // 32
@@ -68,10 +71,22 @@ class Int4PagedCache:
         self.table.fill_(-1)
         self._rebuild_free()
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self._dev = self.buf.device
+        self._dev_index = self._dev.index if self._dev.index is not None else torch.cuda.current_device()
+        self._status_ptr = self.status.data_ptr()
         self._pt = _C.PageTable(self.table.data_ptr(), max_blocks, self.lens.data_ptr(), self.refs.data_ptr(),
                                 self.free_bits.data_ptr(), max_seqs, max_blocks, n_pages)
         self._ws: dict = {}
+        self._ws_need: dict = {}
+        self._scale = 1.0 / math.sqrt(head_dim)
+        self._pt_ref = ctypes.byref(self._pt)
+        # the page operations of one cache follow one another (they change one table), so they share a workspace
+        self._page_ws_bytes = int(self._lib.akv_pages_workspace_bytes(n_pages, _ROWS_PER_CALL))
+        self._page_ws = torch.empty(self._page_ws_bytes, dtype=torch.uint8, device=device)
+        self._page_ws_ptr = self._page_ws.data_ptr()
+        self._pool_ptr, self._layer_bytes, self._page_bytes = self.buf.data_ptr(), self.buf.stride(0), self.buf.stride(1)
         self._views = [self._view(layer) for layer in range(n_layers)]
+        self._view_ptrs = [ctypes.addressof(v) for v in self._views]
 
     # ------------------------------------------------------------------ state
     @property
@@ -134,33 +149,40 @@ class Int4PagedCache:
         """A contiguous int32 vector on the cache's device (lists are copied over)."""
         if x is None:
             return None
-        if not torch.is_tensor(x):
-            x = torch.tensor(x, dtype=torch.int32, device=self.device)
-        if x.device != self.device:
-            raise ValueError(f"{what} must be on {self.device}")
-        if x.dtype != torch.int32 or x.dim() != 1:
+        if not isinstance(x, torch.Tensor):
+            x = torch.tensor(x, dtype=torch.int32, device=self._dev)
+        shape = x.shape
+        if x.dtype is not torch.int32 or len(shape) != 1:
             raise ValueError(f"{what} must be an int32 vector")
-        if n is not None and x.numel() != n:
-            raise ValueError(f"{what} needs {n} entries (got {x.numel()})")
+        if x.device != self._dev:
+            raise ValueError(f"{what} must be on {self._dev}")
+        if n is not None and shape[0] != n:
+            raise ValueError(f"{what} needs {n} entries (got {shape[0]})")
         return x if x.is_contiguous() else x.contiguous()
 
-    def _layer(self, layer: int) -> "_C.Int4Cache":
+    def _layer(self, layer: int) -> int:
         if not 0 <= layer < self.n_layers:
             raise ValueError(f"layer {layer} of {self.n_layers}")
-        return self._views[layer]
+        return self._view_ptrs[layer]
 
-    def _count(self, rows, n: int) -> None:
-        if rows is None and n > self.max_seqs:
-            raise ValueError(f"{n} rows, but the cache holds {self.max_seqs} sequences")
+    def _rows(self, rows, n_new, R: int) -> tuple:
+        """The row and count vectors of a call over R rows, and their pointers (0: none)."""
+        if rows is not None:
+            rows = self._ints(rows, "rows", R)
+        elif R > self.max_seqs:
+            raise ValueError(f"{R} rows, but the cache holds {self.max_seqs} sequences")
+        if n_new is not None:
+            n_new = self._ints(n_new, "n_new", R)
+        return (rows, n_new, 0 if rows is None else rows.data_ptr(), 0 if n_new is None else n_new.data_ptr())
 
     def _workspace(self, need: int, stream: int) -> torch.Tensor:
         """Zeroed scratch for attention on a stream: kept per stream (calls on two streams may overlap), its own
         for each call of a captured graph (replays may overlap eager calls)."""
         if torch.cuda.is_current_stream_capturing():
-            return torch.zeros(need, dtype=torch.uint8, device=self.device)
+            return torch.zeros(need, dtype=torch.uint8, device=self._dev)
         ws = self._ws.get(stream)
         if ws is None or ws.numel() < need:
-            ws = self._ws[stream] = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=self.device)
+            ws = self._ws[stream] = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=self._dev)
         return ws
 
     # ------------------------------------------------------------------ pages
@@ -168,70 +190,79 @@ class Int4PagedCache:
         """Room for ``n_new`` (int32 vector, or one number for all) more tokens in each of ``rows`` (None: all,
         in order), the lengths advanced.  Returns the tokens granted per row, n_new or 0 where the request was
         refused: pass it to ``append`` and ``attend`` as their ``n_new``."""
-        lib = _C.load()
         rows = self._ints(rows, "rows")
-        n = self.max_seqs if rows is None else rows.numel()
-        one = isinstance(n_new, int)
-        if one and n_new < 0:
-            raise ValueError("n_new is negative")
+        n = self.max_seqs if rows is None else rows.shape[0]
+        counts = None
+        if isinstance(n_new, int):
+            if n_new < 0:
+                raise ValueError("n_new is negative")
+        else:
+            counts = self._ints(n_new, "n_new", n)
+            n_new = 0
         if rows is None and n > _ROWS_PER_CALL:
-            rows = torch.arange(n, dtype=torch.int32, device=self.device)
-        counts = None if one else self._ints(n_new, "n_new", n)
-        granted = torch.empty(n, dtype=torch.int32, device=self.device)
-        need = _C.workspace_bytes("akv_pages_workspace_bytes", self.n_pages, min(n, _ROWS_PER_CALL))
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            rows = torch.arange(n, dtype=torch.int32, device=self._dev)
+        granted = torch.empty(n, dtype=torch.int32, device=self._dev)
+        rp, cp, gp = _C.ptr(rows), _C.ptr(counts), granted.data_ptr()
+        stream = _C.raw_stream(self._dev_index)
         for a in range(0, n, _ROWS_PER_CALL):
-            b = min(n, a + _ROWS_PER_CALL)
-            rc = lib.akv_pages_reserve(
-                ctypes.byref(self._pt), None if rows is None else rows.data_ptr() + 4 * a,
-                None if one else counts.data_ptr() + 4 * a, n_new if one else 0, b - a, granted.data_ptr() + 4 * a,
-                self.buf.data_ptr(), self.n_layers, self.buf.stride(0), self.buf.stride(1), ws.data_ptr(), need,
-                self.status.data_ptr(), _C.stream_of(self.buf))
-            _C.check(rc, "akv_pages_reserve")
+            rc = self._lib.akv_pages_reserve(
+                self._pt_ref, None if rp is None else rp + 4 * a, None if cp is None else cp + 4 * a, n_new,
+                min(n - a, _ROWS_PER_CALL), gp + 4 * a, self._pool_ptr, self.n_layers, self._layer_bytes,
+                self._page_bytes, self._page_ws_ptr, self._page_ws_bytes, self._status_ptr, stream)
+            if rc:
+                _C.check(rc, "akv_pages_reserve")
         return granted
 
     def fork(self, parents, children) -> None:
         """Row ``children[i]`` (empty) continues row ``parents[i]``: it shares the parent's pages, and whichever
         of them next writes into a shared, partly filled page gets its own copy (``reserve``)."""
         parents = self._ints(parents, "parents")
-        children = self._ints(children, "children", parents.numel())
-        _C.check(_C.load().akv_pages_fork(ctypes.byref(self._pt), parents.data_ptr(), children.data_ptr(),
-                                          parents.numel(), self.status.data_ptr(), _C.stream_of(self.buf)),
-                 "akv_pages_fork")
+        n = parents.shape[0]
+        children = self._ints(children, "children", n)
+        rc = self._lib.akv_pages_fork(self._pt_ref, parents.data_ptr(), children.data_ptr(), n, self._status_ptr,
+                                      _C.raw_stream(self._dev_index))
+        if rc:
+            _C.check(rc, "akv_pages_fork")
+
+    def _truncate(self, rows, n: int, new_lens) -> None:
+        rc = self._lib.akv_pages_truncate(self._pt_ref, _C.ptr(rows), _C.ptr(new_lens), n, self._status_ptr,
+                                          _C.raw_stream(self._dev_index))
+        if rc:
+            _C.check(rc, "akv_pages_truncate")
 
     def truncate(self, rows, new_lens) -> None:
         """Rows shortened to ``new_lens`` tokens (int32 vector); pages beyond go back to the pool."""
+        if new_lens is None:
+            raise ValueError("new_lens is missing (free() empties rows)")
         rows = self._ints(rows, "rows")
-        n = self.max_seqs if rows is None else rows.numel()
-        new_lens = self._ints(new_lens, "new_lens", n)
-        _C.check(_C.load().akv_pages_truncate(ctypes.byref(self._pt), _C.ptr(rows), _C.ptr(new_lens), n,
-                                              self.status.data_ptr(), _C.stream_of(self.buf)), "akv_pages_truncate")
+        n = self.max_seqs if rows is None else rows.shape[0]
+        self._truncate(rows, n, self._ints(new_lens, "new_lens", n))
 
     def free(self, rows) -> None:
         """The sequences' pages given back, their rows empty."""
         rows = self._ints(rows, "rows")
-        n = self.max_seqs if rows is None else rows.numel()
-        _C.check(_C.load().akv_pages_truncate(ctypes.byref(self._pt), _C.ptr(rows), None, n, self.status.data_ptr(),
-                                              _C.stream_of(self.buf)), "akv_pages_truncate")
+        self._truncate(rows, self.max_seqs if rows is None else rows.shape[0], None)
 
     def compact(self) -> torch.Tensor:
         """Live pages moved to the low end of the pool, tables following.  Returns their number (int32, device)."""
-        live = torch.empty(1, dtype=torch.int32, device=self.device)
-        need = _C.workspace_bytes("akv_pages_workspace_bytes", self.n_pages, 0)
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        rc = _C.load().akv_pages_compact(ctypes.byref(self._pt), self.buf.data_ptr(), self.n_layers,
-                                         self.buf.stride(0), self.buf.stride(1), live.data_ptr(), ws.data_ptr(), need,
-                                         self.status.data_ptr(), _C.stream_of(self.buf))
-        _C.check(rc, "akv_pages_compact")
+        live = torch.empty(1, dtype=torch.int32, device=self._dev)
+        rc = self._lib.akv_pages_compact(self._pt_ref, self._pool_ptr, self.n_layers, self._layer_bytes,
+                                         self._page_bytes, live.data_ptr(), self._page_ws_ptr, self._page_ws_bytes,
+                                         self._status_ptr, _C.raw_stream(self._dev_index))
+        if rc:
+            _C.check(rc, "akv_pages_compact")
         return live
 
     def copy_pages(self, src, dst) -> None:
         """The bytes of pages ``src`` copied over pages ``dst`` in every layer (no page in both)."""
         src = self._ints(src, "src")
-        dst = self._ints(dst, "dst", src.numel())
-        _C.check(_C.load().akv_pages_copy(self.buf.data_ptr(), self.n_layers, self.buf.stride(0), self.buf.stride(1),
-                                          self.n_pages, src.data_ptr(), dst.data_ptr(), src.numel(),
-                                          self.status.data_ptr(), _C.stream_of(self.buf)), "akv_pages_copy")
+        n = src.shape[0]
+        dst = self._ints(dst, "dst", n)
+        rc = self._lib.akv_pages_copy(self._pool_ptr, self.n_layers, self._layer_bytes, self._page_bytes, self.n_pages,
+                                      src.data_ptr(), dst.data_ptr(), n, self._status_ptr,
+                                      _C.raw_stream(self._dev_index))
+        if rc:
+            _C.check(rc, "akv_pages_copy")
 
     # ------------------------------------------------------------------ tokens
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows=None, n_new=None) -> None:
@@ -240,42 +271,54 @@ class Int4PagedCache:
         k, v (R, kv_heads, M, head_dim) fp16 or bf16, any strides: row i's last ``n_new[i]`` tokens (None: M)
         are k[i, :, :n_new[i]]."""
         view = self._layer(layer)
-        _C.require_cuda(k, v)
-        dt = _half_dtype(k, v)
-        if k.shape != v.shape or k.dim() != 4 or k.shape[1] != self.H or k.shape[3] != self.D:
+        dt = _half_dtype(k)
+        if v.dtype is not k.dtype:
+            raise TypeError(f"k and v must be of one type (got {k.dtype}, {v.dtype})")
+        shape = k.shape
+        if len(shape) != 4 or v.shape != shape or shape[1] != self.H or shape[3] != self.D:
             raise ValueError(f"k and v must be (rows, {self.H}, tokens, {self.D})")
-        k = k if k.stride(-1) == 1 else k.contiguous()
-        v = v if v.stride(-1) == 1 else v.contiguous()
-        R, _, M, _ = k.shape
-        rows, n_new = self._ints(rows, "rows", R), self._ints(n_new, "n_new", R)
-        self._count(rows, R)
-        rc = _C.load().akv_int4_append(ctypes.byref(view), _C.ptr(rows), _C.ptr(n_new), R, M,
-                                       k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                                       v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), dt,
-                                       self.status.data_ptr(), _C.stream_of(k))
-        _C.check(rc, "akv_int4_append")
+        if k.device != self._dev or v.device != self._dev:
+            raise RuntimeError(f"akv: k and v must be on {self._dev} (no CPU fallback)")
+        ks, vs = k.stride(), v.stride()
+        if ks[3] != 1:
+            k = k.contiguous()
+            ks = k.stride()
+        if vs[3] != 1:
+            v = v.contiguous()
+            vs = v.stride()
+        R, M = shape[0], shape[2]
+        rows, n_new, rp, np_ = self._rows(rows, n_new, R)
+        rc = self._lib.akv_int4_append(
+            _C.IO_ARGS.pack(view, rp, np_, 0, k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
+                            self._status_ptr, R, M, dt, 0), _C.raw_stream(self._dev_index))
+        if rc:
+            _C.check(rc, "akv_int4_append")
 
     def read(self, layer: int, n_tokens: int, rows=None, start=None, n_new=None, dtype=torch.float16):
         """The K and V values the cache stands for, (R, kv_heads, n_tokens, head_dim) in ``dtype``: tokens
         ``start[i]`` onwards of each row, or with ``start`` None its last ``n_new[i]`` (None: n_tokens); 0 past
         the row's end."""
         view = self._layer(layer)
-        if dtype not in (torch.float16, torch.bfloat16):
+        dt = _HALF.get(dtype)
+        if dt is None:
             raise TypeError(f"dtype must be fp16 or bf16 (got {dtype})")
         if n_tokens < 0:
             raise ValueError("n_tokens is negative")
-        rows = self._ints(rows, "rows")
-        given = [x for x in (rows, start, n_new) if x is not None]
-        R = len(given[0]) if given else self.max_seqs
-        start, n_new = self._ints(start, "start", R), self._ints(n_new, "n_new", R)
-        self._count(rows, R)
-        k = torch.empty(R, self.H, n_tokens, self.D, dtype=dtype, device=self.device)
-        v = torch.empty_like(k)
-        rc = _C.load().akv_int4_read(ctypes.byref(view), _C.ptr(rows), _C.ptr(start), _C.ptr(n_new), R, n_tokens,
-                                     k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                                     v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), _DTYPES[dtype],
-                                     self.status.data_ptr(), _C.stream_of(self.buf))
-        _C.check(rc, "akv_int4_read")
+        given = rows if rows is not None else (start if start is not None else n_new)
+        R = self.max_seqs if given is None else len(given)
+        rows, n_new, rp, np_ = self._rows(rows, n_new, R)
+        start = self._ints(start, "start", R)
+        kv = torch.empty((2, R, self.H, n_tokens, self.D), dtype=dtype, device=self._dev)
+        k, v = kv.unbind(0)
+        sm = self.D
+        sh = sm * n_tokens
+        sr = sh * self.H
+        kp = kv.data_ptr()
+        rc = self._lib.akv_int4_read(
+            _C.IO_ARGS.pack(view, rp, np_, 0 if start is None else start.data_ptr(), kp, sr, sh, sm, kp + 2 * sr * R,
+                            sr, sh, sm, self._status_ptr, R, n_tokens, dt, 0), _C.raw_stream(self._dev_index))
+        if rc:
+            _C.check(rc, "akv_int4_read")
         return k, v
 
     def attend(self, layer: int, query: torch.Tensor, rows=None, n_new=None, sm_scale: Optional[float] = None,
@@ -284,34 +327,50 @@ class Int4PagedCache:
 
         query (R, Hq, M, head_dim), or (R, Hq, head_dim) for one token, fp16 or bf16, any strides: query m of
         row i is its token lens - n_new[i] + m (``n_new`` None: M) and sees the tokens up to itself.  Queries
-        past n_new[i] give zero rows.  Returns the output in the query's shape and type, and with
-        ``return_lse`` the natural-log LSE (R, Hq, M) fp32."""
+        past n_new[i] give zero rows.  Returns the output in the query's shape, type and (where it is dense)
+        layout, and with ``return_lse`` the natural-log LSE (R, Hq, M) fp32."""
         view = self._layer(layer)
-        _C.require_cuda(query)
         dt = _half_dtype(query)
-        q = query.unsqueeze(2) if query.dim() == 3 else query
-        if q.dim() != 4 or q.shape[3] != self.D or q.shape[1] % self.H:
+        one = query.dim() == 3
+        q = query.unsqueeze(2) if one else query
+        shape = q.shape
+        if len(shape) != 4 or shape[3] != self.D or shape[1] % self.H or not shape[1]:
             raise ValueError(f"query must be (rows, a multiple of {self.H} heads, tokens, {self.D})")
-        q = q if q.stride(-1) == 1 else q.contiguous()
-        R, Hq, M, D = q.shape
-        rows, n_new = self._ints(rows, "rows", R), self._ints(n_new, "n_new", R)
-        self._count(rows, R)
+        if q.device != self._dev:
+            raise RuntimeError(f"akv: the query must be on {self._dev} (no CPU fallback)")
+        R, Hq, M, D = shape
+        qs = q.stride()
+        if qs[3] != 1:
+            q = q.contiguous()
+            qs = q.stride()
+        rows, n_new, rp, np_ = self._rows(rows, n_new, R)
         if out is None:
-            o = torch.empty(R, Hq, M, D, dtype=q.dtype, device=q.device)
+            o = torch.empty_like(q)
+            os_ = o.stride()
+            if os_[3] != 1:  # a query whose layout does not carry over
+                o = torch.empty(shape, dtype=q.dtype, device=self._dev)
+                os_ = o.stride()
         else:
             o = out.unsqueeze(2) if out.dim() == 3 else out
-            if o.shape != q.shape or o.dtype != q.dtype or o.stride(-1) != 1 or o.device != q.device:
+            os_ = o.stride()
+            if o.shape != shape or o.dtype is not q.dtype or os_[-1] != 1 or o.device != self._dev:
                 raise ValueError("out must have the query's shape, type and device, its last dim contiguous")
-        lse = torch.empty(R, Hq, M, dtype=torch.float32, device=q.device) if return_lse else None
-        lib = _C.load()
-        need = _C.workspace_bytes("akv_int4_attention_workspace_bytes", R, M, Hq, self.H, D, self.max_blocks)
-        stream = _C.stream_of(q)
+        lse = torch.empty(shape[:3], dtype=torch.float32, device=self._dev) if return_lse else None
+        stream = _C.raw_stream(self._dev_index)
+        key = (R, M, Hq)
+        need = self._ws_need.get(key)
+        if need is None:
+            need = self._ws_need[key] = int(self._lib.akv_int4_attention_workspace_bytes(R, M, Hq, self.H, D,
+                                                                                         self.max_blocks))
+            if need == 0:
+                raise ValueError(f"unsupported attention shape: {M} tokens of {Hq} heads")
         ws = self._workspace(need, stream)
-        rc = lib.akv_int4_attention(ctypes.byref(view), _C.ptr(rows), _C.ptr(n_new), R, M, Hq,
-                                    q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
-                                    1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
-                                    o.data_ptr(), o.stride(0), o.stride(1), o.stride(2), _C.ptr(lse), dt,
-                                    ws.data_ptr(), need, self.status.data_ptr(), stream)
-        _C.check(rc, "akv_int4_attention")
-        res = o.squeeze(2) if query.dim() == 3 else o
+        rc = self._lib.akv_int4_attention(
+            _C.ATTENTION_ARGS.pack(view, rp, np_, q.data_ptr(), qs[0], qs[1], qs[2], o.data_ptr(), os_[0], os_[1],
+                                   os_[2], 0 if lse is None else lse.data_ptr(), ws.data_ptr(), need,
+                                   self._status_ptr, R, M, Hq, dt,
+                                   self._scale if sm_scale is None else float(sm_scale), 0), stream)
+        if rc:
+            _C.check(rc, "akv_int4_attention")
+        res = o.squeeze(2) if one else o
         return (res, lse) if return_lse else res

@@ -30,38 +30,51 @@ def verify_draft(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor]
     target's own samples.  Probabilities are counted in whole units of 2^-40, so the result depends on the
     inputs alone.  Returns (accepted int32 (B,), tokens int64 (B, K+1): kept drafts, the next token, then -1).
     A drafted token outside the vocabulary counts as rejected and sets ``status`` (int32 (1,)) if given."""
-    _C.require_cuda(target_probs, draft_probs, draft_tokens, accept_u, sample_u, n_draft)
-    if target_probs.dtype not in _DTYPES:
-        raise TypeError(f"probabilities must be fp32, fp16 or bf16 (got {target_probs.dtype})")
-    if target_probs.dim() != 3 or draft_tokens.dim() != 2:
+    p, q, x = target_probs, draft_probs, draft_tokens
+    dt = _DTYPES.get(p.dtype)
+    if dt is None:
+        raise TypeError(f"probabilities must be fp32, fp16 or bf16 (got {p.dtype})")
+    dev = p.device
+    if dev.type != "cuda":
+        raise RuntimeError("akv: verify_draft runs on CUDA tensors only (no CPU fallback)")
+    if p.dim() != 3 or x.dim() != 2:
         raise ValueError("target_probs must be (B, K+1, V) and draft_tokens (B, K)")
-    B, K1, V = target_probs.shape
+    B, K1, V = p.shape
     K = K1 - 1
-    if tuple(draft_tokens.shape) != (B, K) or draft_tokens.dtype != torch.int64:
-        raise ValueError(f"draft_tokens must be int64 ({B}, {K})")
-    if draft_probs is not None and (tuple(draft_probs.shape) != (B, K, V) or draft_probs.dtype != target_probs.dtype):
-        raise ValueError(f"draft_probs must be ({B}, {K}, {V}) {target_probs.dtype}")
-    if tuple(accept_u.shape) != (B, K) or tuple(sample_u.shape) != (B,) or accept_u.dtype != torch.float32 or \
-            sample_u.dtype != torch.float32:
-        raise ValueError(f"accept_u ({B}, {K}) and sample_u ({B},) must be fp32")
-    if n_draft is not None and (tuple(n_draft.shape) != (B,) or n_draft.dtype != torch.int32):
-        raise ValueError(f"n_draft must be int32 ({B},)")
-    for t in (draft_probs, draft_tokens, accept_u, sample_u, n_draft, status):
-        if t is not None and t.device != target_probs.device:
-            raise ValueError("all tensors must be on one device")
-    p = target_probs if target_probs.stride(-1) == 1 else target_probs.contiguous()
-    q = draft_probs
-    if q is not None and q.stride(-1) != 1:
-        q = q.contiguous()
-    tokens, au, su = draft_tokens.contiguous(), accept_u.contiguous(), sample_u.contiguous()
-    nd = None if n_draft is None else n_draft.contiguous()
-    accepted = torch.empty(B, dtype=torch.int32, device=p.device)
-    out = torch.empty(B, K1, dtype=torch.int64, device=p.device)
-    has_q = q is not None and K > 0
-    rc = _C.load().akv_verify_draft(p.data_ptr(), p.stride(0), p.stride(1),
-                                    q.data_ptr() if has_q else None, q.stride(0) if has_q else 0,
-                                    q.stride(1) if has_q else 0, tokens.data_ptr(), _C.ptr(nd), au.data_ptr(),
-                                    su.data_ptr(), B, K, V, _DTYPES[p.dtype], accepted.data_ptr(), out.data_ptr(),
-                                    _C.ptr(status), _C.stream_of(p))
-    _C.check(rc, "akv_verify_draft")
+    if x.shape != (B, K) or x.dtype is not torch.int64 or x.device != dev:
+        raise ValueError(f"draft_tokens must be int64 ({B}, {K}) on {dev}")
+    ps, qp, qs = p.stride(), 0, (0, 0, 1)
+    if ps[2] != 1:
+        p = p.contiguous()
+        ps = p.stride()
+    if q is not None:
+        if q.shape != (B, K, V) or q.dtype is not p.dtype or q.device != dev:
+            raise ValueError(f"draft_probs must be ({B}, {K}, {V}) {p.dtype} on {dev}")
+        qs = q.stride()
+        if qs[2] != 1:
+            q = q.contiguous()
+            qs = q.stride()
+        if K:
+            qp = q.data_ptr()
+    au, su = accept_u, sample_u
+    if au.shape != (B, K) or su.shape != (B,) or au.dtype is not torch.float32 or su.dtype is not torch.float32 or \
+            au.device != dev or su.device != dev:
+        raise ValueError(f"accept_u ({B}, {K}) and sample_u ({B},) must be fp32 on {dev}")
+    nd = n_draft
+    if nd is not None:
+        if nd.shape != (B,) or nd.dtype is not torch.int32 or nd.device != dev:
+            raise ValueError(f"n_draft must be int32 ({B},) on {dev}")
+        nd = nd.contiguous()
+    if status is not None and (status.dtype is not torch.int32 or status.device != dev):
+        raise ValueError(f"status must be int32 on {dev}")
+    x, au, su = x.contiguous(), au.contiguous(), su.contiguous()
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    out = torch.empty((B, K1), dtype=torch.int64, device=dev)
+    rc = _C.load().akv_verify_draft(
+        _C.VERIFY_ARGS.pack(p.data_ptr(), ps[0], ps[1], qp, qs[0], qs[1], x.data_ptr(),
+                            0 if nd is None else nd.data_ptr(), au.data_ptr(), su.data_ptr(), accepted.data_ptr(),
+                            out.data_ptr(), 0 if status is None else status.data_ptr(), B, K, V, dt),
+        _C.raw_stream(dev.index if dev.index is not None else torch.cuda.current_device()))
+    if rc:
+        _C.check(rc, "akv_verify_draft")
     return accepted, out

@@ -43,46 +43,46 @@ extern "C" size_t akv_int4_attention_workspace_bytes(int R, int M, int Hq, int k
   return p.arrived + p.meta + p.part;
 }
 
-extern "C" int akv_int4_attention(const akv_int4_cache* c, const int32_t* rows, const int32_t* n_new, int R, int M,
-                                  int Hq, const void* q, int64_t q_sr, int64_t q_sh, int64_t q_sm, float sm_scale,
-                                  void* out, int64_t o_sr, int64_t o_sh, int64_t o_sm, float* lse, int dtype,
-                                  void* workspace, size_t workspace_bytes, int* status, void* stream) {
+extern "C" int akv_int4_attention(const akv_int4_attention_args* a, void* stream) {
+  if (!a) return AKV_ERR_NULL;
+  const akv_int4_cache* c = a->cache;
   const int rc = int4_check(c);
   if (rc) return rc;
-  if (dtype != AKV_FP16 && dtype != AKV_BF16) return AKV_ERR_UNSUPPORTED;
-  if (R < 0 || M < 0 || Hq <= 0 || Hq % c->kv_heads) return AKV_ERR_SHAPE;
-  if (R == 0 || M == 0) return AKV_OK;
-  if (!q || !out || !workspace) return AKV_ERR_NULL;
-  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 1) ||
-      (reinterpret_cast<uintptr_t>(workspace) & 15))
+  if (a->dtype != AKV_FP16 && a->dtype != AKV_BF16) return AKV_ERR_UNSUPPORTED;
+  if (a->R < 0 || a->M < 0 || a->Hq <= 0 || a->Hq % c->kv_heads) return AKV_ERR_SHAPE;
+  if (a->R == 0 || a->M == 0) return AKV_OK;
+  if (!a->q || !a->out || !a->workspace) return AKV_ERR_NULL;
+  if (((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 1) ||
+      (reinterpret_cast<uintptr_t>(a->workspace) & 15))
     return AKV_ERR_ALIGN;
-  const size_t need = akv_int4_attention_workspace_bytes(R, M, Hq, c->kv_heads, c->head_dim, c->max_blocks);
+  const size_t need =
+      akv_int4_attention_workspace_bytes(a->R, a->M, a->Hq, c->kv_heads, c->head_dim, c->max_blocks);
   if (need == 0) return AKV_ERR_UNSUPPORTED;  // more query rows than one launch lists
-  if (workspace_bytes < need) return AKV_ERR_WORKSPACE;
-  const Plan plan = attn_plan(R, M, Hq, c->kv_heads, c->head_dim, c->max_blocks);
+  if (a->workspace_bytes < need) return AKV_ERR_WORKSPACE;
+  const Plan plan = attn_plan(a->R, a->M, a->Hq, c->kv_heads, c->head_dim, c->max_blocks);
   Int4AttnParams p{};
   p.c = *c;
-  p.rows = rows;
-  p.n_new = n_new;
-  p.M = M;
-  p.Hq = Hq;
+  p.rows = a->rows;
+  p.n_new = a->n_new;
+  p.M = a->M;
+  p.Hq = a->Hq;
   p.tiles = plan.tiles;
-  p.q = static_cast<const uint16_t*>(q);
-  p.q_sr = q_sr; p.q_sh = q_sh; p.q_sm = q_sm;
-  p.scale = sm_scale;
-  p.out = static_cast<uint16_t*>(out);
-  p.o_sr = o_sr; p.o_sh = o_sh; p.o_sm = o_sm;
-  p.lse = lse;
-  p.bf16 = dtype == AKV_BF16;
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.q_sr = a->q_sr; p.q_sh = a->q_sh; p.q_sm = a->q_sm;
+  p.scale = a->sm_scale;
+  p.out = static_cast<uint16_t*>(a->out);
+  p.o_sr = a->o_sr; p.o_sh = a->o_sh; p.o_sm = a->o_sm;
+  p.lse = a->lse;
+  p.bf16 = a->dtype == AKV_BF16;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   p.arrived = reinterpret_cast<unsigned*>(ws);
   p.meta = plan.fused ? nullptr : reinterpret_cast<int2*>(ws + plan.arrived);
   p.part = reinterpret_cast<float*>(ws + plan.arrived + plan.meta);
-  p.status = status;
+  p.status = a->status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  for (int r = 0; r < R; r += plan.rows) {
+  for (int r = 0; r < a->R; r += plan.rows) {
     p.row0 = r;
-    p.R = R - r < plan.rows ? R - r : plan.rows;
+    p.R = a->R - r < plan.rows ? a->R - r : plan.rows;
     const int e = c->head_dim == 64 ? int4_attn_64(p, plan.nt, st)
                   : c->head_dim == 128 ? int4_attn_128(p, plan.nt, st) : int4_attn_256(p, plan.nt, st);
     if (e) return e;

@@ -354,44 +354,34 @@ extern "C" int akv_int4_layout_init(int head_dim, int group, akv_int4_layout* ou
 
 // argument checks and launch of append and read
 template <bool WRITE>
-static int int4_io(const akv_int4_cache* c, const int32_t* rows, const int32_t* start, const int32_t* n_new, int R, int M,
-                   const void* k, int64_t k_sr, int64_t k_sh, int64_t k_sm, const void* v, int64_t v_sr, int64_t v_sh,
-                   int64_t v_sm, int dtype, int* status, void* stream) {
-  const int rc = int4_check(c);
+static int int4_io(const akv_int4_io_args* x, void* stream) {
+  if (!x) return AKV_ERR_NULL;
+  const int rc = int4_check(x->cache);
   if (rc) return rc;
-  if (dtype != AKV_FP16 && dtype != AKV_BF16) return AKV_ERR_UNSUPPORTED;
-  if (R < 0 || M < 0) return AKV_ERR_SHAPE;
-  if (R == 0 || M == 0) return AKV_OK;
-  if (!k || !v) return AKV_ERR_NULL;
-  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 1) return AKV_ERR_ALIGN;
-  if (R > 65535 || c->kv_heads > (1 << 20) || M > INT32_MAX - 64) return AKV_ERR_UNSUPPORTED;
+  if (x->dtype != AKV_FP16 && x->dtype != AKV_BF16) return AKV_ERR_UNSUPPORTED;
+  if (x->R < 0 || x->M < 0) return AKV_ERR_SHAPE;
+  if (x->R == 0 || x->M == 0) return AKV_OK;
+  if (!x->k || !x->v) return AKV_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(x->k) | reinterpret_cast<uintptr_t>(x->v)) & 1) return AKV_ERR_ALIGN;
+  if (x->R > 65535 || x->cache->kv_heads > (1 << 20) || x->M > INT32_MAX - 64) return AKV_ERR_UNSUPPORTED;
   Int4Io a{};
-  a.c = *c;
-  a.rows = rows;
-  a.n_new = n_new;
-  a.start = start;
-  a.M = M;
-  a.k = static_cast<uint16_t*>(const_cast<void*>(k));
-  a.k_sr = k_sr; a.k_sh = k_sh; a.k_sm = k_sm;
-  a.v = static_cast<uint16_t*>(const_cast<void*>(v));
-  a.v_sr = v_sr; a.v_sh = v_sh; a.v_sm = v_sm;
-  a.status = status;
+  a.c = *x->cache;
+  a.rows = x->rows;
+  a.n_new = x->n_new;
+  a.start = WRITE ? nullptr : x->start;
+  a.M = x->M;
+  a.k = static_cast<uint16_t*>(x->k);
+  a.k_sr = x->k_sr; a.k_sh = x->k_sh; a.k_sm = x->k_sm;
+  a.v = static_cast<uint16_t*>(x->v);
+  a.v_sr = x->v_sr; a.v_sh = x->v_sh; a.v_sm = x->v_sm;
+  a.status = x->status;
   // M tokens from any slot on touch at most this many pages
-  const int blocks = (M + 2 * kBlockTokens - 2) / kBlockTokens;
-  const bool aligned = rows_aligned16(k, k_sr, k_sh, k_sm) && rows_aligned16(v, v_sr, v_sh, v_sm);
-  io_launch<WRITE>(a, dim3(blocks, R), dtype == AKV_BF16, aligned, static_cast<cudaStream_t>(stream));
+  const int blocks = (x->M + 2 * kBlockTokens - 2) / kBlockTokens;
+  const bool aligned = rows_aligned16(x->k, x->k_sr, x->k_sh, x->k_sm) && rows_aligned16(x->v, x->v_sr, x->v_sh, x->v_sm);
+  io_launch<WRITE>(a, dim3(blocks, x->R), x->dtype == AKV_BF16, aligned, static_cast<cudaStream_t>(stream));
   return cudaGetLastError() == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH;
 }
 
-extern "C" int akv_int4_append(const akv_int4_cache* c, const int32_t* rows, const int32_t* n_new, int R, int M,
-                               const void* k, int64_t k_sr, int64_t k_sh, int64_t k_sm,
-                               const void* v, int64_t v_sr, int64_t v_sh, int64_t v_sm, int dtype, int* status,
-                               void* stream) {
-  return int4_io<true>(c, rows, nullptr, n_new, R, M, k, k_sr, k_sh, k_sm, v, v_sr, v_sh, v_sm, dtype, status, stream);
-}
+extern "C" int akv_int4_append(const akv_int4_io_args* a, void* stream) { return int4_io<true>(a, stream); }
 
-extern "C" int akv_int4_read(const akv_int4_cache* c, const int32_t* rows, const int32_t* start, const int32_t* n_new,
-                             int R, int N, void* k, int64_t k_sr, int64_t k_sh, int64_t k_sm,
-                             void* v, int64_t v_sr, int64_t v_sh, int64_t v_sm, int dtype, int* status, void* stream) {
-  return int4_io<false>(c, rows, start, n_new, R, N, k, k_sr, k_sh, k_sm, v, v_sr, v_sh, v_sm, dtype, status, stream);
-}
+extern "C" int akv_int4_read(const akv_int4_io_args* a, void* stream) { return int4_io<false>(a, stream); }

@@ -327,24 +327,23 @@ static cudaError_t verify_launch(const VerifyParams& p, int B, bool draft, cudaS
   return draft ? cudaLaunchKernelEx(&cfg, verify_kernel<DT, true>, p) : cudaLaunchKernelEx(&cfg, verify_kernel<DT, false>, p);
 }
 
-extern "C" int akv_verify_draft(const void* target, int64_t t_sb, int64_t t_sj, const void* draft, int64_t d_sb,
-                                int64_t d_sj, const int64_t* tokens, const int32_t* n_draft, const float* accept_u,
-                                const float* sample_u, int B, int K, int vocab, int dtype, int32_t* accepted,
-                                int64_t* out, int* status, void* stream) {
-  if (B < 0 || K < 0 || vocab <= 0 || vocab > (1 << 23)) return AKV_ERR_SHAPE;  // 2^23 units of 2^40 stay below 2^63
-  if (dtype != AKV_FP32 && dtype != AKV_FP16 && dtype != AKV_BF16) return AKV_ERR_UNSUPPORTED;
-  if (B > 65535) return AKV_ERR_UNSUPPORTED;
-  if (B == 0) return AKV_OK;
-  if (!target || !sample_u || !accepted || !out || (K && (!tokens || !accept_u))) return AKV_ERR_NULL;
-  const uintptr_t mask = dtype == AKV_FP32 ? 3 : 1;
-  if ((reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft)) & mask) return AKV_ERR_ALIGN;
-  VerifyParams p{target, t_sb, t_sj, draft, d_sb, d_sj, tokens, n_draft, accept_u, sample_u, K, vocab, accepted, out,
-                 status};
+extern "C" int akv_verify_draft(const akv_verify_args* a, void* stream) {
+  if (!a) return AKV_ERR_NULL;
+  if (a->B < 0 || a->K < 0 || a->vocab <= 0 || a->vocab > (1 << 23)) return AKV_ERR_SHAPE;  // 2^63 units
+  if (a->dtype != AKV_FP32 && a->dtype != AKV_FP16 && a->dtype != AKV_BF16) return AKV_ERR_UNSUPPORTED;
+  if (a->B > 65535) return AKV_ERR_UNSUPPORTED;
+  if (a->B == 0) return AKV_OK;
+  if (!a->target || !a->sample_u || !a->accepted || !a->out || (a->K && (!a->tokens || !a->accept_u)))
+    return AKV_ERR_NULL;
+  const uintptr_t mask = a->dtype == AKV_FP32 ? 3 : 1;
+  if ((reinterpret_cast<uintptr_t>(a->target) | reinterpret_cast<uintptr_t>(a->draft)) & mask) return AKV_ERR_ALIGN;
+  const VerifyParams p{a->target, a->t_sb,     a->t_sj,     a->draft,    a->d_sb, a->d_sj,     a->tokens,
+                       a->n_draft, a->accept_u, a->sample_u, a->K,       a->vocab, a->accepted, a->out, a->status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  const bool d = draft != nullptr;
-  if (dtype == AKV_FP32) e = verify_launch<AKV_FP32>(p, B, d, st);
-  else if (dtype == AKV_FP16) e = verify_launch<AKV_FP16>(p, B, d, st);
-  else e = verify_launch<AKV_BF16>(p, B, d, st);
+  const bool d = a->draft != nullptr;
+  if (a->dtype == AKV_FP32) e = verify_launch<AKV_FP32>(p, a->B, d, st);
+  else if (a->dtype == AKV_FP16) e = verify_launch<AKV_FP16>(p, a->B, d, st);
+  else e = verify_launch<AKV_BF16>(p, a->B, d, st);
   return e == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH;
 }

@@ -666,17 +666,26 @@ typedef struct {
  * NaN counts as 0, infinities as +-65504; per group, in fp32:
  *   zero = fp16(min), scale = fp16((max - zero) / 15),
  *   code = clamp(rint((x - zero) / scale), 0, 15), 0 where scale is 0. */
-int akv_int4_append(const akv_int4_cache* c, const int32_t* rows, const int32_t* n_new, int R, int M,
-                    const void* k, int64_t k_sr, int64_t k_sh, int64_t k_sm,
-                    const void* v, int64_t v_sr, int64_t v_sh, int64_t v_sm, int dtype, int* status, void* stream);
+typedef struct {
+  const akv_int4_cache* cache;
+  const int32_t* rows;
+  const int32_t* n_new;
+  const int32_t* start;          /* akv_int4_read only */
+  void* k;
+  int64_t k_sr, k_sh, k_sm;
+  void* v;
+  int64_t v_sr, v_sh, v_sm;
+  int* status;
+  int32_t R, M, dtype, reserved; /* reserved: 0 */
+} akv_int4_io_args;
 
-/* The values the cache stands for: out (i, h, t, d), t < N, is token
+int akv_int4_append(const akv_int4_io_args* a, void* stream);
+
+/* The values the cache stands for: k / v element (i, h, t, d), t < M, is token
  * start[i] + t of sequence rows[i] (start NULL: its last n_new[i] tokens,
- * n_new NULL: N), 0 where there is no such token; fp16 results are held to
+ * n_new NULL: M), 0 where there is no such token; fp16 results are held to
  * +-65504. */
-int akv_int4_read(const akv_int4_cache* c, const int32_t* rows, const int32_t* start, const int32_t* n_new, int R,
-                  int N, void* k, int64_t k_sr, int64_t k_sh, int64_t k_sm,
-                  void* v, int64_t v_sr, int64_t v_sh, int64_t v_sm, int dtype, int* status, void* stream);
+int akv_int4_read(const akv_int4_io_args* a, void* stream);
 
 /* Attention of M query tokens per call row over its sequence.  Query m <
  * n_new[i] stands at position lens - n_new + m and sees every token up to its
@@ -687,11 +696,25 @@ int akv_int4_read(const akv_int4_cache* c, const int32_t* rows, const int32_t* s
  * Workspace: akv_int4_attention_workspace_bytes(...), 16-byte aligned, zeroed
  * once before its first use (its counters are 0 again after every call, so
  * calls in order on one stream may share it, whatever their shapes). */
+typedef struct {
+  const akv_int4_cache* cache;
+  const int32_t* rows;
+  const int32_t* n_new;
+  const void* q;
+  int64_t q_sr, q_sh, q_sm;
+  void* out;
+  int64_t o_sr, o_sh, o_sm;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+  int* status;
+  int32_t R, M, Hq, dtype;
+  float sm_scale;
+  int32_t reserved;              /* 0 */
+} akv_int4_attention_args;
+
 size_t akv_int4_attention_workspace_bytes(int R, int M, int Hq, int kv_heads, int head_dim, int max_blocks);
-int akv_int4_attention(const akv_int4_cache* c, const int32_t* rows, const int32_t* n_new, int R, int M, int Hq,
-                       const void* q, int64_t q_sr, int64_t q_sh, int64_t q_sm, float sm_scale,
-                       void* out, int64_t o_sr, int64_t o_sh, int64_t o_sm, float* lse, int dtype,
-                       void* workspace, size_t workspace_bytes, int* status, void* stream);
+int akv_int4_attention(const akv_int4_attention_args* a, void* stream);
 
 /* ------------------------------------------------------------------------
  * Ownership of the pages, kept on the device so that no step of a serving
@@ -765,9 +788,22 @@ int akv_pages_copy(uint8_t* pool, int n_layers, int64_t layer_stride, int64_t pa
  * [B][K+1] = them, the drawn token, then -1.  A token outside [0, vocab) is
  * rejected (AKV_ERR_SHAPE in *status).
  * ---------------------------------------------------------------------- */
-int akv_verify_draft(const void* target, int64_t t_sb, int64_t t_sj, const void* draft, int64_t d_sb, int64_t d_sj,
-                     const int64_t* tokens, const int32_t* n_draft, const float* accept_u, const float* sample_u,
-                     int B, int K, int vocab, int dtype, int32_t* accepted, int64_t* out, int* status, void* stream);
+typedef struct {
+  const void* target;
+  int64_t t_sb, t_sj;
+  const void* draft;
+  int64_t d_sb, d_sj;
+  const int64_t* tokens;
+  const int32_t* n_draft;
+  const float* accept_u;
+  const float* sample_u;
+  int32_t* accepted;
+  int64_t* out;
+  int* status;
+  int32_t B, K, vocab, dtype;
+} akv_verify_args;
+
+int akv_verify_draft(const akv_verify_args* a, void* stream);
 
 #ifdef __cplusplus
 }

@@ -29,6 +29,25 @@ def test_struct_matches_header(tmp_path, struct, name):
     assert out[1:] == [getattr(S, f).offset for f in fields]
 
 
+@pytest.mark.parametrize("packer,name,last", [("IO_ARGS", "akv_int4_io_args", "reserved"),
+                                              ("ATTENTION_ARGS", "akv_int4_attention_args", "reserved"),
+                                              ("VERIFY_ARGS", "akv_verify_args", "dtype")])
+def test_packed_args_match_header(tmp_path, packer, name, last):
+    """The packed argument structs have the header's size, and their last field its place."""
+    from akv import _C
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    src = tmp_path / "s.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "akv_b200.h"\nint main(void){\n'
+                   f'printf("%zu %zu\\n", sizeof({name}), offsetof({name}, {last}));return 0;}}\n')
+    exe = tmp_path / "s"
+    subprocess.run([cc, "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    size, off = map(int, subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split())
+    S = getattr(_C, packer)
+    assert (S.size, S.size - 4) == (size, off)
+
+
 def test_layout():
     from akv import _C
     for d in (64, 128, 256):
@@ -56,7 +75,8 @@ def test_host_refusals():
         return ctypes.byref(_C.Int4Cache(*[d[f[0]] for f in _C.Int4Cache._fields_]))
 
     def append(c, k=256, dtype=0, R=1, M=1):
-        return lib.akv_int4_append(c, None, None, R, M, k, 0, 0, 0, 256, 0, 0, 0, dtype, None, None)
+        return lib.akv_int4_append(_C.IO_ARGS.pack(0 if c is None else ctypes.addressof(c._obj), 0, 0, 0, k or 0, 0, 0,
+                                                   0, 256, 0, 0, 0, 0, R, M, dtype, 0), None)
 
     assert append(None) == -7 and append(cache(pool=0)) == -7 and append(cache(), k=None) == -7
     assert append(cache(head_dim=96)) == -1 and append(cache(table_stride=3)) == -1 and append(cache(), R=-1) == -1
@@ -68,8 +88,9 @@ def test_host_refusals():
     assert need > 0 and lib.akv_int4_attention_workspace_bytes(1, 1, 3, 2, 128, 4) == 0
 
     def attend(c, Hq=4, q=256, ws=256, n=need, dtype=0):
-        return lib.akv_int4_attention(c, None, None, 1, 1, Hq, q, 0, 0, 0, 1.0, 256, 0, 0, 0, None, dtype, ws, n, None,
-                                      None)
+        return lib.akv_int4_attention(_C.ATTENTION_ARGS.pack(0 if c is None else ctypes.addressof(c._obj), 0, 0, q or 0,
+                                                             0, 0, 0, 256, 0, 0, 0, 0, ws or 0, n, 0, 1, 1, Hq, dtype,
+                                                             1.0, 0), None)
 
     assert attend(None) == -7 and attend(cache(), q=None) == -7 and attend(cache(), ws=None) == -7
     assert attend(cache(), Hq=3) == -1 and attend(cache(), ws=264) == -3 and attend(cache(), n=need - 1) == -8
@@ -91,8 +112,8 @@ def test_host_refusals():
     assert lib.akv_pages_copy(256, 1, 0, 4352, 4, None, 256, 1, None, None) == -7
 
     def verify(target=256, K=2, V=10, dtype=2, B=1, tokens=256):
-        return lib.akv_verify_draft(target, 0, 0, 256, 0, 0, tokens, None, 256, 256, B, K, V, dtype, 256, 256, None,
-                                    None)
+        return lib.akv_verify_draft(_C.VERIFY_ARGS.pack(target or 0, 0, 0, 256, 0, 0, tokens or 0, 0, 256, 256, 256, 256,
+                                                        0, B, K, V, dtype), None)
 
     assert verify(target=None) == -7 and verify(tokens=None) == -7 and verify(V=0) == -1 and verify(K=-1) == -1
     assert verify(dtype=3) == -4 and verify(target=257) == -3 and verify(B=0) == 0 and verify(V=1 << 24) == -1
