@@ -18,6 +18,8 @@ Plan attn_plan(int R, int M, int Hq, int kv_heads, int D, int max_blocks) {
   p.nt = attn_nt(D, q_rows);
   p.tiles = (q_rows + 8 * p.nt - 1) / (8 * p.nt);
   p.rows = kAttnEntries / p.tiles;
+  const int64_t row_pages = static_cast<int64_t>(p.tiles) * kv_heads * max_blocks;
+  if (p.rows > INT32_MAX / row_pages) p.rows = static_cast<int>(INT32_MAX / row_pages);  // 0: too many
   if (p.rows > R) p.rows = R;
   const size_t units = static_cast<size_t>(p.rows) * p.tiles * kv_heads;
   // the most CTAs that can share a unit, and the query rows each leaves there
@@ -28,7 +30,7 @@ Plan attn_plan(int R, int M, int Hq, int kv_heads, int D, int max_blocks) {
   p.meta = (units * sizeof(int2) + 15) / 16 * 16;
   // a CTA and a unit meet at most once, and along the list of pages their
   // numbers' sum only grows: it is the slot of the partial result
-  p.part = (units + kSMs * attn_occ(D, p.nt)) * 8 * p.nt * (D + 2) * sizeof(float);
+  p.part = (units + kSMs * attn_occ(D, p.nt) * WAVES) * 8 * p.nt * (D + 2) * sizeof(float);
   return p;
 }
 
@@ -40,6 +42,7 @@ extern "C" size_t akv_int4_attention_workspace_bytes(int R, int M, int Hq, int k
   if (R == 0 || M == 0) return 16;
   if (static_cast<int64_t>(M) * (Hq / kv_heads) > 8 * kAttnEntries) return 0;
   const Plan p = attn_plan(R, M, Hq, kv_heads, head_dim, max_blocks);
+  if (p.rows == 0 || static_cast<int64_t>(R) * Hq * M > INT32_MAX) return 0;
   return p.arrived + p.meta + p.part;
 }
 

@@ -30,6 +30,13 @@ constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kAttnEntries = 1024;  // (row, row tile) pairs of one launch
 constexpr int kAttnMinPages = 4;    // pages of a CTA's share, at least (one per warp)
 constexpr int kAttnFused = 1024;    // partial rows of a unit that its last CTA merges by itself
+#ifndef UNROLL
+#define UNROLL 1
+#define STG (NT > 1 || G == 1 ? 3 : 2)
+#define OCC1 4
+#define OCC2 3
+#define WAVES 1
+#endif
 constexpr float kLazyLog2 = 6.f;    // weights may reach 2^6 before the maximum moves
 
 struct Int4AttnParams {
@@ -51,6 +58,9 @@ struct Int4AttnParams {
   int* status;
 };
 
+// resident CTAs of an SM: what the registers of 128 threads leave
+constexpr int attn_occ(int D, int nt) { return nt == 1 ? (D == 256 ? 2 : OCC1) : (nt == 2 ? (D == 256 ? 2 : OCC2) : 2); }
+
 template <int D, int G, int NT>
 struct AttnShape {
   static constexpr int GS = D / G;              // channels of a group
@@ -58,23 +68,27 @@ struct AttnShape {
   static constexpr int BV = GS / 16;            // V bytes of a thread per token and group
   static constexpr int REC = int4_layout(D, G).bytes;
   static constexpr int ROWS = 8 * NT;           // query rows of a CTA
-  static constexpr int STAGES = D == 64 ? 4 : (D == 128 && (NT > 1 || G == 1) ? 3 : 2);
+  static constexpr int U = UNROLL;              // pages of an iteration
+  static constexpr int STAGES = D == 64 ? 4 : (D == 128 ? STG : 2);
   static constexpr int RING = kAttnWarps * STAGES * REC;
   static constexpr int PITCH = D + 4;
   static constexpr int MERGE = kAttnWarps * ROWS * PITCH * 4;
   static constexpr int BUF = RING > MERGE ? RING : MERGE;
   static constexpr int FRAG = D / 16 * NT * 32 * 8;
   // ring / merge buffer, fragments, then: group sums of q, exponent factors,
-  // visible lengths, (y, l) per warp and row, barriers; per entry: prefix sums
-  // of pages, lengths, new tokens
+  // visible lengths, output offsets, (y, l) per warp and row, barriers; per
+  // entry: prefix sums of pages, lengths, new tokens
   static constexpr int OFF_FRAG = (BUF + 127) / 128 * 128;
   static constexpr int OFF_QS = OFF_FRAG + FRAG;
   static constexpr int OFF_CQ = OFF_QS + ROWS * G * 4;
   static constexpr int OFF_SEE = OFF_CQ + ROWS * 4;
-  static constexpr int OFF_ML = OFF_SEE + ROWS * 4;
+  static constexpr int OFF_OUT = OFF_SEE + ROWS * 4;
+  static constexpr int OFF_LSE = OFF_OUT + ROWS * 8;
+  static constexpr int OFF_ON = OFF_LSE + ROWS * 4;
+  static constexpr int OFF_ML = OFF_ON + ROWS * 4;
   static constexpr int OFF_BAR = OFF_ML + kAttnWarps * ROWS * 8;
   static constexpr int OFF_PREF = OFF_BAR + kAttnWarps * STAGES * 8;
-  static constexpr int OCC = NT == 1 ? (D == 256 ? 2 : 4) : (NT == 2 ? (D == 256 ? 2 : 3) : 2);
+  static constexpr int OCC = attn_occ(D, NT);
   static constexpr int smem(int entries) { return OFF_PREF + (3 * entries + 1) * 4; }
   static_assert(OCC * (smem(64) + 1024) <= 228 * 1024, "resident CTAs do not fit");
 };
@@ -123,32 +137,34 @@ AKV_DEV int visible_pages(const Int4Row& r, int m_last) {
   return see > 0 ? (see + kBlockTokens - 1) / kBlockTokens : 0;
 }
 
-// Output channels of accumulator pair p (order of the merge buffer) of query
-// row rr of (call row i, KV head h); its lse with pair 0.
+// Element offset of the output row of query row rr of (call row i, KV head h).
+AKV_DEV int64_t out_row(const Int4AttnParams& P, int i, int hq, int m) {
+  return i * P.o_sr + hq * P.o_sh + m * P.o_sm;
+}
+
+// Output channels of accumulator pair p (order of the merge buffer) of the row
+// at `row`; its lse with pair 0.  L 0: a row that sees nothing.
 template <int D, int G>
-AKV_DEV void store_pair(const Int4AttnParams& P, int i, int h, int rep, int rr, int n_new, int p, float2 v, float top,
-                        float L) {
+AKV_DEV void store_pair(const Int4AttnParams& P, int64_t row, float* lse, int p, float2 v, float top, float L) {
   constexpr int GS = D / G, BV = GS / 16;
   const int j = p / 8, g = p % 8;
   const int ch = j / BV * GS + g * 2 * BV + 2 * (j % BV);
-  const int m = rr / rep, hq = h * rep + rr % rep;
-  const bool on = m < n_new && L > 0.f;
+  const bool on = L > 0.f;
   const float inv = on ? 1.f / L : 0.f;
   v.x = on ? v.x * inv : 0.f;
   v.y = on ? v.y * inv : 0.f;
-  uint16_t* o = P.out + i * P.o_sr + hq * P.o_sh + m * P.o_sm + ch;
+  uint16_t* o = P.out + row + ch;
   const uint32_t w = P.bf16 ? pack_elems<true>(v.x, v.y) : pack_elems<false>(v.x, v.y);
   o[0] = static_cast<uint16_t>(w);
   o[1] = static_cast<uint16_t>(w >> 16);
-  if (P.lse && p == 0)
-    P.lse[(static_cast<int64_t>(i) * P.Hq + hq) * P.M + m] = on ? (top + log2f(L)) * 0.6931471805599453f : -INFINITY;
+  if (lse && p == 0) *lse = on ? (top + log2f(L)) * 0.6931471805599453f : -INFINITY;
 }
 
 // One CTA merges the parts of a unit (segs * 8 NT <= kAttnFused, so their
 // weights fit the buffer w).
 template <int D, int G, int NT>
-AKV_DEV void merge_parts(const Int4AttnParams& P, const float* part, int segs, int i, int h, int rep, int tile,
-                         int valid, int n_new, float* w) {
+AKV_DEV void merge_parts(const Int4AttnParams& P, const float* part, int segs, const int64_t* s_out, const int* s_lse,
+                         int valid, float* w) {
   constexpr int ROWS = 8 * NT;
   constexpr int64_t STEP = static_cast<int64_t>(ROWS) * (D + 2);
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -181,7 +197,7 @@ AKV_DEV void merge_parts(const Int4AttnParams& P, const float* part, int segs, i
       acc.x = fmaf(x, v.x, acc.x);
       acc.y = fmaf(x, v.y, acc.y);
     }
-    store_pair<D, G>(P, i, h, rep, tile * ROWS + n, n_new, p, acc, s_tl[n].x, s_tl[n].y);
+    store_pair<D, G>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, p, acc, s_tl[n].x, s_tl[n].y);
   }
 }
 
@@ -193,6 +209,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
   float* s_qs = reinterpret_cast<float*>(smem + S::OFF_QS);
   float* s_cq = reinterpret_cast<float*>(smem + S::OFF_CQ);
   int* s_see = reinterpret_cast<int*>(smem + S::OFF_SEE);
+  int* s_on = reinterpret_cast<int*>(smem + S::OFF_ON);
+  int* s_lse = reinterpret_cast<int*>(smem + S::OFF_LSE);
+  int64_t* s_out = reinterpret_cast<int64_t*>(smem + S::OFF_OUT);
   float2* s_ml = reinterpret_cast<float2*>(smem + S::OFF_ML);
   uint64_t* s_bar = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
   int* s_pref = reinterpret_cast<int*>(smem + S::OFF_PREF);
@@ -259,28 +278,30 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
       const int rr = e % P.tiles * S::ROWS + k / D, m = rr / rep;
       if (m >= P.M) break;
       const int hq = h * rep + rr % rep;
-      P.out[i * P.o_sr + hq * P.o_sh + m * P.o_sm + k % D] = 0;
-      if (P.lse && k % D == 0) P.lse[(static_cast<int64_t>(i) * P.Hq + hq) * P.M + m] = -INFINITY;
+      P.out[out_row(P, i, hq, m) + k % D] = 0;
+      if (P.lse && k % D == 0) P.lse[(i * P.Hq + hq) * P.M + m] = -INFINITY;
     }
   }
 
-  // This CTA's share of all pages, a contiguous run over (row, tile, head, page).
-  const int64_t total = static_cast<int64_t>(s_pref[entries]) * H;
-  int64_t share = (total + gridDim.x - 1) / gridDim.x;
+  // This CTA's share of all pages, a contiguous run over (row, tile, head, page);
+  // their number fits 31 bits (the caller sees to it).
+  const int total = s_pref[entries] * H;
+  int share = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   {
     int least = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
     if (least > kAttnMinPages) least = kAttnMinPages;
     if (share < least) share = least;
   }
-  int64_t pos = share * blockIdx.x;
-  const int64_t end = pos + share < total ? pos + share : total;
-  if (pos >= end) return;
+  if (static_cast<int64_t>(share) * blockIdx.x >= total) return;
+  const int begin = share * blockIdx.x;
+  const int end = total - begin > share ? begin + share : total;
+  int pos = begin;
   int e = 0;
   {
     int hi = entries;  // the last entry that starts at or before pos
     while (hi - e > 1) {
       const int mid = (e + hi) / 2;
-      if (static_cast<int64_t>(s_pref[mid]) * H <= pos) e = mid; else hi = mid;
+      if (s_pref[mid] * H <= pos) e = mid; else hi = mid;
     }
   }
   uint32_t stage = 0, phase = 0;
@@ -290,15 +311,15 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
 
   while (pos < end) {
     while (s_pref[e + 1] == s_pref[e]) ++e;
-    const int64_t e_start = static_cast<int64_t>(s_pref[e]) * H;
+    const int e_start = s_pref[e] * H;
     const int pages = s_pref[e + 1] - s_pref[e];
-    const int h = static_cast<int>((pos - e_start) / pages);
-    const int page0 = static_cast<int>((pos - e_start) % pages);
+    const int h = (pos - e_start) / pages;
+    const int u_start = e_start + h * pages;
+    const int page0 = pos - u_start;
     int n_pages = pages - page0;
-    if (n_pages > end - pos) n_pages = static_cast<int>(end - pos);
+    if (n_pages > end - pos) n_pages = end - pos;
     const int unit = e * H + h;
-    const int64_t u_start = e_start + static_cast<int64_t>(h) * pages;
-    const int cta0 = static_cast<int>(u_start / share), cta1 = static_cast<int>((u_start + pages - 1) / share);
+    const bool whole = u_start >= begin && u_start + pages <= end;
     const int i = P.row0 + e / P.tiles, tile = e % P.tiles;
     const int len = s_len[e], n_new = s_new[e];
     const int seq = P.rows ? __ldg(P.rows + i) : i;  // in range: its pages are not 0
@@ -388,6 +409,12 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
           // log2 e * scale in units of the MMA result; never 0, so that -inf stays -inf
           s_cq[n] = fmaxf(ldexpf(fabsf(P.scale) * 1.4426950408889634f, 20 - ex), 1e-37f);
           s_see[n] = len - n_new + (m < n_new ? m : n_new - 1) + 1;
+          s_on[n] = m < n_new;
+          if (m < P.M) {
+            const int hq = h * rep + (tile * S::ROWS + n) - m * rep;
+            s_out[n] = out_row(P, i, hq, m);
+            s_lse[n] = (i * P.Hq + hq) * P.M + m;
+          }
         }
       }
     }
@@ -423,102 +450,117 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
       for (int j = 0; j < D / 16; ++j)
 #pragma unroll
         for (int k = 0; k < 4; ++k) O[nt][j][k] = 0.f;
-    float vref = 0.f, vinv = 0.f, vunit = 0.f;  // power of two above the V scales seen so far, its inverse
+    float vref = 0.f, vinv = 0.f;  // power of two above the V scales seen so far, its inverse
 
-    for (int k = 0; k < mine; ++k) {
-      if (!alive || !__all_sync(~0u, mbar_wait(bars + stage, phase, P.status))) {
-        // a copy never came: take no more, but see the ones in flight land
+    for (int k = 0; k < mine; k += S::U) {
+      // a copy that never comes: take no more, but see the ones in flight land
+      bool ok = alive;
+#pragma unroll
+      for (int u = 0; u < S::U; ++u) {
+        const uint32_t st = stage + u;
+        if (ok && k + u < mine)
+          ok = __all_sync(~0u, mbar_wait(bars + st % S::STAGES, st >= S::STAGES ? phase ^ 1 : phase, P.status));
+      }
+      if (!ok) {
         if (alive)
-          for (int r = 1; r < S::STAGES && k + r < mine; ++r) {
-            const uint32_t st = (stage + r) % S::STAGES;
-            mbar_wait(bars + st, stage + r >= S::STAGES ? phase ^ 1 : phase, P.status);
+          for (int r = 0; r < S::STAGES && k + r < mine; ++r) {
+            const uint32_t st = stage + r;
+            mbar_wait(bars + st % S::STAGES, st >= S::STAGES ? phase ^ 1 : phase, P.status);
           }
         alive = false;
         break;
       }
-      const uint8_t* rec = ring + stage * S::REC;
-      const int tok0 = (page0 + warp + k * kAttnWarps) * kBlockTokens;
+      const uint8_t* rec[S::U];
+      int tok0[S::U];
+#pragma unroll
+      for (int u = 0; u < S::U; ++u) {
+        rec[u] = ring + (stage + u) % S::STAGES * S::REC;
+        // an iteration's page that does not exist counts as one past every row's end
+        tok0[u] = k + u < mine ? (page0 + warp + (k + u) * kAttnWarps) * kBlockTokens : INT32_MAX - 2 * kBlockTokens;
+      }
 
       // ---- scores: tokens are the MMA's rows, queries its columns
-      float x[2][NT][4];
-      const __half2* kp = reinterpret_cast<const __half2*>(rec + int4_layout(D, G).kp);
+      float x[S::U][2][NT][4];
 #pragma unroll
-      for (int gi = 0; gi < G; ++gi) {
-        uint32_t kw[4][S::BK < 4 ? 1 : S::BK / 4];
+      for (int u = 0; u < S::U; ++u) {
+        const __half2* kp = reinterpret_cast<const __half2*>(rec[u] + int4_layout(D, G).kp);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          lds_bytes<S::BK>(rec + (r * 8 + tile_token(g)) * (D / 2) + gi * (S::GS / 2) + q4 * S::BK, kw[r]);
-        float acc[2][NT][4];
+        for (int gi = 0; gi < G; ++gi) {
+          uint32_t kw[4][S::BK < 4 ? 1 : S::BK / 4];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+          for (int r = 0; r < 4; ++r)
+            lds_bytes<S::BK>(rec[u] + (r * 8 + tile_token(g)) * (D / 2) + gi * (S::GS / 2) + q4 * S::BK, kw[r]);
+          float acc[2][NT][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[mt][nt][c] = 0.f;
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int s = 0; s < S::GS / 16; ++s) {
-          const int ks = gi * (S::GS / 16) + s;
-          uint2 b[NT];
+              for (int c = 0; c < 4; ++c) acc[mt][nt][c] = 0.f;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) b[nt] = NT == 1 ? qf[NT == 1 ? ks : 0] : frag2[(ks * NT + nt) * 32];
+          for (int s = 0; s < S::GS / 16; ++s) {
+            const int ks = gi * (S::GS / 16) + s;
+            uint2 b[NT];
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
-            // codes of the step's two channel pairs, at bits 4..7 of each half
-            uint32_t a[4];
+            for (int nt = 0; nt < NT; ++nt) b[nt] = NT == 1 ? qf[NT == 1 ? ks : 0] : frag2[(ks * NT + nt) * 32];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              if constexpr (S::BK >= 4) {
-                const uint32_t w = kw[2 * mt + r][s / 2];
-                a[r] = (s & 1 ? w >> 4 : w << 4) & 0x00F000F0u;
-                a[2 + r] = (s & 1 ? w >> 8 : w) & 0x00F000F0u;
-              } else {
-                const uint32_t w = prmt(kw[2 * mt + r][0], 0u, 0x4140);
-                a[r] = (w << 4) & 0x00F000F0u;
+            for (int mt = 0; mt < 2; ++mt) {
+              // codes of the step's two channel pairs, at bits 4..7 of each half
+              uint32_t a[4];
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                uint32_t w;
+                if constexpr (S::BK >= 4) w = s & 1 ? kw[2 * mt + r][s / 2] >> 8 : kw[2 * mt + r][s / 2];
+                else w = prmt(kw[2 * mt + r][0], 0u, 0x4140);
+                a[r] = (w * 16u) & 0x00F000F0u;  // a product: the shifts' pipe is the busy one
                 a[2 + r] = w & 0x00F000F0u;
               }
-            }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_16816(acc[mt][nt], a[0], a[1], a[2], a[3], b[nt].x, b[nt].y);
+              for (int nt = 0; nt < NT; ++nt) mma_16816(acc[mt][nt], a[0], a[1], a[2], a[3], b[nt].x, b[nt].y);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float2 sz = __half22float2(kp[(r * 8 + tile_token(g)) * G + gi]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                float& v = x[u][r >> 1][nt][(r & 1) * 2 + c];
+                const float zq = gi == 0 ? sz.y * qs[nt][c][gi] : fmaf(sz.y, qs[nt][c][gi], v);
+                v = fmaf(acc[r >> 1][nt][(r & 1) * 2 + c], sz.x, zq);
+              }
           }
         }
+      }
+      const bool tail = tok0[S::U - 1] + kBlockTokens > see_min;
+      if (tail) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float2 sz = __half22float2(kp[(r * 8 + tile_token(g)) * G + gi]);
+        for (int u = 0; u < S::U; ++u)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float& v = x[r >> 1][nt][(r & 1) * 2 + c];
-              const float zq = gi == 0 ? sz.y * qs[nt][c][gi] : fmaf(sz.y, qs[nt][c][gi], v);
-              v = fmaf(acc[r >> 1][nt][(r & 1) * 2 + c], sz.x, zq);
+              const int see = s_see[nt * 8 + q4 * 2 + c] - tok0[u];
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (r * 8 + tile_token(g) >= see) x[u][r >> 1][nt][(r & 1) * 2 + c] = -INFINITY;
             }
-        }
-      }
-      const bool tail = tok0 + kBlockTokens > see_min;
-      if (tail) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int see = s_see[nt * 8 + q4 * 2 + c] - tok0;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (r * 8 + tile_token(g) >= see) x[r >> 1][nt][(r & 1) * 2 + c] = -INFINITY;
-          }
       }
       // ---- V scales and zeros of this thread's tokens
-      float vs[4][G], vz[4][G];
-      {
-        const __half2* vp = reinterpret_cast<const __half2*>(rec + int4_layout(D, G).vp);
+      float vs[S::U][4][G], vz[S::U][4][G];
+#pragma unroll
+      for (int u = 0; u < S::U; ++u) {
+        const __half2* vp = reinterpret_cast<const __half2*>(rec[u] + int4_layout(D, G).vp);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
           for (int gi = 0; gi < G; ++gi) {
             float2 sz = __half22float2(vp[(r * 8 + tile_token(g)) * G + gi]);
             // slots past the row's end hold anything: nothing of them may reach a sum
-            if (tail && tok0 + r * 8 + tile_token(g) >= len) sz = make_float2(0.f, 0.f);
-            vs[r][gi] = sz.x;
-            vz[r][gi] = fmaf(8.f, sz.x, sz.y);
+            if (tail && tok0[u] + r * 8 + tile_token(g) >= len) sz = make_float2(0.f, 0.f);
+            vs[u][r][gi] = sz.x;
+            vz[u][r][gi] = fmaf(8.f, sz.x, sz.y);
           }
       }
       // ---- running maximum and V unit move together, rarely
@@ -528,14 +570,20 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          top[nt][c] = fmaxf(fmaxf(x[0][nt][c], x[0][nt][2 + c]), fmaxf(x[1][nt][c], x[1][nt][2 + c]));
+          top[nt][c] = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < S::U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top[nt][c] = fmaxf(top[nt][c], x[u][r >> 1][nt][(r & 1) * 2 + c]);
           move |= top[nt][c] > lim[nt][c];
         }
       float vtop = 0.f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int u = 0; u < S::U; ++u)
 #pragma unroll
-        for (int gi = 0; gi < G; ++gi) vtop = fmaxf(vtop, fabsf(vs[r][gi]));
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int gi = 0; gi < G; ++gi) vtop = fmaxf(vtop, fabsf(vs[u][r][gi]));
       move |= vtop > vref;
       if (__any_sync(~0u, move)) {
 #pragma unroll
@@ -547,7 +595,6 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
           fv = vref > 0.f ? vref / ref : 1.f;
           vref = ref;
           vinv = 1.f / ref;
-          vunit = ref;
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -575,69 +622,89 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
       }
       // ---- weights
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int u = 0; u < S::U; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float& v = x[r >> 1][nt][(r & 1) * 2 + c];
-            v = fast_exp2(fmaf(v, cq[nt][c], -mc[nt][c]));
-            l[nt][c] += v;
+          for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int gi = 0; gi < G; ++gi) zs[nt][c][gi] = fmaf(v, vz[r][gi], zs[nt][c][gi]);
-          }
+            for (int c = 0; c < 2; ++c) {
+              float& v = x[u][r >> 1][nt][(r & 1) * 2 + c];
+              v = fast_exp2(fmaf(v, cq[nt][c], -mc[nt][c]));
+              l[nt][c] += v;
+#pragma unroll
+              for (int gi = 0; gi < G; ++gi) zs[nt][c][gi] = fmaf(v, vz[u][r][gi], zs[nt][c][gi]);
+            }
       // ---- values: channels are the MMA's rows, tokens its depth
 #pragma unroll
-      for (int gi = 0; gi < G; ++gi) {
-        uint32_t pb[4][NT], pl[LO ? 4 : 1][LO ? NT : 1];
+      for (int gi = 0; gi < G; ++gi)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float sn = vs[r][gi] * vinv;
+        for (int u = 0; u < S::U; ++u) {
+          uint32_t pb[4][NT], pl[LO ? 4 : 1][LO ? NT : 1];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float w0 = x[r >> 1][nt][(r & 1) * 2] * sn, w1 = x[r >> 1][nt][(r & 1) * 2 + 1] * sn;
-            const uint32_t hi = pack_h2(w0, w1);
-            pb[r][nt] = movmatrix_trans(hi);
-            if constexpr (LO) {
-              const float2 back = __half22float2(u32_as_h2(hi));
-              pl[r][nt] = movmatrix_trans(pack_h2(w0 - back.x, w1 - back.y));
-            }
-          }
-        }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          constexpr int NW = S::BV < 4 ? 1 : S::BV / 4;
-          uint32_t va[2][NW], vb[2][NW];  // the two tokens of each 8-token tile
-#pragma unroll
-          for (int T = 0; T < 2; ++T) {
-            const uint8_t* vr = rec + int4_layout(D, G).vc + ((2 * kk + T) * 8) * (D / 2) + gi * (S::GS / 2) + g * S::BV;
-            lds_bytes<S::BV>(vr + tile_token(2 * q4) * (D / 2), va[T]);
-            lds_bytes<S::BV>(vr + tile_token(2 * q4 + 1) * (D / 2), vb[T]);
-          }
-#pragma unroll
-          for (int b = 0; b < S::BV; ++b) {
-            // bytes b of both tokens, the first in the low half
-            const uint32_t y0 = prmt(va[0][b / 4], vb[0][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
-            const uint32_t y1 = prmt(va[1][b / 4], vb[1][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
+          for (int r = 0; r < 4; ++r) {
+            const float sn = vs[u][r][gi] * vinv;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const uint32_t a0 = low_code(y0), a1 = high_code(y0), a2 = low_code(y1), a3 = high_code(y1);
-              mma_16816(O[nt][gi * S::BV + b], a0, a1, a2, a3, pb[2 * kk][nt], pb[2 * kk + 1][nt]);
-              if constexpr (LO)
-                mma_16816(O[nt][gi * S::BV + b], a0, a1, a2, a3, pl[2 * kk][nt], pl[2 * kk + 1][nt]);
+              const float w0 = x[u][r >> 1][nt][(r & 1) * 2] * sn, w1 = x[u][r >> 1][nt][(r & 1) * 2 + 1] * sn;
+              const uint32_t hi = pack_h2(w0, w1);
+              pb[r][nt] = movmatrix_trans(hi);
+              if constexpr (LO) {
+                const float2 back = __half22float2(u32_as_h2(hi));
+                pl[r][nt] = movmatrix_trans(pack_h2(w0 - back.x, w1 - back.y));
+              }
+            }
+          }
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk) {
+            constexpr int NW = S::BV < 4 ? 1 : S::BV / 4;
+            uint32_t va[2][NW], vb[2][NW];  // the two tokens of each 8-token tile
+#pragma unroll
+            for (int T = 0; T < 2; ++T) {
+              const uint8_t* vr =
+                  rec[u] + int4_layout(D, G).vc + ((2 * kk + T) * 8) * (D / 2) + gi * (S::GS / 2) + g * S::BV;
+              lds_bytes<S::BV>(vr + tile_token(2 * q4) * (D / 2), va[T]);
+              lds_bytes<S::BV>(vr + tile_token(2 * q4 + 1) * (D / 2), vb[T]);
+            }
+            // two channels' bytes at a time: the two terms of a sum stand apart
+#pragma unroll
+            for (int b0 = 0; b0 < S::BV; b0 += 2) {
+              constexpr int BB = S::BV < 2 ? 1 : 2;
+              uint32_t a[BB][4];
+#pragma unroll
+              for (int b2 = 0; b2 < BB; ++b2) {
+                const int b = b0 + b2;
+                // bytes b of both tokens, the first in the low half
+                const uint32_t y0 = prmt(va[0][b / 4], vb[0][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
+                const uint32_t y1 = prmt(va[1][b / 4], vb[1][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
+                a[b2][0] = low_code(y0), a[b2][1] = high_code(y0), a[b2][2] = low_code(y1), a[b2][3] = high_code(y1);
+              }
+#pragma unroll
+              for (int term = 0; term < (LO ? 2 : 1); ++term)
+#pragma unroll
+                for (int b2 = 0; b2 < BB; ++b2)
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+                    mma_16816(O[nt][gi * S::BV + b0 + b2], a[b2][0], a[b2][1], a[b2][2], a[b2][3],
+                              term ? pl[LO ? 2 * kk : 0][LO ? nt : 0] : pb[2 * kk][nt],
+                              term ? pl[LO ? 2 * kk + 1 : 0][LO ? nt : 0] : pb[2 * kk + 1][nt]);
             }
           }
         }
-      }
-      // ---- the stage is free: the page STAGES ahead
+      // ---- the stages are free: the pages STAGES ahead
       __syncwarp();
-      const int next = k + S::STAGES;
-      if (next < mine) {
-        if ((next & 31) == 0) ids = page_ids(next);
-        const int p = __shfl_sync(~0u, ids, next & 31);
-        issue(p, stage);
+#pragma unroll
+      for (int u = 0; u < S::U; ++u) {
+        const int next = k + u + S::STAGES;
+        if (k + u < mine) {
+          if (next < mine) {
+            if ((next & 31) == 0) ids = page_ids(next);
+            const int p = __shfl_sync(~0u, ids, next & 31);
+            issue(p, stage);
+          }
+          if (++stage == S::STAGES) stage = 0, phase ^= 1;
+        }
       }
-      if (++stage == S::STAGES) stage = 0, phase ^= 1;
     }
 
     // ---- the warps' results meet
@@ -679,14 +746,13 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float2 v;  // even channel (high nibble), odd channel
-            v.x = f[nt][c] * fmaf(O[nt][j][2 + c], vunit, zs[nt][c][gi]);
-            v.y = f[nt][c] * fmaf(O[nt][j][c], vunit, zs[nt][c][gi]);
+            v.x = f[nt][c] * fmaf(O[nt][j][2 + c], vref, zs[nt][c][gi]);
+            v.y = f[nt][c] * fmaf(O[nt][j][c], vref, zs[nt][c][gi]);
             *reinterpret_cast<float2*>(merge + (warp * S::ROWS + nt * 8 + q4 * 2 + c) * S::PITCH + j * 16 + g * 2) = v;
           }
         }
     __syncthreads();
     const int valid = min(S::ROWS, P.M * rep - tile * S::ROWS);  // query rows of this tile
-    const bool whole = cta0 == cta1;
     constexpr int64_t STEP = static_cast<int64_t>(S::ROWS) * (D + 2);
     float* part = P.part + (static_cast<int64_t>(blockIdx.x) + unit) * STEP;
     for (int k = t; k < valid * (D / 2); k += kAttnThreads) {
@@ -703,15 +769,18 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
         v.x += o.x, v.y += o.y;
       }
       if (whole) {
-        store_pair<D, G>(P, i, h, rep, tile * S::ROWS + n, n_new, p, v, top, L);
+        store_pair<D, G>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, p, v, top, s_on[n] ? L : 0.f);
       } else {
         *reinterpret_cast<float2*>(part + n * (D + 2) + 2 * p) = v;
-        if (p == 0) *reinterpret_cast<float2*>(part + n * (D + 2) + D) = make_float2(top, L);
+        if (p == 0) *reinterpret_cast<float2*>(part + n * (D + 2) + D) = make_float2(top, s_on[n] ? L : 0.f);
       }
     }
-    if (!whole) {
+    if (whole) {
+      if (t == 0 && P.meta) P.meta[unit] = make_int2(0, 0);
+    } else {
+      const int cta0 = u_start / share, cta1 = (u_start + pages - 1) / share;
       if (P.meta) {
-        if (t == 0 && cta0 == static_cast<int>(blockIdx.x)) P.meta[unit] = make_int2(cta0, cta1);
+        if (t == 0 && page0 == 0) P.meta[unit] = make_int2(cta0, cta1);
       } else {
         // the last of the unit's CTAs to arrive merges their parts
         __threadfence();
@@ -723,8 +792,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
         __syncthreads();
         if (s_last) {
           __threadfence();
-          merge_parts<D, G, NT>(P, P.part + (static_cast<int64_t>(cta0) + unit) * STEP, cta1 - cta0 + 1, i, h, rep, tile,
-                                valid, n_new, reinterpret_cast<float*>(smem));
+          merge_parts<D, G, NT>(P, P.part + (static_cast<int64_t>(cta0) + unit) * STEP, cta1 - cta0 + 1, s_out, s_lse, valid,
+                                reinterpret_cast<float*>(smem));
         }
       }
     }
@@ -732,7 +801,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
     fence_proxy_async_shared();
     __syncthreads();
     pos += n_pages;
-    if (pos - e_start >= static_cast<int64_t>(pages) * H) ++e;
+    if (pos - e_start >= pages * H) ++e;
   }
 }
 
@@ -752,7 +821,6 @@ __global__ void __launch_bounds__(128) int4_combine_kernel(const Int4AttnParams 
   const int e = unit / H, h = unit % H, i = P.row0 + e / P.tiles;
   const int rr = e % P.tiles * ROWS + n;
   if (rr / rep >= P.M) return;
-  const Int4Row row = int4_row(P.c, P.rows, P.n_new, i, P.M, nullptr);
   const float* part = P.part + (static_cast<int64_t>(cta.x) + unit) * STEP + n * (D + 2);
   float top = -INFINITY;
   for (int s = t; s < segs; s += 128) top = fmaxf(top, part[s * STEP + D]);
@@ -795,7 +863,8 @@ __global__ void __launch_bounds__(128) int4_combine_kernel(const Int4AttnParams 
     acc.x += s_acc[(w - 1) * PAIRS + p].x;
     acc.y += s_acc[(w - 1) * PAIRS + p].y;
   }
-  store_pair<D, G>(P, i, h, rep, rr, row.n_new, p, acc, top, L);
+  const int m = rr / rep, hq = h * rep + rr % rep;
+  store_pair<D, G>(P, out_row(P, i, hq, m), P.lse ? P.lse + (i * P.Hq + hq) * P.M + m : nullptr, p, acc, top, L);
 }
 
 // ---------------------------------------------------------------- host
@@ -808,7 +877,6 @@ inline int attn_nt(int D, int rows) {
   return nt < most ? nt : most;
 }
 
-inline int attn_occ(int D, int nt) { return nt == 1 ? (D == 256 ? 2 : 4) : (nt == 2 ? (D == 256 ? 2 : 3) : 2); }
 
 template <int D, int G, int NT, bool LO>
 int attn_launch(const Int4AttnParams& p, cudaStream_t st) {
@@ -816,7 +884,7 @@ int attn_launch(const Int4AttnParams& p, cudaStream_t st) {
   const int entries = p.R * p.tiles;
   const int smem = S::smem(entries);
   if (!ensure_dynamic_smem<int4_attn_kernel<D, G, NT, LO>>(S::smem(kAttnEntries))) return AKV_ERR_LAUNCH;
-  const int grid = kSMs * S::OCC;
+  const int grid = kSMs * S::OCC * WAVES;
   int4_attn_kernel<D, G, NT, LO><<<grid, kAttnThreads, smem, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return AKV_ERR_LAUNCH;
   if (!p.meta) return AKV_OK;
