@@ -36,6 +36,7 @@ constexpr int kAttnFused = 1024;    // partial rows of a unit that its last CTA 
 #define OCC1 4
 #define OCC2 3
 #define WAVES 1
+#define AVMIN 4
 #endif
 constexpr float kLazyLog2 = 6.f;    // weights may reach 2^6 before the maximum moves
 
@@ -61,11 +62,20 @@ struct Int4AttnParams {
 // resident CTAs of an SM: what the registers of 128 threads leave
 constexpr int attn_occ(int D, int nt) { return nt == 1 ? (D == 256 ? 2 : OCC1) : (nt == 2 ? (D == 256 ? 2 : OCC2) : 2); }
 
-template <int D, int G, int NT>
+// A bf16 output leaves room to round each value of V to fp16 as it is unpacked,
+// scale and zero applied (AttnShape::AV); the weights are then the same for
+// every group.  It costs a second fp16 operation for each pair of codes and
+// saves per group and query tile what the weights cost: it pays from four
+// (group, tile) pairs on.
+constexpr bool attn_av(int G, int NT, bool LO) { return !LO && G * NT >= AVMIN; }
+
+template <int D, int G, int NT, bool LO>
 struct AttnShape {
   static constexpr int GS = D / G;              // channels of a group
   static constexpr int BK = GS / 8;             // K bytes of a thread per token and group
-  static constexpr int BV = GS / 16;            // V bytes of a thread per token and group
+  static constexpr bool AV = attn_av(G, NT, LO);
+  static constexpr int GV = AV ? 1 : G;         // groups the weights differ for
+  static constexpr int BV = D / GV / 16;        // V bytes of a thread per token and such group
   static constexpr int REC = int4_layout(D, G).bytes;
   static constexpr int ROWS = 8 * NT;           // query rows of a CTA
   static constexpr int U = UNROLL;              // pages of an iteration
@@ -128,6 +138,19 @@ AKV_DEV void lds_bytes(const uint8_t* p, uint32_t (&w)[BYTES < 4 ? 1 : BYTES / 4
     w[0] = *reinterpret_cast<const uint16_t*>(p);
   } else {
     w[0] = *p;
+  }
+}
+
+// the (scale, zero) pairs of a token
+template <int G>
+AKV_DEV void lds_pairs(const uint8_t* p, uint32_t (&w)[G]) {
+  if constexpr (G == 4) {
+    lds_u32x4(p, w);
+  } else if constexpr (G == 2) {
+    const uint2 v = lds_v2(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = lds_u32(p);
   }
 }
 
@@ -202,8 +225,8 @@ AKV_DEV void merge_parts(const Int4AttnParams& P, const float* part, int segs, c
 }
 
 template <int D, int G, int NT, bool LO>
-__global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_attn_kernel(const Int4AttnParams P) {
-  using S = AttnShape<D, G, NT>;
+__global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) int4_attn_kernel(const Int4AttnParams P) {
+  using S = AttnShape<D, G, NT, LO>;
   constexpr int KS = D / 16;  // MMA steps of q.K
   extern __shared__ __align__(128) uint8_t smem[];
   float* s_qs = reinterpret_cast<float*>(smem + S::OFF_QS);
@@ -404,7 +427,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
         constexpr int GL = 32 / G;  // lanes of a group
 #pragma unroll
         for (int o = 1; o < GL; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        if (lane % GL == 0) s_qs[n * G + lane / GL] = sum * 9.5367431640625e-7f;  // 2^-20, the codes' unit
+        if (lane % GL == 0) s_qs[lane / GL * S::ROWS + n] = sum * 9.5367431640625e-7f;  // 2^-20, the codes' unit
         if (lane == 0) {
           // log2 e * scale in units of the MMA result; never 0, so that -inf stays -inf
           s_cq[n] = fmaxf(ldexpf(fabsf(P.scale) * 1.4426950408889634f, 20 - ex), 1e-37f);
@@ -426,22 +449,26 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) qf[ks] = frag2[ks * 32];
     }
-    float qs[NT][2][G], cq[NT][2];
-    float mx[NT][2], mc[NT][2], lim[NT][2], l[NT][2], zs[NT][2][G];
+    // Per pair of queries (columns 2 q4, 2 q4 + 1), as packed fp32 pairs: group
+    // sums of q (in registers where they are few), exponent factors, minus the
+    // exponent of the maximum (0 before any token), sums of weights and of
+    // weights times zeros; and the score from which the maximum moves.
+    constexpr bool QS_REG = NT * G <= 2;
+    const uint64_t* s_qs2 = reinterpret_cast<const uint64_t*>(s_qs) + q4;
+    uint64_t qs[QS_REG ? NT : 1][QS_REG ? G : 1], cq[NT], nm[NT], l[NT], zs[NT][S::AV ? 1 : G];
+    float lim[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      cq[nt] = f2_make(s_cq[nt * 8 + q4 * 2], s_cq[nt * 8 + q4 * 2 + 1]);
+      nm[nt] = l[nt] = 0;
+      lim[nt][0] = lim[nt][1] = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int n = nt * 8 + q4 * 2 + c;
-        cq[nt][c] = s_cq[n];
-        mx[nt][c] = lim[nt][c] = -INFINITY;
-        mc[nt][c] = l[nt][c] = 0.f;
-#pragma unroll
-        for (int gi = 0; gi < G; ++gi) {
-          qs[nt][c][gi] = s_qs[n * G + gi];
-          zs[nt][c][gi] = 0.f;
-        }
+      for (int gi = 0; gi < G; ++gi) {
+        if constexpr (QS_REG) qs[nt][gi] = s_qs2[(gi * S::ROWS + nt * 8) / 2];
+        if constexpr (!S::AV) zs[nt][gi] = 0;
       }
+      if constexpr (S::AV) zs[nt][0] = 0;
+    }
     const int see_min = s_see[0];
     float O[NT][D / 16][4];
 #pragma unroll
@@ -479,11 +506,14 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
         tok0[u] = k + u < mine ? (page0 + warp + (k + u) * kAttnWarps) * kBlockTokens : INT32_MAX - 2 * kBlockTokens;
       }
 
-      // ---- scores: tokens are the MMA's rows, queries its columns
-      float x[S::U][2][NT][4];
+      // ---- scores: tokens are the MMA's rows, queries its columns; x holds the
+      // pairs of a token row (mt, half) as (2 q4, 2 q4 + 1)
+      uint64_t x[S::U][4][NT];
 #pragma unroll
       for (int u = 0; u < S::U; ++u) {
-        const __half2* kp = reinterpret_cast<const __half2*>(rec[u] + int4_layout(D, G).kp);
+        uint32_t kp[4][G];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) lds_pairs<G>(rec[u] + int4_layout(D, G).kp + (r * 8 + tile_token(g)) * G * 4, kp[r]);
 #pragma unroll
         for (int gi = 0; gi < G; ++gi) {
           uint32_t kw[4][S::BK < 4 ? 1 : S::BK / 4];
@@ -521,15 +551,15 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float2 sz = __half22float2(kp[(r * 8 + tile_token(g)) * G + gi]);
+            const float2 sz = __half22float2(u32_as_h2(kp[r][gi]));
+            const uint64_t s2 = f2_make(sz.x, sz.x), z2 = f2_make(sz.y, sz.y);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                float& v = x[u][r >> 1][nt][(r & 1) * 2 + c];
-                const float zq = gi == 0 ? sz.y * qs[nt][c][gi] : fmaf(sz.y, qs[nt][c][gi], v);
-                v = fmaf(acc[r >> 1][nt][(r & 1) * 2 + c], sz.x, zq);
-              }
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint64_t q2 = QS_REG ? qs[QS_REG ? nt : 0][QS_REG ? gi : 0] : s_qs2[(gi * S::ROWS + nt * 8) / 2];
+              const float* a = acc[r >> 1][nt] + (r & 1) * 2;
+              const uint64_t zq = gi == 0 ? f2_mul(z2, q2) : f2_fma(z2, q2, x[u][r][nt]);
+              x[u][r][nt] = f2_fma(f2_make(a[0], a[1]), s2, zq);
+            }
           }
         }
       }
@@ -538,82 +568,96 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
 #pragma unroll
         for (int u = 0; u < S::U; ++u)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            const int see0 = s_see[nt * 8 + q4 * 2] - tok0[u], see1 = s_see[nt * 8 + q4 * 2 + 1] - tok0[u];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int see = s_see[nt * 8 + q4 * 2 + c] - tok0[u];
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (r * 8 + tile_token(g) >= see) x[u][r >> 1][nt][(r & 1) * 2 + c] = -INFINITY;
+            for (int r = 0; r < 4; ++r) {
+              float2 v = f2_split(x[u][r][nt]);
+              if (r * 8 + tile_token(g) >= see0) v.x = -INFINITY;
+              if (r * 8 + tile_token(g) >= see1) v.y = -INFINITY;
+              x[u][r][nt] = f2_make(v.x, v.y);
             }
+          }
       }
-      // ---- V scales and zeros of this thread's tokens
-      float vs[S::U][4][G], vz[S::U][4][G];
+      // ---- V scales and zeros of this thread's tokens (slots past the row's end
+      // hold anything: nothing of them may reach a sum)
+      uint32_t vp[S::AV ? 1 : S::U][4][G];
+      if constexpr (!S::AV) {
 #pragma unroll
-      for (int u = 0; u < S::U; ++u) {
-        const __half2* vp = reinterpret_cast<const __half2*>(rec[u] + int4_layout(D, G).vp);
+        for (int u = 0; u < S::U; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+          for (int r = 0; r < 4; ++r) {
+            lds_pairs<G>(rec[u] + int4_layout(D, G).vp + (r * 8 + tile_token(g)) * G * 4, vp[u][r]);
 #pragma unroll
-          for (int gi = 0; gi < G; ++gi) {
-            float2 sz = __half22float2(vp[(r * 8 + tile_token(g)) * G + gi]);
-            // slots past the row's end hold anything: nothing of them may reach a sum
-            if (tail && tok0[u] + r * 8 + tile_token(g) >= len) sz = make_float2(0.f, 0.f);
-            vs[u][r][gi] = sz.x;
-            vz[u][r][gi] = fmaf(8.f, sz.x, sz.y);
+            for (int gi = 0; gi < G; ++gi)
+              if (tail && tok0[u] + r * 8 + tile_token(g) >= len) vp[u][r][gi] = 0u;
           }
       }
       // ---- running maximum and V unit move together, rarely
       bool move = false;
       float top[NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        top[nt][0] = top[nt][1] = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          top[nt][c] = -INFINITY;
+        for (int u = 0; u < S::U; ++u)
 #pragma unroll
-          for (int u = 0; u < S::U; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) top[nt][c] = fmaxf(top[nt][c], x[u][r >> 1][nt][(r & 1) * 2 + c]);
-          move |= top[nt][c] > lim[nt][c];
-        }
+          for (int r = 0; r < 4; ++r) {
+            const float2 v = f2_split(x[u][r][nt]);
+            top[nt][0] = fmaxf(top[nt][0], v.x);
+            top[nt][1] = fmaxf(top[nt][1], v.y);
+          }
+        move |= top[nt][0] > lim[nt][0];
+        move |= top[nt][1] > lim[nt][1];
+      }
       float vtop = 0.f;
+      if constexpr (!S::AV) {
+        __half2 vtop2 = u32_as_h2(0u);
 #pragma unroll
-      for (int u = 0; u < S::U; ++u)
+        for (int u = 0; u < S::U; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+          for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int gi = 0; gi < G; ++gi) vtop = fmaxf(vtop, fabsf(vs[u][r][gi]));
-      move |= vtop > vref;
+            for (int gi = 0; gi < G; ++gi) vtop2 = __hmax2(vtop2, __habs2(u32_as_h2(vp[u][r][gi])));
+        vtop = __low2float(vtop2);
+        move |= vtop > vref;
+      }
       if (__any_sync(~0u, move)) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(~0u, vtop, o));
         float fv = 1.f;
-        if (vtop > vref) {
-          // the power of two above vtop (scales are finite fp16 values)
-          const float ref = __uint_as_float((__float_as_uint(vtop) & 0x7F800000u) + 0x00800000u);
-          fv = vref > 0.f ? vref / ref : 1.f;
-          vref = ref;
-          vinv = 1.f / ref;
+        if constexpr (!S::AV) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(~0u, vtop, o));
+          if (vtop > vref) {
+            // the power of two above vtop (scales are finite fp16 values)
+            const float ref = __uint_as_float((__float_as_uint(vtop) & 0x7F800000u) + 0x00800000u);
+            fv = vref > 0.f ? vref / ref : 1.f;
+            vref = ref;
+            vinv = 1.f / ref;
+          }
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+          const float2 c2 = f2_split(cq[nt]);
+          float2 n2 = f2_split(nm[nt]);
           float f[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float m = top[nt][c];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-            m = fmaxf(m, mx[nt][c]);
-            const float y = m == -INFINITY ? 0.f : m * cq[nt][c];
-            f[c] = mx[nt][c] == -INFINITY ? 0.f : exp2f(mc[nt][c] - y);
-            mx[nt][c] = m;
-            mc[nt][c] = y;
-            lim[nt][c] = m + kLazyLog2 / cq[nt][c];
-            l[nt][c] *= f[c];
-#pragma unroll
-            for (int gi = 0; gi < G; ++gi) zs[nt][c][gi] *= f[c];
+            const float cqc = c ? c2.y : c2.x, old = -(c ? n2.y : n2.x);
+            const bool any = lim[nt][c] != -INFINITY;
+            float y = m == -INFINITY ? 0.f : m * cqc;
+            if (any) y = fmaxf(y, old);
+            f[c] = any ? exp2f(old - y) : 0.f;
+            if (any || m != -INFINITY) lim[nt][c] = (y + kLazyLog2) / cqc;
+            (c ? n2.y : n2.x) = -y;
           }
+          nm[nt] = f2_make(n2.x, n2.y);
+          const uint64_t f2 = f2_make(f[0], f[1]);
+          l[nt] = f2_mul(l[nt], f2);
+#pragma unroll
+          for (int gi = 0; gi < S::GV; ++gi) zs[nt][gi] = f2_mul(zs[nt][gi], f2);
 #pragma unroll
           for (int j = 0; j < D / 16; ++j)
 #pragma unroll
@@ -624,34 +668,45 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
 #pragma unroll
       for (int u = 0; u < S::U; ++u)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int r = 0; r < 4; ++r) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
+          for (int nt = 0; nt < NT; ++nt) {
+            const float2 v = f2_split(f2_fma(x[u][r][nt], cq[nt], nm[nt]));
+            x[u][r][nt] = f2_make(fast_exp2(v.x), fast_exp2(v.y));
+            l[nt] = f2_add(l[nt], x[u][r][nt]);
+          }
+          if constexpr (!S::AV) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float& v = x[u][r >> 1][nt][(r & 1) * 2 + c];
-              v = fast_exp2(fmaf(v, cq[nt][c], -mc[nt][c]));
-              l[nt][c] += v;
+            for (int gi = 0; gi < G; ++gi) {
+              const float2 sz = __half22float2(u32_as_h2(vp[u][r][gi]));
+              const float z8 = fmaf(8.f, sz.x, sz.y);
+              const uint64_t z2 = f2_make(z8, z8);
 #pragma unroll
-              for (int gi = 0; gi < G; ++gi) zs[nt][c][gi] = fmaf(v, vz[u][r][gi], zs[nt][c][gi]);
+              for (int nt = 0; nt < NT; ++nt) zs[nt][gi] = f2_fma(x[u][r][nt], z2, zs[nt][gi]);
             }
+          }
+        }
       // ---- values: channels are the MMA's rows, tokens its depth
 #pragma unroll
-      for (int gi = 0; gi < G; ++gi)
+      for (int gi = 0; gi < S::GV; ++gi)
 #pragma unroll
         for (int u = 0; u < S::U; ++u) {
           uint32_t pb[4][NT], pl[LO ? 4 : 1][LO ? NT : 1];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float sn = vs[u][r][gi] * vinv;
+            uint64_t sn2 = 0;
+            if constexpr (!S::AV) {
+              const float sn = __low2float(u32_as_h2(vp[u][r][gi])) * vinv;
+              sn2 = f2_make(sn, sn);
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const float w0 = x[u][r >> 1][nt][(r & 1) * 2] * sn, w1 = x[u][r >> 1][nt][(r & 1) * 2 + 1] * sn;
-              const uint32_t hi = pack_h2(w0, w1);
+              const float2 w = f2_split(S::AV ? x[u][r][nt] : f2_mul(x[u][r][nt], sn2));
+              const uint32_t hi = pack_h2(w.x, w.y);
               pb[r][nt] = movmatrix_trans(hi);
               if constexpr (LO) {
                 const float2 back = __half22float2(u32_as_h2(hi));
-                pl[r][nt] = movmatrix_trans(pack_h2(w0 - back.x, w1 - back.y));
+                pl[r][nt] = movmatrix_trans(pack_h2(w.x - back.x, w.y - back.y));
               }
             }
           }
@@ -659,13 +714,28 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
           for (int kk = 0; kk < 2; ++kk) {
             constexpr int NW = S::BV < 4 ? 1 : S::BV / 4;
             uint32_t va[2][NW], vb[2][NW];  // the two tokens of each 8-token tile
+            uint32_t vs2[2], vz2[2];        // AV: their scales, zeros + 8 scales
 #pragma unroll
             for (int T = 0; T < 2; ++T) {
-              const uint8_t* vr =
-                  rec[u] + int4_layout(D, G).vc + ((2 * kk + T) * 8) * (D / 2) + gi * (S::GS / 2) + g * S::BV;
-              lds_bytes<S::BV>(vr + tile_token(2 * q4) * (D / 2), va[T]);
-              lds_bytes<S::BV>(vr + tile_token(2 * q4 + 1) * (D / 2), vb[T]);
+              const int t0 = (2 * kk + T) * 8 + tile_token(2 * q4), t1 = (2 * kk + T) * 8 + tile_token(2 * q4 + 1);
+              const uint8_t* vr = rec[u] + int4_layout(D, G).vc + gi * (S::GS / 2) + g * S::BV;
+              lds_bytes<S::BV>(vr + t0 * (D / 2), va[T]);
+              lds_bytes<S::BV>(vr + t1 * (D / 2), vb[T]);
+              if constexpr (S::AV) {
+                const uint8_t* pr = rec[u] + int4_layout(D, G).vp + g * (D / 8) / S::GS * 4;
+                uint32_t w0 = lds_u32(pr + t0 * G * 4), w1 = lds_u32(pr + t1 * G * 4);
+                if (tail) {
+                  if (tok0[u] + t0 >= len) w0 = 0u;
+                  if (tok0[u] + t1 >= len) w1 = 0u;
+                }
+                vs2[T] = prmt(w0, w1, 0x5410);
+                vz2[T] = h2_as_u32(__hfma2(u32_as_h2(vs2[T]), u32_as_h2(0x48004800u), u32_as_h2(prmt(w0, w1, 0x7632))));
+              }
             }
+            auto value = [&](uint32_t c, int T) -> uint32_t {
+              if constexpr (S::AV) return h2_as_u32(__hfma2(u32_as_h2(c), u32_as_h2(vs2[T]), u32_as_h2(vz2[T])));
+              return c;
+            };
             // two channels' bytes at a time: the two terms of a sum stand apart
 #pragma unroll
             for (int b0 = 0; b0 < S::BV; b0 += 2) {
@@ -677,7 +747,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
                 // bytes b of both tokens, the first in the low half
                 const uint32_t y0 = prmt(va[0][b / 4], vb[0][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
                 const uint32_t y1 = prmt(va[1][b / 4], vb[1][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
-                a[b2][0] = low_code(y0), a[b2][1] = high_code(y0), a[b2][2] = low_code(y1), a[b2][3] = high_code(y1);
+                a[b2][0] = value(low_code(y0), 0), a[b2][1] = value(high_code(y0), 0);
+                a[b2][2] = value(low_code(y1), 1), a[b2][3] = value(high_code(y1), 1);
               }
 #pragma unroll
               for (int term = 0; term < (LO ? 2 : 1); ++term)
@@ -708,46 +779,60 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
     }
 
     // ---- the warps' results meet
+    float2 zf[NT][S::GV];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      float2 lf = f2_split(l[nt]), nf = f2_split(nm[nt]);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int gi = 0; gi < S::GV; ++gi) zf[nt][gi] = f2_split(zs[nt][gi]);
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          l[nt][c] += __shfl_xor_sync(~0u, l[nt][c], o);
+      for (int o = 4; o < 32; o <<= 1) {
+        lf.x += __shfl_xor_sync(~0u, lf.x, o);
+        lf.y += __shfl_xor_sync(~0u, lf.y, o);
+        if constexpr (!S::AV) {
 #pragma unroll
-          for (int gi = 0; gi < G; ++gi) zs[nt][c][gi] += __shfl_xor_sync(~0u, zs[nt][c][gi], o);
+          for (int gi = 0; gi < G; ++gi) {
+            zf[nt][gi].x += __shfl_xor_sync(~0u, zf[nt][gi].x, o);
+            zf[nt][gi].y += __shfl_xor_sync(~0u, zf[nt][gi].y, o);
+          }
         }
-        if (g == 0)
-          s_ml[warp * S::ROWS + nt * 8 + q4 * 2 + c] = make_float2(mx[nt][c] == -INFINITY ? -INFINITY : mc[nt][c], l[nt][c]);
       }
+      if (g == 0) {
+        float2* ml = s_ml + warp * S::ROWS + nt * 8 + q4 * 2;
+        ml[0] = make_float2(lim[nt][0] == -INFINITY ? -INFINITY : -nf.x, lf.x);
+        ml[1] = make_float2(lim[nt][1] == -INFINITY ? -INFINITY : -nf.y, lf.y);
+      }
+    }
     __syncthreads();  // every warp is done with its ring
     float* merge = reinterpret_cast<float*>(smem);
     float f[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      const float2 nf = f2_split(nm[nt]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int n = nt * 8 + q4 * 2 + c;
         float m = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kAttnWarps; ++w) m = fmaxf(m, s_ml[w * S::ROWS + n].x);
-        f[nt][c] = mx[nt][c] == -INFINITY ? 0.f : exp2f(mc[nt][c] - m);
+        f[nt][c] = lim[nt][c] == -INFINITY ? 0.f : exp2f(-(c ? nf.y : nf.x) - m);
       }
+    }
     // each warp's share, scaled to the common maximum; within a row the
     // channels stand in the accumulators' order, 16 (j, g, parity) at a time
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int gi = 0; gi < G; ++gi)
+      for (int gi = 0; gi < S::GV; ++gi)
 #pragma unroll
         for (int b = 0; b < S::BV; ++b) {
           const int j = gi * S::BV + b;
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float2 v;  // even channel (high nibble), odd channel
-            v.x = f[nt][c] * fmaf(O[nt][j][2 + c], vref, zs[nt][c][gi]);
-            v.y = f[nt][c] * fmaf(O[nt][j][c], vref, zs[nt][c][gi]);
+            const float z = S::AV ? 0.f : (c ? zf[nt][gi].y : zf[nt][gi].x), unit = S::AV ? 1.f : vref;
+            v.x = f[nt][c] * fmaf(O[nt][j][2 + c], unit, z);
+            v.y = f[nt][c] * fmaf(O[nt][j][c], unit, z);
             *reinterpret_cast<float2*>(merge + (warp * S::ROWS + nt * 8 + q4 * 2 + c) * S::PITCH + j * 16 + g * 2) = v;
           }
         }
@@ -769,7 +854,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
         v.x += o.x, v.y += o.y;
       }
       if (whole) {
-        store_pair<D, G>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, p, v, top, s_on[n] ? L : 0.f);
+        store_pair<D, S::GV>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, p, v, top, s_on[n] ? L : 0.f);
       } else {
         *reinterpret_cast<float2*>(part + n * (D + 2) + 2 * p) = v;
         if (p == 0) *reinterpret_cast<float2*>(part + n * (D + 2) + D) = make_float2(top, s_on[n] ? L : 0.f);
@@ -792,7 +877,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT>::OCC) int4_a
         __syncthreads();
         if (s_last) {
           __threadfence();
-          merge_parts<D, G, NT>(P, P.part + (static_cast<int64_t>(cta0) + unit) * STEP, cta1 - cta0 + 1, s_out, s_lse, valid,
+          merge_parts<D, S::GV, NT>(P, P.part + (static_cast<int64_t>(cta0) + unit) * STEP, cta1 - cta0 + 1, s_out, s_lse, valid,
                                 reinterpret_cast<float*>(smem));
         }
       }
@@ -880,7 +965,7 @@ inline int attn_nt(int D, int rows) {
 
 template <int D, int G, int NT, bool LO>
 int attn_launch(const Int4AttnParams& p, cudaStream_t st) {
-  using S = AttnShape<D, G, NT>;
+  using S = AttnShape<D, G, NT, LO>;
   const int entries = p.R * p.tiles;
   const int smem = S::smem(entries);
   if (!ensure_dynamic_smem<int4_attn_kernel<D, G, NT, LO>>(S::smem(kAttnEntries))) return AKV_ERR_LAUNCH;
@@ -898,7 +983,7 @@ int attn_launch(const Int4AttnParams& p, cudaStream_t st) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, int4_combine_kernel<D, G, NT>, p) == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, int4_combine_kernel<D, S::GV, NT>, p) == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH;
 }
 
 template <int D, int G, int NT>

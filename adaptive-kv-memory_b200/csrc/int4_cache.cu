@@ -85,12 +85,6 @@ AKV_DEV float recip(float s) {
   return __fmaf_rn(__fmaf_rn(-s, r, 1.f), r, r);
 }
 
-AKV_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 template <bool BF>
 AKV_DEV uint32_t min2(uint32_t a, uint32_t b) {
   uint32_t r;
