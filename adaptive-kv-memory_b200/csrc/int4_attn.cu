@@ -30,7 +30,7 @@ Plan attn_plan(int R, int M, int Hq, int kv_heads, int D, int max_blocks) {
   p.meta = (units * sizeof(int2) + 15) / 16 * 16;
   // a CTA and a unit meet at most once, and along the list of pages their
   // numbers' sum only grows: it is the slot of the partial result
-  p.part = (units + kSMs * attn_occ(D, p.nt) * WAVES) * 8 * p.nt * (D + 2) * sizeof(float);
+  p.part = (units + kSMs * attn_occ(D, p.nt)) * 8 * p.nt * (D + 2) * sizeof(float);
   return p;
 }
 

@@ -28,16 +28,8 @@ namespace akv {
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kAttnEntries = 1024;  // (row, row tile) pairs of one launch
-constexpr int kAttnMinPages = 4;    // pages of a CTA's share, at least (one per warp)
+constexpr int kAttnMinPages = 8;    // pages of a CTA's share, at least (two per warp) where a unit has them
 constexpr int kAttnFused = 1024;    // partial rows of a unit that its last CTA merges by itself
-#ifndef UNROLL
-#define UNROLL 1
-#define STG (NT > 1 || G == 1 ? 3 : 2)
-#define OCC1 4
-#define OCC2 3
-#define WAVES 1
-#define AVMIN 4
-#endif
 constexpr float kLazyLog2 = 6.f;    // weights may reach 2^6 before the maximum moves
 
 struct Int4AttnParams {
@@ -60,16 +52,21 @@ struct Int4AttnParams {
 };
 
 // resident CTAs of an SM: what the registers of 128 threads leave
-constexpr int attn_occ(int D, int nt) { return nt == 1 ? (D == 256 ? 2 : OCC1) : (nt == 2 ? (D == 256 ? 2 : OCC2) : 2); }
+constexpr int attn_occ(int D, int nt) { return D == 256 ? 2 : (nt == 1 ? 4 : 3); }
 
+// Terms of a weight in P.V (LO): 0 one fp16 term; 1 two, the second the first's
+// error, in an MMA of its own; 2 two, the second in columns 4..7, where the
+// queries of columns 0..3 stand once more (at most four query rows: a grouped
+// decode step's usual count leaves those columns free).
+//
 // A bf16 output leaves room to round each value of V to fp16 as it is unpacked,
 // scale and zero applied (AttnShape::AV); the weights are then the same for
 // every group.  It costs a second fp16 operation for each pair of codes and
 // saves per group and query tile what the weights cost: it pays from four
 // (group, tile) pairs on.
-constexpr bool attn_av(int G, int NT, bool LO) { return !LO && G * NT >= AVMIN; }
+constexpr bool attn_av(int G, int NT, int LO) { return !LO && G * NT >= 4; }
 
-template <int D, int G, int NT, bool LO>
+template <int D, int G, int NT, int LO>
 struct AttnShape {
   static constexpr int GS = D / G;              // channels of a group
   static constexpr int BK = GS / 8;             // K bytes of a thread per token and group
@@ -78,8 +75,7 @@ struct AttnShape {
   static constexpr int BV = D / GV / 16;        // V bytes of a thread per token and such group
   static constexpr int REC = int4_layout(D, G).bytes;
   static constexpr int ROWS = 8 * NT;           // query rows of a CTA
-  static constexpr int U = UNROLL;              // pages of an iteration
-  static constexpr int STAGES = D == 64 ? 4 : (D == 128 ? STG : 2);
+  static constexpr int STAGES = D == 64 ? 4 : (D == 128 && (NT > 1 || G == 1) ? 3 : 2);
   static constexpr int RING = kAttnWarps * STAGES * REC;
   static constexpr int PITCH = D + 4;
   static constexpr int MERGE = kAttnWarps * ROWS * PITCH * 4;
@@ -141,6 +137,12 @@ AKV_DEV void lds_bytes(const uint8_t* p, uint32_t (&w)[BYTES < 4 ? 1 : BYTES / 4
   }
 }
 
+// the query row that stands in column n of a tile
+template <int LO>
+AKV_DEV int tile_row(int n) {
+  return LO == 2 ? n & 3 : n;
+}
+
 // the (scale, zero) pairs of a token
 template <int G>
 AKV_DEV void lds_pairs(const uint8_t* p, uint32_t (&w)[G]) {
@@ -195,11 +197,14 @@ AKV_DEV void merge_parts(const Int4AttnParams& P, const float* part, int segs, c
   for (int n = warp; n < valid; n += kAttnWarps) {
     const float* ml = part + n * (D + 2) + D;
     float top = -INFINITY, L = 0.f;
-    for (int s = lane; s < segs; s += 32) top = fmaxf(top, __ldcg(ml + s * STEP));
+    const float2 none = make_float2(-INFINITY, 0.f);
+    const float2 first = lane < segs ? __ldcg(reinterpret_cast<const float2*>(ml + lane * STEP)) : none;
+    top = first.x;
+    for (int s = lane + 32; s < segs; s += 32) top = fmaxf(top, __ldcg(ml + s * STEP));
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
     for (int s = lane; s < segs; s += 32) {
-      const float2 yl = __ldcg(reinterpret_cast<const float2*>(ml + s * STEP));
+      const float2 yl = s < 32 ? first : __ldcg(reinterpret_cast<const float2*>(ml + s * STEP));
       const float x = yl.x == -INFINITY ? 0.f : exp2f(yl.x - top);
       w[n * segs + s] = x;
       L = fmaf(x, yl.y, L);
@@ -209,22 +214,37 @@ AKV_DEV void merge_parts(const Int4AttnParams& P, const float* part, int segs, c
     if (lane == 0) s_tl[n] = make_float2(top, L);
   }
   __syncthreads();
-  for (int k = t; k < valid * (D / 2); k += kAttnThreads) {
-    const int n = k / (D / 2), p = k % (D / 2);
-    const float* at = part + n * (D + 2) + 2 * p;
-    float2 acc = make_float2(0.f, 0.f);
-#pragma unroll 8
-    for (int s = 0; s < segs; ++s) {
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(at + s * STEP));
-      const float x = w[n * segs + s];
-      acc.x = fmaf(x, v.x, acc.x);
-      acc.y = fmaf(x, v.y, acc.y);
+  constexpr int T = 4;  // output pairs of a thread at a time
+  for (int k0 = t; k0 < valid * (D / 2); k0 += T * kAttnThreads) {
+    const float* at[T];
+    const float* wn[T];
+    float2 acc[T];
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      const int k = min(k0 + j * kAttnThreads, valid * (D / 2) - 1);
+      at[j] = part + k / (D / 2) * (D + 2) + 2 * (k % (D / 2));
+      wn[j] = w + k / (D / 2) * segs;
+      acc[j] = make_float2(0.f, 0.f);
     }
-    store_pair<D, G>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, p, acc, s_tl[n].x, s_tl[n].y);
+#pragma unroll 8
+    for (int s = 0; s < segs; ++s)
+#pragma unroll
+      for (int j = 0; j < T; ++j) {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(at[j] + s * STEP));
+        acc[j].x = fmaf(wn[j][s], v.x, acc[j].x);
+        acc[j].y = fmaf(wn[j][s], v.y, acc[j].y);
+      }
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      const int k = k0 + j * kAttnThreads;
+      if (k >= valid * (D / 2)) break;
+      const int n = k / (D / 2);
+      store_pair<D, G>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, k % (D / 2), acc[j], s_tl[n].x, s_tl[n].y);
+    }
   }
 }
 
-template <int D, int G, int NT, bool LO>
+template <int D, int G, int NT, int LO>
 __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) int4_attn_kernel(const Int4AttnParams P) {
   using S = AttnShape<D, G, NT, LO>;
   constexpr int KS = D / 16;  // MMA steps of q.K
@@ -384,7 +404,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
       uint16_t raw[RW][PER];
 #pragma unroll
       for (int k2 = 0; k2 < RW; ++k2) {
-        const int rr = tile * S::ROWS + k2 * kAttnWarps + warp, m = rr / rep;
+        const int rr = tile * S::ROWS + tile_row<LO>(k2 * kAttnWarps + warp), m = rr / rep;
         const uint16_t* src = P.q + i * P.q_sr + (h * rep + rr % rep) * P.q_sh + m * P.q_sm + lane * PER;
 #pragma unroll
         for (int k = 0; k < PER; ++k) raw[k2][k] = m < n_new ? src[k] : 0;
@@ -392,7 +412,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
 #pragma unroll
       for (int k2 = 0; k2 < RW; ++k2) {
         const int n = k2 * kAttnWarps + warp;
-        const int m = (tile * S::ROWS + n) / rep;
+        const int nr = tile_row<LO>(n), m = (tile * S::ROWS + nr) / rep;
         float x[PER];
         float top = 0.f;
 #pragma unroll
@@ -434,7 +454,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
           s_see[n] = len - n_new + (m < n_new ? m : n_new - 1) + 1;
           s_on[n] = m < n_new;
           if (m < P.M) {
-            const int hq = h * rep + (tile * S::ROWS + n) - m * rep;
+            const int hq = h * rep + (tile * S::ROWS + nr) - m * rep;
             s_out[n] = out_row(P, i, hq, m);
             s_lse[n] = (i * P.Hq + hq) * P.M + m;
           }
@@ -479,119 +499,99 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
         for (int k = 0; k < 4; ++k) O[nt][j][k] = 0.f;
     float vref = 0.f, vinv = 0.f;  // power of two above the V scales seen so far, its inverse
 
-    for (int k = 0; k < mine; k += S::U) {
-      // a copy that never comes: take no more, but see the ones in flight land
-      bool ok = alive;
-#pragma unroll
-      for (int u = 0; u < S::U; ++u) {
-        const uint32_t st = stage + u;
-        if (ok && k + u < mine)
-          ok = __all_sync(~0u, mbar_wait(bars + st % S::STAGES, st >= S::STAGES ? phase ^ 1 : phase, P.status));
-      }
-      if (!ok) {
+    for (int k = 0; k < mine; ++k) {
+      if (!alive || !__all_sync(~0u, mbar_wait(bars + stage, phase, P.status))) {
+        // a copy never came: take no more, but see the ones in flight land
         if (alive)
-          for (int r = 0; r < S::STAGES && k + r < mine; ++r) {
+          for (int r = 1; r < S::STAGES && k + r < mine; ++r) {
             const uint32_t st = stage + r;
             mbar_wait(bars + st % S::STAGES, st >= S::STAGES ? phase ^ 1 : phase, P.status);
           }
         alive = false;
         break;
       }
-      const uint8_t* rec[S::U];
-      int tok0[S::U];
-#pragma unroll
-      for (int u = 0; u < S::U; ++u) {
-        rec[u] = ring + (stage + u) % S::STAGES * S::REC;
-        // an iteration's page that does not exist counts as one past every row's end
-        tok0[u] = k + u < mine ? (page0 + warp + (k + u) * kAttnWarps) * kBlockTokens : INT32_MAX - 2 * kBlockTokens;
-      }
+      const uint8_t* rec = ring + stage * S::REC;
+      const int tok0 = (page0 + warp + k * kAttnWarps) * kBlockTokens;
 
       // ---- scores: tokens are the MMA's rows, queries its columns; x holds the
       // pairs of a token row (mt, half) as (2 q4, 2 q4 + 1)
-      uint64_t x[S::U][4][NT];
+      uint64_t x[4][NT];
+      uint32_t kp[4][G];
 #pragma unroll
-      for (int u = 0; u < S::U; ++u) {
-        uint32_t kp[4][G];
+      for (int r = 0; r < 4; ++r) lds_pairs<G>(rec + int4_layout(D, G).kp + (r * 8 + tile_token(g)) * G * 4, kp[r]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) lds_pairs<G>(rec[u] + int4_layout(D, G).kp + (r * 8 + tile_token(g)) * G * 4, kp[r]);
+      for (int gi = 0; gi < G; ++gi) {
+        uint32_t kw[4][S::BK < 4 ? 1 : S::BK / 4];
 #pragma unroll
-        for (int gi = 0; gi < G; ++gi) {
-          uint32_t kw[4][S::BK < 4 ? 1 : S::BK / 4];
+        for (int r = 0; r < 4; ++r)
+          lds_bytes<S::BK>(rec + (r * 8 + tile_token(g)) * (D / 2) + gi * (S::GS / 2) + q4 * S::BK, kw[r]);
+        float acc[2][NT][4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            lds_bytes<S::BK>(rec[u] + (r * 8 + tile_token(g)) * (D / 2) + gi * (S::GS / 2) + q4 * S::BK, kw[r]);
-          float acc[2][NT][4];
+        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int c = 0; c < 4; ++c) acc[mt][nt][c] = 0.f;
 #pragma unroll
-              for (int c = 0; c < 4; ++c) acc[mt][nt][c] = 0.f;
+        for (int s = 0; s < S::GS / 16; ++s) {
+          const int ks = gi * (S::GS / 16) + s;
+          uint2 b[NT];
 #pragma unroll
-          for (int s = 0; s < S::GS / 16; ++s) {
-            const int ks = gi * (S::GS / 16) + s;
-            uint2 b[NT];
+          for (int nt = 0; nt < NT; ++nt) b[nt] = NT == 1 ? qf[NT == 1 ? ks : 0] : frag2[(ks * NT + nt) * 32];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) b[nt] = NT == 1 ? qf[NT == 1 ? ks : 0] : frag2[(ks * NT + nt) * 32];
+          for (int mt = 0; mt < 2; ++mt) {
+            // codes of the step's two channel pairs, at bits 4..7 of each half
+            uint32_t a[4];
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-              // codes of the step's two channel pairs, at bits 4..7 of each half
-              uint32_t a[4];
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                uint32_t w;
-                if constexpr (S::BK >= 4) w = s & 1 ? kw[2 * mt + r][s / 2] >> 8 : kw[2 * mt + r][s / 2];
-                else w = prmt(kw[2 * mt + r][0], 0u, 0x4140);
-                a[r] = (w * 16u) & 0x00F000F0u;  // a product: the shifts' pipe is the busy one
-                a[2 + r] = w & 0x00F000F0u;
-              }
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma_16816(acc[mt][nt], a[0], a[1], a[2], a[3], b[nt].x, b[nt].y);
+            for (int r = 0; r < 2; ++r) {
+              uint32_t w;
+              if constexpr (S::BK >= 4) w = s & 1 ? kw[2 * mt + r][s / 2] >> 8 : kw[2 * mt + r][s / 2];
+              else w = prmt(kw[2 * mt + r][0], 0u, 0x4140);
+              a[r] = (w * 16u) & 0x00F000F0u;  // a product: the shifts' pipe is the busy one
+              a[2 + r] = w & 0x00F000F0u;
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816(acc[mt][nt], a[0], a[1], a[2], a[3], b[nt].x, b[nt].y);
           }
+        }
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float2 sz = __half22float2(u32_as_h2(kp[r][gi]));
-            const uint64_t s2 = f2_make(sz.x, sz.x), z2 = f2_make(sz.y, sz.y);
+        for (int r = 0; r < 4; ++r) {
+          const float2 sz = __half22float2(u32_as_h2(kp[r][gi]));
+          const uint64_t s2 = f2_make(sz.x, sz.x), z2 = f2_make(sz.y, sz.y);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const uint64_t q2 = QS_REG ? qs[QS_REG ? nt : 0][QS_REG ? gi : 0] : s_qs2[(gi * S::ROWS + nt * 8) / 2];
-              const float* a = acc[r >> 1][nt] + (r & 1) * 2;
-              const uint64_t zq = gi == 0 ? f2_mul(z2, q2) : f2_fma(z2, q2, x[u][r][nt]);
-              x[u][r][nt] = f2_fma(f2_make(a[0], a[1]), s2, zq);
-            }
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint64_t q2 = QS_REG ? qs[QS_REG ? nt : 0][QS_REG ? gi : 0] : s_qs2[(gi * S::ROWS + nt * 8) / 2];
+            const float* a = acc[r >> 1][nt] + (r & 1) * 2;
+            const uint64_t zq = gi == 0 ? f2_mul(z2, q2) : f2_fma(z2, q2, x[r][nt]);
+            x[r][nt] = f2_fma(f2_make(a[0], a[1]), s2, zq);
           }
         }
       }
-      const bool tail = tok0[S::U - 1] + kBlockTokens > see_min;
+      const bool tail = tok0 + kBlockTokens > see_min;
       if (tail) {
 #pragma unroll
-        for (int u = 0; u < S::U; ++u)
+        for (int nt = 0; nt < NT; ++nt) {
+          const int see0 = s_see[nt * 8 + q4 * 2] - tok0, see1 = s_see[nt * 8 + q4 * 2 + 1] - tok0;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const int see0 = s_see[nt * 8 + q4 * 2] - tok0[u], see1 = s_see[nt * 8 + q4 * 2 + 1] - tok0[u];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              float2 v = f2_split(x[u][r][nt]);
-              if (r * 8 + tile_token(g) >= see0) v.x = -INFINITY;
-              if (r * 8 + tile_token(g) >= see1) v.y = -INFINITY;
-              x[u][r][nt] = f2_make(v.x, v.y);
-            }
+          for (int r = 0; r < 4; ++r) {
+            float2 v = f2_split(x[r][nt]);
+            if (r * 8 + tile_token(g) >= see0) v.x = -INFINITY;
+            if (r * 8 + tile_token(g) >= see1) v.y = -INFINITY;
+            x[r][nt] = f2_make(v.x, v.y);
           }
+        }
       }
       // ---- V scales and zeros of this thread's tokens (slots past the row's end
       // hold anything: nothing of them may reach a sum)
-      uint32_t vp[S::AV ? 1 : S::U][4][G];
+      uint32_t vp[4][G];
       if constexpr (!S::AV) {
 #pragma unroll
-        for (int u = 0; u < S::U; ++u)
+        for (int r = 0; r < 4; ++r) {
+          lds_pairs<G>(rec + int4_layout(D, G).vp + (r * 8 + tile_token(g)) * G * 4, vp[r]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            lds_pairs<G>(rec[u] + int4_layout(D, G).vp + (r * 8 + tile_token(g)) * G * 4, vp[u][r]);
-#pragma unroll
-            for (int gi = 0; gi < G; ++gi)
-              if (tail && tok0[u] + r * 8 + tile_token(g) >= len) vp[u][r][gi] = 0u;
-          }
+          for (int gi = 0; gi < G; ++gi)
+            if (tail && tok0 + r * 8 + tile_token(g) >= len) vp[r][gi] = 0u;
+        }
       }
       // ---- running maximum and V unit move together, rarely
       bool move = false;
@@ -600,13 +600,11 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
       for (int nt = 0; nt < NT; ++nt) {
         top[nt][0] = top[nt][1] = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < S::U; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float2 v = f2_split(x[u][r][nt]);
-            top[nt][0] = fmaxf(top[nt][0], v.x);
-            top[nt][1] = fmaxf(top[nt][1], v.y);
-          }
+        for (int r = 0; r < 4; ++r) {
+          const float2 v = f2_split(x[r][nt]);
+          top[nt][0] = fmaxf(top[nt][0], v.x);
+          top[nt][1] = fmaxf(top[nt][1], v.y);
+        }
         move |= top[nt][0] > lim[nt][0];
         move |= top[nt][1] > lim[nt][1];
       }
@@ -614,11 +612,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
       if constexpr (!S::AV) {
         __half2 vtop2 = u32_as_h2(0u);
 #pragma unroll
-        for (int u = 0; u < S::U; ++u)
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int gi = 0; gi < G; ++gi) vtop2 = __hmax2(vtop2, __habs2(u32_as_h2(vp[u][r][gi])));
+          for (int gi = 0; gi < G; ++gi) vtop2 = __hmax2(vtop2, __habs2(u32_as_h2(vp[r][gi])));
         vtop = __low2float(vtop2);
         move |= vtop > vref;
       }
@@ -666,116 +662,109 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
       }
       // ---- weights
 #pragma unroll
-      for (int u = 0; u < S::U; ++u)
+      for (int r = 0; r < 4; ++r) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float2 v = f2_split(f2_fma(x[u][r][nt], cq[nt], nm[nt]));
-            x[u][r][nt] = f2_make(fast_exp2(v.x), fast_exp2(v.y));
-            l[nt] = f2_add(l[nt], x[u][r][nt]);
-          }
-          if constexpr (!S::AV) {
-#pragma unroll
-            for (int gi = 0; gi < G; ++gi) {
-              const float2 sz = __half22float2(u32_as_h2(vp[u][r][gi]));
-              const float z8 = fmaf(8.f, sz.x, sz.y);
-              const uint64_t z2 = f2_make(z8, z8);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) zs[nt][gi] = f2_fma(x[u][r][nt], z2, zs[nt][gi]);
-            }
-          }
+        for (int nt = 0; nt < NT; ++nt) {
+          const float2 v = f2_split(f2_fma(x[r][nt], cq[nt], nm[nt]));
+          x[r][nt] = f2_make(fast_exp2(v.x), fast_exp2(v.y));
+          l[nt] = f2_add(l[nt], x[r][nt]);
         }
-      // ---- values: channels are the MMA's rows, tokens its depth
+        if constexpr (!S::AV) {
 #pragma unroll
-      for (int gi = 0; gi < S::GV; ++gi)
+          for (int gi = 0; gi < G; ++gi) {
+            const float2 sz = __half22float2(u32_as_h2(vp[r][gi]));
+            const float z8 = fmaf(8.f, sz.x, sz.y);
+            const uint64_t z2 = f2_make(z8, z8);
 #pragma unroll
-        for (int u = 0; u < S::U; ++u) {
-          uint32_t pb[4][NT], pl[LO ? 4 : 1][LO ? NT : 1];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            uint64_t sn2 = 0;
-            if constexpr (!S::AV) {
-              const float sn = __low2float(u32_as_h2(vp[u][r][gi])) * vinv;
-              sn2 = f2_make(sn, sn);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const float2 w = f2_split(S::AV ? x[u][r][nt] : f2_mul(x[u][r][nt], sn2));
-              const uint32_t hi = pack_h2(w.x, w.y);
-              pb[r][nt] = movmatrix_trans(hi);
-              if constexpr (LO) {
-                const float2 back = __half22float2(u32_as_h2(hi));
-                pl[r][nt] = movmatrix_trans(pack_h2(w.x - back.x, w.y - back.y));
-              }
-            }
+            for (int nt = 0; nt < NT; ++nt) zs[nt][gi] = f2_fma(x[r][nt], z2, zs[nt][gi]);
           }
-#pragma unroll
-          for (int kk = 0; kk < 2; ++kk) {
-            constexpr int NW = S::BV < 4 ? 1 : S::BV / 4;
-            uint32_t va[2][NW], vb[2][NW];  // the two tokens of each 8-token tile
-            uint32_t vs2[2], vz2[2];        // AV: their scales, zeros + 8 scales
-#pragma unroll
-            for (int T = 0; T < 2; ++T) {
-              const int t0 = (2 * kk + T) * 8 + tile_token(2 * q4), t1 = (2 * kk + T) * 8 + tile_token(2 * q4 + 1);
-              const uint8_t* vr = rec[u] + int4_layout(D, G).vc + gi * (S::GS / 2) + g * S::BV;
-              lds_bytes<S::BV>(vr + t0 * (D / 2), va[T]);
-              lds_bytes<S::BV>(vr + t1 * (D / 2), vb[T]);
-              if constexpr (S::AV) {
-                const uint8_t* pr = rec[u] + int4_layout(D, G).vp + g * (D / 8) / S::GS * 4;
-                uint32_t w0 = lds_u32(pr + t0 * G * 4), w1 = lds_u32(pr + t1 * G * 4);
-                if (tail) {
-                  if (tok0[u] + t0 >= len) w0 = 0u;
-                  if (tok0[u] + t1 >= len) w1 = 0u;
-                }
-                vs2[T] = prmt(w0, w1, 0x5410);
-                vz2[T] = h2_as_u32(__hfma2(u32_as_h2(vs2[T]), u32_as_h2(0x48004800u), u32_as_h2(prmt(w0, w1, 0x7632))));
-              }
-            }
-            auto value = [&](uint32_t c, int T) -> uint32_t {
-              if constexpr (S::AV) return h2_as_u32(__hfma2(u32_as_h2(c), u32_as_h2(vs2[T]), u32_as_h2(vz2[T])));
-              return c;
-            };
-            // two channels' bytes at a time: the two terms of a sum stand apart
-#pragma unroll
-            for (int b0 = 0; b0 < S::BV; b0 += 2) {
-              constexpr int BB = S::BV < 2 ? 1 : 2;
-              uint32_t a[BB][4];
-#pragma unroll
-              for (int b2 = 0; b2 < BB; ++b2) {
-                const int b = b0 + b2;
-                // bytes b of both tokens, the first in the low half
-                const uint32_t y0 = prmt(va[0][b / 4], vb[0][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
-                const uint32_t y1 = prmt(va[1][b / 4], vb[1][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
-                a[b2][0] = value(low_code(y0), 0), a[b2][1] = value(high_code(y0), 0);
-                a[b2][2] = value(low_code(y1), 1), a[b2][3] = value(high_code(y1), 1);
-              }
-#pragma unroll
-              for (int term = 0; term < (LO ? 2 : 1); ++term)
-#pragma unroll
-                for (int b2 = 0; b2 < BB; ++b2)
-#pragma unroll
-                  for (int nt = 0; nt < NT; ++nt)
-                    mma_16816(O[nt][gi * S::BV + b0 + b2], a[b2][0], a[b2][1], a[b2][2], a[b2][3],
-                              term ? pl[LO ? 2 * kk : 0][LO ? nt : 0] : pb[2 * kk][nt],
-                              term ? pl[LO ? 2 * kk + 1 : 0][LO ? nt : 0] : pb[2 * kk + 1][nt]);
-            }
-          }
-        }
-      // ---- the stages are free: the pages STAGES ahead
-      __syncwarp();
-#pragma unroll
-      for (int u = 0; u < S::U; ++u) {
-        const int next = k + u + S::STAGES;
-        if (k + u < mine) {
-          if (next < mine) {
-            if ((next & 31) == 0) ids = page_ids(next);
-            const int p = __shfl_sync(~0u, ids, next & 31);
-            issue(p, stage);
-          }
-          if (++stage == S::STAGES) stage = 0, phase ^= 1;
         }
       }
+      // ---- values: channels are the MMA's rows, tokens its depth
+#pragma unroll
+      for (int gi = 0; gi < S::GV; ++gi) {
+        uint32_t pb[4][NT], pl[LO == 1 ? 4 : 1][LO == 1 ? NT : 1];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          uint64_t sn2 = 0;
+          if constexpr (!S::AV) {
+            const float sn = __low2float(u32_as_h2(vp[r][gi])) * vinv;
+            sn2 = f2_make(sn, sn);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float2 w = f2_split(S::AV ? x[r][nt] : f2_mul(x[r][nt], sn2));
+            uint32_t hi = pack_h2(w.x, w.y);
+            if constexpr (LO) {
+              const float2 back = __half22float2(u32_as_h2(hi));
+              const uint32_t lo = pack_h2(w.x - back.x, w.y - back.y);
+              if constexpr (LO == 1) pl[r][nt] = movmatrix_trans(lo);
+              else hi = q4 < 2 ? hi : lo;
+            }
+            pb[r][nt] = movmatrix_trans(hi);
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          constexpr int NW = S::BV < 4 ? 1 : S::BV / 4;
+          uint32_t va[2][NW], vb[2][NW];  // the two tokens of each 8-token tile
+          uint32_t vs2[2], vz2[2];        // AV: their scales, zeros + 8 scales
+#pragma unroll
+          for (int T = 0; T < 2; ++T) {
+            const int t0 = (2 * kk + T) * 8 + tile_token(2 * q4), t1 = (2 * kk + T) * 8 + tile_token(2 * q4 + 1);
+            const uint8_t* vr = rec + int4_layout(D, G).vc + gi * (S::GS / 2) + g * S::BV;
+            lds_bytes<S::BV>(vr + t0 * (D / 2), va[T]);
+            lds_bytes<S::BV>(vr + t1 * (D / 2), vb[T]);
+            if constexpr (S::AV) {
+              const uint8_t* pr = rec + int4_layout(D, G).vp + g * (D / 8) / S::GS * 4;
+              uint32_t w0 = lds_u32(pr + t0 * G * 4), w1 = lds_u32(pr + t1 * G * 4);
+              if (tail) {
+                if (tok0 + t0 >= len) w0 = 0u;
+                if (tok0 + t1 >= len) w1 = 0u;
+              }
+              vs2[T] = prmt(w0, w1, 0x5410);
+              vz2[T] = h2_as_u32(__hfma2(u32_as_h2(vs2[T]), u32_as_h2(0x48004800u), u32_as_h2(prmt(w0, w1, 0x7632))));
+            }
+          }
+          auto value = [&](uint32_t c, int T) -> uint32_t {
+            if constexpr (S::AV) return h2_as_u32(__hfma2(u32_as_h2(c), u32_as_h2(vs2[T]), u32_as_h2(vz2[T])));
+            return c;
+          };
+          // two channels' bytes at a time: the two terms of a sum stand apart
+#pragma unroll
+          for (int b0 = 0; b0 < S::BV; b0 += 2) {
+            constexpr int BB = S::BV < 2 ? 1 : 2;
+            uint32_t a[BB][4];
+#pragma unroll
+            for (int b2 = 0; b2 < BB; ++b2) {
+              const int b = b0 + b2;
+              // bytes b of both tokens, the first in the low half
+              const uint32_t y0 = prmt(va[0][b / 4], vb[0][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
+              const uint32_t y1 = prmt(va[1][b / 4], vb[1][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
+              a[b2][0] = value(low_code(y0), 0), a[b2][1] = value(high_code(y0), 0);
+              a[b2][2] = value(low_code(y1), 1), a[b2][3] = value(high_code(y1), 1);
+            }
+#pragma unroll
+            for (int term = 0; term < (LO == 1 ? 2 : 1); ++term)
+#pragma unroll
+              for (int b2 = 0; b2 < BB; ++b2)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                  mma_16816(O[nt][gi * S::BV + b0 + b2], a[b2][0], a[b2][1], a[b2][2], a[b2][3],
+                            term ? pl[LO == 1 ? 2 * kk : 0][LO == 1 ? nt : 0] : pb[2 * kk][nt],
+                            term ? pl[LO == 1 ? 2 * kk + 1 : 0][LO == 1 ? nt : 0] : pb[2 * kk + 1][nt]);
+          }
+        }
+      }
+      // ---- the stage is free: the page STAGES ahead
+      __syncwarp();
+      const int next = k + S::STAGES;
+      if (next < mine) {
+        if ((next & 31) == 0) ids = page_ids(next);
+        const int p = __shfl_sync(~0u, ids, next & 31);
+        issue(p, stage);
+      }
+      if (++stage == S::STAGES) stage = 0, phase ^= 1;
     }
 
     // ---- the warps' results meet
@@ -830,7 +819,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float2 v;  // even channel (high nibble), odd channel
-            const float z = S::AV ? 0.f : (c ? zf[nt][gi].y : zf[nt][gi].x), unit = S::AV ? 1.f : vref;
+            const float z = S::AV || (LO == 2 && q4 >= 2) ? 0.f : (c ? zf[nt][gi].y : zf[nt][gi].x), unit = S::AV ? 1.f : vref;
             v.x = f[nt][c] * fmaf(O[nt][j][2 + c], unit, z);
             v.y = f[nt][c] * fmaf(O[nt][j][c], unit, z);
             *reinterpret_cast<float2*>(merge + (warp * S::ROWS + nt * 8 + q4 * 2 + c) * S::PITCH + j * 16 + g * 2) = v;
@@ -852,6 +841,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
         if (a.x != -INFINITY) L = fmaf(a.y, exp2f(a.x - top), L);
         const float2 o = *reinterpret_cast<const float2*>(merge + (w * S::ROWS + n) * S::PITCH + 2 * p);
         v.x += o.x, v.y += o.y;
+        if constexpr (LO == 2) {
+          const float2 o2 = *reinterpret_cast<const float2*>(merge + (w * S::ROWS + n + 4) * S::PITCH + 2 * p);
+          v.x += o2.x, v.y += o2.y;
+        }
       }
       if (whole) {
         store_pair<D, S::GV>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, p, v, top, s_on[n] ? L : 0.f);
@@ -957,19 +950,17 @@ constexpr int kSMs = 148;
 
 // column tiles of 8 query rows for `rows` rows of a (sequence, KV head)
 inline int attn_nt(int D, int rows) {
-  const int most = D == 256 ? 2 : 4;
-  const int nt = (rows + 7) / 8;
-  return nt < most ? nt : most;
+  return rows <= 8 ? 1 : 2;
 }
 
 
-template <int D, int G, int NT, bool LO>
+template <int D, int G, int NT, int LO>
 int attn_launch(const Int4AttnParams& p, cudaStream_t st) {
   using S = AttnShape<D, G, NT, LO>;
   const int entries = p.R * p.tiles;
   const int smem = S::smem(entries);
   if (!ensure_dynamic_smem<int4_attn_kernel<D, G, NT, LO>>(S::smem(kAttnEntries))) return AKV_ERR_LAUNCH;
-  const int grid = kSMs * S::OCC * WAVES;
+  const int grid = kSMs * S::OCC;
   int4_attn_kernel<D, G, NT, LO><<<grid, kAttnThreads, smem, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return AKV_ERR_LAUNCH;
   if (!p.meta) return AKV_OK;
@@ -988,18 +979,15 @@ int attn_launch(const Int4AttnParams& p, cudaStream_t st) {
 
 template <int D, int G, int NT>
 int attn_dispatch_lo(const Int4AttnParams& p, cudaStream_t st) {
-  return p.bf16 ? attn_launch<D, G, NT, false>(p, st) : attn_launch<D, G, NT, true>(p, st);
+  if (p.bf16) return attn_launch<D, G, NT, 0>(p, st);
+  if constexpr (NT == 1)
+    if (p.M * (p.Hq / p.c.kv_heads) <= 4) return attn_launch<D, G, NT, 2>(p, st);
+  return attn_launch<D, G, NT, 1>(p, st);
 }
 
 template <int D, int G>
 int attn_dispatch_nt(const Int4AttnParams& p, int nt, cudaStream_t st) {
-  if (nt == 1) return attn_dispatch_lo<D, G, 1>(p, st);
-  if (nt == 2) return attn_dispatch_lo<D, G, 2>(p, st);
-  if constexpr (D != 256) {
-    if (nt == 3) return attn_dispatch_lo<D, G, 3>(p, st);
-    if (nt == 4) return attn_dispatch_lo<D, G, 4>(p, st);
-  }
-  return AKV_ERR_UNSUPPORTED;
+  return nt == 1 ? attn_dispatch_lo<D, G, 1>(p, st) : attn_dispatch_lo<D, G, 2>(p, st);
 }
 
 template <int D>
