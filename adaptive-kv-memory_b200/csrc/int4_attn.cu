@@ -75,6 +75,7 @@ extern "C" int akv_int4_attention(const akv_int4_attention_args* a, void* stream
   p.scale = a->sm_scale;
   p.out = static_cast<uint16_t*>(a->out);
   p.o_sr = a->o_sr; p.o_sh = a->o_sh; p.o_sm = a->o_sm;
+  p.out4 = ((reinterpret_cast<uintptr_t>(a->out) & 3) | ((a->o_sr | a->o_sh | a->o_sm) & 1)) == 0;
   p.lse = a->lse;
   p.bf16 = a->dtype == AKV_BF16;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);

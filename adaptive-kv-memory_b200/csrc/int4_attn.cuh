@@ -45,6 +45,7 @@ struct Int4AttnParams {
   int64_t o_sr, o_sh, o_sm;
   float* lse;
   int bf16;
+  int out4;  // output rows on 4-byte boundaries
   float* part;         // [slot][8 NT][D + 2]
   unsigned* arrived;   // per unit: CTAs that have stored their part; 0 between calls
   int2* meta;          // per unit: first and last CTA, for the combine kernel (NULL: the last CTA merges)
@@ -82,8 +83,8 @@ struct AttnShape {
   static constexpr int BUF = RING > MERGE ? RING : MERGE;
   static constexpr int FRAG = D / 16 * NT * 32 * 8;
   // ring / merge buffer, fragments, then: group sums of q, exponent factors,
-  // visible lengths, output offsets, (y, l) per warp and row, barriers; per
-  // entry: prefix sums of pages, lengths, new tokens
+  // visible lengths, output offsets, (y, l) per warp and row and of all warps,
+  // barriers; per entry: prefix sums of pages, lengths, new tokens
   static constexpr int OFF_FRAG = (BUF + 127) / 128 * 128;
   static constexpr int OFF_QS = OFF_FRAG + FRAG;
   static constexpr int OFF_CQ = OFF_QS + ROWS * G * 4;
@@ -92,7 +93,8 @@ struct AttnShape {
   static constexpr int OFF_LSE = OFF_OUT + ROWS * 8;
   static constexpr int OFF_ON = OFF_LSE + ROWS * 4;
   static constexpr int OFF_ML = OFF_ON + ROWS * 4;
-  static constexpr int OFF_BAR = OFF_ML + kAttnWarps * ROWS * 8;
+  static constexpr int OFF_TL = OFF_ML + kAttnWarps * ROWS * 8;
+  static constexpr int OFF_BAR = OFF_TL + ROWS * 8;
   static constexpr int OFF_PREF = OFF_BAR + kAttnWarps * STAGES * 8;
   static constexpr int OCC = attn_occ(D, NT);
   static constexpr int smem(int entries) { return OFF_PREF + (3 * entries + 1) * 4; }
@@ -180,8 +182,12 @@ AKV_DEV void store_pair(const Int4AttnParams& P, int64_t row, float* lse, int p,
   v.y = on ? v.y * inv : 0.f;
   uint16_t* o = P.out + row + ch;
   const uint32_t w = P.bf16 ? pack_elems<true>(v.x, v.y) : pack_elems<false>(v.x, v.y);
-  o[0] = static_cast<uint16_t>(w);
-  o[1] = static_cast<uint16_t>(w >> 16);
+  if (P.out4) {
+    *reinterpret_cast<uint32_t*>(o) = w;
+  } else {
+    o[0] = static_cast<uint16_t>(w);
+    o[1] = static_cast<uint16_t>(w >> 16);
+  }
   if (lse && p == 0) *lse = on ? (top + log2f(L)) * 0.6931471805599453f : -INFINITY;
 }
 
@@ -256,6 +262,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
   int* s_lse = reinterpret_cast<int*>(smem + S::OFF_LSE);
   int64_t* s_out = reinterpret_cast<int64_t*>(smem + S::OFF_OUT);
   float2* s_ml = reinterpret_cast<float2*>(smem + S::OFF_ML);
+  float2* s_tl = reinterpret_cast<float2*>(smem + S::OFF_TL);
   uint64_t* s_bar = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
   int* s_pref = reinterpret_cast<int*>(smem + S::OFF_PREF);
   __shared__ int s_scan[kAttnWarps], s_max[kAttnWarps], s_last;
@@ -793,6 +800,17 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
       }
     }
     __syncthreads();  // every warp is done with its ring
+    if (t < S::ROWS) {  // maximum and sum of a row over the warps
+      float top = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, s_ml[w * S::ROWS + t].x);
+#pragma unroll
+      for (int w = 0; w < kAttnWarps; ++w) {
+        const float2 a = s_ml[w * S::ROWS + t];
+        if (a.x != -INFINITY) L = fmaf(a.y, exp2f(a.x - top), L);
+      }
+      s_tl[t] = make_float2(top, s_on[t] ? L : 0.f);
+    }
     float* merge = reinterpret_cast<float*>(smem);
     float f[NT][2];
 #pragma unroll
@@ -831,14 +849,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
     float* part = P.part + (static_cast<int64_t>(blockIdx.x) + unit) * STEP;
     for (int k = t; k < valid * (D / 2); k += kAttnThreads) {
       const int n = k / (D / 2), p = k % (D / 2);
-      float top = -INFINITY, L = 0.f;
-#pragma unroll
-      for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, s_ml[w * S::ROWS + n].x);
       float2 v = make_float2(0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kAttnWarps; ++w) {
-        const float2 a = s_ml[w * S::ROWS + n];
-        if (a.x != -INFINITY) L = fmaf(a.y, exp2f(a.x - top), L);
         const float2 o = *reinterpret_cast<const float2*>(merge + (w * S::ROWS + n) * S::PITCH + 2 * p);
         v.x += o.x, v.y += o.y;
         if constexpr (LO == 2) {
@@ -846,11 +859,12 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
           v.x += o2.x, v.y += o2.y;
         }
       }
+      const float2 tl = s_tl[n];
       if (whole) {
-        store_pair<D, S::GV>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, p, v, top, s_on[n] ? L : 0.f);
+        store_pair<D, S::GV>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, p, v, tl.x, tl.y);
       } else {
         *reinterpret_cast<float2*>(part + n * (D + 2) + 2 * p) = v;
-        if (p == 0) *reinterpret_cast<float2*>(part + n * (D + 2) + D) = make_float2(top, s_on[n] ? L : 0.f);
+        if (p == 0) *reinterpret_cast<float2*>(part + n * (D + 2) + D) = tl;
       }
     }
     if (whole) {
