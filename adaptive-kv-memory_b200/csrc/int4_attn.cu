@@ -9,7 +9,7 @@ namespace {
 struct Plan {
   int nt, tiles, rows;
   bool fused;  // each unit's last CTA merges its parts: no second launch
-  size_t arrived, meta, part;
+  size_t meta, part;
 };
 
 Plan attn_plan(int R, int M, int Hq, int kv_heads, int D, int max_blocks) {
@@ -20,13 +20,15 @@ Plan attn_plan(int R, int M, int Hq, int kv_heads, int D, int max_blocks) {
   p.rows = kAttnEntries / p.tiles;
   const int64_t row_pages = static_cast<int64_t>(p.tiles) * kv_heads * max_blocks;
   if (p.rows > INT32_MAX / row_pages) p.rows = static_cast<int>(INT32_MAX / row_pages);  // 0: too many
+  // a counter for every unit, in a region of its own at the workspace's start
+  const int64_t row_units = static_cast<int64_t>(p.tiles) * kv_heads;
+  if (p.rows > kAttnUnits / row_units) p.rows = static_cast<int>(kAttnUnits / row_units);
   if (p.rows > R) p.rows = R;
   const size_t units = static_cast<size_t>(p.rows) * p.tiles * kv_heads;
   // the most CTAs that can share a unit, and the query rows each leaves there
   const int segs = max_blocks / kAttnMinPages + 2;
   const int q_rows_tile = q_rows < 8 * p.nt ? q_rows : 8 * p.nt;
   p.fused = static_cast<int64_t>(segs) * q_rows_tile <= kAttnFused;
-  p.arrived = (units * sizeof(unsigned) + 15) / 16 * 16;
   p.meta = (units * sizeof(int2) + 15) / 16 * 16;
   // a CTA and a unit meet at most once, and along the list of pages their
   // numbers' sum only grows: it is the slot of the partial result
@@ -43,7 +45,7 @@ extern "C" size_t akv_int4_attention_workspace_bytes(int R, int M, int Hq, int k
   if (static_cast<int64_t>(M) * (Hq / kv_heads) > 8 * kAttnEntries) return 0;
   const Plan p = attn_plan(R, M, Hq, kv_heads, head_dim, max_blocks);
   if (p.rows == 0 || static_cast<int64_t>(R) * Hq * M > INT32_MAX) return 0;
-  return p.arrived + p.meta + p.part;
+  return kAttnUnits * sizeof(unsigned) + p.meta + p.part;
 }
 
 extern "C" int akv_int4_attention(const akv_int4_attention_args* a, void* stream) {
@@ -80,8 +82,9 @@ extern "C" int akv_int4_attention(const akv_int4_attention_args* a, void* stream
   p.bf16 = a->dtype == AKV_BF16;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   p.arrived = reinterpret_cast<unsigned*>(ws);
-  p.meta = plan.fused ? nullptr : reinterpret_cast<int2*>(ws + plan.arrived);
-  p.part = reinterpret_cast<float*>(ws + plan.arrived + plan.meta);
+  ws += kAttnUnits * sizeof(unsigned);
+  p.meta = plan.fused ? nullptr : reinterpret_cast<int2*>(ws);
+  p.part = reinterpret_cast<float*>(ws + plan.meta);
   p.status = a->status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (int r = 0; r < a->R; r += plan.rows) {

@@ -28,6 +28,7 @@ namespace akv {
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kAttnEntries = 1024;  // (row, row tile) pairs of one launch
+constexpr int kAttnUnits = 16384;    // units of one launch
 constexpr int kAttnMinPages = 8;    // pages of a CTA's share, at least (two per warp) where a unit has them
 constexpr int kAttnFused = 1024;    // partial rows of a unit that its last CTA merges by itself
 constexpr float kLazyLog2 = 6.f;    // weights may reach 2^6 before the maximum moves
@@ -278,8 +279,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
   fence_mbar_init();
 
   // Pages of every (row, row tile), as a prefix sum; all heads of a row alike.
+  bool empty;  // some see no token
   {
     int base = 0, most = 0;
+    empty = false;
     for (int e0 = 0; e0 < entries; e0 += kAttnThreads) {
       const int e = e0 + t;
       int n = 0;
@@ -310,7 +313,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
       }
       if (e < entries) s_pref[e + 1] = before + x;
       base = sum;
-      __syncthreads();
+      empty |= __syncthreads_or(e < entries && n == 0);
     }
     most = __reduce_max_sync(~0u, most);
     if (lane == 0) s_max[warp] = most;
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
   }
 
   // rows without any visible token: zero output
-  for (int u = blockIdx.x; u < entries * H; u += gridDim.x) {
+  for (int u = empty ? blockIdx.x : entries * H; u < entries * H; u += gridDim.x) {
     const int e = u / H, h = u % H;
     if (s_pref[e + 1] != s_pref[e]) continue;
     const int i = P.row0 + e / P.tiles;
@@ -397,6 +400,17 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
       }
     };
     int ids = page_ids(0);
+    // the query rows this warp prepares, on their way with the page numbers
+    constexpr int PER = D / 32;
+    constexpr int RW = S::ROWS / kAttnWarps;  // rows of a warp, all loads in flight at once
+    uint16_t raw[RW][PER];
+#pragma unroll
+    for (int k2 = 0; k2 < RW; ++k2) {
+      const int rr = tile * S::ROWS + tile_row<LO>(k2 * kAttnWarps + warp), m = rr / rep;
+      const uint16_t* src = P.q + i * P.q_sr + (h * rep + rr % rep) * P.q_sh + m * P.q_sm + lane * PER;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) raw[k2][k] = m < n_new ? src[k] : 0;
+    }
 #pragma unroll
     for (int k = 0; k < S::STAGES; ++k) {
       const int p = __shfl_sync(~0u, ids, k);
@@ -406,16 +420,6 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
     // Queries of the tile: scaled to fp16, placed as MMA operands; sums per group.
     {
       uint16_t* frag = reinterpret_cast<uint16_t*>(smem + S::OFF_FRAG);
-      constexpr int PER = D / 32;
-      constexpr int RW = S::ROWS / kAttnWarps;  // rows of a warp, all loads in flight at once
-      uint16_t raw[RW][PER];
-#pragma unroll
-      for (int k2 = 0; k2 < RW; ++k2) {
-        const int rr = tile * S::ROWS + tile_row<LO>(k2 * kAttnWarps + warp), m = rr / rep;
-        const uint16_t* src = P.q + i * P.q_sr + (h * rep + rr % rep) * P.q_sh + m * P.q_sm + lane * PER;
-#pragma unroll
-        for (int k = 0; k < PER; ++k) raw[k2][k] = m < n_new ? src[k] : 0;
-      }
 #pragma unroll
       for (int k2 = 0; k2 < RW; ++k2) {
         const int n = k2 * kAttnWarps + warp;

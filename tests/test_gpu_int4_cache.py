@@ -312,6 +312,14 @@ def test_attend_same_pages_in_two_rows_and_repeated_calls():
     assert torch.equal(a, b) and torch.equal(a, d)
 
 
+def test_attend_shapes_in_turn_on_one_workspace():
+    """Calls of very different shapes share the stream's scratch: no call may see what another left."""
+    c = _filled([1500, 700, 33, 1], 128, 128, heads=2)
+    shapes = [(4, 2, 1), (1, 8, 2), (4, 16, 3), (2, 4, 12), (4, 2, 1), (1, 2, 1), (4, 16, 8)]
+    for i, (r, hq, m) in enumerate(shapes * 2):
+        _check(c, 0, _rand((r, hq, m, 128), 30 + i, torch.float16), None, None)
+
+
 def test_attend_on_another_stream_and_in_a_graph():
     c = _filled([500, 37], 128, 64)
     q = _rand((2, 4, 2, 128), 22, torch.float16)
