@@ -32,9 +32,11 @@ namespace akv {
 namespace cg = cooperative_groups;
 
 constexpr int kVerifyCluster = 8;
-constexpr int kVerifyThreads = 512;
-constexpr int kVerifyWarps = kVerifyThreads / 32;
-static_assert(kVerifyWarps <= 32, "a lane stands for a warp's sum");
+// Threads of a CTA.  One sequence is a chain of latencies (accept, sums,
+// exchange, draw) that more threads shorten; many sequences want several of
+// their CTAs on an SM, so that one's loads cover another's chain.
+constexpr int kVerifyFew = 512, kVerifyMany = 256;
+constexpr int kVerifyManyFrom = 24;  // sequences
 
 struct VerifyParams {
   const void* target;
@@ -102,12 +104,14 @@ AKV_DEV uint64_t warp_scan_u64(uint64_t x) {
   return x;
 }
 
-template <int DT, bool DRAFT>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyParams P) {
+template <int DT, bool DRAFT, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == kVerifyMany ? 4 : 1) verify_kernel(VerifyParams P) {
+  constexpr int WARPS = THREADS / 32;
+  static_assert(WARPS <= 32, "a lane stands for a warp's sum");
   using E = ProbElem<DT>;
   using T = typename E::type;
   cg::cluster_group cluster = cg::this_cluster();
-  __shared__ uint64_t s_w[kVerifyWarps];  // units in each warp's range
+  __shared__ uint64_t s_w[WARPS];  // units in each warp's range
   __shared__ uint64_t s_sum, s_before, s_total;
   __shared__ int s_acc;
   const int b = blockIdx.y, part = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -167,9 +171,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyParams P) 
 
   // this CTA's part, a contiguous range for each warp
   constexpr int VE = 16 / sizeof(T);  // elements of a 16-byte load
-  int per_warp = (P.vocab + kVerifyCluster * kVerifyWarps - 1) / (kVerifyCluster * kVerifyWarps);
+  int per_warp = (P.vocab + kVerifyCluster * WARPS - 1) / (kVerifyCluster * WARPS);
   per_warp = (per_warp + VE - 1) / VE * VE;
-  const int first = min((part * kVerifyWarps + warp) * per_warp, P.vocab);
+  const int first = min((part * WARPS + warp) * per_warp, P.vocab);
   const int end = min(first + per_warp, P.vocab);
 
   // sum of the weights of [first, end), without the hot token's correction
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyParams P) 
     if (lane == 0) s_w[warp] = sum;
     __syncthreads();
     if (warp == 0) {
-      const uint64_t a = warp_sum_u64(lane < kVerifyWarps ? s_w[lane] : 0);
+      const uint64_t a = warp_sum_u64(lane < WARPS ? s_w[lane] : 0);
       if (lane == 0) s_sum = a;
     }
     cluster.sync();
@@ -276,7 +280,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyParams P) 
     cluster.barrier_arrive();  // no CTA reuses or leaves its sum while another reads it
     const uint64_t all = s_total;
     if (part == 0 && pass == 0) {
-      for (int j = t; j <= P.K; j += kVerifyThreads)
+      for (int j = t; j <= P.K; j += THREADS)
         if (j != acc) out[j] = j < acc ? tok[j] : -1;
       if (t == 0) P.accepted[b] = acc;
     }
@@ -285,18 +289,18 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyParams P) 
     const uint64_t goal = (all >> 24) * u24 + (((all & 0xFFFFFFull) * u24) >> 24);
     uint64_t base = s_before;
     if (all && goal >= base && goal - base < s_sum) {  // the goal is in this CTA's part
-      const uint64_t w_sum = lane < kVerifyWarps ? s_w[lane] : 0, w_inc = warp_scan_u64(w_sum);
+      const uint64_t w_sum = lane < WARPS ? s_w[lane] : 0, w_inc = warp_scan_u64(w_sum);
       const int w = __ffs(__ballot_sync(~0u, base + w_inc > goal)) - 1;
       base += __shfl_sync(~0u, w_inc - w_sum, w);
-      const int f0 = (part * kVerifyWarps + w) * per_warp, f1 = min(f0 + per_warp, P.vocab);
-      for (int x0 = f0; x0 < f1 && base <= goal; x0 += kVerifyThreads) {
+      const int f0 = (part * WARPS + w) * per_warp, f1 = min(f0 + per_warp, P.vocab);
+      for (int x0 = f0; x0 < f1 && base <= goal; x0 += THREADS) {
         const int x = x0 + t;
         const uint64_t mine = x < f1 ? weight(x, over) : 0;
         uint64_t inc = warp_scan_u64(mine);
         __syncthreads();  // the sums of warps are read above, and in the round before
         if (lane == 31) s_w[warp] = inc;
         __syncthreads();
-        const uint64_t v = lane < kVerifyWarps ? s_w[lane] : 0, v_inc = warp_scan_u64(v);
+        const uint64_t v = lane < WARPS ? s_w[lane] : 0, v_inc = warp_scan_u64(v);
         inc += base + __shfl_sync(~0u, v_inc - v, warp);
         if (mine && inc > goal && inc - mine <= goal) out[acc] = x;
         base += __shfl_sync(~0u, v_inc, 31);
@@ -311,11 +315,11 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyParams P) 
 
 using namespace akv;
 
-template <int DT>
-static cudaError_t verify_launch(const VerifyParams& p, int B, bool draft, cudaStream_t st) {
+template <int DT, int THREADS>
+static cudaError_t verify_launch(const VerifyParams& p, int B, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(kVerifyCluster, B);
-  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.blockDim = dim3(THREADS);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -324,7 +328,15 @@ static cudaError_t verify_launch(const VerifyParams& p, int B, bool draft, cudaS
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return draft ? cudaLaunchKernelEx(&cfg, verify_kernel<DT, true>, p) : cudaLaunchKernelEx(&cfg, verify_kernel<DT, false>, p);
+  return p.draft ? cudaLaunchKernelEx(&cfg, verify_kernel<DT, true, THREADS>, p)
+                 : cudaLaunchKernelEx(&cfg, verify_kernel<DT, false, THREADS>, p);
+}
+
+// Measured (151,936 fp32 probabilities, draft and target; us with 512 / 256
+// threads): 1 sequence 10.3 / 12.8, 16 12.4 / 14.4, 24 14.4 / 14.4, 64 28.7 / 18.4.
+template <int DT>
+static cudaError_t verify_launch(const VerifyParams& p, int B, cudaStream_t st) {
+  return B >= kVerifyManyFrom ? verify_launch<DT, kVerifyMany>(p, B, st) : verify_launch<DT, kVerifyFew>(p, B, st);
 }
 
 extern "C" int akv_verify_draft(const akv_verify_args* a, void* stream) {
@@ -341,9 +353,8 @@ extern "C" int akv_verify_draft(const akv_verify_args* a, void* stream) {
                        a->n_draft, a->accept_u, a->sample_u, a->K,       a->vocab, a->accepted, a->out, a->status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  const bool d = a->draft != nullptr;
-  if (a->dtype == AKV_FP32) e = verify_launch<AKV_FP32>(p, a->B, d, st);
-  else if (a->dtype == AKV_FP16) e = verify_launch<AKV_FP16>(p, a->B, d, st);
-  else e = verify_launch<AKV_BF16>(p, a->B, d, st);
+  if (a->dtype == AKV_FP32) e = verify_launch<AKV_FP32>(p, a->B, st);
+  else if (a->dtype == AKV_FP16) e = verify_launch<AKV_FP16>(p, a->B, st);
+  else e = verify_launch<AKV_BF16>(p, a->B, st);
   return e == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH;
 }
