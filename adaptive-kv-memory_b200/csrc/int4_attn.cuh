@@ -30,6 +30,8 @@ constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kAttnEntries = 1024;  // (row, row tile) pairs of one launch
 constexpr int kAttnUnits = 16384;    // units of one launch
 constexpr int kAttnMinPages = 8;    // pages of a CTA's share, at least (two per warp) where a unit has them
+constexpr int kAttnWhole = 32;       // pages up to which no unit is split
+constexpr int kAttnSetup = 16;       // pages that such a unit's set-up counts for
 constexpr int kAttnFused = 1024;    // partial rows of a unit that its last CTA merges by itself
 constexpr float kLazyLog2 = 6.f;    // weights may reach 2^6 before the maximum moves
 
@@ -159,28 +161,27 @@ AKV_DEV void lds_pairs(const uint8_t* p, uint32_t (&w)[G]) {
   }
 }
 
-// tokens that query tokens [0, m_last] of call row i see, in pages
-AKV_DEV int visible_pages(const Int4Row& r, int m_last) {
-  const int see = r.len - r.n_new + m_last + 1;
-  return see > 0 ? (see + kBlockTokens - 1) / kBlockTokens : 0;
-}
-
-// Element offset of the output row of query row rr of (call row i, KV head h).
+// Element offset of the output row of query token m, head hq of call row i.
 AKV_DEV int64_t out_row(const Int4AttnParams& P, int i, int hq, int m) {
   return i * P.o_sr + hq * P.o_sh + m * P.o_sm;
 }
 
+// What a row's maximum (log2) and sum L make of its output: its lse, and the
+// factor of the sums of p V.  L 0: a row that sees nothing.
+AKV_DEV float2 row_scale(float top, float L) {
+  return L > 0.f ? make_float2((top + log2f(L)) * 0.6931471805599453f, 1.f / L) : make_float2(-INFINITY, 0.f);
+}
+
 // Output channels of accumulator pair p (order of the merge buffer) of the row
-// at `row`; its lse with pair 0.  L 0: a row that sees nothing.
+// at `row`; its lse with pair 0.  scale: row_scale().
 template <int D, int G>
-AKV_DEV void store_pair(const Int4AttnParams& P, int64_t row, float* lse, int p, float2 v, float top, float L) {
+AKV_DEV void store_pair(const Int4AttnParams& P, int64_t row, float* lse, int p, float2 v, float2 scale) {
   constexpr int GS = D / G, BV = GS / 16;
   const int j = p / 8, g = p % 8;
   const int ch = j / BV * GS + g * 2 * BV + 2 * (j % BV);
-  const bool on = L > 0.f;
-  const float inv = on ? 1.f / L : 0.f;
-  v.x = on ? v.x * inv : 0.f;
-  v.y = on ? v.y * inv : 0.f;
+  const bool on = scale.y > 0.f;
+  v.x = on ? v.x * scale.y : 0.f;
+  v.y = on ? v.y * scale.y : 0.f;
   uint16_t* o = P.out + row + ch;
   const uint32_t w = P.bf16 ? pack_elems<true>(v.x, v.y) : pack_elems<false>(v.x, v.y);
   if (P.out4) {
@@ -189,7 +190,7 @@ AKV_DEV void store_pair(const Int4AttnParams& P, int64_t row, float* lse, int p,
     o[0] = static_cast<uint16_t>(w);
     o[1] = static_cast<uint16_t>(w >> 16);
   }
-  if (lse && p == 0) *lse = on ? (top + log2f(L)) * 0.6931471805599453f : -INFINITY;
+  if (lse && p == 0) *lse = scale.x;
 }
 
 // One CTA merges the parts of a unit (segs * 8 NT <= kAttnFused, so their
@@ -200,7 +201,7 @@ AKV_DEV void merge_parts(const Int4AttnParams& P, const float* part, int segs, c
   constexpr int ROWS = 8 * NT;
   constexpr int64_t STEP = static_cast<int64_t>(ROWS) * (D + 2);
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  float2* s_tl = reinterpret_cast<float2*>(w + kAttnFused);  // per row: maximum, sum
+  float2* s_tl = reinterpret_cast<float2*>(w + kAttnFused);  // per row: lse, factor
   for (int n = warp; n < valid; n += kAttnWarps) {
     const float* ml = part + n * (D + 2) + D;
     float top = -INFINITY, L = 0.f;
@@ -218,7 +219,7 @@ AKV_DEV void merge_parts(const Int4AttnParams& P, const float* part, int segs, c
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
-    if (lane == 0) s_tl[n] = make_float2(top, L);
+    if (lane == 0) s_tl[n] = row_scale(top, L);
   }
   __syncthreads();
   constexpr int T = 4;  // output pairs of a thread at a time
@@ -246,7 +247,7 @@ AKV_DEV void merge_parts(const Int4AttnParams& P, const float* part, int segs, c
       const int k = k0 + j * kAttnThreads;
       if (k >= valid * (D / 2)) break;
       const int n = k / (D / 2);
-      store_pair<D, G>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, k % (D / 2), acc[j], s_tl[n].x, s_tl[n].y);
+      store_pair<D, G>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, k % (D / 2), acc[j], s_tl[n]);
     }
   }
 }
@@ -278,26 +279,32 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
   if (lane < S::STAGES) mbar_init(s_bar + warp * S::STAGES + lane, 1);
   fence_mbar_init();
 
-  // Pages of every (row, row tile), as a prefix sum; all heads of a row alike.
-  bool empty;  // some see no token
-  {
+  // Pages of every entry (row, row tile); all heads of a row alike.
+  for (int e = t; e < entries; e += kAttnThreads) {
+    const Int4Row r = int4_row(P.c, P.rows, P.n_new, P.row0 + e / P.tiles, P.M, P.status);
+    s_len[e] = r.len;
+    s_new[e] = r.n_new;
+  }
+  auto pages_of = [&](int e) -> int {
+    const int tile = e % P.tiles, n_new = s_new[e];
+    const int first = tile * S::ROWS / rep;  // its first query token
+    const int last = min((tile * S::ROWS + S::ROWS - 1) / rep, n_new - 1);
+    const int see = s_len[e] - n_new + last + 1;
+    return first <= last && see > 0 ? (see + kBlockTokens - 1) / kBlockTokens : 0;
+  };
+  // Prefix sums of (pages + extra) over the entries that have any; whether some
+  // have none, and the longest.
+  bool empty = false;
+  int longest = 0;
+  auto scan = [&](int extra) {
     int base = 0, most = 0;
-    empty = false;
     for (int e0 = 0; e0 < entries; e0 += kAttnThreads) {
+      __syncthreads();
       const int e = e0 + t;
-      int n = 0;
-      if (e < entries) {
-        const int i = P.row0 + e / P.tiles, tile = e % P.tiles;
-        const Int4Row r = int4_row(P.c, P.rows, P.n_new, i, P.M, P.status);
-        const int first = tile * S::ROWS / rep;  // its first query token
-        int last = (tile * S::ROWS + S::ROWS - 1) / rep;
-        if (last >= r.n_new) last = r.n_new - 1;
-        if (first <= last) n = visible_pages(r, last);
-        s_len[e] = r.len;
-        s_new[e] = r.n_new;
-      }
-      most = n > most ? n : most;
-      int x = n;
+      const int n = e < entries ? pages_of(e) : 0;
+      empty |= e < entries && n == 0;
+      most = max(most, n);
+      int x = n ? n + extra : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(~0u, x, o);
@@ -313,13 +320,18 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
       }
       if (e < entries) s_pref[e + 1] = before + x;
       base = sum;
-      empty |= __syncthreads_or(e < entries && n == 0);
     }
     most = __reduce_max_sync(~0u, most);
     if (lane == 0) s_max[warp] = most;
     if (t == 0) s_pref[0] = 0;
-    __syncthreads();
-  }
+    empty = __syncthreads_or(empty);
+    longest = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+  };
+  scan(0);
+  // Where every unit is short, none is split (below), and a unit's cost is more
+  // its set-up than its pages: it counts as so many pages more.
+  const int extra = longest <= kAttnWhole ? kAttnSetup : 0;
+  if (extra) scan(extra);
 
   // rows without any visible token: zero output
   for (int u = empty ? blockIdx.x : entries * H; u < entries * H; u += gridDim.x) {
@@ -327,36 +339,54 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
     if (s_pref[e + 1] != s_pref[e]) continue;
     const int i = P.row0 + e / P.tiles;
     if (t == 0 && P.meta) P.meta[u] = make_int2(0, 0);
-    for (int k = t; k < S::ROWS * D; k += kAttnThreads) {
-      const int rr = e % P.tiles * S::ROWS + k / D, m = rr / rep;
+    for (int n = warp; n < S::ROWS; n += kAttnWarps) {
+      const int rr = e % P.tiles * S::ROWS + n, m = rr / rep;
       if (m >= P.M) break;
-      const int hq = h * rep + rr % rep;
-      P.out[out_row(P, i, hq, m) + k % D] = 0;
-      if (P.lse && k % D == 0) P.lse[(i * P.Hq + hq) * P.M + m] = -INFINITY;
+      const int hq = h * rep + rr - m * rep;
+      uint16_t* o = P.out + out_row(P, i, hq, m);
+      for (int c = lane; c < D / 2; c += 32) {
+        if (P.out4) {
+          reinterpret_cast<uint32_t*>(o)[c] = 0u;
+        } else {
+          o[2 * c] = 0;
+          o[2 * c + 1] = 0;
+        }
+      }
+      if (P.lse && lane == 0) P.lse[(i * P.Hq + hq) * P.M + m] = -INFINITY;
     }
   }
 
   // This CTA's share of all pages, a contiguous run over (row, tile, head, page);
-  // their number fits 31 bits (the caller sees to it).
+  // their number fits 31 bits (the caller sees to it).  Where every unit (row,
+  // tile, head) is short, a share's ends move up to the next unit's start:
+  // no unit is split, so none has parts to merge.
   const int total = s_pref[entries] * H;
   int share = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-  {
-    int least = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
-    if (least > kAttnMinPages) least = kAttnMinPages;
-    if (share < least) share = least;
-  }
+  const bool keep = extra > 0;
+  if (!keep && share < kAttnMinPages) share = kAttnMinPages;
   if (static_cast<int64_t>(share) * blockIdx.x >= total) return;
-  const int begin = share * blockIdx.x;
-  const int end = total - begin > share ? begin + share : total;
-  int pos = begin;
-  int e = 0;
-  {
-    int hi = entries;  // the last entry that starts at or before pos
-    while (hi - e > 1) {
-      const int mid = (e + hi) / 2;
-      if (s_pref[mid] * H <= pos) e = mid; else hi = mid;
+  int begin = share * blockIdx.x;
+  int end = total - begin > share ? begin + share : total;
+  auto entry_at = [&](int pos) -> int {  // the last entry that starts at or before pos
+    int lo = 0, hi = entries;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (s_pref[mid] * H <= pos) lo = mid; else hi = mid;
     }
+    return lo;
+  };
+  if (keep) {
+    auto next_unit = [&](int pos) -> int {
+      if (pos >= total) return total;
+      const int x = entry_at(pos), start = s_pref[x] * H, pages = s_pref[x + 1] - s_pref[x];
+      return start + (pos - start + pages - 1) / pages * pages;
+    };
+    begin = next_unit(begin);
+    end = next_unit(end);
+    if (begin >= end) return;
   }
+  int pos = begin;
+  int e = entry_at(begin);
   uint32_t stage = 0, phase = 0;
   bool alive = true;
   uint8_t* ring = smem + warp * S::STAGES * S::REC;
@@ -365,14 +395,14 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
   while (pos < end) {
     while (s_pref[e + 1] == s_pref[e]) ++e;
     const int e_start = s_pref[e] * H;
-    const int pages = s_pref[e + 1] - s_pref[e];
-    const int h = (pos - e_start) / pages;
-    const int u_start = e_start + h * pages;
+    const int weight = s_pref[e + 1] - s_pref[e], pages = weight - extra;
+    const int h = (pos - e_start) / weight;
+    const int u_start = e_start + h * weight;
     const int page0 = pos - u_start;
     int n_pages = pages - page0;
     if (n_pages > end - pos) n_pages = end - pos;
     const int unit = e * H + h;
-    const bool whole = u_start >= begin && u_start + pages <= end;
+    const bool whole = u_start >= begin && u_start + weight <= end;
     const int i = P.row0 + e / P.tiles, tile = e % P.tiles;
     const int len = s_len[e], n_new = s_new[e];
     const int seq = P.rows ? __ldg(P.rows + i) : i;  // in range: its pages are not 0
@@ -813,7 +843,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
         const float2 a = s_ml[w * S::ROWS + t];
         if (a.x != -INFINITY) L = fmaf(a.y, exp2f(a.x - top), L);
       }
-      s_tl[t] = make_float2(top, s_on[t] ? L : 0.f);
+      if (!s_on[t]) L = 0.f;
+      s_tl[t] = whole ? row_scale(top, L) : make_float2(top, L);
     }
     float* merge = reinterpret_cast<float*>(smem);
     float f[NT][2];
@@ -851,6 +882,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
     const int valid = min(S::ROWS, P.M * rep - tile * S::ROWS);  // query rows of this tile
     constexpr int64_t STEP = static_cast<int64_t>(S::ROWS) * (D + 2);
     float* part = P.part + (static_cast<int64_t>(blockIdx.x) + unit) * STEP;
+#pragma unroll 2
     for (int k = t; k < valid * (D / 2); k += kAttnThreads) {
       const int n = k / (D / 2), p = k % (D / 2);
       float2 v = make_float2(0.f, 0.f);
@@ -865,7 +897,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
       }
       const float2 tl = s_tl[n];
       if (whole) {
-        store_pair<D, S::GV>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, p, v, tl.x, tl.y);
+        store_pair<D, S::GV>(P, s_out[n], P.lse ? P.lse + s_lse[n] : nullptr, p, v, tl);
       } else {
         *reinterpret_cast<float2*>(part + n * (D + 2) + 2 * p) = v;
         if (p == 0) *reinterpret_cast<float2*>(part + n * (D + 2) + D) = tl;
@@ -896,8 +928,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
     // the merge buffer goes back to the copies
     fence_proxy_async_shared();
     __syncthreads();
-    pos += n_pages;
-    if (pos - e_start >= pages * H) ++e;
+    pos += n_pages + extra;
+    if (pos - e_start >= weight * H) ++e;
   }
 }
 
@@ -960,7 +992,8 @@ __global__ void __launch_bounds__(128) int4_combine_kernel(const Int4AttnParams 
     acc.y += s_acc[(w - 1) * PAIRS + p].y;
   }
   const int m = rr / rep, hq = h * rep + rr % rep;
-  store_pair<D, G>(P, out_row(P, i, hq, m), P.lse ? P.lse + (i * P.Hq + hq) * P.M + m : nullptr, p, acc, top, L);
+  store_pair<D, G>(P, out_row(P, i, hq, m), P.lse ? P.lse + (i * P.Hq + hq) * P.M + m : nullptr, p, acc,
+                   row_scale(top, L));
 }
 
 // ---------------------------------------------------------------- host
