@@ -19,6 +19,27 @@
 // fp16 term for a bf16 output (an eighth of that output's own rounding), as
 // two, the second holding the first's error, for an fp16 output (LO).  The
 // zero-point sum, l and the partial results are fp32.
+//
+// Work.  A unit is one (row, tile of 8 or 16 query rows, KV head); the units'
+// pages form one list that is cut into equal shares, one per resident CTA, from
+// the lengths on the device: ragged batches balance and the host needs no
+// length.  A unit cut in two or more is merged by the last of its CTAs to
+// finish (or, with many query rows over a long table, by a second kernel); a
+// call of short units keeps each whole.  A warp streams every fourth page of
+// its share through its own ring of bulk copies and meets the others in shared
+// memory at a unit's end.  Sums are taken in an order that the lengths alone
+// decide, so a call repeated gives the same bits.
+//
+// Bound and measured (B200, 32 / 8 heads of 128, 16 x 32K tokens).  The pages
+// alone stream in 95 us (6.0 TB/s).  One query token, group 128: 135 us fp16
+// (4.2 TB/s).  Per page and warp some 630 instructions, 40 % of them unpacking
+// (256 codes a lane); issue slots 60 %, the integer pipe 52 %, tensor cores
+// 25 % busy, and fewer or more warps change nothing: instruction throughput
+// bounds it.  Five tokens, groups of 32, bf16: 236 us; the same bound, the
+// per-group scaling of scores above all.  What was tried and did not help: two
+// pages per iteration, one CTA of 16 warps an SM, keeping warps in step, three
+// or four query tiles a CTA (the registers leave too few warps), three or more
+// CTAs' worth of shares.
 #pragma once
 
 #include "int4.cuh"
@@ -28,12 +49,22 @@ namespace akv {
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kAttnEntries = 1024;  // (row, row tile) pairs of one launch
-constexpr int kAttnUnits = 16384;    // units of one launch
-constexpr int kAttnMinPages = 8;    // pages of a CTA's share, at least (two per warp) where a unit has them
-constexpr int kAttnWhole = 32;       // pages up to which no unit is split
-constexpr int kAttnSetup = 16;       // pages that such a unit's set-up counts for
-constexpr int kAttnFused = 1024;    // partial rows of a unit that its last CTA merges by itself
-constexpr float kLazyLog2 = 6.f;    // weights may reach 2^6 before the maximum moves
+constexpr int kAttnUnits = 16384;   // units of one launch
+// Pages of a CTA's share, at least (two per warp): with 4 more parts are merged,
+// with 16 a share takes longer (1 x 4K tokens 15.3 / 14.6 / 16.6 us, 1 x 32K
+// 30.9 / 22.7 / 20.6 us with 4 / 8 / 16).
+constexpr int kAttnMinPages = 8;
+// Up to this many pages no unit is split, where all are so short (64 x 100-300
+// tokens: 24.7 us split, 18.5 us whole; 64 x 400-1000 32.8 and 30.8).
+constexpr int kAttnWhole = 32;
+// The pages that such a unit's set-up counts for in its share (90 short rows of
+// 12 drafted tokens: 107 us with 0, 80 with 4, 72 with 8 and 16; 64 x 100-300
+// tokens 18.5, 18.6, 16.5 and 15.5).
+constexpr int kAttnSetup = 16;
+constexpr int kAttnFused = 1024;  // partial rows of a unit that its last CTA merges by itself
+// Weights may reach 2^6 before the maximum moves: the rescaling of the sums
+// becomes rare, and fp16 holds such weights with the same relative error.
+constexpr float kLazyLog2 = 6.f;
 
 struct Int4AttnParams {
   akv_int4_cache c;
@@ -102,6 +133,7 @@ struct AttnShape {
   static constexpr int OCC = attn_occ(D, NT);
   static constexpr int smem(int entries) { return OFF_PREF + (3 * entries + 1) * 4; }
   static_assert(OCC * (smem(64) + 1024) <= 228 * 1024, "resident CTAs do not fit");
+  static_assert(kAttnFused * 4 + ROWS * 8 <= BUF, "the merge of a unit's parts does not fit the buffer");
 };
 
 // token of tile row g: a permutation within 8 that spreads the V loads of the
