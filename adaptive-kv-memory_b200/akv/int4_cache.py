@@ -110,6 +110,8 @@ class Int4PagedCache:
 
     def set_page_state(self, state: torch.Tensor) -> None:
         """The bookkeeping put back as ``page_state`` returned it (the pages' bytes are not touched)."""
+        if state.shape != self._state.shape or state.dtype is not torch.int32:
+            raise ValueError("the state does not match the cache")
         self._state.copy_(state)
 
     def load_state(self, buf: torch.Tensor, table: torch.Tensor, lens: torch.Tensor) -> None:
@@ -117,6 +119,8 @@ class Int4PagedCache:
         counts follow from the table."""
         if buf.shape != self.buf.shape or table.shape != self.table.shape or lens.shape != self.lens.shape:
             raise ValueError("the state's shapes do not match the cache")
+        if int(lens.min()) < 0 or int(lens.max()) > self.max_blocks * BLOCK:
+            raise ValueError(f"a length is outside 0 to {self.max_blocks * BLOCK}")
         t = table.to(self.device)
         used = torch.arange(self.max_blocks, device=self.device)[None, :] < \
             ((lens.to(self.device).long() + BLOCK - 1) // BLOCK)[:, None]

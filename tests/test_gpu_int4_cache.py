@@ -110,6 +110,43 @@ def test_append_special_values():
         assert (err <= step * (0.5 + 15 * 2.0 ** -11) + 2.0 ** -10 * r.abs().amax(1) + 1e-7).all()
 
 
+@pytest.mark.parametrize("dim,group", [(64, 16), (128, 32), (128, 128), (256, 128)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_append_unusual_tokens_among_ordinary_ones(dim, group, dtype):
+    """NaN, infinities, a range past fp16's, a rounded-up minimum or a scale without its bits in single tokens:
+    they get the formula's codes, and their neighbours what they get alone."""
+    k = _rand((1, 2, 37, dim), 31, dtype)
+    k[0, :, 20] = 0
+    odd = k.clone()
+    odd[0, 0, 2, 5] = float("nan")
+    odd[0, 1, 7, 0], odd[0, 1, 7, group - 1] = float("inf"), -float("inf")
+    odd[0, 0, 11, 9] = -float("inf")
+    odd[0, 1, 13] *= 1e-6                   # the scale below fp16's normal range
+    odd[0, 0, 18] = odd[0, 0, 18].abs() + 1.0000001e-7
+    if dtype is torch.bfloat16:
+        odd[0, 1, 22, 4], odd[0, 0, 30] = 1e5, 70000.0
+        odd[0, 0, 26] = odd[0, 0, 26].abs() * 1e-5 + 1.1e-7  # minima that fp16 does not hold
+    a, b, c = (_cache(heads=2, dim=dim, group=group) for _ in range(3))
+    for cache, x in ((a, k), (b, odd)):
+        cache.append(0, x, x, [0], cache.reserve([0], 37))
+        cache.check()
+    for t in range(37):
+        c.append(0, odd[:, :, t:t + 1], odd[:, :, t:t + 1], [0], c.reserve([0], 1))
+    assert torch.equal(b.buf, c.buf)        # in one call and one at a time
+    same = (k == odd).all(-1)[0].cpu()
+    for t in range(37):
+        for h in range(2):
+            f, g = _fields(b, 0, t // 32, h, t % 32), _fields(a, 0, t // 32, h, t % 32)
+            if same[h, t]:
+                assert all((x == y).all() for x, y in zip(f, g))
+            q, s, z = _np_quantise(odd[0, h, t].double().cpu().numpy(), group)
+            np.testing.assert_array_equal(f[2][:, 0], s)
+            np.testing.assert_array_equal(f[2][:, 1], z)
+            near = np.abs(q - f[0]) <= 0.5 * (1 + 2.0 ** -20)
+            assert near.all() or (f[0][~near] == q[~near].round().clip(0, 15)).all()
+            assert (f[0] == f[1]).all() and (f[2] == f[3]).all()
+
+
 @pytest.mark.parametrize("layout", ["token_major", "odd_stride", "odd_offset", "last_dim"])
 def test_append_strides(layout):
     a, b = _cache(heads=2), _cache(heads=2)
@@ -415,3 +452,19 @@ def test_refusals():
     assert c.attend(0, q[:0], []).shape == (0, 4, 1, 128)
     assert c.attend(0, q[:, :, :0]).shape == (2, 4, 0, 128)
     c.check()
+
+
+def test_state_refusals():
+    c = _filled([64, 40], 128, 128)
+    state = c.page_state()
+    for bad in (-1, c.max_blocks * 32 + 1):
+        lens = c.lens.clone()
+        lens[1] = bad
+        with pytest.raises(ValueError):
+            c.load_state(c.buf, c.table, lens)
+    for bad in (state[:1], state[:-1], state.long()):
+        with pytest.raises(ValueError):
+            c.set_page_state(bad)
+    assert torch.equal(c.page_state(), state)
+    c.set_page_state(state)
+    assert torch.equal(c.page_state(), state)
