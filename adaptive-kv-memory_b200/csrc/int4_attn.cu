@@ -15,7 +15,7 @@ struct Plan {
 Plan attn_plan(int R, int M, int Hq, int kv_heads, int D, int max_blocks) {
   Plan p{};
   const int q_rows = M * (Hq / kv_heads);
-  p.nt = attn_nt(D, q_rows);
+  p.nt = attn_nt(q_rows);
   p.tiles = (q_rows + 8 * p.nt - 1) / (8 * p.nt);
   p.rows = kAttnEntries / p.tiles;
   const int64_t row_pages = static_cast<int64_t>(p.tiles) * kv_heads * max_blocks;

@@ -1032,10 +1032,9 @@ __global__ void __launch_bounds__(128) int4_combine_kernel(const Int4AttnParams 
 constexpr int kSMs = 148;
 
 // column tiles of 8 query rows for `rows` rows of a (sequence, KV head)
-inline int attn_nt(int D, int rows) {
+inline int attn_nt(int rows) {
   return rows <= 8 ? 1 : 2;
 }
-
 
 template <int D, int G, int NT, int LO>
 int attn_launch(const Int4AttnParams& p, cudaStream_t st) {

@@ -12,10 +12,11 @@
 // the row and page lookups are paid once.
 //
 // Measured (4 x 32,767 tokens, 8 heads of 128, bf16, groups of 32; 688 MB moved
-// by each direction's kernel): append 170 us (3.9 TB/s; some 120 instructions
-// per 8 values, issue slots 70 %: the exact quotients bound it), read 109 us
-// (6.1 TB/s: memory).  Fewer rows in flight (2) or fewer CTAs (3 an SM) cost
-// append 3 to 5 %.
+// by each direction's kernel): append 138 us (5.0 TB/s; 91 instructions per 8
+// values, issue slots 64 %, the rest waits for loads), read 109 us (6.1 TB/s:
+// memory).  Append with the unusual groups looked for in every row instead of
+// once for four: 147; two rows in flight: 164; three CTAs an SM, no spills: 155;
+// five: 159.
 #include <type_traits>
 
 #include "int4.cuh"
@@ -43,7 +44,7 @@ constexpr int kReadUnroll = 8;  // read (a quarter of the bytes a step)
 // The call tokens of row i that lie on one page: block `blk` of the pages that
 // its tokens start on.  Token m of the call is at position pos0 + m.
 struct IoPage {
-  int seq, page;
+  int page;
   int m0, m1;   // call tokens on it
   int end;      // those from here on do not exist (yet)
   int slot0;    // slot of token m0
@@ -53,7 +54,6 @@ AKV_DEV IoPage io_page(const Int4Io& a, int i, int blk, bool write) {
   int* status = threadIdx.x == 0 ? a.status : nullptr;
   const Int4Row row = int4_row(a.c, a.rows, a.n_new, i, a.M, status);
   IoPage t;
-  t.seq = row.seq;
   t.page = -1;
   const int64_t pos0 = a.start ? static_cast<int64_t>(a.start[i]) : static_cast<int64_t>(row.len) - row.n_new;
   const int64_t b0 = pos0 >= 0 ? pos0 / kBlockTokens : -((kBlockTokens - 1 - pos0) / kBlockTokens);  // floor
@@ -84,7 +84,7 @@ AKV_DEV float div_by(float x, float s, float r) {
   return __fmaf_rn(__fmaf_rn(-s, q, x), r, q);
 }
 
-// the float nearest 1/s for an fp16 value s > 0
+// the float nearest 1/s for an fp16 value s > 0: Newton's step on an estimate
 AKV_DEV float recip(float s) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
@@ -105,52 +105,57 @@ AKV_DEV uint32_t max2(uint32_t a, uint32_t b) {
   else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// the same, but NaN where either is
+template <bool BF>
+AKV_DEV uint32_t min2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (BF) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <bool BF>
+AKV_DEV uint32_t max2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (BF) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
-// Eight channels of a group spread over gl threads: codes (word in the
-// record's byte order), scale and zero.  All lanes of the warp take part.
-template <bool BF, int gl>
-AKV_DEV uint32_t quantise8(uint4 raw, __half2& sz) {
+template <bool BF>
+AKV_DEV void floats_of(uint4 raw, float (&x)[8]) {
   const uint32_t e[4] = {raw.x, raw.y, raw.z, raw.w};
-  // a bit 15 / 31 where an element is NaN, infinite or past 65504
-  constexpr uint32_t PAST = BF ? 0x38803880u : 0x04000400u;
-  uint32_t odd = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) odd |= (e[j] & 0x7FFF7FFFu) + PAST;
-  float x[8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     x[2 * j] = elem_to_float<BF>(static_cast<uint16_t>(e[j]));
     x[2 * j + 1] = BF ? __uint_as_float(e[j] & 0xFFFF0000u) : elem_to_float<BF>(static_cast<uint16_t>(e[j] >> 16));
   }
-  float lo, hi;
-  if (__any_sync(~0u, (odd & 0x80008000u) != 0)) {
-    // NaN counts as 0, anything past fp16's range as its end
+}
+
+// (minimum, negated maximum) of a group spread over gl threads as one 16-bit
+// pair: NaN where an element is, for the caller to see
+template <bool BF, int gl>
+AKV_DEV uint32_t group_range(uint4 e) {
+  const uint32_t a2 = min2_nan<BF>(min2_nan<BF>(e.x, e.y), min2_nan<BF>(e.z, e.w));
+  const uint32_t b2 = max2_nan<BF>(max2_nan<BF>(e.x, e.y), max2_nan<BF>(e.z, e.w)) ^ 0x80008000u;
+  uint32_t p = min2_nan<BF>(prmt(a2, b2, 0x5410), prmt(a2, b2, 0x7632));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = x[j] == x[j] ? fminf(fmaxf(x[j], -65504.f), 65504.f) : 0.f;
-    lo = hi = x[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]);
-#pragma unroll
-    for (int o = 1; o < gl; o <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
-    }
-  } else {
-    // (minimum, negated maximum) of the group as one 16-bit pair
-    const uint32_t a2 = min2<BF>(min2<BF>(e[0], e[1]), min2<BF>(e[2], e[3]));
-    const uint32_t b2 = max2<BF>(max2<BF>(e[0], e[1]), max2<BF>(e[2], e[3])) ^ 0x80008000u;
-    uint32_t p = min2<BF>(prmt(a2, b2, 0x5410), prmt(a2, b2, 0x7632));
-#pragma unroll
-    for (int o = 1; o < gl; o <<= 1) p = min2<BF>(p, __shfl_xor_sync(~0u, p, o));
-    lo = elem_to_float<BF>(static_cast<uint16_t>(p));
-    hi = -elem_to_float<BF>(static_cast<uint16_t>(p >> 16));
-  }
-  const __half zh = __float2half_rn(lo);
-  const float z = __half2float(zh);
-  const __half sh = __float2half_rn(div_by(__fsub_rn(hi, z), 15.f, 1.f / 15.f));
-  const float s = __half2float(sh);
+  for (int o = 1; o < gl; o <<= 1) p = min2_nan<BF>(p, __shfl_xor_sync(~0u, p, o));
+  return p;
+}
+
+// the scale of values from z to hi; the (scale, zero) of values from lo to hi
+AKV_DEV __half scale_of(float z, float hi) { return __float2half_rn(div_by(__fsub_rn(hi, z), 15.f, 1.f / 15.f)); }
+
+AKV_DEV __half2 scale_zero(float lo, float hi) {
+  const __half z = __float2half_rn(lo);
+  return __halves2half2(scale_of(__half2float(z), hi), z);
+}
+
+// Codes of eight channels (word in the record's byte order).
+template <bool CLAMP>
+AKV_DEV uint32_t codes8(const float (&x)[8], __half2 sz) {
+  const float s = __low2float(sz), z = __high2float(sz);
   const float r = s > 0.f ? recip(s) : 0.f;  // scale 0: every quotient 0
-  sz = __halves2half2(sh, zh);
   // 1.5 * 2^23 + quotient: the sum rounds half to even and holds the code in its low bits
   const uint64_t nz = f2_make(-z, -z), r2 = f2_make(r, r), ns = f2_make(-s, -s), magic = f2_make(12582912.f, 12582912.f);
   float c[8];
@@ -162,9 +167,7 @@ AKV_DEV uint32_t quantise8(uint4 raw, __half2& sz) {
     const float2 v = f2_split(f2_add(q, magic));
     c[2 * j] = v.x, c[2 * j + 1] = v.y;
   }
-  // Quotients leave [0, 15.5) only where the zero was rounded up or the scale
-  // has lost bits (below fp16's normal range).
-  if (__any_sync(~0u, z > lo || s < 6.103515625e-5f)) {
+  if constexpr (CLAMP) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) c[j] = fminf(fmaxf(c[j], 12582912.f), 12582927.f);
   }
@@ -178,6 +181,66 @@ AKV_DEV uint32_t quantise8(uint4 raw, __half2& sz) {
   w = w * 16u + __float_as_uint(c[0]);
   w = w * 16u + __float_as_uint(c[1]);
   return w - 0x4B400000u * 0x11111111u;
+}
+
+// Steps with NaN, elements past fp16's range, or quotients past the codes: NaN
+// counts as 0, anything out of range as its end.
+template <bool BF, int gl>
+AKV_DEV uint32_t quantise8_any(uint4 raw, __half2& sz) {
+  float x[8];
+  floats_of<BF>(raw, x);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = x[j] == x[j] ? fminf(fmaxf(x[j], -65504.f), 65504.f) : 0.f;
+  float lo = x[0], hi = x[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]);
+#pragma unroll
+  for (int o = 1; o < gl; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
+  }
+  sz = scale_zero(lo, hi);
+  return codes8<true>(x, sz);
+}
+
+// kIoUnroll steps of eight channels a thread, each group spread over gl
+// threads; one vote sends the unusual ones to the general form.  All lanes of
+// the warp take part.
+template <bool BF, int gl, class Store>
+AKV_DEV void quantise_steps(const uint4 (&raw)[kIoUnroll], Store store) {
+  constexpr uint32_t PAST = BF ? 0x38803880u : 0x04000400u;  // carries into bits 15 / 31 past 65504, and for NaN
+  __half2 sz[kIoUnroll];
+  bool odd = false;
+#pragma unroll
+  for (int u = 0; u < kIoUnroll; ++u) {
+    const uint32_t p = group_range<BF, gl>(raw[u]);
+    const float lo = elem_to_float<BF>(static_cast<uint16_t>(p));
+    const float hi = -elem_to_float<BF>(static_cast<uint16_t>(p >> 16));
+    odd |= (((p & 0x7FFF7FFFu) + PAST) & 0x80008000u) != 0;
+    // quotients leave [0, 15.5) only where the zero was rounded up (an fp16
+    // minimum is its own zero) or the scale has lost bits (below the normal range)
+    if constexpr (BF) {
+      sz[u] = scale_zero(lo, hi);
+      odd |= __high2float(sz[u]) > lo;
+    } else {
+      sz[u] = __halves2half2(scale_of(lo, hi), __ushort_as_half(static_cast<uint16_t>(p)));
+    }
+    odd |= __half_as_ushort(__low2half(sz[u])) - 1u < 0x3FFu;
+  }
+  if (__any_sync(~0u, odd)) {
+#pragma unroll
+    for (int u = 0; u < kIoUnroll; ++u) {
+      const uint32_t w = quantise8_any<BF, gl>(raw[u], sz[u]);
+      store(u, w, sz[u]);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < kIoUnroll; ++u) {
+      float x[8];
+      floats_of<BF>(raw[u], x);
+      store(u, codes8<false>(x, sz[u]), sz[u]);
+    }
+  }
 }
 
 // A CTA takes one page of one call row, a warp one (head, K / V) of it at a
@@ -208,7 +271,7 @@ __global__ void __launch_bounds__(kIoThreads, 4) int4_append_kernel(const Int4Io
       for (int u = 0; u < kIoUnroll; ++u) {
         if (!WHOLE) raw[u] = make_uint4(0u, 0u, 0u, 0u);
         if (WHOLE || m + u * TW + tw < n) {
-          const uint16_t* p = src + (m + u * TW) * sm;
+          const uint16_t* p = src + u * (TW * sm);
           if constexpr (AL) {
             raw[u] = ldg_nc_v4(p);
           } else {
@@ -219,16 +282,15 @@ __global__ void __launch_bounds__(kIoThreads, 4) int4_append_kernel(const Int4Io
           }
         }
       }
-#pragma unroll
-      for (int u = 0; u < kIoUnroll; ++u) {
-        if (!WHOLE && m + u * TW >= n) break;  // the whole warp
-        __half2 sz;
-        const uint32_t w = quantise8<BF, gl>(raw[u], sz);
+      quantise_steps<BF, gl>(raw, [&](int u, uint32_t w, __half2 sz) {
         if (WHOLE || m + u * TW + tw < n) {
-          *reinterpret_cast<uint32_t*>(codes + (m + u * TW) * (D / 2)) = w;
-          if (lead) *reinterpret_cast<__half2*>(pairs + (m + u * TW) * G * 4) = sz;
+          *reinterpret_cast<uint32_t*>(codes + u * (TW * D / 2)) = w;
+          if (lead) *reinterpret_cast<__half2*>(pairs + u * (TW * G * 4)) = sz;
         }
-      }
+      });
+      src += TW * kIoUnroll * sm;
+      codes += TW * kIoUnroll * (D / 2);
+      pairs += TW * kIoUnroll * G * 4;
     };
     int m = 0;
     for (; m + TW * kIoUnroll <= n; m += TW * kIoUnroll) round(m, std::true_type{});
