@@ -205,7 +205,7 @@ class Int4PagedCache:
             n_new = 0
         if rows is None and n > _ROWS_PER_CALL:
             rows = torch.arange(n, dtype=torch.int32, device=self._dev)
-        granted = torch.empty(n, dtype=torch.int32, device=self._dev)
+        granted = torch.empty_strided((n,), (1,), dtype=torch.int32, device=self._dev)
         rp, cp, gp = _C.ptr(rows), _C.ptr(counts), granted.data_ptr()
         stream = _C.raw_stream(self._dev_index)
         for a in range(0, n, _ROWS_PER_CALL):
@@ -249,7 +249,7 @@ class Int4PagedCache:
 
     def compact(self) -> torch.Tensor:
         """Live pages moved to the low end of the pool, tables following.  Returns their number (int32, device)."""
-        live = torch.empty(1, dtype=torch.int32, device=self._dev)
+        live = torch.empty_strided((1,), (1,), dtype=torch.int32, device=self._dev)
         rc = self._lib.akv_pages_compact(self._pt_ref, self._pool_ptr, self.n_layers, self._layer_bytes,
                                          self._page_bytes, live.data_ptr(), self._page_ws_ptr, self._page_ws_bytes,
                                          self._status_ptr, _C.raw_stream(self._dev_index))
@@ -312,15 +312,17 @@ class Int4PagedCache:
         R = self.max_seqs if given is None else len(given)
         rows, n_new, rp, np_ = self._rows(rows, n_new, R)
         start = self._ints(start, "start", R)
-        kv = torch.empty((2, R, self.H, n_tokens, self.D), dtype=dtype, device=self._dev)
-        k, v = kv.unbind(0)
+        shape = (R, self.H, n_tokens, self.D)
         sm = self.D
         sh = sm * n_tokens
         sr = sh * self.H
-        kp = kv.data_ptr()
+        # empty_strided: 1.5 us of host time, torch.empty with its keywords 2.3
+        k = torch.empty_strided(shape, (sr, sh, sm, 1), dtype=dtype, device=self._dev)
+        v = torch.empty_strided(shape, (sr, sh, sm, 1), dtype=dtype, device=self._dev)
         rc = self._lib.akv_int4_read(
-            _C.IO_ARGS.pack(view, rp, np_, 0 if start is None else start.data_ptr(), kp, sr, sh, sm, kp + 2 * sr * R,
-                            sr, sh, sm, self._status_ptr, R, n_tokens, dt, 0), _C.raw_stream(self._dev_index))
+            _C.IO_ARGS.pack(view, rp, np_, 0 if start is None else start.data_ptr(), k.data_ptr(), sr, sh, sm,
+                            v.data_ptr(), sr, sh, sm, self._status_ptr, R, n_tokens, dt, 0),
+            _C.raw_stream(self._dev_index))
         if rc:
             _C.check(rc, "akv_int4_read")
         return k, v
@@ -359,7 +361,8 @@ class Int4PagedCache:
             os_ = o.stride()
             if o.shape != shape or o.dtype is not q.dtype or os_[-1] != 1 or o.device != self._dev:
                 raise ValueError("out must have the query's shape, type and device, its last dim contiguous")
-        lse = torch.empty(shape[:3], dtype=torch.float32, device=self._dev) if return_lse else None
+        lse = torch.empty_strided((R, Hq, M), (Hq * M, M, 1), dtype=torch.float32,
+                                  device=self._dev) if return_lse else None
         stream = _C.raw_stream(self._dev_index)
         key = (R, M, Hq)
         need = self._ws_need.get(key)

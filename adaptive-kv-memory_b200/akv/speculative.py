@@ -68,8 +68,9 @@ def verify_draft(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor]
     if status is not None and (status.dtype is not torch.int32 or status.device != dev):
         raise ValueError(f"status must be int32 on {dev}")
     x, au, su = x.contiguous(), au.contiguous(), su.contiguous()
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
-    out = torch.empty((B, K1), dtype=torch.int64, device=dev)
+    # empty_strided: 1.5 us of host time, torch.empty with its keywords 2.3
+    accepted = torch.empty_strided((B,), (1,), dtype=torch.int32, device=dev)
+    out = torch.empty_strided((B, K1), (K1, 1), dtype=torch.int64, device=dev)
     rc = _C.load().akv_verify_draft(
         _C.VERIFY_ARGS.pack(p.data_ptr(), ps[0], ps[1], qp, qs[0], qs[1], x.data_ptr(),
                             0 if nd is None else nd.data_ptr(), au.data_ptr(), su.data_ptr(), accepted.data_ptr(),

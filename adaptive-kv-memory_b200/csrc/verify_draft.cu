@@ -110,7 +110,8 @@ AKV_DEV uint64_t warp_scan_u64(uint64_t x) {
 }
 
 template <int DT, bool DRAFT, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == kVerifyMany ? 4 : 1) verify_kernel(VerifyParams P) {
+__global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(THREADS, THREADS == kVerifyMany ? 4 : 1)
+    verify_kernel(VerifyParams P) {
   constexpr int WARPS = THREADS / 32;
   static_assert(WARPS <= 32, "a lane stands for a warp's sum");
   using E = ProbElem<DT>;
@@ -322,19 +323,10 @@ using namespace akv;
 
 template <int DT, int THREADS>
 static cudaError_t verify_launch(const VerifyParams& p, int B, cudaStream_t st) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(kVerifyCluster, B);
-  cfg.blockDim = dim3(THREADS);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = kVerifyCluster;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return p.draft ? cudaLaunchKernelEx(&cfg, verify_kernel<DT, true, THREADS>, p)
-                 : cudaLaunchKernelEx(&cfg, verify_kernel<DT, false, THREADS>, p);
+  const dim3 grid(kVerifyCluster, B);
+  if (p.draft) verify_kernel<DT, true, THREADS><<<grid, THREADS, 0, st>>>(p);
+  else verify_kernel<DT, false, THREADS><<<grid, THREADS, 0, st>>>(p);
+  return cudaGetLastError();
 }
 
 // Measured (151,936 fp32 probabilities, draft and target; us with 512 / 256
