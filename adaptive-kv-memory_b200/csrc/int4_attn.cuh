@@ -42,6 +42,8 @@
 // CTAs' worth of shares.
 #pragma once
 
+#include <type_traits>
+
 #include "int4.cuh"
 
 namespace akv {
@@ -782,6 +784,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
           constexpr int NW = S::BV < 4 ? 1 : S::BV / 4;
           uint32_t va[2][NW], vb[2][NW];  // the two tokens of each 8-token tile
           uint32_t vs2[2], vz2[2];        // AV: their scales, zeros + 8 scales
+          uint32_t far = 0u;              // AV: the furthest that a code may lie from 0
 #pragma unroll
           for (int T = 0; T < 2; ++T) {
             const int t0 = (2 * kk + T) * 8 + tile_token(2 * q4), t1 = (2 * kk + T) * 8 + tile_token(2 * q4 + 1);
@@ -797,35 +800,51 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
               }
               vs2[T] = prmt(w0, w1, 0x5410);
               vz2[T] = h2_as_u32(__hfma2(u32_as_h2(vs2[T]), u32_as_h2(0x48004800u), u32_as_h2(prmt(w0, w1, 0x7632))));
+              const __half2 reach = __hfma2(u32_as_h2(vs2[T]), u32_as_h2(0x48004800u), __habs2(u32_as_h2(vz2[T])));
+              far = h2_as_u32(__hmax2(u32_as_h2(far), reach));
             }
           }
-          auto value = [&](uint32_t c, int T) -> uint32_t {
-            if constexpr (S::AV) return h2_as_u32(__hfma2(u32_as_h2(c), u32_as_h2(vs2[T]), u32_as_h2(vz2[T])));
-            return c;
-          };
-          // two channels' bytes at a time: the two terms of a sum stand apart
+          auto products = [&](auto held) {
+            auto value = [&](uint32_t c, int T) -> uint32_t {
+              if constexpr (!S::AV) return c;
+              __half2 v = __hfma2(u32_as_h2(c), u32_as_h2(vs2[T]), u32_as_h2(vz2[T]));
+              if constexpr (decltype(held)::value) v = __hmax2(__hmin2(v, u32_as_h2(0x7BFF7BFFu)), u32_as_h2(0xFBFFFBFFu));
+              return h2_as_u32(v);
+            };
+            // two channels' bytes at a time: the two terms of a sum stand apart
 #pragma unroll
-          for (int b0 = 0; b0 < S::BV; b0 += 2) {
-            constexpr int BB = S::BV < 2 ? 1 : 2;
-            uint32_t a[BB][4];
+            for (int b0 = 0; b0 < S::BV; b0 += 2) {
+              constexpr int BB = S::BV < 2 ? 1 : 2;
+              uint32_t a[BB][4];
 #pragma unroll
-            for (int b2 = 0; b2 < BB; ++b2) {
-              const int b = b0 + b2;
-              // bytes b of both tokens, the first in the low half
-              const uint32_t y0 = prmt(va[0][b / 4], vb[0][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
-              const uint32_t y1 = prmt(va[1][b / 4], vb[1][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
-              a[b2][0] = value(low_code(y0), 0), a[b2][1] = value(high_code(y0), 0);
-              a[b2][2] = value(low_code(y1), 1), a[b2][3] = value(high_code(y1), 1);
+              for (int b2 = 0; b2 < BB; ++b2) {
+                const int b = b0 + b2;
+                // bytes b of both tokens, the first in the low half
+                const uint32_t y0 = prmt(va[0][b / 4], vb[0][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
+                const uint32_t y1 = prmt(va[1][b / 4], vb[1][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
+                a[b2][0] = value(low_code(y0), 0), a[b2][1] = value(high_code(y0), 0);
+                a[b2][2] = value(low_code(y1), 1), a[b2][3] = value(high_code(y1), 1);
+              }
+#pragma unroll
+              for (int term = 0; term < (LO == 1 ? 2 : 1); ++term)
+#pragma unroll
+                for (int b2 = 0; b2 < BB; ++b2)
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+                    mma_16816(O[nt][gi * S::BV + b0 + b2], a[b2][0], a[b2][1], a[b2][2], a[b2][3],
+                              term ? pl[LO == 1 ? 2 * kk : 0][LO == 1 ? nt : 0] : pb[2 * kk][nt],
+                              term ? pl[LO == 1 ? 2 * kk + 1 : 0][LO == 1 ? nt : 0] : pb[2 * kk + 1][nt]);
             }
-#pragma unroll
-            for (int term = 0; term < (LO == 1 ? 2 : 1); ++term)
-#pragma unroll
-              for (int b2 = 0; b2 < BB; ++b2)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                  mma_16816(O[nt][gi * S::BV + b0 + b2], a[b2][0], a[b2][1], a[b2][2], a[b2][3],
-                            term ? pl[LO == 1 ? 2 * kk : 0][LO == 1 ? nt : 0] : pb[2 * kk][nt],
-                            term ? pl[LO == 1 ? 2 * kk + 1 : 0][LO == 1 ? nt : 0] : pb[2 * kk + 1][nt]);
+          };
+          // Codes 0 and 15 of a group that append held to +-65504 can round to
+          // infinity, and a token that a query does not see has weight 0 times
+          // that.  Where the sum 8 s + |z + 8 s| is infinite (no code's value is
+          // otherwise) the warp takes the values with a clamp.
+          if constexpr (S::AV) {
+            if (__any_sync(~0u, max(far & 0x7FFFu, far >> 16) >= 0x7C00u)) products(std::true_type{});
+            else products(std::false_type{});
+          } else {
+            products(std::false_type{});
           }
         }
       }
