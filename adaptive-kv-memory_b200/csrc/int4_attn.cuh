@@ -4,15 +4,17 @@
 // Mathematics.  With token t's value c*s_tg + z_tg in channel group g,
 //   q.K_t = sum_g  s_tg (q_g . c_tg) + z_tg sum(q_g)
 //   O     = sum_t p_t V_t
-//         = sum_t (p_t s_tg)(c - 8) + sum_t p_t (z_tg + 8 s_tg)
+//         = sum_t (p_t s_tg)(c - m_t) + sum_t p_t (z_tg + m_t s_tg)
 // so both contractions run on codes.  For K a code needs no conversion: alone
 // in bits 4..7 of a half it is the fp16 subnormal c * 2^-20, one shift and one
 // AND for two codes of a word.  (The MMA aligns its products by the operands'
 // nominal exponents and cuts them off, so bits 0..3 would lose 4 bits more of
 // the sum.)  Over the thousands of additions of P.V that cutting off is a
 // drift of the growing sum; there the codes are centred, exactly, by one fp16
-// operation more, and the sums stay as small as the output.  Online softmax,
-// maximum and sums in fp32.
+// operation more, and the sums stay as small as the output: m_t is 8 and 7 in
+// turn, 16 tokens each, since codes lie around 7.5 (with 8 alone a CTA that
+// takes 32K tokens of a row left an fp16 output 1.1 to 1.4 times as far off as
+// its own rounding; with both, 1.00).  Online softmax, maximum and sums in fp32.
 //
 // Roundings: q is scaled per row by a power of two into fp16's middle range
 // (exact unless 2^-24 of the row's largest).  p_t s_tg enters the MMA as one
@@ -142,17 +144,23 @@ struct AttnShape {
 // four thread columns over the banks (rows of both parities in every load)
 AKV_DEV int tile_token(int g) { return g ^ ((g >> 2) & 1); }
 
-// the codes in bits 0..3 (4..7) of both halves, as the fp16 pair c - 8
-AKV_DEV uint32_t low_code(uint32_t y) {
+// m_t for the tokens of each P.V step.  Codes lie around 7.5: with one of them
+// the sums would grow by half a scale a token, far past the output.
+AKV_DEV constexpr int code_centre(int step) { return step ? 7 : 8; }
+
+// the codes in bits 0..3 (4..7) of both halves, as the fp16 pair c - centre
+AKV_DEV uint32_t low_code(uint32_t y, int centre) {
+  const uint32_t back = 0x10001u * (0xE400u + centre);  // -(1024 + centre)
   uint32_t r;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(lop_magic<0x000F000Fu>(y)), "r"(0xE408E408u));  // 1024 + c - 1032
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(lop_magic<0x000F000Fu>(y)), "r"(back));  // 1024 + c - ...
   return r;
 }
-AKV_DEV uint32_t high_code(uint32_t y) {
+AKV_DEV uint32_t high_code(uint32_t y, int centre) {
+  const uint32_t back = 0x10001u * (0xD400u + 16 * centre);  // -(64 + centre)
   uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;"  // (1024 + 16 c) / 16 - 72
+  asm("fma.rn.f16x2 %0, %1, %2, %3;"  // (1024 + 16 c) / 16 - ...
       : "=r"(r)
-      : "r"(lop_magic<0x00F000F0u>(y)), "r"(0x2C002C00u), "r"(0xD480D480u));
+      : "r"(lop_magic<0x00F000F0u>(y)), "r"(0x2C002C00u), "r"(back));
   return r;
 }
 
@@ -748,8 +756,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
 #pragma unroll
           for (int gi = 0; gi < G; ++gi) {
             const float2 sz = __half22float2(u32_as_h2(vp[r][gi]));
-            const float z8 = fmaf(8.f, sz.x, sz.y);
-            const uint64_t z2 = f2_make(z8, z8);
+            const float mid = fmaf(static_cast<float>(code_centre(r / 2)), sz.x, sz.y);
+            const uint64_t z2 = f2_make(mid, mid);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) zs[nt][gi] = f2_fma(x[r][nt], z2, zs[nt][gi]);
           }
@@ -782,6 +790,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
           constexpr int NW = S::BV < 4 ? 1 : S::BV / 4;
+          const int mid = S::AV ? 8 : code_centre(kk);
           uint32_t va[2][NW], vb[2][NW];  // the two tokens of each 8-token tile
           uint32_t vs2[2], vz2[2];        // AV: their scales, zeros + 8 scales
           uint32_t far = 0u;              // AV: the furthest that a code may lie from 0
@@ -822,8 +831,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
                 // bytes b of both tokens, the first in the low half
                 const uint32_t y0 = prmt(va[0][b / 4], vb[0][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
                 const uint32_t y1 = prmt(va[1][b / 4], vb[1][b / 4], (b & 2) ? 0x7632 : 0x5410) >> (8 * (b & 1));
-                a[b2][0] = value(low_code(y0), 0), a[b2][1] = value(high_code(y0), 0);
-                a[b2][2] = value(low_code(y1), 1), a[b2][3] = value(high_code(y1), 1);
+                a[b2][0] = value(low_code(y0, mid), 0), a[b2][1] = value(high_code(y0, mid), 0);
+                a[b2][2] = value(low_code(y1, mid), 1), a[b2][3] = value(high_code(y1, mid), 1);
               }
 #pragma unroll
               for (int term = 0; term < (LO == 1 ? 2 : 1); ++term)
