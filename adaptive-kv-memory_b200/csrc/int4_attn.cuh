@@ -66,9 +66,13 @@ constexpr int kAttnWhole = 32;
 // tokens 18.5, 18.6, 16.5 and 15.5).
 constexpr int kAttnSetup = 16;
 constexpr int kAttnFused = 1024;  // partial rows of a unit that its last CTA merges by itself
-// Weights may reach 2^6 before the maximum moves: the rescaling of the sums
-// becomes rare, and fp16 holds such weights with the same relative error.
-constexpr float kLazyLog2 = 6.f;
+// The maximum's weight stands at 2^9, and weights may reach 2^15, fp16's last
+// binade, before the maximum moves: the rescaling of the sums becomes rare.
+// fp16 loses bits below 2^-14, so a weight keeps 11 of them down to 2^-23 of
+// the maximum, and the 22 of two terms down to 2^-12.  (With the maximum at 2^0
+// and 90 % of the weight on a token of value 0, the many small weights beside it
+// left the output off by 4 to 9 times its own rounding; with 99 %, by 40 to 150.)
+constexpr float kTopLog2 = 9.f, kMostLog2 = 15.f;
 
 struct Int4AttnParams {
   akv_int4_cache c;
@@ -726,10 +730,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
             for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
             const float cqc = c ? c2.y : c2.x, old = -(c ? n2.y : n2.x);
             const bool any = lim[nt][c] != -INFINITY;
-            float y = m == -INFINITY ? 0.f : m * cqc;
+            float y = m == -INFINITY ? 0.f : fmaf(m, cqc, -kTopLog2);
             if (any) y = fmaxf(y, old);
             f[c] = any ? exp2f(old - y) : 0.f;
-            if (any || m != -INFINITY) lim[nt][c] = (y + kLazyLog2) / cqc;
+            if (any || m != -INFINITY) lim[nt][c] = (y + kMostLog2) / cqc;
             (c ? n2.y : n2.x) = -y;
           }
           nm[nt] = f2_make(n2.x, n2.y);

@@ -86,6 +86,15 @@ def test_sums_over_many_tokens(hq, m, dtype):
     assert _one_prompt(0.0, True, hq, m, dtype) <= 1.1
 
 
+@pytest.mark.parametrize("share", [0.5, 0.9, 0.99])
+@pytest.mark.parametrize("own_value", [True, False])
+@pytest.mark.parametrize("hq,m,dtype", [(32, 1, torch.float16), (64, 1, torch.float16), (32, 4, torch.float16),
+                                        (64, 1, torch.bfloat16)])
+def test_most_of_the_weight_on_the_first_token(share, own_value, hq, m, dtype):
+    """The other tokens' weights, each a 32768th of what is left, still make the output as exact as its type."""
+    assert _one_prompt(share, own_value, hq, m, dtype) <= 1.1
+
+
 @pytest.mark.parametrize("dim,group", [(64, 64), (64, 32), (64, 16), (128, 128), (128, 64), (128, 32),
                                        (256, 256), (256, 128), (256, 64)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -100,3 +109,31 @@ def test_every_shape(dim, group, dtype, rep, m):
     out = c.attend(0, q)
     c.check()
     assert _ratio(out, _formula(*_fields(c, [0, 1]), q)[0]) <= 1.1
+
+
+@pytest.mark.parametrize("dim,group,dtype", [(64, 64, torch.float16), (128, 128, torch.float16),
+                                             (128, 32, torch.float16), (256, 128, torch.float16),
+                                             (128, 128, torch.bfloat16), (128, 32, torch.bfloat16)])
+@pytest.mark.parametrize("rep,m,where", [(4, 1, "light"), (8, 1, "light"), (4, 4, "light"), (4, 4, "unseen")])
+def test_one_token_of_much_larger_values(dim, group, dtype, rep, m, where):
+    """A token whose values are 3,000 times the others' and that hardly counts, or is the last new one."""
+    n = 1111
+    c = base._cache(1, 80, 2, dim, group, 2, 36)
+    g = torch.Generator(device=DEV).manual_seed(dim + group + m)
+    k, v = (torch.randn(2, 2, n, dim, generator=g, device=DEV) for _ in range(2))
+    q = torch.randn(2, 2 * rep, m, dim, generator=g, device=DEV)
+    v *= 0.01
+    q[..., 0], k[..., 0] = 4, 0
+    at = n - 1 if where == "unseen" else 500
+    v[:, :, at] *= 3000
+    if where == "light":
+        k[:, :, at] = 0
+        k[:, :, at, 0] = -20 * math.sqrt(dim) / 4            # its logit: -20
+    c.append(0, k.half(), v.half(), None, c.reserve(None, n))
+    q = q.to(dtype)
+    out = c.attend(0, q)
+    c.check()
+    ref = _formula(*_fields(c, [0, 1]), q)[0]
+    if where == "unseen":
+        out, ref = out[:, :, :-1], ref[:, :, :-1]
+    assert _ratio(out, ref) <= 1.1
