@@ -333,8 +333,9 @@ class Int4PagedCache:
 
         query (R, Hq, M, head_dim), or (R, Hq, head_dim) for one token, fp16 or bf16, any strides: query m of
         row i is its token lens - n_new[i] + m (``n_new`` None: M) and sees the tokens up to itself.  Queries
-        past n_new[i] give zero rows.  Returns the output in the query's shape, type and (where it is dense)
-        layout, and with ``return_lse`` the natural-log LSE (R, Hq, M) fp32."""
+        past n_new[i] give zero rows, queries with NaN or infinities rows of NaN.  Returns the output in the
+        query's shape, type and (where it is dense) layout, and with ``return_lse`` the natural-log LSE (R, Hq, M)
+        fp32."""
         view = self._layer(layer)
         dt = _half_dtype(query)
         one = query.dim() == 3

@@ -213,9 +213,10 @@ AKV_DEV int64_t out_row(const Int4AttnParams& P, int i, int hq, int m) {
 }
 
 // What a row's maximum (log2) and sum L make of its output: its lse, and the
-// factor of the sums of p V.  L 0: a row that sees nothing.
+// factor of the sums of p V.  L 0: a row that sees nothing.  L NaN (a query
+// that is not finite, scores past fp32): both NaN.
 AKV_DEV float2 row_scale(float top, float L) {
-  return L > 0.f ? make_float2((top + log2f(L)) * 0.6931471805599453f, 1.f / L) : make_float2(-INFINITY, 0.f);
+  return L == 0.f ? make_float2(-INFINITY, 0.f) : make_float2((top + log2f(L)) * 0.6931471805599453f, 1.f / L);
 }
 
 // Output channels of accumulator pair p (order of the merge buffer) of the row
@@ -225,7 +226,7 @@ AKV_DEV void store_pair(const Int4AttnParams& P, int64_t row, float* lse, int p,
   constexpr int GS = D / G, BV = GS / 16;
   const int j = p / 8, g = p % 8;
   const int ch = j / BV * GS + g * 2 * BV + 2 * (j % BV);
-  const bool on = scale.y > 0.f;
+  const bool on = scale.y != 0.f;
   v.x = on ? v.x * scale.y : 0.f;
   v.y = on ? v.y * scale.y : 0.f;
   uint16_t* o = P.out + row + ch;
@@ -306,7 +307,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
   float* s_qs = reinterpret_cast<float*>(smem + S::OFF_QS);
   float* s_cq = reinterpret_cast<float*>(smem + S::OFF_CQ);
   int* s_see = reinterpret_cast<int*>(smem + S::OFF_SEE);
-  int* s_on = reinterpret_cast<int*>(smem + S::OFF_ON);
+  float* s_on = reinterpret_cast<float*>(smem + S::OFF_ON);  // 1; 0 past n_new; NaN for a query that is not finite
   int* s_lse = reinterpret_cast<int*>(smem + S::OFF_LSE);
   int64_t* s_out = reinterpret_cast<int64_t*>(smem + S::OFF_OUT);
   float2* s_ml = reinterpret_cast<float2*>(smem + S::OFF_ML);
@@ -501,23 +502,23 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
         const int n = k2 * kAttnWarps + warp;
         const int nr = tile_row<LO>(n), m = (tile * S::ROWS + nr) / rep;
         float x[PER];
-        float top = 0.f;
+        uint32_t top = 0u;  // bits of the largest magnitude: infinity, then NaN, above all others
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
           x[k] = P.bf16 ? elem_to_float<true>(raw[k2][k]) : elem_to_float<false>(raw[k2][k]);
-          top = fmaxf(top, fabsf(x[k]));
+          top = max(top, __float_as_uint(x[k]) & 0x7FFFFFFFu);
         }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        top = __reduce_max_sync(~0u, top);
+        const bool bad = top >= 0x7F800000u;  // no softmax: computed as zeros, NaN at the end
         int ex = 0;  // 2^ex brings the largest into [2^9, 2^10)
-        if (top > 0.f) ex = 9 - (static_cast<int>(__float_as_uint(top) >> 23) - 127);
+        if (top && !bad) ex = 9 - (static_cast<int>(top >> 23) - 127);
         ex = ex > 120 ? 120 : (ex < -120 ? -120 : ex);
         const float up = exp2f(static_cast<float>(ex)) * (P.scale < 0.f ? -1.f : 1.f);
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
           const int c = lane * PER + k;
-          const __half hv = __float2half_rn(x[k] * up);
+          const __half hv = __float2half_rn(bad ? 0.f : x[k] * up);
           sum += __half2float(hv);
           const int gi = c / S::GS, r = c % S::GS, col = r / (S::GS / 4), r2 = r % (S::GS / 4);
           int ks, reg, half;
@@ -538,8 +539,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
         if (lane == 0) {
           // log2 e * scale in units of the MMA result; never 0, so that -inf stays -inf
           s_cq[n] = fmaxf(ldexpf(fabsf(P.scale) * 1.4426950408889634f, 20 - ex), 1e-37f);
-          s_see[n] = len - n_new + (m < n_new ? m : n_new - 1) + 1;
-          s_on[n] = m < n_new;
+          const int see = len - n_new + (m < n_new ? m : n_new - 1) + 1;
+          s_see[n] = see;
+          s_on[n] = m < n_new ? (bad && see > 0 ? NAN : 1.f) : 0.f;
           if (m < P.M) {
             const int hq = h * rep + (tile * S::ROWS + nr) - m * rep;
             s_out[n] = out_row(P, i, hq, m);
@@ -907,7 +909,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, G, NT, LO>::OCC) in
         const float2 a = s_ml[w * S::ROWS + t];
         if (a.x != -INFINITY) L = fmaf(a.y, exp2f(a.x - top), L);
       }
-      if (!s_on[t]) L = 0.f;
+      if (s_on[t] != 1.f) L = s_on[t];
       s_tl[t] = whole ? row_scale(top, L) : make_float2(top, L);
     }
     float* merge = reinterpret_cast<float*>(smem);

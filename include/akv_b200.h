@@ -690,7 +690,8 @@ int akv_int4_read(const akv_int4_io_args* a, void* stream);
 /* Attention of M query tokens per call row over its sequence.  Query m <
  * n_new[i] stands at position lens - n_new + m and sees every token up to its
  * own; a query with m >= n_new[i], or that sees no token, gets a zero row and
- * lse -inf.  q element (i, hq, m, d) at q + i*q_sr + hq*q_sh + m*q_sm + d, out
+ * lse -inf; one that is not finite, or whose scores pass fp32's range, a row of
+ * NaN and lse NaN.  q element (i, hq, m, d) at q + i*q_sr + hq*q_sh + m*q_sm + d, out
  * alike, both dtype AKV_FP16 or AKV_BF16; lse fp32 [R][Hq][M] (nullable,
  * natural log).  Query head hq reads KV head hq / (Hq / kv_heads).
  * Workspace: akv_int4_attention_workspace_bytes(...), 16-byte aligned, zeroed
