@@ -18,12 +18,14 @@ and ``fork`` / ``free`` / ``compact`` manage whole sequences.  Page tables,
 lengths and reference counts live on the device and every call is a few
 launches on the current stream: nothing waits for the host, so accepted
 counts that only the device knows drive the next step, and a step can be
-captured in a CUDA graph.  Errors found on the device (a bad row, an exhausted
+captured in a CUDA graph.  A call runs on the cache's GPU, whichever is current,
+on that GPU's current stream.  Errors found on the device (a bad row, an exhausted
 pool) go to ``cache.status``; ``check()`` reads it.
 """
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -43,6 +45,17 @@ def _half_dtype(t: torch.Tensor) -> int:
     if d is None:
         raise TypeError(f"fp16 or bf16 wanted (got {t.dtype})")
     return d
+
+
+def _on_its_gpu(method):
+    """The call made with the cache's GPU current: the default stream's handle, 0, does not say whose it is."""
+    @functools.wraps(method)
+    def call(self, *args, **kw):
+        if torch.cuda.current_device() == self._dev_index:
+            return method(self, *args, **kw)
+        with torch.cuda.device(self._dev_index):
+            return method(self, *args, **kw)
+    return call
 
 
 class Int4PagedCache:
@@ -190,6 +203,7 @@ class Int4PagedCache:
         return ws
 
     # ------------------------------------------------------------------ pages
+    @_on_its_gpu
     def reserve(self, rows, n_new) -> torch.Tensor:
         """Room for ``n_new`` (int32 vector, or one number for all) more tokens in each of ``rows`` (None: all,
         in order), the lengths advanced.  Returns the tokens granted per row, n_new or 0 where the request was
@@ -217,6 +231,7 @@ class Int4PagedCache:
                 _C.check(rc, "akv_pages_reserve")
         return granted
 
+    @_on_its_gpu
     def fork(self, parents, children) -> None:
         """Row ``children[i]`` (empty) continues row ``parents[i]``: it shares the parent's pages, and whichever
         of them next writes into a shared, partly filled page gets its own copy (``reserve``)."""
@@ -228,6 +243,7 @@ class Int4PagedCache:
         if rc:
             _C.check(rc, "akv_pages_fork")
 
+    @_on_its_gpu
     def _truncate(self, rows, n: int, new_lens) -> None:
         rc = self._lib.akv_pages_truncate(self._pt_ref, _C.ptr(rows), _C.ptr(new_lens), n, self._status_ptr,
                                           _C.raw_stream(self._dev_index))
@@ -247,6 +263,7 @@ class Int4PagedCache:
         rows = self._ints(rows, "rows")
         self._truncate(rows, self.max_seqs if rows is None else rows.shape[0], None)
 
+    @_on_its_gpu
     def compact(self) -> torch.Tensor:
         """Live pages moved to the low end of the pool, tables following.  Returns their number (int32, device)."""
         live = torch.empty_strided((1,), (1,), dtype=torch.int32, device=self._dev)
@@ -257,6 +274,7 @@ class Int4PagedCache:
             _C.check(rc, "akv_pages_compact")
         return live
 
+    @_on_its_gpu
     def copy_pages(self, src, dst) -> None:
         """The bytes of pages ``src`` copied over pages ``dst`` in every layer (no page in both)."""
         src = self._ints(src, "src")
@@ -269,6 +287,7 @@ class Int4PagedCache:
             _C.check(rc, "akv_pages_copy")
 
     # ------------------------------------------------------------------ tokens
+    @_on_its_gpu
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows=None, n_new=None) -> None:
         """Quantise the newest tokens of each row into its pages (``reserve`` made the room).
 
@@ -298,6 +317,7 @@ class Int4PagedCache:
         if rc:
             _C.check(rc, "akv_int4_append")
 
+    @_on_its_gpu
     def read(self, layer: int, n_tokens: int, rows=None, start=None, n_new=None, dtype=torch.float16):
         """The K and V values the cache stands for, (R, kv_heads, n_tokens, head_dim) in ``dtype``: tokens
         ``start[i]`` onwards of each row, or with ``start`` None its last ``n_new[i]`` (None: n_tokens); 0 past
@@ -327,6 +347,7 @@ class Int4PagedCache:
             _C.check(rc, "akv_int4_read")
         return k, v
 
+    @_on_its_gpu
     def attend(self, layer: int, query: torch.Tensor, rows=None, n_new=None, sm_scale: Optional[float] = None,
                out: Optional[torch.Tensor] = None, return_lse: bool = False):
         """softmax(q K^T * sm_scale) V of each row's newest tokens over its sequence, causal by position.

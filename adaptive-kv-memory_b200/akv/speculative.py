@@ -37,6 +37,10 @@ def verify_draft(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor]
     dev = p.device
     if dev.type != "cuda":
         raise RuntimeError("akv: verify_draft runs on CUDA tensors only (no CPU fallback)")
+    index = torch.cuda.current_device()
+    if dev.index is not None and dev.index != index:  # launches go to the current GPU
+        with torch.cuda.device(dev.index):
+            return verify_draft(p, q, x, accept_u, sample_u, n_draft, status)
     if p.dim() != 3 or x.dim() != 2:
         raise ValueError("target_probs must be (B, K+1, V) and draft_tokens (B, K)")
     B, K1, V = p.shape
@@ -75,7 +79,7 @@ def verify_draft(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor]
         _C.VERIFY_ARGS.pack(p.data_ptr(), ps[0], ps[1], qp, qs[0], qs[1], x.data_ptr(),
                             0 if nd is None else nd.data_ptr(), au.data_ptr(), su.data_ptr(), accepted.data_ptr(),
                             out.data_ptr(), 0 if status is None else status.data_ptr(), B, K, V, dt),
-        _C.raw_stream(dev.index if dev.index is not None else torch.cuda.current_device()))
+        _C.raw_stream(index))
     if rc:
         _C.check(rc, "akv_verify_draft")
     return accepted, out
