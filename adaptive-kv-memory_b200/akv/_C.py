@@ -192,6 +192,8 @@ SIGNATURES = {
     "akv_pages_fork": (c_int, [POINTER(PageTable), c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "akv_pages_reserve": (c_int, [POINTER(PageTable), c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
                                   c_int64, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "akv_pages_reserve_many": (c_int, [POINTER(PageTable), c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
+                                       c_int64, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
     "akv_pages_truncate": (c_int, [POINTER(PageTable), c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "akv_pages_compact": (c_int, [POINTER(PageTable), c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p,
                                   c_size_t, c_void_p, c_void_p]),

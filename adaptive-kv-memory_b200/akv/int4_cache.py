@@ -34,7 +34,7 @@ import torch
 from . import _C
 
 BLOCK = _C.BLOCK_TOKENS
-_ROWS_PER_CALL = 1024  # requests one reserve plan holds
+_REQUESTS = 1024  # requests that a call may hold however few the sequences
 
 
 _HALF = {torch.float16: 0, torch.bfloat16: 1}
@@ -94,7 +94,8 @@ class Int4PagedCache:
         self._scale = 1.0 / math.sqrt(head_dim)
         self._pt_ref = ctypes.byref(self._pt)
         # the page operations of one cache follow one another (they change one table), so they share a workspace
-        self._page_ws_bytes = int(self._lib.akv_pages_workspace_bytes(n_pages, _ROWS_PER_CALL))
+        self._most_requests = max(_REQUESTS, max_seqs)
+        self._page_ws_bytes = int(self._lib.akv_pages_workspace_bytes(n_pages, self._most_requests))
         self._page_ws = torch.empty(self._page_ws_bytes, dtype=torch.uint8, device=device)
         self._page_ws_ptr = self._page_ws.data_ptr()
         self._pool_ptr, self._layer_bytes, self._page_bytes = self.buf.data_ptr(), self.buf.stride(0), self.buf.stride(1)
@@ -207,7 +208,8 @@ class Int4PagedCache:
     def reserve(self, rows, n_new) -> torch.Tensor:
         """Room for ``n_new`` (int32 vector, or one number for all) more tokens in each of ``rows`` (None: all,
         in order), the lengths advanced.  Returns the tokens granted per row, n_new or 0 where the request was
-        refused: pass it to ``append`` and ``attend`` as their ``n_new``."""
+        refused: pass it to ``append`` and ``attend`` as their ``n_new``.  When the pool runs out, that request and
+        all after it are refused; so is a row that was already asked for in the call."""
         rows = self._ints(rows, "rows")
         n = self.max_seqs if rows is None else rows.shape[0]
         counts = None
@@ -217,18 +219,15 @@ class Int4PagedCache:
         else:
             counts = self._ints(n_new, "n_new", n)
             n_new = 0
-        if rows is None and n > _ROWS_PER_CALL:
-            rows = torch.arange(n, dtype=torch.int32, device=self._dev)
+        if n > self._most_requests:
+            raise ValueError(f"{n} requests for {self.max_seqs} sequences")
         granted = torch.empty_strided((n,), (1,), dtype=torch.int32, device=self._dev)
-        rp, cp, gp = _C.ptr(rows), _C.ptr(counts), granted.data_ptr()
-        stream = _C.raw_stream(self._dev_index)
-        for a in range(0, n, _ROWS_PER_CALL):
-            rc = self._lib.akv_pages_reserve(
-                self._pt_ref, None if rp is None else rp + 4 * a, None if cp is None else cp + 4 * a, n_new,
-                min(n - a, _ROWS_PER_CALL), gp + 4 * a, self._pool_ptr, self.n_layers, self._layer_bytes,
-                self._page_bytes, self._page_ws_ptr, self._page_ws_bytes, self._status_ptr, stream)
-            if rc:
-                _C.check(rc, "akv_pages_reserve")
+        rc = self._lib.akv_pages_reserve_many(
+            self._pt_ref, _C.ptr(rows), _C.ptr(counts), n_new, n, granted.data_ptr(), self._pool_ptr, self.n_layers,
+            self._layer_bytes, self._page_bytes, self._page_ws_ptr, self._page_ws_bytes, self._status_ptr,
+            _C.raw_stream(self._dev_index))
+        if rc:
+            _C.check(rc, "akv_pages_reserve_many")
         return granted
 
     @_on_its_gpu

@@ -63,20 +63,31 @@ AKV_DEV int block_scan(int x, int* warp_sums, int& total) {
 }
 
 // ---------------------------------------------------------------- reserve
+// Requests go through 1,024 at a time, in order; what one round takes, copies
+// and refuses the next one sees (free bits and reference counts are read from
+// L2, where this CTA's atomics change them).
 __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(akv_page_table T, const int32_t* rows,
-                                                                    const int32_t* n_new, int n_new_all, int n,
+                                                                    const int32_t* n_new, int n_new_all, int n_all,
                                                                     int32_t* granted, PageWs ws, int* status) {
   __shared__ int s_row[kPlanThreads], s_page[kPlanThreads], s_off[kPlanThreads + 1], s_block[kPlanThreads];
   __shared__ int s_warp[32];
   __shared__ int s_found, s_fail, s_copies;
   const int t = threadIdx.x;
-  // the request of this thread
-  int row = -1, add = 0, len = 0, nb0 = 0, nb1 = 0, last = -1;
-  bool part = false;
-  if (t < n) {
-    row = rows ? rows[t] : t;
-    add = n_new ? n_new[t] : n_new_all;
-    bool ok = row >= 0 && row < T.max_seqs && add >= 0;
+  const int words = (T.n_pages + 31) / 32;
+  if (t == 0) s_copies = 0;
+  int first = 0;
+  for (; first < n_all; first += kPlanThreads) {
+    const int n = n_all - first < kPlanThreads ? n_all - first : kPlanThreads, i = first + t;
+    // the request of this thread
+    int row = -1, add = 0, len = 0, nb0 = 0, nb1 = 0, last = -1;
+    bool ok = false, part = false;
+    if (t < n) {
+      row = rows ? rows[i] : i;
+      add = n_new ? n_new[i] : n_new_all;
+      ok = row >= 0 && row < T.max_seqs && add >= 0;
+    }
+    s_row[t] = row;
+    if (t == 0) s_found = 0, s_fail = n;
     if (ok) {
       len = T.lens[row];
       const int64_t end = static_cast<int64_t>(len) + add;
@@ -91,84 +102,79 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(akv_page_tab
         }
       }
     }
+    __syncthreads();
+    if (ok && rows) {
+      bool twice = false;
+      for (int s = 0; s < first; ++s) twice |= rows[s] == row;
+      for (int s = 0; s < t; ++s) twice |= s_row[s] == row;
+      ok = !twice;
+    }
     if (!ok) {
-      set_status(status, AKV_ERR_SHAPE);
-      row = -1;
+      if (t < n) set_status(status, AKV_ERR_SHAPE);
       add = nb0 = nb1 = 0;
       part = false;
     }
-  }
-  s_row[t] = row;
-  if (t == 0) s_found = s_copies = 0, s_fail = n;
-  __syncthreads();
-  if (row >= 0) {
-    bool twice = false;
-    for (int s = 0; s < t; ++s) twice |= s_row[s] == row;
-    if (twice) {
-      set_status(status, AKV_ERR_SHAPE);
-      row = -1;
-      add = nb0 = nb1 = 0;
-      part = false;
+    s_page[t] = part ? last : -1;
+    __syncthreads();
+    bool cow = false;
+    if (part) {  // earlier requests that share this page leave it before this one
+      int before = 0;
+      for (int s = 0; s < t; ++s) before += s_page[s] == last;
+      cow = __ldcg(T.refs + last) - before > 1;
     }
-  }
-  s_page[t] = part ? last : -1;
-  __syncthreads();
-  bool cow = false;
-  if (part) {  // earlier requests that share this page leave it before this one
-    int before = 0;
-    for (int s = 0; s < t; ++s) before += s_page[s] == last;
-    cow = T.refs[last] - before > 1;
-  }
-  const int need = nb1 - nb0 + (cow ? 1 : 0);
-  int total;
-  const int off = block_scan(need, s_warp, total) - need;
-  s_off[t] = off;
-  s_block[t] = nb0 - (cow ? 1 : 0);
-  // the first `total` free pages, lowest first
-  const int words = (T.n_pages + 31) / 32;
-  for (int base = 0; base < words; base += kPlanThreads) {
-    const int w = base + t;
-    uint32_t bits = w < words ? T.free_bits[w] : 0u;
-    int sum;
-    int rank = s_found + block_scan(__popc(bits), s_warp, sum) - __popc(bits);
-    while (bits && rank < total) {
-      ws.list[rank++] = w * 32 + __ffs(bits) - 1;
-      bits &= bits - 1;
+    const int need = nb1 - nb0 + (cow ? 1 : 0);
+    int total;
+    const int off = block_scan(need, s_warp, total) - need;
+    s_off[t] = off;
+    s_block[t] = nb0 - (cow ? 1 : 0);
+    // the first `total` free pages, lowest first
+    for (int base = 0; base < words; base += kPlanThreads) {
+      const int w = base + t;
+      uint32_t bits = w < words ? __ldcg(T.free_bits + w) : 0u;
+      int sum;
+      int rank = s_found + block_scan(__popc(bits), s_warp, sum) - __popc(bits);
+      while (bits && rank < total) {
+        ws.list[rank++] = w * 32 + __ffs(bits) - 1;
+        bits &= bits - 1;
+      }
+      __syncthreads();
+      if (t == 0) s_found += sum;
+      __syncthreads();
+      if (s_found >= total) break;
+    }
+    const int have = s_found < total ? s_found : total;
+    // in order until the pool runs out
+    if (t < n && need > 0 && off + need > have) atomicMin(&s_fail, t);
+    __syncthreads();
+    const int fail = s_fail;
+    const int used = fail < n ? s_off[fail] : total;
+    if (t == 0 && fail < n) set_status(status, AKV_ERR_EXHAUSTED);
+    if (t < n) granted[i] = t < fail ? add : 0;
+    if (t < fail && ok) {
+      T.lens[row] = len + add;
+      if (cow) {
+        const int k = atomicAdd(&s_copies, 1);
+        ws.src[k] = last;
+        ws.dst[k] = ws.list[off];
+        atomicSub(T.refs + last, 1);
+      }
+    }
+    for (int k = t; k < used; k += kPlanThreads) {
+      const int page = ws.list[k];
+      atomicAnd(T.free_bits + (page >> 5), ~(1u << (page & 31)));
+      T.refs[page] = 1;
+      int lo = 0, hi = n;  // the last request whose first page is at or before k
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (s_off[mid] <= k) lo = mid; else hi = mid;
+      }
+      T.table[s_row[lo] * T.table_stride + s_block[lo] + (k - s_off[lo])] = page;
     }
     __syncthreads();
-    if (t == 0) s_found += sum;
-    __syncthreads();
-    if (s_found >= total) break;
+    if (fail < n) break;
   }
-  const int have = s_found < total ? s_found : total;
-  // in order until the pool runs out
-  if (t < n && need > 0 && off + need > have) atomicMin(&s_fail, t);
-  __syncthreads();
-  const int fail = s_fail;
-  const int used = fail < n ? s_off[fail] : total;
-  if (t == 0 && fail < n) set_status(status, AKV_ERR_EXHAUSTED);
-  if (t < n) granted[t] = t < fail ? add : 0;
-  if (t < fail && row >= 0) {
-    T.lens[row] = len + add;
-    if (cow) {
-      const int k = atomicAdd(&s_copies, 1);
-      ws.src[k] = last;
-      ws.dst[k] = ws.list[off];
-      atomicSub(T.refs + last, 1);
-    }
-  }
-  for (int i = t; i < used; i += kPlanThreads) {
-    const int page = ws.list[i];
-    atomicAnd(T.free_bits + (page >> 5), ~(1u << (page & 31)));
-    T.refs[page] = 1;
-    int lo = 0, hi = n;  // the last request whose first page is at or before i
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (s_off[mid] <= i) lo = mid; else hi = mid;
-    }
-    T.table[s_row[lo] * T.table_stride + s_block[lo] + (i - s_off[lo])] = page;
-  }
-  __syncthreads();
+  // the pool ran out: whatever follows is refused
+  for (int i = first + kPlanThreads + t; i < n_all; i += kPlanThreads) granted[i] = 0;
   if (t == 0) *ws.count = s_copies;
 }
 
@@ -380,15 +386,14 @@ extern "C" int akv_pages_fork(const akv_page_table* t, const int32_t* parents, c
   return launched();
 }
 
-extern "C" int akv_pages_reserve(const akv_page_table* t, const int32_t* rows, const int32_t* n_new, int n_new_all,
-                                 int n, int32_t* granted, uint8_t* pool, int n_layers, int64_t layer_stride,
-                                 int64_t page_bytes, void* workspace, size_t workspace_bytes, int* status,
-                                 void* stream) {
+extern "C" int akv_pages_reserve_many(const akv_page_table* t, const int32_t* rows, const int32_t* n_new,
+                                      int n_new_all, int n, int32_t* granted, uint8_t* pool, int n_layers,
+                                      int64_t layer_stride, int64_t page_bytes, void* workspace,
+                                      size_t workspace_bytes, int* status, void* stream) {
   int rc = table_check(t);
   if (rc) return rc;
   if ((rc = pool_check(pool, n_layers, layer_stride, page_bytes))) return rc;
   if (n < 0) return AKV_ERR_SHAPE;
-  if (n > kPlanThreads) return AKV_ERR_UNSUPPORTED;
   if (n == 0) return AKV_OK;
   if (!granted || !workspace) return AKV_ERR_NULL;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return AKV_ERR_ALIGN;
@@ -401,6 +406,15 @@ extern "C" int akv_pages_reserve(const akv_page_table* t, const int32_t* rows, c
       pool, n_layers, layer_stride, page_bytes, ws.src, ws.dst, ws.count, 0, t->n_pages, nullptr, 0, 0, 1, nullptr,
       nullptr, status);
   return launched();
+}
+
+extern "C" int akv_pages_reserve(const akv_page_table* t, const int32_t* rows, const int32_t* n_new, int n_new_all,
+                                 int n, int32_t* granted, uint8_t* pool, int n_layers, int64_t layer_stride,
+                                 int64_t page_bytes, void* workspace, size_t workspace_bytes, int* status,
+                                 void* stream) {
+  if (t && n > kPlanThreads) return AKV_ERR_UNSUPPORTED;
+  return akv_pages_reserve_many(t, rows, n_new, n_new_all, n, granted, pool, n_layers, layer_stride, page_bytes,
+                                workspace, workspace_bytes, status, stream);
 }
 
 extern "C" int akv_pages_truncate(const akv_page_table* t, const int32_t* rows, const int32_t* new_lens, int n,

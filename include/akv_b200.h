@@ -755,6 +755,12 @@ int akv_pages_reserve(const akv_page_table* t, const int32_t* rows, const int32_
                       int32_t* granted, uint8_t* pool, int n_layers, int64_t layer_stride, int64_t page_bytes,
                       void* workspace, size_t workspace_bytes, int* status, void* stream);
 
+/* The same for any number of requests: a pool that has run out refuses all that
+ * follow, and a row already asked for is refused wherever it comes again. */
+int akv_pages_reserve_many(const akv_page_table* t, const int32_t* rows, const int32_t* n_new, int n_new_all, int n,
+                           int32_t* granted, uint8_t* pool, int n_layers, int64_t layer_stride, int64_t page_bytes,
+                           void* workspace, size_t workspace_bytes, int* status, void* stream);
+
 /* Row rows[i] (NULL: i) shortened to new_lens[i] (NULL: 0) tokens; pages
  * beyond it lose this holder and, with the last one gone, become free. */
 int akv_pages_truncate(const akv_page_table* t, const int32_t* rows, const int32_t* new_lens, int n, int* status,
