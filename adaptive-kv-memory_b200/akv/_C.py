@@ -257,6 +257,18 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_get_device = None
+
+
+def current_device() -> int:
+    """The current GPU's index, by torch's raw accessor where it has one."""
+    global _get_device
+    if _get_device is None:
+        import torch
+        _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    return _get_device()
+
+
 _raw_stream = None
 
 

@@ -25,7 +25,6 @@ pool) go to ``cache.status``; ``check()`` reads it.
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 from typing import Optional
 
@@ -45,17 +44,6 @@ def _half_dtype(t: torch.Tensor) -> int:
     if d is None:
         raise TypeError(f"fp16 or bf16 wanted (got {t.dtype})")
     return d
-
-
-def _on_its_gpu(method):
-    """The call made with the cache's GPU current: the default stream's handle, 0, does not say whose it is."""
-    @functools.wraps(method)
-    def call(self, *args, **kw):
-        if torch.cuda.current_device() == self._dev_index:
-            return method(self, *args, **kw)
-        with torch.cuda.device(self._dev_index):
-            return method(self, *args, **kw)
-    return call
 
 
 class Int4PagedCache:
@@ -85,6 +73,7 @@ class Int4PagedCache:
         self._rebuild_free()
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self._dev = self.buf.device
+        # the default stream's handle, 0, does not say whose it is: every call makes this GPU current to launch
         self._dev_index = self._dev.index if self._dev.index is not None else torch.cuda.current_device()
         self._status_ptr = self.status.data_ptr()
         self._pt = _C.PageTable(self.table.data_ptr(), max_blocks, self.lens.data_ptr(), self.refs.data_ptr(),
@@ -204,12 +193,14 @@ class Int4PagedCache:
         return ws
 
     # ------------------------------------------------------------------ pages
-    @_on_its_gpu
     def reserve(self, rows, n_new) -> torch.Tensor:
         """Room for ``n_new`` (int32 vector, or one number for all) more tokens in each of ``rows`` (None: all,
         in order), the lengths advanced.  Returns the tokens granted per row, n_new or 0 where the request was
         refused: pass it to ``append`` and ``attend`` as their ``n_new``.  When the pool runs out, that request and
         all after it are refused; so is a row that was already asked for in the call."""
+        if _C.current_device() != self._dev_index:
+            with torch.cuda.device(self._dev_index):
+                return self.reserve(rows, n_new)
         rows = self._ints(rows, "rows")
         n = self.max_seqs if rows is None else rows.shape[0]
         counts = None
@@ -230,10 +221,12 @@ class Int4PagedCache:
             _C.check(rc, "akv_pages_reserve_many")
         return granted
 
-    @_on_its_gpu
     def fork(self, parents, children) -> None:
         """Row ``children[i]`` (empty) continues row ``parents[i]``: it shares the parent's pages, and whichever
         of them next writes into a shared, partly filled page gets its own copy (``reserve``)."""
+        if _C.current_device() != self._dev_index:
+            with torch.cuda.device(self._dev_index):
+                return self.fork(parents, children)
         parents = self._ints(parents, "parents")
         n = parents.shape[0]
         children = self._ints(children, "children", n)
@@ -242,8 +235,10 @@ class Int4PagedCache:
         if rc:
             _C.check(rc, "akv_pages_fork")
 
-    @_on_its_gpu
     def _truncate(self, rows, n: int, new_lens) -> None:
+        if _C.current_device() != self._dev_index:
+            with torch.cuda.device(self._dev_index):
+                return self._truncate(rows, n, new_lens)
         rc = self._lib.akv_pages_truncate(self._pt_ref, _C.ptr(rows), _C.ptr(new_lens), n, self._status_ptr,
                                           _C.raw_stream(self._dev_index))
         if rc:
@@ -262,9 +257,11 @@ class Int4PagedCache:
         rows = self._ints(rows, "rows")
         self._truncate(rows, self.max_seqs if rows is None else rows.shape[0], None)
 
-    @_on_its_gpu
     def compact(self) -> torch.Tensor:
         """Live pages moved to the low end of the pool, tables following.  Returns their number (int32, device)."""
+        if _C.current_device() != self._dev_index:
+            with torch.cuda.device(self._dev_index):
+                return self.compact()
         live = torch.empty_strided((1,), (1,), dtype=torch.int32, device=self._dev)
         rc = self._lib.akv_pages_compact(self._pt_ref, self._pool_ptr, self.n_layers, self._layer_bytes,
                                          self._page_bytes, live.data_ptr(), self._page_ws_ptr, self._page_ws_bytes,
@@ -273,9 +270,11 @@ class Int4PagedCache:
             _C.check(rc, "akv_pages_compact")
         return live
 
-    @_on_its_gpu
     def copy_pages(self, src, dst) -> None:
         """The bytes of pages ``src`` copied over pages ``dst`` in every layer (no page in both)."""
+        if _C.current_device() != self._dev_index:
+            with torch.cuda.device(self._dev_index):
+                return self.copy_pages(src, dst)
         src = self._ints(src, "src")
         n = src.shape[0]
         dst = self._ints(dst, "dst", n)
@@ -286,12 +285,14 @@ class Int4PagedCache:
             _C.check(rc, "akv_pages_copy")
 
     # ------------------------------------------------------------------ tokens
-    @_on_its_gpu
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows=None, n_new=None) -> None:
         """Quantise the newest tokens of each row into its pages (``reserve`` made the room).
 
         k, v (R, kv_heads, M, head_dim) fp16 or bf16, any strides: row i's last ``n_new[i]`` tokens (None: M)
         are k[i, :, :n_new[i]]."""
+        if _C.current_device() != self._dev_index:
+            with torch.cuda.device(self._dev_index):
+                return self.append(layer, k, v, rows, n_new)
         view = self._layer(layer)
         dt = _half_dtype(k)
         if v.dtype is not k.dtype:
@@ -316,11 +317,13 @@ class Int4PagedCache:
         if rc:
             _C.check(rc, "akv_int4_append")
 
-    @_on_its_gpu
     def read(self, layer: int, n_tokens: int, rows=None, start=None, n_new=None, dtype=torch.float16):
         """The K and V values the cache stands for, (R, kv_heads, n_tokens, head_dim) in ``dtype``: tokens
         ``start[i]`` onwards of each row, or with ``start`` None its last ``n_new[i]`` (None: n_tokens); 0 past
         the row's end."""
+        if _C.current_device() != self._dev_index:
+            with torch.cuda.device(self._dev_index):
+                return self.read(layer, n_tokens, rows, start, n_new, dtype)
         view = self._layer(layer)
         dt = _HALF.get(dtype)
         if dt is None:
@@ -346,7 +349,6 @@ class Int4PagedCache:
             _C.check(rc, "akv_int4_read")
         return k, v
 
-    @_on_its_gpu
     def attend(self, layer: int, query: torch.Tensor, rows=None, n_new=None, sm_scale: Optional[float] = None,
                out: Optional[torch.Tensor] = None, return_lse: bool = False):
         """softmax(q K^T * sm_scale) V of each row's newest tokens over its sequence, causal by position.
@@ -356,6 +358,9 @@ class Int4PagedCache:
         past n_new[i] give zero rows, queries with NaN or infinities rows of NaN.  Returns the output in the
         query's shape, type and (where it is dense) layout, and with ``return_lse`` the natural-log LSE (R, Hq, M)
         fp32."""
+        if _C.current_device() != self._dev_index:
+            with torch.cuda.device(self._dev_index):
+                return self.attend(layer, query, rows, n_new, sm_scale, out, return_lse)
         view = self._layer(layer)
         dt = _half_dtype(query)
         one = query.dim() == 3

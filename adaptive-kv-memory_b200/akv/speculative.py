@@ -37,7 +37,7 @@ def verify_draft(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor]
     dev = p.device
     if dev.type != "cuda":
         raise RuntimeError("akv: verify_draft runs on CUDA tensors only (no CPU fallback)")
-    index = torch.cuda.current_device()
+    index = _C.current_device()
     if dev.index is not None and dev.index != index:  # launches go to the current GPU
         with torch.cuda.device(dev.index):
             return verify_draft(p, q, x, accept_u, sample_u, n_draft, status)

@@ -14,7 +14,9 @@ class Gpu:
     """The current GPU (0 at first), and what each call of the library found as current."""
 
     def __init__(self, monkeypatch):
+        from akv import _C
         self.now, self.calls = 0, []
+        monkeypatch.setattr(_C, "current_device", lambda: self.now)
         monkeypatch.setattr(torch.cuda, "current_device", lambda: self.now)
         monkeypatch.setattr(torch.cuda, "device", self.device)
         monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
