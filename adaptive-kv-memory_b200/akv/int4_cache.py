@@ -205,8 +205,8 @@ class Int4PagedCache:
         n = self.max_seqs if rows is None else rows.shape[0]
         counts = None
         if isinstance(n_new, int):
-            if n_new < 0:
-                raise ValueError("n_new is negative")
+            if not 0 <= n_new < 1 << 31:
+                raise ValueError(f"n_new must be 0 to 2^31 - 1 (got {n_new})")
         else:
             counts = self._ints(n_new, "n_new", n)
             n_new = 0

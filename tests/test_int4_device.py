@@ -118,3 +118,13 @@ def test_verification_launches_on_its_tensors_gpu(gpu, monkeypatch, index):
                      Fake((1, 2), f32, index), Fake((1,), f32, index))
     assert gpu.calls == [("akv_verify_draft", index)] and gpu.now == 0
     assert isinstance(akv, types.ModuleType)
+
+
+@pytest.mark.parametrize("n_new", [-1, 1 << 31, (1 << 32) + 5])
+def test_reserve_refuses_a_count_past_32_bits(gpu, n_new):
+    """The entry takes a 32-bit count; a larger one would be cut to its low bits."""
+    c = _cache(gpu, 0)
+    gpu.calls.clear()
+    with pytest.raises(ValueError):
+        c.reserve([0], n_new)
+    assert not gpu.calls
