@@ -286,13 +286,8 @@ def stream_of(t) -> int:
 
     Called on every op of the hot path, so it asks torch's raw-stream accessor
     (a few hundred ns) rather than building a Stream object (~10 us)."""
-    global _raw_stream
-    import torch
-    if _raw_stream is None:
-        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", False)
-    if _raw_stream:
-        return _raw_stream(t.device.index if t.device.index is not None else torch.cuda.current_device())
-    return torch.cuda.current_stream(t.device).cuda_stream
+    i = t.device.index
+    return raw_stream(current_device() if i is None else i)
 
 
 def require_cuda(*tensors) -> None:
