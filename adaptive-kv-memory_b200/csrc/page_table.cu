@@ -62,6 +62,11 @@ AKV_DEV int block_scan(int x, int* warp_sums, int& total) {
   return x + (warp ? before : 0);
 }
 
+AKV_DEV uint32_t page_mask(int w, int n_pages) {  // the bits of word w that are pages
+  const int left = n_pages - w * 32;
+  return left >= 32 ? ~0u : (left <= 0 ? 0u : (1u << left) - 1u);
+}
+
 // ---------------------------------------------------------------- reserve
 // Requests go through 1,024 at a time, in order; what one round takes, copies
 // and refuses the next one sees (free bits and reference counts are read from
@@ -130,7 +135,8 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(akv_page_tab
     // the first `total` free pages, lowest first
     for (int base = 0; base < words; base += kPlanThreads) {
       const int w = base + t;
-      uint32_t bits = w < words ? __ldcg(T.free_bits + w) : 0u;
+      // a bit past the pool, of a state from elsewhere, is no page
+      uint32_t bits = w < words ? __ldcg(T.free_bits + w) & page_mask(w, T.n_pages) : 0u;
       int sum;
       int rank = s_found + block_scan(__popc(bits), s_warp, sum) - __popc(bits);
       while (bits && rank < total) {
@@ -286,11 +292,6 @@ __global__ void __launch_bounds__(128) truncate_kernel(akv_page_table T, const i
 }
 
 // ---------------------------------------------------------------- compact
-AKV_DEV uint32_t page_mask(int w, int n_pages) {  // the bits of word w that are pages
-  const int left = n_pages - w * 32;
-  return left >= 32 ? ~0u : (left <= 0 ? 0u : (1u << left) - 1u);
-}
-
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(akv_page_table T, int32_t* n_live, PageWs ws) {
   __shared__ int s_warp[32];
   __shared__ int s_below;  // live pages below n_live

@@ -112,3 +112,13 @@ def test_too_many_requests():
     with pytest.raises(ValueError):
         c.reserve([0] * 1025, 1)
     assert c.lens.tolist() == [1] + [0] * 8
+
+
+def test_free_bits_past_the_pool_are_no_pages():
+    """A state whose last word has bits that stand for no page: as many pages are handed out as there are."""
+    c, m, content = base._make(layers=1, pages=35, seqs=9, blocks=6)
+    c.free_bits.fill_(-1)
+    assert c.reserve(list(range(9)), 160).tolist() == m.reserve(list(range(9)), [160] * 9) == [160] * 7 + [0, 0]
+    assert _status(c) == -9
+    c.free_bits[1] &= 7                                  # what is left of them
+    base._same(c, m, content)
