@@ -33,11 +33,11 @@
 // decide, so a call repeated gives the same bits.
 //
 // Bound and measured (B200, 32 / 8 heads of 128, 16 x 32K tokens).  The pages
-// alone stream in 95 us (6.0 TB/s).  One query token, group 128: 135 us fp16
-// (4.2 TB/s).  Per page and warp some 630 instructions, 40 % of them unpacking
+// alone stream in 95 us (6.0 TB/s).  One query token, group 128: 139 us fp16
+// (4.1 TB/s).  Per page and warp some 630 instructions, 40 % of them unpacking
 // (256 codes a lane); issue slots 60 %, the integer pipe 52 %, tensor cores
 // 25 % busy, and fewer or more warps change nothing: instruction throughput
-// bounds it.  Five tokens, groups of 32, bf16: 236 us; the same bound, the
+// bounds it.  Five tokens, groups of 32, bf16: 243 us; the same bound, the
 // per-group scaling of scores above all.  What was tried and did not help: two
 // pages per iteration, one CTA of 16 warps an SM, keeping warps in step, three
 // or four query tiles a CTA (the registers leave too few warps), three or more
@@ -104,9 +104,11 @@ constexpr int attn_occ(int D, int nt) { return D == 256 ? 2 : (nt == 1 ? 4 : 3);
 //
 // A bf16 output leaves room to round each value of V to fp16 as it is unpacked,
 // scale and zero applied (AttnShape::AV); the weights are then the same for
-// every group.  It costs a second fp16 operation for each pair of codes and
-// saves per group and query tile what the weights cost: it pays from four
-// (group, tile) pairs on.
+// every group.  It costs a second fp16 operation for each pair of codes, and a
+// look for values past fp16's range (1 to 4 % of the time), and saves per group
+// and query tile what the weights cost: it pays from four (group, tile) pairs
+// on.  Against the formula a bf16 output is then 1.01 to 1.03 times as far off
+// as by its own rounding.
 constexpr bool attn_av(int G, int NT, int LO) { return !LO && G * NT >= 4; }
 
 template <int D, int G, int NT, int LO>

@@ -11,9 +11,9 @@
 // 16-bit pair in log2(g/8) shuffles.  A CTA takes one page of one sequence, so
 // the row and page lookups are paid once.
 //
-// Measured (4 x 32,767 tokens, 8 heads of 128, bf16, groups of 32; 688 MB moved
-// by each direction's kernel): append 138 us (5.0 TB/s; 91 instructions per 8
-// values, issue slots 64 %, the rest waits for loads), read 109 us (6.1 TB/s:
+// Measured (4 x 32,767 tokens, 8 heads of 128, bf16, groups of 32; 705 MB moved
+// by each direction's kernel): append 137 us (5.1 TB/s; 91 instructions per 8
+// values, issue slots 64 %, the rest waits for loads), read 118 us (6.0 TB/s:
 // memory).  Append with the unusual groups looked for in every row instead of
 // once for four: 147; two rows in flight: 164; three CTAs an SM, no spills: 155;
 // five: 159.

@@ -22,10 +22,11 @@
 // units(max(p, q)) - units(q), because units() is monotone: no comparison of
 // the two-part numbers.
 //
-// Measured (151,936 fp32 probabilities, draft and target): 64 sequences 17 us
-// (4.6 TB/s of the 78 MB; the chain of a CTA, half of it not loads, shows), one
-// sequence 10.4 us, all latency: accept 1.4, sums 1.5, two cluster exchanges
-// 2.5, draw 1, launch.
+// Measured (151,936 fp32 probabilities, draft and target, inputs from DRAM,
+// launches of a graph): 64 sequences 23.1 us (3.4 TB/s of the 78 MB, 1.9 times
+// the bytes' time: all CTAs go through accept, sums, exchange and draw in step,
+// and only the sums stream), one sequence 7.8 us, all latency: accept 1.4, sums
+// 1.5, two cluster exchanges 2.5, draw 1, launch.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -329,8 +330,9 @@ static cudaError_t verify_launch(const VerifyParams& p, int B, cudaStream_t st) 
   return cudaGetLastError();
 }
 
-// Measured (151,936 fp32 probabilities, draft and target; us with 512 / 256
-// threads): 1 sequence 10.3 / 12.8, 16 12.4 / 14.4, 24 14.4 / 14.4, 64 28.7 / 18.4.
+// Measured (151,936 fp32 probabilities, draft and target, inputs from DRAM,
+// launches of a graph; us with 512 / 256 threads): 1 sequence 7.8 / 10.5, 16
+// 15.3 / 15.0, 24 17.2 / 15.6, 32 23.1 / 16.9, 64 39.7 / 23.1.
 template <int DT>
 static cudaError_t verify_launch(const VerifyParams& p, int B, cudaStream_t st) {
   return B >= kVerifyManyFrom ? verify_launch<DT, kVerifyMany>(p, B, st) : verify_launch<DT, kVerifyFew>(p, B, st);
