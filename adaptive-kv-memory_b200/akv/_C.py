@@ -92,6 +92,7 @@ class PageTable(ctypes.Structure):
 IO_ARGS = struct.Struct("13q4i")         # akv_int4_io_args
 ATTENTION_ARGS = struct.Struct("15q4ifi")  # akv_int4_attention_args
 VERIFY_ARGS = struct.Struct("13q4i")     # akv_verify_args
+LOGPROBS_ARGS = struct.Struct("8q4i")    # akv_logprobs_args
 
 # name -> (restype, argtypes); must list every function declared in akv_b200.h
 SIGNATURES = {
@@ -200,6 +201,7 @@ SIGNATURES = {
     "akv_pages_copy": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p,
                                c_void_p]),
     "akv_verify_draft": (c_int, [c_char_p, c_void_p]),
+    "akv_token_logprobs": (c_int, [c_char_p, c_void_p]),
     "akv_selftest_wait": (c_int, [c_int, c_int64, c_void_p, c_void_p, c_void_p]),
     "akv_cold_copy": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
 }

@@ -15,6 +15,7 @@ from .packed_layout import WarmArena, measure_packed_bytes
 from .drop_in import AKVCache, AKVLayer, recommend_preset
 from .graphs import DecodeGraph
 from .int4_cache import Int4PagedCache
+from .logprobs import TokenLogprobs, token_logprobs
 from .speculative import verify_draft
 from .tiering import fused_importance_update
 from .triton_ops import HAS_TRITON, fused_mixed_precision_attention, fused_quantized_attention
@@ -29,6 +30,6 @@ __all__ = [
     "int4_group_dequant", "prefill_attention",
     "HAS_TRITON", "fused_quantized_attention", "fused_mixed_precision_attention", "fused_importance_update",
     "fused_decode_attention", "fused_quantize_evict",
-    "Int4PagedCache", "verify_draft",
+    "Int4PagedCache", "verify_draft", "TokenLogprobs", "token_logprobs",
     "pack", "unpack", "packed_bytes",
 ]

@@ -1,0 +1,369 @@
+// Log probabilities of given tokens, with entropy, rank and the top alternatives.
+//
+// Of a row x of logits, with M = max x, u = x - M, Z = sum e^u:
+//   logprob = u[token] - ln Z     entropy = ln Z - sum(e^u u) / Z
+//   rank    = 1 + the number of logits above the token's
+// and the k largest logits, the lowest index first among equal ones.  One pass:
+// a thread keeps the running maximum of what it has seen, Z and sum(e^u u)
+// relative to it (in log2 units), and rescales both when the maximum moves.
+// All sums are fp32; u is clamped to -160 in log2 units, where e^u is 0 in fp32,
+// so that -inf logits add 0 and not 0 * -inf.
+//
+// Top alternatives: a warp holds the best 32 it has met, one a lane in
+// descending order, as 64-bit keys (value's order << 32 | ~index): they decide
+// ties, so the result depends on the inputs alone.  A batch of 32 elements a
+// lane is looked through only if its maximum reaches the k-th key.  The lists
+// of warps and CTAs are merged pairwise (maximum of one and the other reversed
+// is the bitonic top half).
+//
+// Bound by memory: every logit is read once.  Few rows are split over clusters
+// of up to 8 CTAs.
+#include <cooperative_groups.h>
+
+#include "int4.cuh"
+
+namespace akv {
+
+namespace cg = cooperative_groups;
+
+constexpr int kLogpThreads = 256;
+constexpr int kLogpWarps = kLogpThreads / 32;
+constexpr int kLogpVecs = 4;         // 16-byte loads of a thread in flight
+constexpr int kLogpMaxTop = 32;
+constexpr int kLogpMaxCluster = 8;
+constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct LogpParams {
+  const void* logits;
+  int64_t row_stride;
+  const int64_t* tokens;
+  float* logprob;
+  float* entropy;
+  int32_t* rank;
+  int64_t* top_tokens;
+  float* top_logprobs;
+  int vocab, top;
+};
+
+// max that gives NaN for NaN
+AKV_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+template <int DT>
+struct LogitElem {  // two 16-bit logits a word
+  using type = uint16_t;
+  static constexpr int N = 8;  // logits of a 16-byte vector
+  static constexpr uint32_t kNone = DT == AKV_BF16 ? 0xFF80FF80u : 0xFC00FC00u;  // -inf
+  AKV_DEV static float get(uint16_t u) { return elem_to_float<DT == AKV_BF16>(u); }
+  AKV_DEV static void unpack(uint32_t w, float (&x)[2]) {
+    if constexpr (DT == AKV_BF16) {
+      x[0] = __uint_as_float(w << 16);
+      x[1] = __uint_as_float(w & 0xFFFF0000u);
+    } else {
+      const float2 f = __half22float2(u32_as_h2(w));
+      x[0] = f.x, x[1] = f.y;
+    }
+  }
+  AKV_DEV static uint32_t max_word(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (DT == AKV_BF16)
+      asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+      asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  AKV_DEV static float max_of(uint32_t w) {
+    float x[2];
+    unpack(w, x);
+    return fmaxf(x[0], x[1]);
+  }
+};
+template <>
+struct LogitElem<AKV_FP32> {
+  using type = float;
+  static constexpr int N = 4;
+  static constexpr uint32_t kNone = 0xFF800000u;
+  AKV_DEV static float get(float u) { return u; }
+  AKV_DEV static uint32_t max_word(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+  AKV_DEV static float max_of(uint32_t w) { return __uint_as_float(w); }
+};
+
+// 32-bit order of a logit (-0 as +0); never called for NaN
+AKV_DEV uint32_t logit_order(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+}
+AKV_DEV float order_logit(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+
+AKV_DEV uint64_t logit_key(float x, int index) {
+  return static_cast<uint64_t>(logit_order(x)) << 32 | static_cast<uint32_t>(~index);
+}
+
+// What a part of a row comes to: maximum, and relative to it the sums of e^u and
+// e^u u (u in log2 units).
+struct LogpSums {
+  float m, s, t;
+};
+AKV_DEV LogpSums join(LogpSums a, LogpSums b) {
+  LogpSums r;
+  r.m = max_nan(a.m, b.m);
+  // a part without anything has s = t = 0; far below the other, it only has to vanish
+  const float da = a.m == -INFINITY ? 0.f : fmaxf((a.m - r.m) * kLog2E, -1e4f);
+  const float db = b.m == -INFINITY ? 0.f : fmaxf((b.m - r.m) * kLog2E, -1e4f);
+  const float fa = exp2f(da), fb = exp2f(db);
+  r.s = fa * a.s + fb * b.s;
+  r.t = fa * fmaf(da, a.s, a.t) + fb * fmaf(db, b.s, b.t);
+  return r;
+}
+
+// descending order over the lanes of a bitonic sequence of keys
+AKV_DEV uint64_t bitonic_merge(uint64_t k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const uint64_t y = __shfl_xor_sync(~0u, k, o);
+    k = (lane & o) ? (k < y ? k : y) : (k > y ? k : y);
+  }
+  return k;
+}
+
+template <int DT, bool TOP>
+__global__ void __launch_bounds__(kLogpThreads, 4) token_logprobs_kernel(const LogpParams P) {
+  using E = LogitElem<DT>;
+  using T = typename E::type;
+  constexpr int W = kLogpVecs * 4;                 // words of a batch
+  constexpr int PER = E::N / 4;                    // logits of a word
+  __shared__ LogpSums s_sums[kLogpWarps];
+  __shared__ int s_above[kLogpWarps];
+  __shared__ uint64_t s_keys[TOP ? kLogpWarps : 1][32];
+
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = cluster.num_blocks(), rank = cluster.block_rank();
+  const int row = blockIdx.x / C;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const T* x0 = static_cast<const T*>(P.logits) + row * P.row_stride;
+  const int64_t token = P.tokens ? __ldg(P.tokens + row) : -1;
+  const bool have = static_cast<uint64_t>(token) < static_cast<uint64_t>(P.vocab);
+  const float mine = have ? E::get(__ldg(x0 + token)) : NAN;
+
+  // 16-byte vectors from the first boundary on; what stands before and after them is taken one by one
+  const int head = min(P.vocab, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x0) & 15)) % 16 / sizeof(T)));
+  const int n_vec = (P.vocab - head) / E::N;
+  const int tail0 = head + n_vec * E::N;
+  const int v0 = static_cast<int>(static_cast<int64_t>(n_vec) * rank / C);
+  const int v1 = static_cast<int>(static_cast<int64_t>(n_vec) * (rank + 1) / C);
+  const uint4* xv = reinterpret_cast<const uint4*>(x0 + head);
+
+  LogpSums a{-INFINITY, 0.f, 0.f};
+  float base = 0.f;  // the maximum, or 0 while there is none: -inf - base stays -inf
+  int above = 0;
+  uint64_t best = 0, least = 0;  // this lane's key; the k-th key of the warp
+
+  auto raise = [&](float m) {
+    if (a.m != -INFINITY) {
+      const float d = fmaxf((a.m - m) * kLog2E, -1e4f), f = exp2f(d);
+      a.t = f * fmaf(d, a.s, a.t);
+      a.s *= f;
+    }
+    a.m = m;
+    base = m;
+  };
+  auto add = [&](float x) {
+    const float u = max_nan((x - base) * kLog2E, -160.f);
+    const float e = fast_exp2(u);
+    a.s += e;
+    a.t = fmaf(e, u, a.t);
+  };
+  // one candidate of each lane (key 0: none) into the warp's list
+  auto offer = [&](uint64_t key) {
+    for (uint32_t who = __ballot_sync(~0u, key > least); who; who &= who - 1) {
+      const uint64_t k = __shfl_sync(~0u, key, __ffs(who) - 1);
+      if (k <= least) continue;
+      const uint64_t up = __shfl_up_sync(~0u, best, 1);
+      if (best < k) best = lane == 0 || up > k ? k : up;
+      least = __shfl_sync(~0u, best, P.top - 1);
+    }
+  };
+
+  for (int v = v0; v < v1; v += kLogpVecs * kLogpThreads) {
+    uint32_t w[W];
+#pragma unroll
+    for (int j = 0; j < kLogpVecs; ++j) {
+      const int at = v + j * kLogpThreads + t;
+      const uint4 q = at < v1 ? ldg_nc_v4(xv + at) : make_uint4(E::kNone, E::kNone, E::kNone, E::kNone);
+      w[4 * j] = q.x, w[4 * j + 1] = q.y, w[4 * j + 2] = q.z, w[4 * j + 3] = q.w;
+    }
+    uint32_t top = w[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) top = E::max_word(top, w[i]);
+    const float m = E::max_of(top);
+    if (!(m <= a.m)) raise(m);
+    const bool count = m > mine;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (PER == 2) {
+        float x[2];
+        E::unpack(w[i], x);
+        add(x[0]);
+        add(x[1]);
+        if (count) above += (x[0] > mine) + (x[1] > mine);
+      } else {
+        add(__uint_as_float(w[i]));
+        if (count) above += __uint_as_float(w[i]) > mine;
+      }
+    }
+    if constexpr (TOP) {
+      const bool look = m == m && logit_order(m) >= static_cast<uint32_t>(least >> 32);
+      if (__any_sync(~0u, look)) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const int at = v + (i / 4) * kLogpThreads + t;
+          const int c = head + at * E::N + (i % 4) * PER;
+          if constexpr (PER == 2) {
+            float x[2];
+            E::unpack(w[i], x);
+            offer(look && at < v1 ? logit_key(x[0], c) : 0);
+            offer(look && at < v1 ? logit_key(x[1], c + 1) : 0);
+          } else {
+            offer(look && at < v1 ? logit_key(__uint_as_float(w[i]), c) : 0);
+          }
+        }
+      }
+    }
+  }
+  // the row's ends: fewer than 16 logits, by the first warp of the last CTA
+  if (rank == C - 1 && warp == 0) {
+    const int c = lane < head ? lane : tail0 + lane - head;
+    const bool on = c < P.vocab;
+    const float x = on ? E::get(x0[c]) : -INFINITY;
+    if (!(x <= a.m)) raise(x);
+    add(x);
+    above += x > mine;
+    if constexpr (TOP) offer(on && x == x ? logit_key(x, c) : 0);
+  }
+
+  // warps, then CTAs
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const LogpSums b{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.t, o)};
+    // both lanes join in the same order
+    a = (lane & o) ? join(b, a) : join(a, b);
+  }
+  above = __reduce_add_sync(~0u, above);
+  if (lane == 0) {
+    s_sums[warp] = a;
+    s_above[warp] = above;
+  }
+  if constexpr (TOP) {
+    s_keys[warp][lane] = best;
+#pragma unroll
+    for (int o = 1; o < kLogpWarps; o *= 2) {
+      __syncthreads();
+      if (warp % (2 * o) == 0) {
+        const uint64_t other = s_keys[warp + o][31 - lane];
+        best = bitonic_merge(best > other ? best : other);
+        s_keys[warp][lane] = best;
+      }
+    }
+  }
+  __syncthreads();
+  if (t == 0) {
+    for (int i = 1; i < kLogpWarps; ++i) {
+      a = join(a, s_sums[i]);
+      above += s_above[i];
+    }
+    s_sums[0] = a;
+    s_above[0] = above;
+  }
+  cluster.sync();
+  if (rank == 0 && warp == 0) {
+    for (int i = 1; i < C; ++i) {
+      a = join(i == 1 ? s_sums[0] : a, *cluster.map_shared_rank(&s_sums[0], i));
+      above = (i == 1 ? s_above[0] : above) + *cluster.map_shared_rank(&s_above[0], i);
+      if constexpr (TOP) {
+        const uint64_t other = cluster.map_shared_rank(&s_keys[0][0], i)[31 - lane];
+        best = bitonic_merge(best > other ? best : other);
+      }
+    }
+    if (C == 1) {
+      a = s_sums[0];
+      above = s_above[0];
+    }
+    // no distribution: NaN or +inf among the logits, or all of them -inf
+    const bool bad = !(fabsf(a.m) < INFINITY) || a.s != a.s;
+    const float logz = logf(a.s);
+    if (lane == 0) {
+      P.logprob[row] = bad || !have ? NAN : (mine - a.m) - logz;
+      P.entropy[row] = bad ? NAN : logz - a.t / a.s * kLn2;
+      P.rank[row] = bad || !have ? 0 : above + 1;
+    }
+    if constexpr (TOP) {
+      if (lane < P.top) {
+        const float x = order_logit(static_cast<uint32_t>(best >> 32));
+        P.top_tokens[static_cast<int64_t>(row) * P.top + lane] = bad ? -1 : static_cast<int>(~static_cast<uint32_t>(best));
+        P.top_logprobs[static_cast<int64_t>(row) * P.top + lane] = bad ? NAN : (x - a.m) - logz;
+      }
+    }
+  }
+  cluster.sync();  // the first CTA has read the others' shared memory
+}
+
+template <int DT, bool TOP>
+static int launch_logprobs(const LogpParams& p, int n, int cluster, cudaStream_t st) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(n) * cluster);
+  cfg.blockDim = dim3(kLogpThreads);
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<DT, TOP>, p) == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH;
+}
+
+}  // namespace akv
+
+using namespace akv;
+
+extern "C" int akv_token_logprobs(const akv_logprobs_args* a, void* stream) {
+  if (!a) return AKV_ERR_NULL;
+  if (a->n < 0 || a->vocab <= 0 || a->top < 0 || a->top > kLogpMaxTop || a->top > a->vocab) return AKV_ERR_SHAPE;
+  if (a->n > (1 << 28) || a->vocab > INT32_MAX - 64) return AKV_ERR_SHAPE;
+  if (a->dtype != AKV_FP32 && a->dtype != AKV_FP16 && a->dtype != AKV_BF16) return AKV_ERR_UNSUPPORTED;
+  if (a->n == 0) return AKV_OK;
+  if (!a->logits || !a->tokens || !a->logprob || !a->entropy || !a->rank ||
+      (a->top && (!a->top_tokens || !a->top_logprobs)))
+    return AKV_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(a->logits) & (a->dtype == AKV_FP32 ? 3 : 1)) return AKV_ERR_ALIGN;
+  LogpParams p{};
+  p.logits = a->logits;
+  p.row_stride = a->row_stride;
+  p.tokens = a->tokens;
+  p.logprob = a->logprob;
+  p.entropy = a->entropy;
+  p.rank = a->rank;
+  p.top_tokens = a->top_tokens;
+  p.top_logprobs = a->top_logprobs;
+  p.vocab = a->vocab;
+  p.top = a->top;
+  // as many CTAs a row as fill the GPU, each with a batch's worth of logits at least
+  const int batch = kLogpThreads * kLogpVecs * (a->dtype == AKV_FP32 ? 4 : 8);
+  int cluster = 1;
+  while (cluster < kLogpMaxCluster && a->n * cluster * 2 <= 148 * 4 && a->vocab > batch * cluster) cluster *= 2;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (a->dtype * 2 + (a->top > 0)) {
+    case AKV_FP32 * 2: return launch_logprobs<AKV_FP32, false>(p, a->n, cluster, st);
+    case AKV_FP32 * 2 + 1: return launch_logprobs<AKV_FP32, true>(p, a->n, cluster, st);
+    case AKV_FP16 * 2: return launch_logprobs<AKV_FP16, false>(p, a->n, cluster, st);
+    case AKV_FP16 * 2 + 1: return launch_logprobs<AKV_FP16, true>(p, a->n, cluster, st);
+    case AKV_BF16 * 2: return launch_logprobs<AKV_BF16, false>(p, a->n, cluster, st);
+    default: return launch_logprobs<AKV_BF16, true>(p, a->n, cluster, st);
+  }
+}

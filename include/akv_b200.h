@@ -812,6 +812,33 @@ typedef struct {
 
 int akv_verify_draft(const akv_verify_args* a, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Log probabilities of given tokens.  Row i < n of the logits: element x at
+ * logits + i*row_stride + x (elements), dtype AKV_FP32, AKV_FP16 or AKV_BF16,
+ * any alignment of its elements' size.  Per row, in fp32:
+ *   logprob[i]  log softmax at tokens[i] (NaN where it is outside [0, vocab))
+ *   entropy[i]  of the row's softmax, in nats
+ *   rank[i]     1 + the logits above the token's (0 where that is no token)
+ * and, top > 0, int64 / fp32 [n][top]: the tokens of the largest logits in
+ * descending order, the lowest first among equal ones, with their log
+ * probabilities.  A logit of -inf has probability 0.  A row without a
+ * distribution (NaN or +inf in it, or -inf alone) gives NaN, rank 0 and tokens
+ * -1.  top <= 32 and <= vocab.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  const void* logits;
+  int64_t row_stride;
+  const int64_t* tokens;
+  float* logprob;
+  float* entropy;
+  int32_t* rank;
+  int64_t* top_tokens;
+  float* top_logprobs;
+  int32_t n, vocab, top, dtype;
+} akv_logprobs_args;
+
+int akv_token_logprobs(const akv_logprobs_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
