@@ -91,6 +91,8 @@ class PageTable(ctypes.Structure):
 # tenth of converting as many ctypes arguments): pointers and 64-bit fields first, then 32-bit ones.
 IO_ARGS = struct.Struct("13q4i")         # akv_int4_io_args
 ATTENTION_ARGS = struct.Struct("15q4ifi")  # akv_int4_attention_args
+WEIGH_ARGS = struct.Struct("11q4ifi")  # akv_int4_weigh_args
+EVICT_ARGS = struct.Struct("12q8i")      # akv_int4_evict_args
 VERIFY_ARGS = struct.Struct("13q4i")     # akv_verify_args
 LOGPROBS_ARGS = struct.Struct("8q4i")    # akv_logprobs_args
 
@@ -189,6 +191,13 @@ SIGNATURES = {
     "akv_int4_read": (c_int, [c_char_p, c_void_p]),
     "akv_int4_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "akv_int4_attention": (c_int, [c_char_p, c_void_p]),
+    "akv_int4_weigh": (c_int, [c_char_p, c_void_p]),
+    "akv_int4_evict_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "akv_int4_evict": (c_int, [c_char_p, c_void_p]),
+    "akv_int4_weights_clear": (c_int, [POINTER(PageTable), c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p,
+                                       c_int, c_void_p]),
+    "akv_int4_weights_fork": (c_int, [POINTER(PageTable), c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p,
+                                      c_int, c_void_p]),
     "akv_pages_workspace_bytes": (c_size_t, [c_int, c_int]),
     "akv_pages_fork": (c_int, [POINTER(PageTable), c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "akv_pages_reserve": (c_int, [POINTER(PageTable), c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,

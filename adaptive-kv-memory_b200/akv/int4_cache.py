@@ -14,7 +14,13 @@ A serving step is
         out = cache.attend(layer, q, rows, granted)
     cache.truncate(rows, kept_lengths)          # rejected drafts
 
-and ``fork`` / ``free`` / ``compact`` manage whole sequences.  Page tables,
+and ``fork`` / ``free`` / ``compact`` manage whole sequences.  A cache that
+tracks weights holds long sequences within a budget:
+
+    out, lse = cache.attend(layer, q, rows, granted, return_lse=True)
+    cache.weigh(layer, q, lse, rows, granted)   # what each token received
+    kept = cache.evict(rows, budget, first=4, recent=128)
+  Page tables,
 lengths and reference counts live on the device and every call is a few
 launches on the current stream: nothing waits for the host, so accepted
 counts that only the device knows drive the next step, and a step can be
@@ -50,10 +56,13 @@ class Int4PagedCache:
     """``n_layers`` pools of ``n_pages`` pages for ``max_seqs`` sequences of up to ``max_blocks`` pages.
 
     ``group_size`` channels share a scale and zero: head_dim (default),
-    head_dim / 2 or head_dim / 4; head_dim 64, 128 or 256."""
+    head_dim / 2 or head_dim / 4; head_dim 64, 128 or 256.  ``track_weights``: ``weights`` (n_layers, max_seqs,
+    max_blocks * 32) fp32 holds the attention weight that each token of each row has received (``weigh``), 0 for a
+    token when ``reserve`` makes room for it; ``fork`` and ``evict`` take it along.  It may be read, scaled or
+    replaced between calls."""
 
     def __init__(self, n_layers: int, n_pages: int, kv_heads: int, head_dim: int, group_size: Optional[int] = None,
-                 max_seqs: int = 64, max_blocks: int = 1024, device="cuda"):
+                 max_seqs: int = 64, max_blocks: int = 1024, device="cuda", track_weights: bool = False):
         group_size = head_dim if group_size is None else group_size
         self.layout = _C.int4_layout(head_dim, group_size)
         if min(n_layers, n_pages, kv_heads, max_seqs, max_blocks) <= 0:
@@ -88,6 +97,8 @@ class Int4PagedCache:
         self._page_ws = torch.empty(self._page_ws_bytes, dtype=torch.uint8, device=device)
         self._page_ws_ptr = self._page_ws.data_ptr()
         self._pool_ptr, self._layer_bytes, self._page_bytes = self.buf.data_ptr(), self.buf.stride(0), self.buf.stride(1)
+        self.weights = torch.zeros(n_layers, max_seqs, max_blocks * BLOCK, dtype=torch.float32,
+                                   device=device) if track_weights else None
         self._views = [self._view(layer) for layer in range(n_layers)]
         self._view_ptrs = [ctypes.addressof(v) for v in self._views]
 
@@ -119,7 +130,7 @@ class Int4PagedCache:
 
     def load_state(self, buf: torch.Tensor, table: torch.Tensor, lens: torch.Tensor) -> None:
         """Take over pages, table and lengths (a checkpoint's ``buf``, ``table``, ``lens``); the reference
-        counts follow from the table."""
+        counts follow from the table.  Tracked weights are set to 0."""
         if buf.shape != self.buf.shape or table.shape != self.table.shape or lens.shape != self.lens.shape:
             raise ValueError("the state's shapes do not match the cache")
         if int(lens.min()) < 0 or int(lens.max()) > self.max_blocks * BLOCK:
@@ -136,6 +147,8 @@ class Int4PagedCache:
         self.refs.zero_()
         self.refs.index_add_(0, pages, torch.ones_like(pages, dtype=torch.int32))
         self._rebuild_free()
+        if self.weights is not None:
+            self.weights.zero_()
 
     def check(self) -> None:
         """Wait for the device and raise if an operation reported an error since the last check."""
@@ -219,6 +232,11 @@ class Int4PagedCache:
             _C.raw_stream(self._dev_index))
         if rc:
             _C.check(rc, "akv_pages_reserve_many")
+        if self.weights is not None:
+            rc = self._lib.akv_int4_weights_clear(self._pt_ref, *self._weight_args(), _C.ptr(rows),
+                                                  granted.data_ptr(), n, _C.raw_stream(self._dev_index))
+            if rc:
+                _C.check(rc, "akv_int4_weights_clear")
         return granted
 
     def fork(self, parents, children) -> None:
@@ -230,6 +248,11 @@ class Int4PagedCache:
         parents = self._ints(parents, "parents")
         n = parents.shape[0]
         children = self._ints(children, "children", n)
+        if self.weights is not None:
+            rc = self._lib.akv_int4_weights_fork(self._pt_ref, *self._weight_args(), parents.data_ptr(),
+                                                 children.data_ptr(), n, _C.raw_stream(self._dev_index))
+            if rc:
+                _C.check(rc, "akv_int4_weights_fork")
         rc = self._lib.akv_pages_fork(self._pt_ref, parents.data_ptr(), children.data_ptr(), n, self._status_ptr,
                                       _C.raw_stream(self._dev_index))
         if rc:
@@ -283,6 +306,87 @@ class Int4PagedCache:
                                       _C.raw_stream(self._dev_index))
         if rc:
             _C.check(rc, "akv_pages_copy")
+
+    # ------------------------------------------------------------------ eviction
+    def _weight_args(self) -> tuple:
+        """Pointer, layer and row strides of the weights, and the layers."""
+        w = self.weights
+        if w.shape != (self.n_layers, self.max_seqs, self.max_blocks * BLOCK) or w.dtype is not torch.float32 or \
+                w.device != self._dev or not w.is_contiguous():
+            raise ValueError(f"weights must be contiguous fp32 ({self.n_layers}, {self.max_seqs}, "
+                             f"{self.max_blocks * BLOCK}) on {self._dev}")
+        return w.data_ptr(), w.stride(0), w.stride(1), self.n_layers
+
+    def weigh(self, layer: int, query: torch.Tensor, lse: torch.Tensor, rows=None, n_new=None,
+              sm_scale: Optional[float] = None) -> None:
+        """Add the attention weight that the rows' newest tokens give to every token they see to
+        ``weights[layer]``: over all query heads and new tokens, exp(q . K_t * sm_scale - lse).
+
+        query, rows and n_new as in ``attend``; lse (R, Hq, M), or (R, Hq, 1) with a query of one token, fp32, as it
+        returned it.  Queries past n_new[i] add nothing, nor do those that are not finite or whose lse is not.  A row
+        named twice counts once."""
+        if _C.current_device() != self._dev_index:
+            with torch.cuda.device(self._dev_index):
+                return self.weigh(layer, query, lse, rows, n_new, sm_scale)
+        if self.weights is None:
+            raise RuntimeError("the cache does not track weights (track_weights=True)")
+        view = self._layer(layer)
+        dt = _half_dtype(query)
+        q = query.unsqueeze(2) if query.dim() == 3 else query
+        shape = q.shape
+        if len(shape) != 4 or shape[3] != self.D or shape[1] % self.H or not shape[1]:
+            raise ValueError(f"query must be (rows, a multiple of {self.H} heads, tokens, {self.D})")
+        if q.device != self._dev or lse.device != self._dev:
+            raise RuntimeError(f"akv: the query and lse must be on {self._dev} (no CPU fallback)")
+        R, Hq, M, D = shape
+        if lse.shape != (R, Hq, M) or lse.dtype is not torch.float32:
+            raise ValueError(f"lse must be fp32 ({R}, {Hq}, {M})")
+        lse = lse.contiguous()
+        qs = q.stride()
+        if qs[3] != 1:
+            q = q.contiguous()
+            qs = q.stride()
+        rows, n_new, rp, np_ = self._rows(rows, n_new, R)
+        wp, w_layer, w_row, _ = self._weight_args()
+        rc = self._lib.akv_int4_weigh(
+            _C.WEIGH_ARGS.pack(view, rp, np_, q.data_ptr(), qs[0], qs[1], qs[2], lse.data_ptr(),
+                               wp + 4 * layer * w_layer, w_row, self._status_ptr, R, M, Hq, dt,
+                               self._scale if sm_scale is None else float(sm_scale), 0),
+            _C.raw_stream(self._dev_index))
+        if rc:
+            _C.check(rc, "akv_int4_weigh")
+
+    def evict(self, rows, keep: int, first: int = 0, recent: int = 0) -> torch.Tensor:
+        """Bring each of ``rows`` (None: all) that holds more than ``keep`` tokens down to ``keep``: its first
+        ``first`` and last ``recent`` ones and the heaviest of the others by their weights' sum over the layers (the
+        earliest first among equal ones).  They move together in their order, in every layer, as if the others had
+        never been appended (rotary positions are part of the keys and stay); pages left over go back to the pool,
+        pages shared with other rows stay theirs.
+
+        Returns the old positions of the tokens that stay, int32 (rows, keep), -1 past a row's end.  A row that needs
+        new pages for shared ones when the pool has none is refused, as are all after it: they stay as they are, -1
+        everywhere.  So is a row named twice, the second time."""
+        if _C.current_device() != self._dev_index:
+            with torch.cuda.device(self._dev_index):
+                return self.evict(rows, keep, first, recent)
+        if self.weights is None:
+            raise RuntimeError("the cache does not track weights (track_weights=True)")
+        if keep < 1 or first < 0 or recent < 0 or first + recent > keep or keep >= 1 << 31:
+            raise ValueError(f"keep must be positive and first + recent at most that (got {keep}, {first}, {recent})")
+        rows = self._ints(rows, "rows")
+        n = self.max_seqs if rows is None else rows.shape[0]
+        kept = torch.empty_strided((n, keep), (keep, 1), dtype=torch.int32, device=self._dev)
+        need = int(self._lib.akv_int4_evict_workspace_bytes(n, self.max_blocks, self.n_pages)) if n else 0
+        ws = torch.empty(need, dtype=torch.uint8, device=self._dev)
+        wp, w_layer, w_row, _ = self._weight_args()
+        rc = self._lib.akv_int4_evict(
+            _C.EVICT_ARGS.pack(ctypes.addressof(self._pt), self._pool_ptr, self._layer_bytes, self._page_bytes, wp,
+                               w_layer, w_row, _C.ptr(rows) or 0, kept.data_ptr(), ws.data_ptr(), need,
+                               self._status_ptr, n, self.n_layers, self.H, self.D, self.group, keep, first, recent),
+            _C.raw_stream(self._dev_index))
+        if rc:
+            _C.check(rc, "akv_int4_evict")
+        return kept
 
     # ------------------------------------------------------------------ tokens
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows=None, n_new=None) -> None:

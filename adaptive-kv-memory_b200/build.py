@@ -22,7 +22,8 @@ OUT_DIR = os.path.join(HERE, "akv", "_lib")
 LIB = os.path.join(OUT_DIR, "libakv_sm100.so")
 SOURCES = ["quant_pack.cu", "decode_attn.cu", "tiering.cu", "prefill_attn.cu", "group_format.cu", "layer_step.cu", "peer_exchange.cu",
            "int4_cache.cu", "int4_attn.cu", "int4_attn_64.cu", "int4_attn_128.cu", "int4_attn_256.cu",
-           "page_table.cu", "verify_draft.cu", "token_logprobs.cu"]
+           "page_table.cu", "verify_draft.cu", "token_logprobs.cu",
+           "int4_weigh.cu", "int4_evict.cu"]
 
 
 def nvcc() -> str:

@@ -1,0 +1,467 @@
+// Attention weight that the tokens of the 4-bit paged cache receive.
+//
+//   weights[s][t] += sum over query heads h and new tokens m that see t of
+//                    exp(q_hm . K_t * scale - lse_hm)
+// with the log-sum-exp that attention returned, so each query's weights sum to
+// 1 and nothing has to be normalised in a second pass.  Only the K half of the
+// records is read.  With K_t = c s_tg + z_tg in channel group g,
+//   q.K_t = sum_g s_tg (q_g . (c_tg - 8)) + (z_tg + 8 s_tg) sum(q_g)
+// the contraction runs on codes, exact in fp16, and its accumulators, scales
+// and sums are fp32: the only rounding before the exponential is fp32's.
+// (Queries enter fp16 scaled per row by a power of two, exact unless 2^-24 of
+// the row's largest.)
+//
+// A token's sum is formed by one thread set in a fixed order (heads, then
+// queries), so a call repeated gives the same bits.
+//
+// Few queries: the pages of all rows form one list that is cut into equal
+// shares, one per resident CTA, from the lengths on the device.  A warp takes
+// every fourth page of its share and streams the page's heads through its own
+// ring of bulk copies; tokens are the MMA's rows, queries its columns.  The
+// queries of up to kWeighUnits (head, 8 or 16 columns) units stand in shared
+// memory as MMA fragments; more of them take the pages again.
+#include <type_traits>
+
+#include "int4.cuh"
+
+namespace akv {
+
+constexpr int kWeighWarps = 4;
+constexpr int kWeighThreads = kWeighWarps * 32;
+constexpr int kWeighRows = 1024;   // call rows of one launch
+constexpr int kWeighUnits = 8;     // (head, column tile) units prepared at a time
+
+struct WeighParams {
+  akv_int4_cache c;
+  const int32_t* rows;
+  const int32_t* n_new;
+  int row0, R;  // call rows [row0, row0 + R) of this launch
+  int M, Hq;
+  const uint16_t* q;
+  int64_t q_sr, q_sh, q_sm;
+  const float* lse;
+  float scale;
+  float* weights;
+  int64_t w_stride;
+  int bf16;
+  int* status;
+};
+
+template <int D, int G, int NT>
+struct WeighShape {
+  static constexpr int GS = D / G;
+  static constexpr int BK = GS / 8;     // K bytes of a thread per token and group
+  static constexpr int KS = D / 16;     // MMA steps
+  static constexpr int ROWS = 8 * NT;   // query columns of a unit
+  static constexpr int CODES = kBlockTokens * D / 2;
+  static constexpr int PAIRS = kBlockTokens * G * 4;
+  static constexpr int REC = CODES + PAIRS;
+  static constexpr int STAGES = D == 256 ? 3 : 4;
+  static constexpr int OFF_FRAG = kWeighWarps * STAGES * REC;
+  static constexpr int FRAG = KS * NT * 32 * 8;
+  // per unit: fragments, then group sums of q, exponent factors, minus lse, visible lengths
+  static constexpr int OFF_QS = OFF_FRAG + kWeighUnits * FRAG;
+  static constexpr int OFF_CQ = OFF_QS + kWeighUnits * ROWS * G * 4;
+  static constexpr int OFF_L2 = OFF_CQ + kWeighUnits * ROWS * 4;
+  static constexpr int OFF_SEE = OFF_L2 + kWeighUnits * ROWS * 4;
+  static constexpr int OFF_BAR = OFF_SEE + kWeighUnits * ROWS * 4;
+  static constexpr int OFF_PREF = OFF_BAR + kWeighWarps * STAGES * 8;
+  static constexpr int smem(int rows) { return OFF_PREF + (3 * rows + 1) * 4; }
+};
+
+// token of tile row g: see the attention kernel's bank note
+AKV_DEV int weigh_token(int g) { return g ^ ((g >> 2) & 1); }
+
+// the codes in bits 0..3 (4..7) of both halves, as the fp16 pair c - 8
+AKV_DEV uint32_t code8_low(uint32_t w) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(lop_magic<0x000F000Fu>(w)), "r"(0xE408E408u));  // - 1032
+  return r;
+}
+AKV_DEV uint32_t code8_high(uint32_t w) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;"  // (1024 + 16 c) / 16 - 72
+      : "=r"(r)
+      : "r"(lop_magic<0x00F000F0u>(w)), "r"(0x2C002C00u), "r"(0xD480D480u));
+  return r;
+}
+
+template <int BYTES>
+AKV_DEV void weigh_lds(const uint8_t* p, uint32_t (&w)[BYTES < 4 ? 1 : BYTES / 4]) {
+  if constexpr (BYTES >= 16) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 v = lds_v4(p + 16 * i);
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (BYTES == 8) {
+    const uint2 v = lds_v2(p);
+    w[0] = v.x, w[1] = v.y;
+  } else if constexpr (BYTES == 4) {
+    w[0] = lds_u32(p);
+  } else {
+    w[0] = *reinterpret_cast<const uint16_t*>(p);
+  }
+}
+
+// Lengths of the call rows [row0, row0 + R) and their pages' prefix sums; a row
+// without new tokens has none, nor has one that an earlier call row names.
+AKV_DEV void weigh_rows(const WeighParams& P, int* s_pref, int* s_len, int* s_new, int* s_scan) {
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, n_warps = blockDim.x >> 5;
+  for (int e = t; e < P.R; e += blockDim.x) {
+    const Int4Row r = int4_row(P.c, P.rows, P.n_new, P.row0 + e, P.M, P.status);
+    s_new[e] = r.n_new;
+    s_len[e] = r.len;
+    if (!P.rows) continue;
+    for (int s = 0; s < P.row0 + e; ++s)
+      if (P.rows[s] == r.seq) {
+        set_status(P.status, AKV_ERR_SHAPE);
+        s_new[e] = 0;
+        break;
+      }
+  }
+  int base = 0;
+  for (int e0 = 0; e0 < P.R; e0 += blockDim.x) {
+    __syncthreads();
+    const int e = e0 + t;
+    int x = e < P.R && s_new[e] > 0 ? (s_len[e] + kBlockTokens - 1) / kBlockTokens : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(~0u, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s_scan[warp] = x;
+    __syncthreads();
+    int before = base, sum = base;
+    for (int w = 0; w < n_warps; ++w) {
+      if (w < warp) before += s_scan[w];
+      sum += s_scan[w];
+    }
+    if (e < P.R) s_pref[e + 1] = before + x;
+    base = sum;
+  }
+  if (t == 0) s_pref[0] = 0;
+  __syncthreads();
+}
+
+template <int D, int G, int NT>
+__global__ void __launch_bounds__(kWeighThreads, D == 256 ? 2 : 3) weigh_few_kernel(const WeighParams P) {
+  using S = WeighShape<D, G, NT>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* s_qs = reinterpret_cast<float*>(smem + S::OFF_QS);   // [unit][G][ROWS]
+  float* s_cq = reinterpret_cast<float*>(smem + S::OFF_CQ);
+  float* s_l2 = reinterpret_cast<float*>(smem + S::OFF_L2);
+  int* s_see = reinterpret_cast<int*>(smem + S::OFF_SEE);
+  uint64_t* s_bar = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
+  int* s_pref = reinterpret_cast<int*>(smem + S::OFF_PREF);
+  int* s_len = s_pref + P.R + 1;
+  int* s_new = s_len + P.R;
+  __shared__ int s_scan[kWeighWarps];
+
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int g = lane >> 2, q4 = lane & 3;
+  const int H = P.c.kv_heads, rep = P.Hq / H;
+
+  if (lane < S::STAGES) mbar_init(s_bar + warp * S::STAGES + lane, 1);
+  fence_mbar_init();
+  weigh_rows(P, s_pref, s_len, s_new, s_scan);
+
+  const int total = s_pref[P.R];
+  const int share = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  int pos = static_cast<int>(min(static_cast<int64_t>(share) * blockIdx.x, static_cast<int64_t>(total)));
+  const int end = min(total, pos + share);
+  int e = 0, hi = P.R;  // the last row that starts at or before pos
+  while (hi - e > 1) {
+    const int mid = (e + hi) / 2;
+    if (s_pref[mid] <= pos) e = mid; else hi = mid;
+  }
+
+  uint8_t* ring = smem + warp * S::STAGES * S::REC;
+  uint64_t* bars = s_bar + warp * S::STAGES;
+  uint32_t stage = 0, phase = 0;
+  bool alive = true;
+
+  while (pos < end) {
+    while (s_pref[e + 1] <= pos) ++e;
+    const int page0 = pos - s_pref[e];
+    const int n_pages = min(s_pref[e + 1], end) - pos;
+    const int i = P.row0 + e, len = s_len[e], n_new = s_new[e];
+    const int seq = P.rows ? __ldg(P.rows + i) : i;
+    const int32_t* table = P.c.table + seq * P.c.table_stride + page0;
+    float* w_row = P.weights + seq * P.w_stride;
+    const int mine = (n_pages - warp + kWeighWarps - 1) / kWeighWarps;  // pages warp, warp + 4, ...
+    const int tiles = (n_new * rep + S::ROWS - 1) / S::ROWS, units = H * tiles;
+
+    for (int u0 = 0; u0 < units; u0 += kWeighUnits) {
+      const int u1 = min(units, u0 + kWeighUnits);
+      const int h0 = u0 / tiles, heads = (u1 - 1) / tiles - h0 + 1;
+      const int items = mine * heads;  // (page, head) records of this warp
+
+      // a page's number, checked; pages are looked up one ahead of their copies
+      auto page_of = [&](int k) -> int {
+        if (k >= mine) return -1;
+        const int p = __ldg(table + warp + k * kWeighWarps);
+        if (p >= 0 && p < P.c.n_pages) return p;
+        set_status(P.status, AKV_ERR_SHAPE);
+        return -1;
+      };
+      int next_k = 0, next_h = 0, next_p = page_of(0);  // the next record to copy
+      auto issue = [&](uint32_t st) {
+        if (next_k < mine) {
+          if (lane == 0) {
+            // a bad page is read as page 0; nothing of it is added
+            const uint8_t* rec = P.c.pool + (next_p < 0 ? 0 : next_p) * P.c.page_stride + (h0 + next_h) * P.c.head_stride;
+            mbar_arrive_expect_tx(bars + st, S::REC);
+            tma_load_1d(ring + st * S::REC, rec + int4_layout(D, G).kc, S::CODES, bars + st);
+            tma_load_1d(ring + st * S::REC + S::CODES, rec + int4_layout(D, G).kp, S::PAIRS, bars + st);
+          }
+          if (++next_h == heads) {
+            next_h = 0;
+            next_p = page_of(++next_k);
+          }
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < S::STAGES; ++k)
+        if (alive) issue((stage + k) % S::STAGES);
+
+      // ---- queries of the units as MMA operands
+      __syncthreads();  // the previous units' are done with
+      constexpr int PER = D / 32;
+      for (int n = warp; n < (u1 - u0) * S::ROWS; n += kWeighWarps) {
+        const int unit = n / S::ROWS, col = n % S::ROWS;
+        const int h = (u0 + unit) / tiles, rr = (u0 + unit) % tiles * S::ROWS + col, m = rr / rep;
+        const int hq = h * rep + rr - m * rep;
+        const bool on = m < n_new;
+        const uint16_t* src = P.q + i * P.q_sr + hq * P.q_sh + m * P.q_sm + lane * PER;
+        float x[PER];
+        uint32_t top = 0u;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const uint16_t raw = on ? src[k] : 0;
+          x[k] = P.bf16 ? elem_to_float<true>(raw) : elem_to_float<false>(raw);
+          top = max(top, __float_as_uint(x[k]) & 0x7FFFFFFFu);
+        }
+        top = __reduce_max_sync(~0u, top);
+        const bool bad = top >= 0x7F800000u;
+        int ex = 0;  // 2^ex brings the largest into [2^9, 2^10)
+        if (top && !bad) ex = 9 - (static_cast<int>(top >> 23) - 127);
+        ex = ex > 120 ? 120 : (ex < -120 ? -120 : ex);
+        const float up = exp2f(static_cast<float>(ex));
+        uint16_t* frag = reinterpret_cast<uint16_t*>(smem + S::OFF_FRAG + unit * S::FRAG);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const int c = lane * PER + k;
+          const __half hv = __float2half_rn(bad ? 0.f : x[k] * up);
+          sum += __half2float(hv);
+          const int gi = c / S::GS, r = c % S::GS, cc = r / (S::GS / 4), r2 = r % (S::GS / 4);
+          int ks, half;
+          if constexpr (S::BK >= 4) {
+            ks = gi * (S::GS / 16) + (r2 / 8) * 2 + ((r2 >> 1) & 1);
+            half = (r2 >> 2) & 1;
+          } else {
+            ks = gi;
+            half = r2 >> 1;
+          }
+          const int reg = c & 1 ? 0 : 1;
+          frag[(((ks * NT + col / 8) * 32 + (col % 8) * 4 + cc) * 2 + reg) * 2 + half] = __half_as_ushort(hv);
+        }
+        constexpr int GL = 32 / G;  // lanes of a group
+#pragma unroll
+        for (int o = 1; o < GL; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (lane % GL == 0) s_qs[(unit * G + lane / GL) * S::ROWS + col] = sum;
+        if (lane == 0) {
+          const float lse = on ? __ldg(P.lse + (static_cast<int64_t>(i) * P.Hq + hq) * P.M + m) : -INFINITY;
+          const bool counts = on && !bad && fabsf(lse) < INFINITY;
+          s_cq[unit * S::ROWS + col] = ldexpf(P.scale * 1.4426950408889634f, -ex);
+          s_l2[unit * S::ROWS + col] = counts ? -lse * 1.4426950408889634f : -INFINITY;
+          s_see[unit * S::ROWS + col] = counts ? len - n_new + m + 1 : 0;
+        }
+      }
+      __syncthreads();
+
+      // ---- this warp's pages: all heads of the units, then the next page
+      for (int k = 0, item = 0; k < mine && alive; ++k) {
+        const int tok0 = (page0 + warp + k * kWeighWarps) * kBlockTokens;
+        const int p = __ldg(table + warp + k * kWeighWarps);
+        float w[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int hh = 0; hh < heads; ++hh, ++item) {
+          if (!__all_sync(~0u, mbar_wait(bars + stage, phase, P.status))) {
+            // a copy never came: take no more, but see the ones in flight land
+            for (int r = 1; r < S::STAGES && item + r < items; ++r) {
+              const uint32_t st = stage + r;
+              mbar_wait(bars + st % S::STAGES, st >= S::STAGES ? phase ^ 1 : phase, P.status);
+            }
+            alive = false;
+            break;
+          }
+          const uint8_t* rec = ring + stage * S::REC;
+          uint32_t kp[4][G];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi)
+              kp[r][gi] = lds_u32(rec + S::CODES + (r * 8 + weigh_token(g)) * G * 4 + gi * 4);
+          const int ub = max(u0, (h0 + hh) * tiles) - u0, ue = min(u1, (h0 + hh + 1) * tiles) - u0;
+          for (int unit = ub; unit < ue; ++unit) {
+            const uint2* frag = reinterpret_cast<const uint2*>(smem + S::OFF_FRAG + unit * S::FRAG) + lane;
+            const uint64_t* qs2 = reinterpret_cast<const uint64_t*>(s_qs + unit * G * S::ROWS) + q4;
+            uint64_t x[4][NT];
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) {
+              uint32_t kw[4][S::BK < 4 ? 1 : S::BK / 4];
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                weigh_lds<S::BK>(rec + (r * 8 + weigh_token(g)) * (D / 2) + gi * (S::GS / 2) + q4 * S::BK, kw[r]);
+              float acc[2][NT][4];
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int c = 0; c < 4; ++c) acc[mt][nt][c] = 0.f;
+#pragma unroll
+              for (int s = 0; s < S::GS / 16; ++s) {
+                const int ks = gi * (S::GS / 16) + s;
+                uint2 b[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) b[nt] = frag[(ks * NT + nt) * 32];
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt) {
+                  uint32_t a[4];
+#pragma unroll
+                  for (int r = 0; r < 2; ++r) {
+                    uint32_t v;
+                    if constexpr (S::BK >= 4) v = s & 1 ? kw[2 * mt + r][s / 2] >> 8 : kw[2 * mt + r][s / 2];
+                    else v = prmt(kw[2 * mt + r][0], 0u, 0x4140);
+                    a[r] = code8_low(v);
+                    a[2 + r] = code8_high(v);
+                  }
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt) mma_16816(acc[mt][nt], a[0], a[1], a[2], a[3], b[nt].x, b[nt].y);
+                }
+              }
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float2 sz = __half22float2(u32_as_h2(kp[r][gi]));
+                const float mid = fmaf(8.f, sz.x, sz.y);
+                const uint64_t s2 = f2_make(sz.x, sz.x), z2 = f2_make(mid, mid);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  const uint64_t q2 = qs2[(gi * S::ROWS + nt * 8) / 2];
+                  const float* a = acc[r >> 1][nt] + (r & 1) * 2;
+                  const uint64_t zq = gi == 0 ? f2_mul(z2, q2) : f2_fma(z2, q2, x[r][nt]);
+                  x[r][nt] = f2_fma(f2_make(a[0], a[1]), s2, zq);
+                }
+              }
+            }
+            const bool tail = tok0 + kBlockTokens > len - n_new;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const int c0 = unit * S::ROWS + nt * 8 + 2 * q4;
+              const float2 cq = *reinterpret_cast<const float2*>(s_cq + c0), l2 = *reinterpret_cast<const float2*>(s_l2 + c0);
+              const int2 see = *reinterpret_cast<const int2*>(s_see + c0);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                float2 y = f2_split(f2_fma(x[r][nt], f2_make(cq.x, cq.y), f2_make(l2.x, l2.y)));
+                if (tail) {
+                  const int tok = tok0 + r * 8 + weigh_token(g);
+                  if (tok >= see.x) y.x = -INFINITY;
+                  if (tok >= see.y) y.y = -INFINITY;
+                }
+                w[r] += fast_exp2(y.x) + fast_exp2(y.y);
+              }
+            }
+          }
+          __syncwarp();
+          if (++stage == S::STAGES) stage = 0, phase ^= 1;
+          issue((stage + S::STAGES - 1) % S::STAGES);
+        }
+        if (!alive) break;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          w[r] += __shfl_xor_sync(~0u, w[r], 1);
+          w[r] += __shfl_xor_sync(~0u, w[r], 2);
+        }
+        const int tok = tok0 + q4 * 8 + weigh_token(g);
+        if (tok < len && p >= 0 && p < P.c.n_pages) w_row[tok] += q4 < 2 ? (q4 == 0 ? w[0] : w[1]) : (q4 == 2 ? w[2] : w[3]);
+      }
+    }
+    pos += n_pages;
+  }
+}
+
+template <int D, int G, int NT>
+static int launch_few(const WeighParams& P, cudaStream_t st) {
+  using S = WeighShape<D, G, NT>;
+  const int smem = S::smem(P.R);
+  if (!ensure_dynamic_smem<weigh_few_kernel<D, G, NT>>(smem)) return AKV_ERR_LAUNCH;
+  constexpr int kPerSm = D == 256 ? 2 : 3;
+  const int64_t pages = static_cast<int64_t>(P.R) * P.c.max_blocks;
+  const int64_t most = 148 * kPerSm, want = (pages + kWeighWarps - 1) / kWeighWarps;
+  weigh_few_kernel<D, G, NT><<<static_cast<int>(want < most ? want : most), kWeighThreads, smem, st>>>(P);
+  return cudaGetLastError() == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH;
+}
+
+template <int D, int NT>
+static int few_by_group(const WeighParams& P, cudaStream_t st) {
+  switch (D / P.c.group) {
+    case 1: return launch_few<D, 1, NT>(P, st);
+    case 2: return launch_few<D, 2, NT>(P, st);
+    default: return launch_few<D, 4, NT>(P, st);
+  }
+}
+
+static int weigh_few(const WeighParams& P, cudaStream_t st) {
+  const bool one = P.M * (P.Hq / P.c.kv_heads) <= 8;
+  switch (P.c.head_dim) {
+    case 64: return one ? few_by_group<64, 1>(P, st) : few_by_group<64, 2>(P, st);
+    case 128: return one ? few_by_group<128, 1>(P, st) : few_by_group<128, 2>(P, st);
+    default: return one ? few_by_group<256, 1>(P, st) : few_by_group<256, 2>(P, st);
+  }
+}
+
+}  // namespace akv
+
+using namespace akv;
+
+extern "C" int akv_int4_weigh(const akv_int4_weigh_args* a, void* stream) {
+  if (!a) return AKV_ERR_NULL;
+  const akv_int4_cache* c = a->cache;
+  const int rc = int4_check(c);
+  if (rc) return rc;
+  if (a->dtype != AKV_FP16 && a->dtype != AKV_BF16) return AKV_ERR_UNSUPPORTED;
+  if (a->R < 0 || a->M < 0 || a->Hq <= 0 || a->Hq % c->kv_heads) return AKV_ERR_SHAPE;
+  if (a->w_stride < static_cast<int64_t>(c->max_blocks) * kBlockTokens) return AKV_ERR_SHAPE;
+  if (a->R == 0 || a->M == 0) return AKV_OK;
+  if (!a->q || !a->lse || !a->weights) return AKV_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(a->q) & 1) ||
+      ((reinterpret_cast<uintptr_t>(a->lse) | reinterpret_cast<uintptr_t>(a->weights)) & 3))
+    return AKV_ERR_ALIGN;
+  // columns and pages of a launch are counted in 32 bits
+  if (static_cast<int64_t>(a->M) * a->Hq > INT32_MAX / 2) return AKV_ERR_UNSUPPORTED;
+  int rows = kWeighRows;
+  if (rows > INT32_MAX / c->max_blocks) rows = INT32_MAX / c->max_blocks;
+  WeighParams p{};
+  p.c = *c;
+  p.rows = a->rows;
+  p.n_new = a->n_new;
+  p.M = a->M;
+  p.Hq = a->Hq;
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.q_sr = a->q_sr; p.q_sh = a->q_sh; p.q_sm = a->q_sm;
+  p.lse = a->lse;
+  p.scale = a->sm_scale;
+  p.weights = a->weights;
+  p.w_stride = a->w_stride;
+  p.bf16 = a->dtype == AKV_BF16;
+  p.status = a->status;
+  for (int r = 0; r < a->R; r += rows) {
+    p.row0 = r;
+    p.R = a->R - r < rows ? a->R - r : rows;
+    const int e = weigh_few(p, static_cast<cudaStream_t>(stream));
+    if (e) return e;
+  }
+  return AKV_OK;
+}

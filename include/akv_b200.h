@@ -717,6 +717,31 @@ typedef struct {
 size_t akv_int4_attention_workspace_bytes(int R, int M, int Hq, int kv_heads, int head_dim, int max_blocks);
 int akv_int4_attention(const akv_int4_attention_args* a, void* stream);
 
+/* Attention weight that the tokens receive, added to a running total:
+ *   weights[s*w_stride + t] += sum over hq, m < n_new[i] with pos(m) >= t of
+ *                              exp(q . K_t * sm_scale - lse[i][hq][m])
+ * for s = rows[i] and t < lens[s]; positions as in akv_int4_attention, q laid
+ * out alike, lse fp32 [R][Hq][M] (natural log) as it returned it.  A query that
+ * is not finite, or whose lse is not, adds nothing.  Sums are taken in an order
+ * that the shapes and lengths alone decide.  A row named twice counts once
+ * (AKV_ERR_SHAPE in *status). */
+typedef struct {
+  const akv_int4_cache* cache;
+  const int32_t* rows;
+  const int32_t* n_new;
+  const void* q;
+  int64_t q_sr, q_sh, q_sm;
+  const float* lse;
+  float* weights;
+  int64_t w_stride;
+  int* status;
+  int32_t R, M, Hq, dtype;
+  float sm_scale;
+  int32_t reserved;              /* 0 */
+} akv_int4_weigh_args;
+
+int akv_int4_weigh(const akv_int4_weigh_args* a, void* stream);
+
 /* ------------------------------------------------------------------------
  * Ownership of the pages, kept on the device so that no step of a serving
  * loop waits for the host.  refs[p] sequences hold page p; bit p of free_bits
@@ -776,6 +801,49 @@ int akv_pages_compact(const akv_page_table* t, uint8_t* pool, int n_layers, int6
  * both lists, nor twice in dst). */
 int akv_pages_copy(uint8_t* pool, int n_layers, int64_t layer_stride, int64_t page_bytes, int n_pages,
                    const int32_t* src, const int32_t* dst, int n, int* status, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Eviction from a 4-bit paged cache.  Row rows[i] (NULL: i) of more than
+ * `keep` tokens is brought down to `keep`: its first `first` and last `recent`
+ * tokens and the largest of the others by fp32(sum over l, in fp64, of
+ * weights[l*w_layer + s*w_row + t]) (NaN below all, the lowest token first
+ * among equal ones).  They move together in their order, in every layer and KV
+ * head, and their weights with them; pages left over lose this holder.  A page
+ * that has other holders and would be written is left to them: the row gets a
+ * free one (the lowest, in order) in its place.  When the pool runs out, that
+ * row and all after it are refused and stay as they are (AKV_ERR_EXHAUSTED);
+ * so is a bad or repeated row (AKV_ERR_SHAPE).  kept int32 [n][keep]: the old
+ * positions of the tokens that stay, ascending, then -1 (all -1 for a refused
+ * row).  keep >= 1, first + recent <= keep.
+ * Workspace: akv_int4_evict_workspace_bytes(...), 16-byte aligned.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  const akv_page_table* table;
+  uint8_t* pool;
+  int64_t layer_stride, page_bytes;
+  float* weights;
+  int64_t w_layer, w_row;        /* in floats; w_row >= 32 * max_blocks */
+  const int32_t* rows;
+  int32_t* kept;
+  void* workspace;
+  size_t workspace_bytes;
+  int* status;
+  int32_t n, n_layers, kv_heads, head_dim, group, keep, first, recent;
+} akv_int4_evict_args;
+
+size_t akv_int4_evict_workspace_bytes(int n, int max_blocks, int n_pages);
+int akv_int4_evict(const akv_int4_evict_args* a, void* stream);
+
+/* The weights of the last n_new[i] tokens of row rows[i] (NULL: i), i < n, set
+ * to 0 in every layer (after a reserve that granted them). */
+int akv_int4_weights_clear(const akv_page_table* t, float* weights, int64_t w_layer, int64_t w_row, int n_layers,
+                           const int32_t* rows, const int32_t* n_new, int n, void* stream);
+
+/* The weights of row parents[i] copied to the empty row children[i] in every
+ * layer (before the fork; a request that fork refuses changes nothing that
+ * counts). */
+int akv_int4_weights_fork(const akv_page_table* t, float* weights, int64_t w_layer, int64_t w_row, int n_layers,
+                          const int32_t* parents, const int32_t* children, int n, void* stream);
 
 /* ------------------------------------------------------------------------
  * Verification of drafted tokens (speculative decoding).  target (b, j, x) at
