@@ -191,6 +191,8 @@ SIGNATURES = {
     "akv_int4_read": (c_int, [c_char_p, c_void_p]),
     "akv_int4_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "akv_int4_attention": (c_int, [c_char_p, c_void_p]),
+    "akv_int4_chunk_workspace_bytes": (c_size_t, [c_int]),
+    "akv_int4_chunk_attention": (c_int, [c_char_p, c_void_p]),
     "akv_int4_weigh": (c_int, [c_char_p, c_void_p]),
     "akv_int4_evict_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "akv_int4_evict": (c_int, [c_char_p, c_void_p]),

@@ -89,6 +89,8 @@ class Int4PagedCache:
                                 self.free_bits.data_ptr(), max_seqs, max_blocks, n_pages)
         self._ws: dict = {}
         self._ws_need: dict = {}
+        self._chunk_ws: dict = {}  # per stream: calls on two streams may overlap
+        self._chunk_ws_bytes = int(self._lib.akv_int4_chunk_workspace_bytes(head_dim))
         self._scale = 1.0 / math.sqrt(head_dim)
         self._pt_ref = ctypes.byref(self._pt)
         # the page operations of one cache follow one another (they change one table), so they share a workspace
@@ -306,6 +308,58 @@ class Int4PagedCache:
                                       _C.raw_stream(self._dev_index))
         if rc:
             _C.check(rc, "akv_pages_copy")
+
+    # ------------------------------------------------------------------ chunks
+    def attend_chunk(self, layer: int, query: torch.Tensor, rows=None, n_new=None, sm_scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None, return_lse: bool = False):
+        """``attend`` for a chunk of new tokens a row (a prompt's, tens to thousands): the same arguments and
+        results, on the tensor cores' tiles of 128 query rows.  query (R, Hq, M, head_dim).
+
+        With a bf16 query K, V and the softmax's weights are rounded to fp16 (an eighth of the output's own
+        rounding each; the lse is off by some 1e-4); with an fp16 query K and the weights keep 22 bits."""
+        if _C.current_device() != self._dev_index:
+            with torch.cuda.device(self._dev_index):
+                return self.attend_chunk(layer, query, rows, n_new, sm_scale, out, return_lse)
+        view = self._layer(layer)
+        dt = _half_dtype(query)
+        q = query
+        shape = q.shape
+        if len(shape) != 4 or shape[3] != self.D or shape[1] % self.H or not shape[1]:
+            raise ValueError(f"query must be (rows, a multiple of {self.H} heads, tokens, {self.D})")
+        if q.device != self._dev:
+            raise RuntimeError(f"akv: the query must be on {self._dev} (no CPU fallback)")
+        R, Hq, M, D = shape
+        qs = q.stride()
+        if qs[3] != 1:
+            q = q.contiguous()
+            qs = q.stride()
+        rows, n_new, rp, np_ = self._rows(rows, n_new, R)
+        o = out
+        if o is None:
+            o = torch.empty_like(q)
+            if o.stride(3) != 1:  # a query whose layout does not carry over
+                o = torch.empty(shape, dtype=q.dtype, device=self._dev)
+        os_ = o.stride()
+        if o.shape != shape or o.dtype is not q.dtype or os_[-1] != 1 or o.device != self._dev:
+            raise ValueError("out must have the query's shape, type and device, its last dim contiguous")
+        lse = torch.empty_strided((R, Hq, M), (Hq * M, M, 1), dtype=torch.float32,
+                                  device=self._dev) if return_lse else None
+        stream = _C.raw_stream(self._dev_index)
+        need = self._chunk_ws_bytes
+        if torch.cuda.is_current_stream_capturing():  # replays may overlap eager calls
+            ws = torch.empty(need, dtype=torch.uint8, device=self._dev)
+        else:
+            ws = self._chunk_ws.get(stream)
+            if ws is None:
+                ws = self._chunk_ws[stream] = torch.empty(need, dtype=torch.uint8, device=self._dev)
+        rc = self._lib.akv_int4_chunk_attention(
+            _C.ATTENTION_ARGS.pack(view, rp, np_, q.data_ptr(), qs[0], qs[1], qs[2], o.data_ptr(), os_[0], os_[1],
+                                   os_[2], 0 if lse is None else lse.data_ptr(), ws.data_ptr(), need,
+                                   self._status_ptr, R, M, Hq, dt,
+                                   self._scale if sm_scale is None else float(sm_scale), 0), stream)
+        if rc:
+            _C.check(rc, "akv_int4_chunk_attention")
+        return (o, lse) if return_lse else o
 
     # ------------------------------------------------------------------ eviction
     def _weight_args(self) -> tuple:

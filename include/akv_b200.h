@@ -717,6 +717,14 @@ typedef struct {
 size_t akv_int4_attention_workspace_bytes(int R, int M, int Hq, int kv_heads, int head_dim, int max_blocks);
 int akv_int4_attention(const akv_int4_attention_args* a, void* stream);
 
+/* The same for a chunk of new tokens (tens to thousands a row), on the fifth-
+ * generation tensor cores: arguments and results as akv_int4_attention, but for
+ * a bf16 query K, V and the softmax's weights are rounded to fp16 once each.
+ * Workspace: akv_int4_chunk_workspace_bytes(...), 16-byte aligned, with any
+ * content; calls in order on one stream may share it. */
+size_t akv_int4_chunk_workspace_bytes(int head_dim);
+int akv_int4_chunk_attention(const akv_int4_attention_args* a, void* stream);
+
 /* Attention weight that the tokens receive, added to a running total:
  *   weights[s*w_stride + t] += sum over hq, m < n_new[i] with pos(m) >= t of
  *                              exp(q . K_t * sm_scale - lse[i][hq][m])
