@@ -91,7 +91,7 @@ class PageTable(ctypes.Structure):
 # tenth of converting as many ctypes arguments): pointers and 64-bit fields first, then 32-bit ones.
 IO_ARGS = struct.Struct("13q4i")         # akv_int4_io_args
 ATTENTION_ARGS = struct.Struct("15q4ifi")  # akv_int4_attention_args
-WEIGH_ARGS = struct.Struct("11q4ifi")  # akv_int4_weigh_args
+WEIGH_ARGS = struct.Struct("13q4ifi")  # akv_int4_weigh_args
 EVICT_ARGS = struct.Struct("12q8i")      # akv_int4_evict_args
 VERIFY_ARGS = struct.Struct("13q4i")     # akv_verify_args
 LOGPROBS_ARGS = struct.Struct("8q4i")    # akv_logprobs_args
@@ -193,6 +193,7 @@ SIGNATURES = {
     "akv_int4_attention": (c_int, [c_char_p, c_void_p]),
     "akv_int4_chunk_workspace_bytes": (c_size_t, [c_int]),
     "akv_int4_chunk_attention": (c_int, [c_char_p, c_void_p]),
+    "akv_int4_weigh_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "akv_int4_weigh": (c_int, [c_char_p, c_void_p]),
     "akv_int4_evict_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "akv_int4_evict": (c_int, [c_char_p, c_void_p]),

@@ -402,9 +402,14 @@ class Int4PagedCache:
             qs = q.stride()
         rows, n_new, rp, np_ = self._rows(rows, n_new, R)
         wp, w_layer, w_row, _ = self._weight_args()
+        need = _C.workspace_bytes("akv_int4_weigh_workspace_bytes", R, M, Hq, self.H, D, self.group)
+        if need == 0:
+            raise ValueError(f"unsupported shape: {M} tokens of {Hq} heads")
+        ws = torch.empty(need, dtype=torch.uint8, device=self._dev) if need > 16 else None
         rc = self._lib.akv_int4_weigh(
             _C.WEIGH_ARGS.pack(view, rp, np_, q.data_ptr(), qs[0], qs[1], qs[2], lse.data_ptr(),
-                               wp + 4 * layer * w_layer, w_row, self._status_ptr, R, M, Hq, dt,
+                               wp + 4 * layer * w_layer, w_row, 0 if ws is None else ws.data_ptr(), need,
+                               self._status_ptr, R, M, Hq, dt,
                                self._scale if sm_scale is None else float(sm_scale), 0),
             _C.raw_stream(self._dev_index))
         if rc:

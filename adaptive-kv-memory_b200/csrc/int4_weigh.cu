@@ -22,30 +22,13 @@
 // memory as MMA fragments; more of them take the pages again.
 #include <type_traits>
 
-#include "int4.cuh"
+#include "int4_weigh.cuh"
 
 namespace akv {
 
 constexpr int kWeighWarps = 4;
 constexpr int kWeighThreads = kWeighWarps * 32;
-constexpr int kWeighRows = 1024;   // call rows of one launch
 constexpr int kWeighUnits = 8;     // (head, column tile) units prepared at a time
-
-struct WeighParams {
-  akv_int4_cache c;
-  const int32_t* rows;
-  const int32_t* n_new;
-  int row0, R;  // call rows [row0, row0 + R) of this launch
-  int M, Hq;
-  const uint16_t* q;
-  int64_t q_sr, q_sh, q_sm;
-  const float* lse;
-  float scale;
-  float* weights;
-  int64_t w_stride;
-  int bf16;
-  int* status;
-};
 
 template <int D, int G, int NT>
 struct WeighShape {
@@ -110,15 +93,8 @@ AKV_DEV void weigh_rows(const WeighParams& P, int* s_pref, int* s_len, int* s_ne
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, n_warps = blockDim.x >> 5;
   for (int e = t; e < P.R; e += blockDim.x) {
     const Int4Row r = int4_row(P.c, P.rows, P.n_new, P.row0 + e, P.M, P.status);
-    s_new[e] = r.n_new;
+    s_new[e] = weigh_new(P, e, r);
     s_len[e] = r.len;
-    if (!P.rows) continue;
-    for (int s = 0; s < P.row0 + e; ++s)
-      if (P.rows[s] == r.seq) {
-        set_status(P.status, AKV_ERR_SHAPE);
-        s_new[e] = 0;
-        break;
-      }
   }
   int base = 0;
   for (int e0 = 0; e0 < P.R; e0 += blockDim.x) {
@@ -422,9 +398,20 @@ static int weigh_few(const WeighParams& P, cudaStream_t st) {
   }
 }
 
+// From this many query columns (new tokens x query heads of a group) on the
+// tensor-memory kernel takes the call.
+constexpr int kWeighMany = 64;
+
 }  // namespace akv
 
 using namespace akv;
+
+extern "C" size_t akv_int4_weigh_workspace_bytes(int R, int M, int Hq, int kv_heads, int head_dim, int group) {
+  if (R < 0 || M < 0 || Hq <= 0 || kv_heads <= 0 || Hq % kv_heads || !int4_shape_ok(head_dim, group)) return 0;
+  if (R == 0 || static_cast<int64_t>(M) * (Hq / kv_heads) < kWeighMany) return 16;
+  if (static_cast<int64_t>(M) * Hq > INT32_MAX / 2) return 0;
+  return weigh_many_workspace(R, M, Hq, kv_heads, head_dim, head_dim / group);
+}
 
 extern "C" int akv_int4_weigh(const akv_int4_weigh_args* a, void* stream) {
   if (!a) return AKV_ERR_NULL;
@@ -441,6 +428,13 @@ extern "C" int akv_int4_weigh(const akv_int4_weigh_args* a, void* stream) {
     return AKV_ERR_ALIGN;
   // columns and pages of a launch are counted in 32 bits
   if (static_cast<int64_t>(a->M) * a->Hq > INT32_MAX / 2) return AKV_ERR_UNSUPPORTED;
+  const bool many = a->M * (a->Hq / c->kv_heads) >= kWeighMany;
+  if (many) {
+    if (!a->workspace) return AKV_ERR_NULL;
+    if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return AKV_ERR_ALIGN;
+    if (a->workspace_bytes < akv_int4_weigh_workspace_bytes(a->R, a->M, a->Hq, c->kv_heads, c->head_dim, c->group))
+      return AKV_ERR_WORKSPACE;
+  }
   int rows = kWeighRows;
   if (rows > INT32_MAX / c->max_blocks) rows = INT32_MAX / c->max_blocks;
   WeighParams p{};
@@ -457,6 +451,7 @@ extern "C" int akv_int4_weigh(const akv_int4_weigh_args* a, void* stream) {
   p.w_stride = a->w_stride;
   p.bf16 = a->dtype == AKV_BF16;
   p.status = a->status;
+  if (many) return weigh_many(p, a->R, a->workspace, static_cast<cudaStream_t>(stream));
   for (int r = 0; r < a->R; r += rows) {
     p.row0 = r;
     p.R = a->R - r < rows ? a->R - r : rows;

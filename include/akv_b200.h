@@ -732,7 +732,9 @@ int akv_int4_chunk_attention(const akv_int4_attention_args* a, void* stream);
  * out alike, lse fp32 [R][Hq][M] (natural log) as it returned it.  A query that
  * is not finite, or whose lse is not, adds nothing.  Sums are taken in an order
  * that the shapes and lengths alone decide.  A row named twice counts once
- * (AKV_ERR_SHAPE in *status). */
+ * (AKV_ERR_SHAPE in *status).
+ * Workspace: akv_int4_weigh_workspace_bytes(...) (16: none is read), 16-byte
+ * aligned, with any content. */
 typedef struct {
   const akv_int4_cache* cache;
   const int32_t* rows;
@@ -742,12 +744,15 @@ typedef struct {
   const float* lse;
   float* weights;
   int64_t w_stride;
+  void* workspace;
+  size_t workspace_bytes;
   int* status;
   int32_t R, M, Hq, dtype;
   float sm_scale;
   int32_t reserved;              /* 0 */
 } akv_int4_weigh_args;
 
+size_t akv_int4_weigh_workspace_bytes(int R, int M, int Hq, int kv_heads, int head_dim, int group);
 int akv_int4_weigh(const akv_int4_weigh_args* a, void* stream);
 
 /* ------------------------------------------------------------------------

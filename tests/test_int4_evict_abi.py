@@ -37,18 +37,23 @@ def test_weigh_refusals():
     from akv import _C
     lib = _C.load()
 
-    def weigh(c=None, Hq=4, q=256, lse=256, w=256, stride=128, R=1, M=1, dtype=0, **kw):
+    need = lib.akv_int4_weigh_workspace_bytes(1, 64, 4, 2, 128, 128)
+    assert need > 16 and lib.akv_int4_weigh_workspace_bytes(1, 1, 4, 2, 128, 128) == 16
+    assert lib.akv_int4_weigh_workspace_bytes(1, 64, 3, 2, 128, 128) == 0
+
+    def weigh(c=None, Hq=4, q=256, lse=256, w=256, stride=128, R=1, M=1, dtype=0, ws=0, nb=0, **kw):
         d = dict(pool=256, page_stride=8704, head_stride=4352, n_pages=4, table=256, table_stride=4, lens=256,
                  max_seqs=2, max_blocks=4, kv_heads=2, head_dim=128, group=128)
         d.update(kw)
         cache = _C.Int4Cache(*[d[f[0]] for f in _C.Int4Cache._fields_])
         return lib.akv_int4_weigh(_C.WEIGH_ARGS.pack(ctypes.addressof(cache) if c is None else c, 0, 0, q, 0, 0, 0, lse,
-                                                     w, stride, 0, R, M, Hq, dtype, 1.0, 0), None)
+                                                     w, stride, ws, nb, 0, R, M, Hq, dtype, 1.0, 0), None)
 
     assert lib.akv_int4_weigh(None, None) == -7 and weigh(c=0) == -7
     assert weigh(q=0) == -7 and weigh(lse=0) == -7 and weigh(w=0) == -7 and weigh(pool=0) == -7
     assert weigh(Hq=3) == -1 and weigh(R=-1) == -1 and weigh(M=-1) == -1 and weigh(stride=127) == -1
     assert weigh(head_dim=96) == -1 and weigh(q=257) == -3 and weigh(lse=258) == -3 and weigh(w=257) == -3
+    assert weigh(M=64) == -7 and weigh(M=64, ws=264, nb=need) == -3 and weigh(M=64, ws=256, nb=need - 1) == -8
     assert weigh(dtype=2) == -4 and weigh(R=0) == 0 and weigh(M=0) == 0 and weigh(M=1 << 29) == -4
 
 
