@@ -41,15 +41,15 @@ extern "C" int akv_int4_chunk_attention(const akv_int4_attention_args* a, void* 
     return AKV_ERR_ALIGN;
   const ChunkWs w = chunk_ws(c->head_dim);
   if (a->workspace_bytes < w.bytes) return AKV_ERR_WORKSPACE;
+  if (a->Hq / c->kv_heads > kChunkRep) return AKV_ERR_UNSUPPORTED;
   const int64_t q_rows = static_cast<int64_t>(a->M) * (a->Hq / c->kv_heads);
   const int64_t tiles = (q_rows + chunk_rows(c->head_dim) - 1) / chunk_rows(c->head_dim);
   if (tiles > kChunkEntries) return AKV_ERR_UNSUPPORTED;  // more query rows than one launch lists
   // rows of a launch: its entries, their units and their token tiles are counted in 32 bits
   int64_t rows = kChunkEntries / tiles;
   if (rows > kChunkRowsMax) rows = kChunkRowsMax;
-  const int64_t row_tiles = tiles * (static_cast<int64_t>(c->max_blocks) + kChunkSetup);
-  if (rows > INT32_MAX / row_tiles) rows = INT32_MAX / row_tiles;
-  if (rows > INT32_MAX / (tiles * c->kv_heads)) rows = INT32_MAX / (tiles * c->kv_heads);
+  const int64_t row_tiles = tiles * (static_cast<int64_t>(c->max_blocks) + kChunkSetup) * c->kv_heads;
+  if (rows > INT32_MAX / 2 / row_tiles) rows = INT32_MAX / 2 / row_tiles;
   if (rows == 0) return AKV_ERR_UNSUPPORTED;
   ChunkParams p{};
   p.c = *c;
@@ -71,6 +71,7 @@ extern "C" int akv_int4_chunk_attention(const akv_int4_attention_args* a, void* 
   p.meta = reinterpret_cast<int4*>(ws);
   p.ml = reinterpret_cast<float2*>(ws + w.ml);
   p.part = reinterpret_cast<float*>(ws + w.part);
+  p.rep_inv = 0xFFFFFFFFu / static_cast<uint32_t>(a->Hq / c->kv_heads) + 1;
   p.status = a->status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (int64_t r = 0; r < a->R; r += rows) {

@@ -446,13 +446,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
           mbar_wait(q_full + x, x >= st ? ph : ph ^ 1, P.status);
         }
     }
-  } else if (lane == 0) {
+  } else {
     // ================================================================ MMA
+    const uint32_t lead = elect_one();
     auto wait = [&](uint64_t* bar, uint32_t phase) {
-      if (ok) ok = mbar_wait(bar, phase, P.status);
+      if (ok) ok = __all_sync(~0u, mbar_wait(bar, phase, P.status));
       return ok;
     };
-    const uint32_t idesc = instr_desc(128, N, 0);
+    constexpr uint32_t IDESC = instr_desc(128, N, 0);
     const uint32_t base = smem_u32(smem);
     int st = 0;
     uint32_t ph_q = 0, ph_a = 0, ph_s = 1;
@@ -462,6 +463,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
       ph_a ^= 1;
       for (int q = u.q0; q < u.q1; ++q) {
         if (!wait(q_full + st, ph_q)) break;
+        const uint32_t tile = desc_lo(base + st * S::REC, N * 16);
         for (int wg = 0; wg < 2; ++wg) {
           if (!wait(s_free + wg, ph_s)) break;
           tc_fence_after();
@@ -471,19 +473,18 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
 #pragma unroll
             for (int k = 0; k < S::KG; ++k) {
               const int step = g * S::KG + k;
-              umma_f16_ts(tS + g * N, tA + 8 * step, smem_desc(base + st * S::REC + step * 2 * N * 16, N * 16, 128), idesc,
-                          k > 0 ? 1u : 0u);
+              umma_ts<desc_hi(128), IDESC>(tS + g * N, tA + 8 * step, tile + step * 2 * N, k > 0 ? 1u : 0u, lead);
             }
-          umma_commit(s_full + wg);
+          umma_commit(s_full + wg, lead);
         }
         if (!ok) break;
         ph_s ^= 1;
-        umma_commit(q_free + st);
+        umma_commit(q_free + st, lead);
         if (++st == S::STAGES) st = 0, ph_q ^= 1;
       }
     }
     if (!ok) {  // see what was issued end before the tensor memory goes
-      umma_commit(drained);
+      umma_commit(drained, lead);
       mbar_wait(drained, 0, P.status);
     }
   }

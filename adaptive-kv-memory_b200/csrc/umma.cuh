@@ -40,10 +40,56 @@ AKV_DEV void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint3
       : "memory");
 }
 
+// The low and the (constant) high word of a descriptor: many of them differ in
+// their addresses alone.
+AKV_DEV constexpr uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4) << 16; }
+AKV_DEV constexpr uint32_t desc_hi(uint32_t sbo) { return (sbo >> 4) | 1u << 14; }
+// ... with the 128-byte swizzle
+AKV_DEV constexpr uint32_t desc_hi_sw128(uint32_t sbo) { return desc_hi(sbo) | 2u << 29; }
+
+// One lane of a converged warp.
+AKV_DEV uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+
+// MMAs by a whole warp, of which the lane with `lead` set issues.  Inside a
+// branch that one lane takes, every operand goes through a vector register
+// first: with the SM's other warps busy an MMA then took 136 cycles to issue;
+// so, with uniform operands, it issues at the tensor cores' pace of 64.
+template <uint32_t A_HI, uint32_t B_HI, uint32_t IDESC>
+AKV_DEV void umma_ss(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t accumulate, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %3, 0;\n\tsetp.ne.b32 q, %8, 0;\n\tmov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %5};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %6, {%7, %7, %7, %7}, p;\n\t}" ::"r"(tmem_d),
+      "r"(a_lo), "r"(b_lo), "r"(accumulate), "n"(A_HI), "n"(B_HI), "r"(IDESC), "r"(0u), "r"(lead)
+      : "memory");
+}
+
+template <uint32_t B_HI, uint32_t IDESC>
+AKV_DEV void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t accumulate, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %3, 0;\n\tsetp.ne.b32 q, %7, 0;\n\tmov.b64 b, {%2, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %5, {%6, %6, %6, %6}, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_lo), "r"(accumulate), "n"(B_HI), "r"(IDESC), "r"(0u), "r"(lead)
+      : "memory");
+}
+
 // Arrive on `bar` once every tcgen05 operation this thread issued has completed.
 AKV_DEV void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
+}
+
+AKV_DEV void umma_commit(uint64_t* bar, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
 }
 
 AKV_DEV void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -62,6 +108,17 @@ AKV_DEV void tmem_ld32(uint32_t taddr, float (&v)[32]) {
       : "r"(taddr));
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+AKV_DEV void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 AKV_DEV void tmem_st32(uint32_t taddr, const float (&v)[32]) {
@@ -101,6 +158,13 @@ AKV_DEV void tmem_st16u(uint32_t taddr, const uint32_t (&v)[16]) {
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
+
+// The register share of the calling warpgroup (all its warps together): the
+// shares' sum may not pass what the block was launched with.
+template <int REGS>
+AKV_DEV void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
+template <int REGS>
+AKV_DEV void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
 
 AKV_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 AKV_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
