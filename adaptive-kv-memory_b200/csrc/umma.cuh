@@ -6,6 +6,24 @@
 
 namespace akv {
 
+// mbar_wait for pipelines whose phases are mostly complete when they are asked
+// for: a plain test first (a potentially suspending one takes longer to say yes).
+AKV_DEV bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+AKV_DEV bool mbar_wait_near(uint64_t* bar, uint32_t parity, int* status) {
+#pragma unroll 1
+  for (int k = 0; k < 16; ++k)
+    if (mbar_test(bar, parity)) return true;
+  return mbar_wait(bar, parity, status);
+}
+
 // Shared-memory matrix descriptor, no swizzle: start address, leading-dimension
 // byte offset (between core matrices along K), stride-dimension byte offset
 // (between 8-row groups along M/N), all >> 4; bits 46-47 = 1 (sm_100 format).
