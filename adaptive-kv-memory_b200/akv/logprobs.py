@@ -50,17 +50,23 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if not 0 <= top <= min(MAX_TOP, V) or V == 0:
         raise ValueError(f"top must be 0 to {min(MAX_TOP, V)} (got {top}), and V positive")
     x = logits if len(shape) == 2 else logits.reshape(-1, V)
-    if x.stride(1) != 1 and V > 1:
+    stride, inner = x.stride()
+    if inner != 1 and V > 1:
         x = x.contiguous()
-    tokens = tokens.contiguous()
-    n, lead = x.shape[0], shape[:-1]
-    logprob = torch.empty(lead, dtype=torch.float32, device=dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-    rank = torch.empty(lead, dtype=torch.int32, device=dev)
-    ids = torch.empty((*lead, top), dtype=torch.int64, device=dev)
-    alt = torch.empty((*lead, top), dtype=torch.float32, device=dev)
+        stride = V
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    n, lead = x.shape[0], tokens.shape
+    # empty_strided: 1.5 us of host time, torch.empty with its keywords 2.3
+    row = tokens.stride()
+    logprob = torch.empty_strided(lead, row, dtype=torch.float32, device=dev)
+    entropy = torch.empty_strided(lead, row, dtype=torch.float32, device=dev)
+    rank = torch.empty_strided(lead, row, dtype=torch.int32, device=dev)
+    many = tuple(s * top for s in row) + (1,)
+    ids = torch.empty_strided((*lead, top), many, dtype=torch.int64, device=dev)
+    alt = torch.empty_strided((*lead, top), many, dtype=torch.float32, device=dev)
     rc = _C.load().akv_token_logprobs(
-        _C.LOGPROBS_ARGS.pack(x.data_ptr(), x.stride(0), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(),
+        _C.LOGPROBS_ARGS.pack(x.data_ptr(), stride, tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(),
                               rank.data_ptr(), ids.data_ptr(), alt.data_ptr(), n, V, top, dt), _C.raw_stream(index))
     if rc:
         _C.check(rc, "akv_token_logprobs")

@@ -17,9 +17,9 @@
 //   softmax  one warpgroup per 128 query rows, thread = row = TMEM lane: query
 //            rows into shared memory, online softmax, P into tensor memory over
 //            S, O out
-//   pages    one warp: a tile's records as they are, by bulk copies
-//   values   two warpgroups: K and V of the tile out of them, into their rings
-//   MMA      a warp per 128 query rows: S = Q K^T from shared memory, O += P V with P from
+//   values   one warpgroup: pages into registers a tile ahead, then the tile's
+//            K and V into their rings
+//   MMA      one warp: S = Q K^T from shared memory, O += P V with P from
 //            tensor memory
 // While one tile's softmax runs, the other's MMAs do.
 //
@@ -41,27 +41,22 @@
 // 0 4 1 5 2 6 3 7, in Q and K alike; V's order is undone when O is stored.
 #pragma once
 
-#include <type_traits>
-
 #include "int4.cuh"
 #include "umma.cuh"
 
 namespace akv {
 
 constexpr int kChunkSMs = 148;      // CTAs: one an SM
-constexpr int kChunkEntries = 1536; // (row, tile) pairs of one launch
-constexpr int kChunkRowsMax = 384;  // call rows of one launch
+constexpr int kChunkEntries = 4096; // (row, tile) pairs of one launch
+constexpr int kChunkRowsMax = 1024; // call rows of one launch
 constexpr int kChunkRep = 4096;     // query heads of a group, at most (the division below)
-constexpr int kChunkSetup = 2;      // token tiles that a unit's set-up counts for
-// When a row's unit is set its maximum stands at 2^9, and a thread's weights of a
-// tile sum up to 2^15 at most before it moves, so that fp16 holds them down to
-// 2^-23 of the maximum with all their bits.  The sum says so without the tile's
-// maximum, which is formed only where a unit moves.
-constexpr float kChunkTop = 9.f, kChunkMost = 32768.f;
-
-// Pairs of weights, of four, whose exponentials run on the FMA pipes where the
-// special-function units bound the softmax (bf16, two query tiles).
-constexpr int kChunkPoly = 0;
+constexpr int kChunkSetup = 4;      // token tiles that a unit's set-up counts for
+constexpr int kChunkShare = 4;      // of a CTA's share, at least
+// A row's maximum stands at 2^7 when its unit is set, and a tile's weights sum up
+// to 2^15 at most before it moves: fp16 holds them down to 2^-21 of the maximum
+// with all their bits.  A sum says so without the tile's maximum: that is formed
+// only where the unit moves.
+constexpr float kChunkTop = 7.f, kChunkMost = 32768.f;
 
 struct ChunkParams {
   akv_int4_cache c;
@@ -87,38 +82,30 @@ struct ChunkParams {
 template <int D, int G, int LO>
 struct ChunkShape {
   static constexpr int NQ = D == 256 ? 1 : 2;
-  static constexpr int TK = 64;                     // tokens of a tile
+  static constexpr int TK = D == 256 || LO ? 64 : 128;
   static constexpr int ROWS = 128 * NQ;
   static constexpr int QB = 128 * D * 2;            // a query tile
   static constexpr int VB = TK * D * 2;             // a tile of V
   static constexpr int KB = VB * (LO ? 2 : 1);      // of K: one or two terms
-  static constexpr int KS = D == 256 ? 1 : (LO ? 2 : 3);          // ring slots
-  static constexpr int VS = D == 256 ? (LO ? 1 : 2) : (LO ? 2 : 3);
-  static constexpr int RS = D == 256 ? (LO ? 3 : 2) : 4;          // of the raw tiles
-  static constexpr int SOFT = 4 * NQ;               // softmax warps
-  static constexpr int THREADS = SOFT * 32 + 256 + 128;
-  // registers of a softmax / value / other thread: 640 threads are launched with 96 each
-  static constexpr bool SPLIT = THREADS == 640;
-  static constexpr int R_SOFT = 136, R_VAL = 72, R_MMA = 64;
-  static_assert(2 * R_SOFT + 2 * R_VAL + R_MMA == 5 * 96, "register shares");
+  static constexpr int KS = D == 256 && LO ? 1 : 2; // ring slots
+  static constexpr int VS = 2;
+  static constexpr int THREADS = 128 * NQ + 128 + 128;
+  // registers of a softmax / value / MMA thread; with 512 threads the launch gives 128 each
+  static constexpr bool SPLIT = THREADS == 512;
+  static constexpr int R_SOFT = 176, R_VAL = 104, R_MMA = 56;
+  static_assert(2 * R_SOFT + R_VAL + R_MMA == 4 * 128, "register shares");
   static constexpr int PARTS = 128 / TK;            // value threads of a token
   static constexpr int CH = D / PARTS;              // channels of a value thread
-  static constexpr int PIECES = CH / 32;            // its 16-byte pieces of codes
-  static constexpr int PAGES = TK / kBlockTokens;
-  // a tile's codes and pairs as they stand in the pages, K or V
-  static constexpr int RAW_CODES = TK * D / 2, RAW = RAW_CODES + TK * G * 4;
-  // pairs of weights, of four, whose exponentials run on the FMA pipes
-  static constexpr int POLY = NQ == 2 && !LO ? kChunkPoly : 0;
+  static constexpr int NG = CH * G / D < 1 ? 1 : CH * G / D;  // groups among them
   static constexpr int OFF_K = NQ * QB;
   static constexpr int OFF_V = OFF_K + KS * KB;
-  static constexpr int OFF_RAW = OFF_V + VS * VB;   // K's slots, then V's
-  static constexpr int OFF_EX = OFF_RAW + 2 * RS * RAW;    // per row: exponent, or a mark for a query that is not finite
+  static constexpr int OFF_EX = OFF_V + VS * VB;    // per row: exponent, or a mark for a query that is not finite
   static constexpr int OFF_BAR = OFF_EX + ROWS * 4;
-  static constexpr int OFF_ROWS = OFF_BAR + 352;    // lengths, new tokens, prefix sums
+  static constexpr int OFF_ROWS = OFF_BAR + 160;    // lengths, new tokens, prefix sums
   static constexpr int smem(int rows, int entries) { return 1024 + OFF_ROWS + (2 * rows + entries + 1) * 4; }
-  // tensor memory: two tiles of S (and P) of each query tile, then O
-  static constexpr int T_S = 0, T_O = NQ * 2 * TK;
-  static_assert(NQ * (2 * TK + D) <= 512, "tensor memory");
+  // tensor memory: S (and P) of each tile, then O
+  static constexpr int T_S = 0, T_O = NQ * TK;
+  static_assert(NQ * (TK + D) <= 512, "tensor memory");
   static_assert(smem(kChunkRowsMax, kChunkEntries) <= 227 * 1024, "shared memory");
 };
 
@@ -210,96 +197,84 @@ AKV_DEV __half2 hold(__half2 x) {  // past fp16's range: its ends
   return __hmax2(__hmin2(x, top), __hneg2(top));
 }
 
-// 32 channels (a 16-byte piece of codes) of one or two terms: c*s + z rounded to
-// fp16, or (TWO) a coarser first term and what it leaves.  dst: the row's 64
-// channels; blk, x: the piece's first block of 8 and the row's permutation, both
-// times 16; second: from the first term to the second.
+// whether a value of the groups reaches `most` in magnitude
+template <int NG>
+AKV_DEV bool far_values(const uint32_t (&pair)[NG], float most) {
+  bool far = false;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    const float2 sz = __half22float2(u32_as_h2(pair[g]));
+    far |= !(fmaxf(fabsf(sz.y), fabsf(fmaf(15.f, sz.x, sz.y))) < most);
+  }
+  return far;
+}
+
+// A row of one or two terms, its first 64 channels at `dst`, the next `next` bytes
+// on, its pieces permuted by x / 16: c*s + z rounded to fp16, or (TWO) a coarser first term and, `second` bytes
+// on, what it leaves.
 //
 // Two terms: with 2^E above the group's magnitudes, M = 1.5 * 2^(E + 1) and z =
 // z1 + z2, z1 = (z + M) - M, both exact, the first term hi = fma(c, s, z1 + M) - M
 // is a multiple of 2^(E - 9), as z1 is, so that z1 - hi is exact, and the second
 // is fma(c, s, z1 - hi) + z2: together 2^(E - 20) or better.  Groups that reach
 // 2^13 (FAR) take the exact difference in halves instead.
-template <bool TWO, bool FAR, int W0, int W1>
-AKV_DEV void store_words(uint4 code, uint32_t sz, unsigned char* dst, int blk, int x, int second) {
-  const uint32_t w[4] = {code.x, code.y, code.z, code.w};
-  const __half2 s = u32_as_h2(prmt(sz, sz, 0x1010)), z = u32_as_h2(prmt(sz, sz, 0x3232));
-  __half2 big = z, z1 = z, z1m = z, z2 = z, sh = s, zh = z;
-  if constexpr (TWO && !FAR) {
-    const float2 f = __half22float2(u32_as_h2(sz));
-    const float most = fmaxf(fabsf(f.y), fabsf(fmaf(15.f, f.x, f.y)));
-    // 2^(E + 1) with 2^(E - 1) <= most < 2^E, 2^-13 at least
-    const int e = max((static_cast<int>(__float_as_uint(most)) >> 23) - 127 + 2, -13);
-    big = __float2half2_rn(__int_as_float((127 + e) << 23) * 1.5f);
-    z1m = __hadd2(z, big);
-    z1 = __hsub2(z1m, big);
-    z2 = __hsub2(z, z1);
-  }
-  if constexpr (TWO && FAR) {
-    const __half2 half = u32_as_h2(0x38003800u);
-    sh = __hmul2(s, half), zh = __hmul2(z, half);
-  }
+template <int NW, int NG, bool TWO, bool FAR>
+AKV_DEV void store_rows(const uint32_t (&w)[NW], const uint32_t (&pair)[NG], unsigned char* dst, int x, int next, int second) {
+  constexpr int PER = NW / NG;  // words (of 8 channels) of a group
 #pragma unroll
-  for (int i = W0; i < W1; ++i) {
-    __half2 c[4], v[4], r[4];
-    codes_of_word(w[i], c);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if constexpr (!TWO) {
-        v[k] = __hfma2(c[k], s, z);
-        if constexpr (FAR) v[k] = hold(v[k]);
-      } else if constexpr (!FAR) {
-        v[k] = __hsub2(__hfma2(c[k], s, z1m), big);
-        r[k] = __hadd2(__hfma2(c[k], s, __hsub2(z1, v[k])), z2);
-      } else {
-        // z - v = d + e exactly, both halved; c*s + d is what v left out, but for e
-        v[k] = hold(__hfma2(c[k], s, z));
-        const __half2 vh = __hmul2_rn(v[k], u32_as_h2(0x38003800u)), d = __hsub2(zh, vh), b = __hsub2(d, zh);
-        const __half2 e = __hsub2(__hsub2(zh, __hsub2(d, b)), __hadd2(vh, b));
-        const __half2 h = __hadd2(__hfma2(c[k], sh, d), e);
-        r[k] = __hadd2(h, h);
-      }
+  for (int g = 0; g < NG; ++g) {
+    const uint32_t sz = pair[g];
+    const __half2 s = u32_as_h2(prmt(sz, sz, 0x1010)), z = u32_as_h2(prmt(sz, sz, 0x3232));
+    __half2 big = z, z1 = z, z1m = z, z2 = z, sh = s, zh = z;
+    if constexpr (TWO && !FAR) {
+      const float2 f = __half22float2(u32_as_h2(sz));
+      const float most = fmaxf(fabsf(f.y), fabsf(fmaf(15.f, f.x, f.y)));
+      // 2^(E + 1) with 2^(E - 1) <= most < 2^E, 2^-13 at least
+      const int e = max((static_cast<int>(__float_as_uint(most)) >> 23) - 127 + 2, -13);
+      big = __float2half2_rn(__int_as_float((127 + e) << 23) * 1.5f);
+      z1m = __hadd2(z, big);
+      z1 = __hsub2(z1m, big);
+      z2 = __hsub2(z, z1);
     }
-    unsigned char* at = dst + ((blk + 16 * i) ^ x);
-    *reinterpret_cast<uint4*>(at) = make_uint4(h2_as_u32(v[0]), h2_as_u32(v[1]), h2_as_u32(v[2]), h2_as_u32(v[3]));
-    if constexpr (TWO)
-      *reinterpret_cast<uint4*>(at + second) =
-          make_uint4(h2_as_u32(r[0]), h2_as_u32(r[1]), h2_as_u32(r[2]), h2_as_u32(r[3]));
+    if constexpr (TWO && FAR) {
+      const __half2 half = u32_as_h2(0x38003800u);
+      sh = __hmul2(s, half), zh = __hmul2(z, half);
+    }
+#pragma unroll
+    for (int i = g * PER; i < (g + 1) * PER; ++i) {
+      __half2 c[4], v[4], r[4];
+      codes_of_word(w[i], c);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (!TWO) {
+          v[k] = __hfma2(c[k], s, z);
+          if constexpr (FAR) v[k] = hold(v[k]);
+        } else if constexpr (!FAR) {
+          v[k] = __hsub2(__hfma2(c[k], s, z1m), big);
+          r[k] = __hadd2(__hfma2(c[k], s, __hsub2(z1, v[k])), z2);
+        } else {
+          // z - v = d + e exactly, both halved; c*s + d is what v left out, but for e
+          v[k] = hold(__hfma2(c[k], s, z));
+          const __half2 vh = __hmul2_rn(v[k], u32_as_h2(0x38003800u)), d = __hsub2(zh, vh), b = __hsub2(d, zh);
+          const __half2 e = __hsub2(__hsub2(zh, __hsub2(d, b)), __hadd2(vh, b));
+          const __half2 h = __hadd2(__hfma2(c[k], sh, d), e);
+          r[k] = __hadd2(h, h);
+        }
+      }
+      unsigned char* at = dst + (i >> 3) * next + ((i & 7) * 16 ^ x);
+      *reinterpret_cast<uint4*>(at) =
+          make_uint4(h2_as_u32(v[0]), h2_as_u32(v[1]), h2_as_u32(v[2]), h2_as_u32(v[3]));
+      if constexpr (TWO)
+        *reinterpret_cast<uint4*>(at + second) =
+            make_uint4(h2_as_u32(r[0]), h2_as_u32(r[1]), h2_as_u32(r[2]), h2_as_u32(r[3]));
+    }
   }
 }
 
-template <bool TWO, bool FAR>
-AKV_DEV void store_piece(uint4 code, uint32_t sz, unsigned char* dst, int blk, int x, int second) {
-  store_words<TWO, FAR, 0, 4>(code, sz, dst, blk, x, second);
-}
-// the same with a pair for each 16 channels
-template <bool TWO, bool FAR>
-AKV_DEV void store_halves(uint4 code, uint32_t s0, uint32_t s1, unsigned char* dst, int blk, int x, int second) {
-  store_words<TWO, FAR, 0, 2>(code, s0, dst, blk, x, second);
-  store_words<TWO, FAR, 2, 4>(code, s1, dst, blk, x, second);
-}
-
-// whether a value of the group reaches `most` in magnitude
-AKV_DEV bool far_values(uint32_t pair, float most) {
-  const float2 sz = __half22float2(u32_as_h2(pair));
-  return !(fmaxf(fabsf(sz.y), fabsf(fmaf(15.f, sz.x, sz.y))) < most);
-}
-
-// 2^y of two values, y held to -126 and more, by a Chebyshev fit of degree 4 of
-// 2^f on [-1/2, 1/2] (2.7e-6 of the value) and its exponent added to the bits.
-AKV_DEV uint64_t exp2_fma(uint64_t y2) {
-  const float2 y = f2_split(y2);
-  const uint64_t v = f2_make(fmaxf(y.x, -126.f), fmaxf(y.y, -126.f));
-  const uint64_t t = f2_add(v, f2_make(12582912.f, 12582912.f));  // 1.5 * 2^23: the whole part in the low bits
-  const uint64_t f = f2_add(v, f2_fma(t, f2_make(-1.f, -1.f), f2_make(12582912.f, 12582912.f)));
-  uint64_t p = f2_make(0.009570102207362652f, 0.009570102207362652f);
-  p = f2_fma(p, f, f2_make(0.05591785907745361f, 0.05591785907745361f));
-  p = f2_fma(p, f, f2_make(0.240247443318367f, 0.240247443318367f));
-  p = f2_fma(p, f, f2_make(0.6931217908859253f, 0.6931217908859253f));
-  p = f2_fma(p, f, f2_make(0.9999992847442627f, 0.9999992847442627f));
-  const float2 a = f2_split(p), n = f2_split(t);
-  return f2_make(__int_as_float(__float_as_int(a.x) + (__float_as_int(n.x) << 23)),
-                 __int_as_float(__float_as_int(a.y) + (__float_as_int(n.y) << 23)));
+template <int NW, int NG, bool TWO>
+AKV_DEV void store_values(const uint32_t (&w)[NW], const uint32_t (&pair)[NG], unsigned char* dst, int x, int next, int second) {
+  if (__any_sync(~0u, far_values(pair, TWO ? 8192.f : 65000.f))) store_rows<NW, NG, TWO, true>(w, pair, dst, x, next, second);
+  else store_rows<NW, NG, TWO, false>(w, pair, dst, x, next, second);
 }
 
 // Lane i of four holds piece k of its row in w[k]: afterwards piece i of row k.
@@ -325,10 +300,9 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
   unsigned char* smem = smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024;
   int* s_ex = reinterpret_cast<int*>(smem + S::OFF_EX);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
-  // per query tile: queries there; [buffer] scores, weights there; P V done.  Rings: [slot] filled, free
-  uint64_t *q_ready = bars, *pv_done = bars + 2, *s_full = bars + 4, *p_ready = bars + 8;
-  uint64_t *k_full = bars + 12, *k_free = bars + 15, *v_full = bars + 18, *v_free = bars + 21;
-  uint64_t *raw_full = bars + 24, *raw_free = bars + 32, *drained = bars + 40, *o_full = bars + 41;  // raw: K's slots, V's slots
+  uint64_t *q_ready = bars, *s_full = bars + 2, *p_ready = bars + 4, *o_full = bars + 6;
+  uint64_t *k_full = bars + 8, *k_free = bars + 10, *v_full = bars + 12, *v_free = bars + 14;
+  uint64_t* drained = bars + 16;
   int* s_len = reinterpret_cast<int*>(smem + S::OFF_ROWS);
   int* s_new = s_len + P.R;
   int* s_pref = s_new + P.R;
@@ -343,25 +317,15 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
   if (t == 0) {
     for (int k = 0; k < 2; ++k) {
       mbar_init(q_ready + k, 128);
-      mbar_init(pv_done + k, 1);
-      mbar_init(o_full + k, 1);
-    }
-    for (int k = 0; k < 3; ++k) {
-      mbar_init(v_full + k, 128);
-      mbar_init(v_free + k, NQ);
-      mbar_init(k_full + k, 128);
-      mbar_init(k_free + k, NQ);
-    }
-    for (int k = 0; k < 4; ++k) {
       mbar_init(s_full + k, 1);
       mbar_init(p_ready + k, 128);
-    }
-    for (int k = 0; k < 8; ++k) {
-      mbar_init(raw_full + k, 1);
-      mbar_init(raw_free + k, 128);
+      mbar_init(o_full + k, 1);
+      mbar_init(k_full + k, 128);
+      mbar_init(k_free + k, 1);
+      mbar_init(v_full + k, 128);
+      mbar_init(v_free + k, 1);
     }
     mbar_init(drained, 1);
-    mbar_init(drained + 3, 1);
     fence_mbar_init();
     P.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
@@ -407,7 +371,7 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
       s_pref[0] = 0;
       const int total = base * H;
       int share = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-      if (share < 2 + kChunkSetup) share = 2 + kChunkSetup;
+      if (share < kChunkShare) share = kChunkShare;
       const int begin = static_cast<int>(min(static_cast<int64_t>(share) * blockIdx.x, static_cast<int64_t>(total)));
       s_list = ChunkList{s_len, s_new, s_pref, share, total - begin > share ? begin + share : total};
       s_begin = chunk_at(P, s_list, begin);
@@ -435,39 +399,38 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
   auto next = [&](ChunkPart& x) { return chunk_next<ROWS>(P, s_list, walk, x); };
   bool ok = true;  // no bounded wait of this warp has run out
   auto wait = [&](uint64_t* bar, uint32_t phase) {  // by whole warps
-    if (ok) ok = __all_sync(~0u, mbar_wait(bar, phase, P.status));
+    if (ok) ok = mbar_wait_warp(bar, phase, P.status);
     return ok;
   };
 
-  if (warp < S::SOFT) {
+  if (warp < 4 * NQ) {
     // ================================================================ softmax
     if constexpr (S::SPLIT) regs_up<S::R_SOFT>();
-    
     const int qt = warp >> 2, r = t & 127;        // query tile, row = TMEM lane
     unsigned char* q_tile = smem + qt * S::QB;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tO = tmem + lanes + S::T_O + qt * D;
+    const uint32_t tS = tmem + lanes + S::T_S + qt * TK, tO = tmem + lanes + S::T_O + qt * D;
 
     // The warp's 32 query rows into shared memory, as fp16; their exponents for
     // later.  A load takes 64 bytes of 8 rows, a store 8 rows of a column block.
     auto load_q = [&](const ChunkPart& x) {
       constexpr int IT = D / 32;             // loads of a row
+      constexpr int GR = D == 256 ? 2 : 4;   // groups of 8 rows in flight
       const int piece = lane >> 3;
-      constexpr int GR = IT < 4 ? 4 : 16 / IT;  // groups of 8 rows in flight
-#pragma unroll 1
+#pragma unroll
       for (int g0 = 0; g0 < 4; g0 += GR) {
-        uint4 va[GR][IT];
+        uint4 v[GR][IT];
 #pragma unroll
         for (int g = 0; g < GR; ++g) {
           const int rr = x.row + qt * 128 + (warp & 3) * 32 + (g0 + g) * 8 + (lane & 7);
           const int m = chunk_token(P, rr), hq = x.h * rep + rr - m * rep;
           const uint16_t* src = P.q + x.i * P.q_sr + hq * P.q_sh + m * P.q_sm + piece * 8;
-          if (m >= x.n_new || g0 + g > 3) {
+          if (m >= x.n_new) {
 #pragma unroll
-            for (int k = 0; k < IT; ++k) va[g][k] = make_uint4(0u, 0u, 0u, 0u);
+            for (int k = 0; k < IT; ++k) v[g][k] = make_uint4(0u, 0u, 0u, 0u);
           } else if (P.q16) {
 #pragma unroll
-            for (int k = 0; k < IT; ++k) va[g][k] = *reinterpret_cast<const uint4*>(src + 32 * k);
+            for (int k = 0; k < IT; ++k) v[g][k] = *reinterpret_cast<const uint4*>(src + 32 * k);
           } else {
 #pragma unroll
             for (int k = 0; k < IT; ++k) {
@@ -475,45 +438,43 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
 #pragma unroll
               for (int c = 0; c < 4; ++c)
                 w[c] = src[32 * k + 2 * c] | static_cast<uint32_t>(src[32 * k + 2 * c + 1]) << 16;
-              va[g][k] = make_uint4(w[0], w[1], w[2], w[3]);
+              v[g][k] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
         }
 #pragma unroll
         for (int g = 0; g < GR; ++g) {
-        if (g0 + g > 3) break;
-        const int row = (warp & 3) * 32 + (g0 + g) * 8 + (lane & 7);
-        const uint4(&v)[IT] = va[g];
-        uint32_t top = 0u;  // largest magnitude of the row, as the 15 bits of the type
+          const int row = (warp & 3) * 32 + (g0 + g) * 8 + (lane & 7);
+          uint32_t top = 0u;  // largest magnitude of the row, as the 15 bits of the type
 #pragma unroll
-        for (int k = 0; k < IT; ++k)
-          top = __vmaxu2(__vmaxu2(top, v[k].x & 0x7FFF7FFFu),
-                         __vmaxu2(v[k].y & 0x7FFF7FFFu, __vmaxu2(v[k].z & 0x7FFF7FFFu, v[k].w & 0x7FFF7FFFu)));
-        top = max(top & 0xFFFFu, top >> 16);
-        top = max(top, __shfl_xor_sync(~0u, top, 8));
-        top = max(top, __shfl_xor_sync(~0u, top, 16));
-        const bool bad = top >= (LO ? 0x7C00u : 0x7F80u);  // no softmax: computed as zeros, NaN at the end
-        int ex = 0;  // bf16: 2^ex brings the largest into [2^9, 2^10)
-        if (!LO && top && !bad) ex = 9 - (static_cast<int>(top >> 7) - 127);
-        ex = ex > 120 ? 120 : (ex < -120 ? -120 : ex);
-        const float up = __int_as_float((127 + ex) << 23) * (P.scale < 0.f ? -1.f : 1.f);
-        const uint32_t flip = P.scale < 0.f ? 0x80008000u : 0u;
+          for (int k = 0; k < IT; ++k)
+            top = __vmaxu2(__vmaxu2(top, v[g][k].x & 0x7FFF7FFFu),
+                           __vmaxu2(v[g][k].y & 0x7FFF7FFFu, __vmaxu2(v[g][k].z & 0x7FFF7FFFu, v[g][k].w & 0x7FFF7FFFu)));
+          top = max(top & 0xFFFFu, top >> 16);
+          top = max(top, __shfl_xor_sync(~0u, top, 8));
+          top = max(top, __shfl_xor_sync(~0u, top, 16));
+          const bool bad = top >= (LO ? 0x7C00u : 0x7F80u);  // no softmax: computed as zeros, NaN at the end
+          int ex = 0;  // bf16: 2^ex brings the largest into [2^9, 2^10)
+          if (!LO && top && !bad) ex = 9 - (static_cast<int>(top >> 7) - 127);
+          ex = ex > 120 ? 120 : (ex < -120 ? -120 : ex);
+          const float up = __int_as_float((127 + ex) << 23) * (P.scale < 0.f ? -1.f : 1.f);
+          const uint32_t flip = P.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-        for (int k = 0; k < IT; ++k) {
-          uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          for (int k = 0; k < IT; ++k) {
+            uint32_t w[4] = {v[g][k].x, v[g][k].y, v[g][k].z, v[g][k].w};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if constexpr (!LO)
-              w[c] = pack_h2(__uint_as_float(w[c] << 16) * up, __uint_as_float(w[c] & 0xFFFF0000u) * up);
-            else
-              w[c] ^= flip;
-            if (bad) w[c] = 0u;
+            for (int c = 0; c < 4; ++c) {
+              if constexpr (!LO)
+                w[c] = pack_h2(__uint_as_float(w[c] << 16) * up, __uint_as_float(w[c] & 0xFFFF0000u) * up);
+              else
+                w[c] ^= flip;
+              if (bad) w[c] = 0u;
+            }
+            *reinterpret_cast<uint4*>(q_tile + (k >> 1) * (128 * 128) + row * 128 + (((4 * (k & 1) + piece) ^ (lane & 7)) * 16)) =
+                make_uint4(prmt(w[0], w[2], 0x5410), prmt(w[0], w[2], 0x7632), prmt(w[1], w[3], 0x5410),
+                           prmt(w[1], w[3], 0x7632));
           }
-          *reinterpret_cast<uint4*>(q_tile + (k >> 1) * (128 * 128) + row * 128 + (((4 * (k & 1) + piece) ^ (lane & 7)) * 16)) =
-              make_uint4(prmt(w[0], w[2], 0x5410), prmt(w[0], w[2], 0x7632), prmt(w[1], w[3], 0x5410),
-                         prmt(w[1], w[3], 0x7632));
-        }
-        if (piece == 0) s_ex[qt * 128 + row] = bad ? INT32_MAX : ex;
+          if (piece == 0) s_ex[qt * 128 + row] = bad ? INT32_MAX : ex;
         }
       }
       fence_proxy_async_shared();
@@ -521,7 +482,7 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
       mbar_arrive(q_ready + qt);
     };
 
-    uint32_t ph_s = 0, ph_o = 0, pv = 0;  // the buffers' phases; P V's so far
+    uint32_t ph_s = 0, ph_o = 0;
     ChunkPos here = walk;  // where the part at hand is decoded from: its fields are not kept over the tiles
     bool more;
     {
@@ -530,17 +491,14 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
       if (more) load_q(u);
     }
     while (more && ok) {
-      int see, tiles;  // tokens that the row sees, from the part's first; tiles
-      bool any;        // it sees one
+      int see, t0, t1;
       {
         ChunkPart u;
         ChunkPos w = here;
         chunk_next<ROWS>(P, s_list, w, u);
         const int m = chunk_token(P, u.row + qt * 128 + r);
-        see = (m < u.n_new ? u.len - u.n_new + m + 1 : 0);
-        tiles = u.t1 - u.t0;
-        see -= u.t0 * TK;  // from the part's first token
-        any = m < u.n_new && u.len - u.n_new + m + 1 > 0;
+        see = m < u.n_new ? u.len - u.n_new + m + 1 : 0;
+        t0 = u.t0, t1 = u.t1;
       }
       const int ex = s_ex[qt * 128 + r];
       const bool bad = ex == INT32_MAX;
@@ -548,41 +506,66 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
       const float sl2 = fmaxf(ldexpf(fabsf(P.scale) * 1.4426950408889634f, bad ? 0 : -ex), 1e-37f);
       float unit = 0.f, l = 0.f;  // weights are 2^(S sl2 - unit), l their sum
       bool fresh = true;          // no token seen: the unit is not set
-      for (int j = 0; j < tiles; ++j) {
-        const int buf = j & 1;
-        const uint32_t tS = tmem + lanes + S::T_S + (2 * qt + buf) * TK;
-        if (!wait(s_full + 2 * qt + buf, ph_s >> buf & 1)) break;
-        ph_s ^= 1u << buf;
+      for (int j = t0; j < t1; ++j) {
+        if (!wait(s_full + qt, ph_s)) break;
+        ph_s ^= 1;
         tc_fence_after();
-        const int n = see - j * TK;  // tokens of the tile that the row sees
-        const bool full = __all_sync(~0u, n >= TK);
+        const int vis = see - j * TK;  // columns of the tile that this row sees
+        const bool full = __all_sync(~0u, vis >= TK);
         uint32_t hi[TK / 32][16], lo[LO ? TK / 32 : 1][16];
-        float part;
-        for (bool moved = false;; moved = true) {
-          const uint64_t sl22 = f2_make(sl2, sl2), un2 = f2_make(-unit, -unit);
+        float part = 0.f;
+        // 0: the unit is set first; 1: weights by the unit there is; 2: again, by a new one
+        for (int round = __any_sync(~0u, fresh && vis > 0) ? 0 : 1;; round = 2) {
+          if (round != 1) {
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < TK / 16; ++c) {
+              float x[16];
+              tmem_ld16(tS + c * 16, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) mx = fmaxf(mx, c * 16 + k < vis ? x[k] : -INFINITY);
+            }
+            const float now = fmaf(mx, sl2, -kChunkTop);
+            float f = 1.f;
+            if (mx > -INFINITY && (fresh || now > unit)) {
+              f = fresh ? 0.f : exp2f(unit - now);
+              unit = now;
+              l *= f;
+              fresh = false;
+            }
+            if (j > t0) {
+#pragma unroll 1
+              for (int c = 0; c < D / 16; ++c) {
+                float o[16];
+                tmem_ld16(tO + c * 16, o);
+                tmem_wait_ld();
+                uint32_t w[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(o[k] * f);
+                tmem_st16u(tO + c * 16, w);
+              }
+            }
+          }
           uint64_t sum = 0;
+          const uint64_t sl22 = f2_make(sl2, sl2), un2 = f2_make(-unit, -unit);
+          float x[2][32];
+          tmem_ld32(tS, x[0]);
 #pragma unroll
           for (int c = 0; c < TK / 32; ++c) {
-            float x[32];
-            tmem_ld32(tS + c * 32, x);
             tmem_wait_ld();
+            if (c + 1 < TK / 32) tmem_ld32(tS + (c + 1) * 32, x[(c + 1) & 1]);
+            float(&v)[32] = x[c & 1];
             if (!full) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) x[k] = c * 32 + k < n ? x[k] : -INFINITY;
+              for (int k = 0; k < 32; ++k) v[k] = c * 32 + k < vis ? v[k] : -INFINITY;
             }
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              uint64_t y2 = f2_fma(f2_make(x[2 * k], x[2 * k + 1]), sl22, un2);
-              float2 y = f2_split(y2);
-              if (k % 4 < S::POLY) {
-                y2 = exp2_fma(y2);
-                y = f2_split(y2);
-              } else {
-                y.x = fast_exp2(y.x);
-                y.y = fast_exp2(y.y);
-                y2 = f2_make(y.x, y.y);
-              }
-              sum = f2_add(sum, y2);
+              float2 y = f2_split(f2_fma(f2_make(v[2 * k], v[2 * k + 1]), sl22, un2));
+              y.x = fast_exp2(y.x);
+              y.y = fast_exp2(y.y);
+              sum = f2_add(sum, f2_make(y.x, y.y));
               hi[c][k] = pack_h2(y.x, y.y);
               if constexpr (LO) {
                 const float2 b = __half22float2(u32_as_h2(hi[c][k]));
@@ -592,39 +575,7 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
           }
           const float2 s2 = f2_split(sum);
           part = s2.x + s2.y;
-          if (moved || __all_sync(~0u, part <= kChunkMost && !(fresh && n > 0))) break;
-          // ---- the unit moves
-          float mx = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < TK / 16; ++c) {
-            float x[16];
-            tmem_ld16(tS + c * 16, x);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 16; ++k) mx = fmaxf(mx, c * 16 + k < n ? x[k] : -INFINITY);
-          }
-          const float to = fmaf(mx, sl2, -kChunkTop);
-          float f = 1.f;
-          if (mx > -INFINITY && (fresh || to > unit)) {
-            f = fresh ? 0.f : exp2f(unit - to);
-            unit = to;
-            l *= f;
-            fresh = false;
-          }
-          if (j > 0) {
-            wait(pv_done + qt, (pv + j - 1) & 1);  // the last tile's P V may still run; those before are done
-            tc_fence_after();
-#pragma unroll 1
-            for (int k = 0; k < D / 16; ++k) {
-              float o[16];
-              tmem_ld16(tO + k * 16, o);
-              tmem_wait_ld();
-              uint32_t w[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(o[i] * f);
-              tmem_st16u(tO + k * 16, w);
-            }
-          }
+          if (round != 1 || __all_sync(~0u, part <= kChunkMost)) break;
         }
         l += part;
 #pragma unroll
@@ -638,10 +589,9 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(p_ready + 2 * qt + buf);
+        mbar_arrive(p_ready + qt);
       }
       if (fresh) l = 0.f;
-      pv += tiles;
       ChunkPart u;
       chunk_next<ROWS>(P, s_list, here, u);
       here = walk;
@@ -657,9 +607,12 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
       const bool whole = u.t0 == 0 && u.t1 == u.tiles;
       const bool in = m < P.M;
       const int64_t row = static_cast<int64_t>(u.i) * P.o_sr + static_cast<int64_t>(hq) * P.o_sh + m * P.o_sm;
-      const float nan = bad && any ? NAN : 0.f;
+      const float nan = bad && see > 0 ? NAN : 0.f;
       const float inv = 1.f / l;
       const bool dead = l == 0.f;  // sees nothing
+      int64_t at[4];  // output rows of the four lanes' query rows; -1: none
+#pragma unroll
+      for (int k = 0; k < 4; ++k) at[k] = __shfl_sync(~0u, in ? row : -1, (lane & 28) + k);
       const int slot = 2 * blockIdx.x + (u.t0 == 0 ? 1 : 0);
       float* part = P.part + static_cast<int64_t>(slot) * ROWS * D + (qt * 128 + r) * 4;
 #pragma unroll 1
@@ -681,10 +634,8 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
             // four lanes exchange, so that a store takes 64 bytes of 8 rows
             transpose4(w);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int64_t at = __shfl_sync(~0u, in ? row : -1, (lane & 28) + k);  // lane k's row
-              if (at >= 0) *reinterpret_cast<uint4*>(P.out + at + c * 32 + (lane & 3) * 8) = w[k];
-            }
+            for (int k = 0; k < 4; ++k)
+              if (at[k] >= 0) *reinterpret_cast<uint4*>(P.out + at[k] + c * 32 + (lane & 3) * 8) = w[k];
           } else if (in) {
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -712,66 +663,96 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
       }
       tc_fence_before();
     }
-  } else if (warp < S::SOFT + 8) {
+  } else if (warp < 4 * NQ + 4) {
     // ================================================================ values
     if constexpr (S::SPLIT) regs_down<S::R_VAL>();
     const int r = (t & 127) % TK, part = (t & 127) / TK;  // token of the tile, channels part * CH on
-    const int page = r / kBlockTokens, slot = r % kBlockTokens;
-    constexpr int NEXT = TK * 128;  // from 64 channels to the next
-    const int x = (r & 7) * 16;
-    // a tile of K or V: raw codes and pairs -> rows of fp16
-    auto unpack = [&](const unsigned char* raw, unsigned char* dst, bool there, auto two) {
-      constexpr bool TWO = decltype(two)::value;
-      const unsigned char* code = raw + page * (kBlockTokens * D / 2) + slot * (D / 2) + part * (S::CH / 2);
-      const uint32_t* pair = reinterpret_cast<const uint32_t*>(raw + S::RAW_CODES) + r * G;
-      dst += r * 128;
-      // the lanes start on different pieces, so that neither their loads nor their stores meet
-#pragma unroll 1
-      for (int k = 0; k < S::PIECES; ++k) {
-        const int p = (k + (r >> 1)) % S::PIECES, ch = part * S::CH + p * 32;
-        const uint4 w = there ? lds_v4(code + p * 16) : make_uint4(0u, 0u, 0u, 0u);
-        unsigned char* at = dst + (ch >> 6) * NEXT;
-        const int blk = (ch & 32) * 2;
-        if constexpr (D / G >= 32) {
-          const uint32_t sz = there ? pair[ch / (D / G)] : 0u;
-          if (__any_sync(~0u, far_values(sz, TWO ? 8192.f : 65000.f))) store_piece<TWO, true>(w, sz, at, blk, x, S::VB);
-          else store_piece<TWO, false>(w, sz, at, blk, x, S::VB);
-        } else {  // two groups of 16 channels
-          const uint32_t s0 = there ? pair[ch / 16] : 0u, s1 = there ? pair[ch / 16 + 1] : 0u;
-          if (__any_sync(~0u, far_values(s0, TWO ? 8192.f : 65000.f) || far_values(s1, TWO ? 8192.f : 65000.f)))
-            store_halves<TWO, true>(w, s0, s1, at, blk, x, S::VB);
-          else
-            store_halves<TWO, false>(w, s0, s1, at, blk, x, S::VB);
-        }
-      }
+    constexpr int NW = S::CH / 8;                          // code words of the thread
+    constexpr Int4Layout L = int4_layout(D, G);
+    uint32_t kw[NW], vw[NW], kp[S::NG], vp[S::NG];
+    const int g0 = part * S::CH / (D / G);                 // its first group
+    const uint8_t* rec = nullptr;  // the token's record; nullptr: no token there
+    auto page_of = [&](const ChunkPart& x, int tile) -> int {  // of the thread's token, as the table has it
+      const int tok = tile * TK + r;
+      const int seq = P.rows ? __ldg(P.rows + x.i) : x.i;  // in range: it has tiles
+      return tok < x.len ? __ldg(P.c.table + seq * P.c.table_stride + tok / kBlockTokens) : 0;
     };
-    const int kv = (warp - S::SOFT) >> 2;  // 0: K, 1: V
-    const int slots = kv ? S::VS : S::KS;
-    uint64_t *full = kv ? v_full : k_full, *freed = kv ? v_free : k_free;
-    int at = 0, rs = 0;
-    uint32_t ph_raw = 0, ph = 1;  // a fresh barrier passes a wait for the phase before its first
-    ChunkPart u;
-    while (ok && next(u)) {
-      for (int j = u.t0; j < u.t1; ++j) {
-        const bool there = j * TK + r < u.len;
-        const int slot_raw = kv * S::RS + rs;
-        const unsigned char* raw = smem + S::OFF_RAW + slot_raw * S::RAW;
-        if (!wait(raw_full + slot_raw, ph_raw) || !wait(freed + at, ph)) break;
-        if (kv) unpack(raw, smem + S::OFF_V + at * S::VB, there, std::false_type());
-        else unpack(raw, smem + S::OFF_K + at * S::KB, there, std::bool_constant<LO != 0>());
-        mbar_arrive(raw_free + slot_raw);
-        fence_proxy_async_shared();
-        mbar_arrive(full + at);
-        if (++at == slots) at = 0, ph ^= 1;
-        if (++rs == S::RS) rs = 0, ph_raw ^= 1;
+    auto fetch_k = [&](const ChunkPart& x, int tile, int p) {
+      const int tok = tile * TK + r;
+      rec = nullptr;
+      if (tok < x.len) {
+        if (p < 0 || p >= P.c.n_pages) {
+          set_status(P.status, AKV_ERR_SHAPE);
+          p = 0;
+        }
+        rec = P.c.pool + p * P.c.page_stride + x.h * P.c.head_stride;
       }
+      const int slot = tok % kBlockTokens;
+#pragma unroll
+      for (int k = 0; k < NW / 4; ++k) {
+        const uint4 v = rec ? ldg_nc_v4(rec + L.kc + slot * (D / 2) + part * (S::CH / 2) + 16 * k) : make_uint4(0, 0, 0, 0);
+        kw[4 * k] = v.x, kw[4 * k + 1] = v.y, kw[4 * k + 2] = v.z, kw[4 * k + 3] = v.w;
+      }
+#pragma unroll
+      for (int k = 0; k < S::NG; ++k)
+        kp[k] = rec ? __ldg(reinterpret_cast<const uint32_t*>(rec + L.kp) + slot * G + g0 + k) : 0u;
+    };
+    auto fetch_v = [&](int tile) {
+      const int slot = (tile * TK + r) % kBlockTokens;
+#pragma unroll
+      for (int k = 0; k < NW / 4; ++k) {
+        const uint4 v = rec ? ldg_nc_v4(rec + L.vc + slot * (D / 2) + part * (S::CH / 2) + 16 * k) : make_uint4(0, 0, 0, 0);
+        vw[4 * k] = v.x, vw[4 * k + 1] = v.y, vw[4 * k + 2] = v.z, vw[4 * k + 3] = v.w;
+      }
+#pragma unroll
+      for (int k = 0; k < S::NG; ++k)
+        vp[k] = rec ? __ldg(reinterpret_cast<const uint32_t*>(rec + L.vp) + slot * G + g0 + k) : 0u;
+    };
+    constexpr int NEXT = TK * 128;  // from 64 channels to the next
+    unsigned char* at = smem + r * 128 + part * (S::CH / 64) * NEXT;
+    const int swz = ((r ^ part * (S::CH / 8)) & 7) * 16;  // half a row of 64 channels starts at its fifth piece
+    int ks = 0, vs = 0;
+    uint32_t kph = 1, vph = 1;  // a fresh barrier passes a wait for the phase before its first
+    ChunkPart u{};
+    bool more = next(u);
+    int j = u.t0;
+    int page = 0;  // of the tile after the next
+    if (more) {
+      fetch_k(u, j, page_of(u, j));
+      fetch_v(j);
+      if (j + 1 < u.t1) page = page_of(u, j + 1);
+    }
+    while (more && ok) {
+      ChunkPart nx = u;
+      int nj = j + 1;
+      bool again = true;
+      if (nj == u.t1) {
+        again = next(nx);
+        nj = nx.t0;
+      }
+      if (!wait(k_free + ks, kph)) break;
+      store_values<NW, S::NG, LO>(kw, kp, at + S::OFF_K + ks * S::KB, swz, NEXT, S::VB);
+      fence_proxy_async_shared();
+      mbar_arrive(k_full + ks);
+      if (++ks == S::KS) ks = 0, kph ^= 1;
+      if (again) {
+        fetch_k(nx, nj, nj == nx.t0 ? page_of(nx, nj) : page);
+        if (nj + 1 < nx.t1) page = page_of(nx, nj + 1);
+      }
+      if (!wait(v_free + vs, vph)) break;
+      store_values<NW, S::NG, false>(vw, vp, at + S::OFF_V + vs * S::VB, swz, NEXT, 0);
+      fence_proxy_async_shared();
+      mbar_arrive(v_full + vs);
+      if (++vs == S::VS) vs = 0, vph ^= 1;
+      if (again) fetch_v(nj);
+      u = nx;
+      j = nj;
+      more = again;
     }
   } else {
     // ================================================================ MMA
     if constexpr (S::SPLIT) regs_down<S::R_MMA>();
-    if (warp < S::SOFT + 8 + NQ) {
-    // a warp for each query tile
-    const int q = warp - S::SOFT - 8;
+    if (warp == 4 * NQ + 4) {
     const uint32_t lead = elect_one();
     constexpr uint32_t NEXT = TK * 128;  // from 64 channels to the next
     constexpr uint32_t HI = desc_hi_sw128(1024);
@@ -780,121 +761,67 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
     const uint32_t base = smem_u32(smem);
     int ks = 0, vs = 0;
     uint32_t kph = 0, vph = 0, ph_p = 0, ph_q = 0;
-    const uint32_t q_tile = desc_lo(base + q * S::QB, 16);
-    const uint32_t tO = tmem + S::T_O + q * D;
-    // S of the next tile into its buffer
-    auto qk = [&](int buf) {
-      const uint32_t b = desc_lo(base + S::OFF_K + ks * S::KB, 16);
-      const uint32_t d = tmem + S::T_S + (2 * q + buf) * TK;
+    auto qk = [&](int q) {
+      const uint32_t a = desc_lo(base + q * S::QB, 16), b = desc_lo(base + S::OFF_K + ks * S::KB, 16);
+      const uint32_t d = tmem + S::T_S + q * TK;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        const uint32_t ak = q_tile + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16, bk = b + ((k >> 2) * NEXT + (k & 3) * 32) / 16;
+        const uint32_t ak = a + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16, bk = b + ((k >> 2) * NEXT + (k & 3) * 32) / 16;
         umma_ss<HI, HI, IDESC_S>(d, ak, bk, k > 0 ? 1u : 0u, lead);
         if constexpr (LO) umma_ss<HI, HI, IDESC_S>(d, ak, bk + S::VB / 16, 1u, lead);
       }
-      umma_commit(s_full + 2 * q + buf, lead);
-      umma_commit(k_free + ks, lead);
-      if (++ks == S::KS) ks = 0, kph ^= 1;
+      umma_commit(s_full + q, lead);
     };
     ChunkPart u;
     while (ok && next(u)) {
-      wait(q_ready + q, ph_q);
+      for (int q = 0; q < NQ; ++q) wait(q_ready + q, ph_q);
       ph_q ^= 1;
-      const int tiles = u.t1 - u.t0;
-      for (int j = 0; j < 2 && j < tiles; ++j) {
-        if (!wait(k_full + ks, kph)) break;
-        tc_fence_after();
-        qk(j);
-      }
-      for (int j = 0; j < tiles; ++j) {
-        const int buf = j & 1;
-        const bool again = j + 2 < tiles;
-        // what is there early first: the weights are what takes its time
-        if (!wait(v_full + vs, vph) || (again && S::KS > 1 && !wait(k_full + ks, kph)) ||
-            !wait(p_ready + 2 * q + buf, ph_p >> buf & 1))
-          break;
-        ph_p ^= 1u << buf;
-        tc_fence_after();
+      if (!wait(k_full + ks, kph)) break;
+      tc_fence_after();
+      for (int q = 0; q < NQ; ++q) qk(q);
+      umma_commit(k_free + ks, lead);
+      if (++ks == S::KS) ks = 0, kph ^= 1;
+      for (int j = u.t0; j < u.t1; ++j) {
+        if (!wait(v_full + vs, vph)) break;
+        const bool again = j + 1 < u.t1;
         const uint32_t v = desc_lo(base + S::OFF_V + vs * S::VB, NEXT);
-        const uint32_t tP = tmem + S::T_S + (2 * q + buf) * TK;
+        for (int q = 0; q < NQ; ++q) {
+          if (!wait(p_ready + q, ph_p)) break;
+          tc_fence_after();
+          const uint32_t tP = tmem + S::T_S + q * TK, tO = tmem + S::T_O + q * D;
 #pragma unroll
-        for (int k = 0; k < TK / 16; ++k) {
-          const uint32_t on = j > 0 || k > 0 ? 1u : 0u;
-          if constexpr (LO) {
-            const uint32_t p = tP + 32 * (k >> 1) + 8 * (k & 1);
-            umma_ts<HI, IDESC_O>(tO, p, v + k * 128, on, lead);
-            umma_ts<HI, IDESC_O>(tO, p + 16, v + k * 128, 1u, lead);
+          for (int k = 0; k < TK / 16; ++k) {
+            const uint32_t on = j > u.t0 || k > 0 ? 1u : 0u;
+            if constexpr (LO) {
+              const uint32_t col = 32 * (k >> 1) + 8 * (k & 1);
+              umma_ts<HI, IDESC_O>(tO, tP + col, v + k * 128, on, lead);
+              umma_ts<HI, IDESC_O>(tO, tP + col + 16, v + k * 128, 1u, lead);
+            } else {
+              umma_ts<HI, IDESC_O>(tO, tP + 8 * k, v + k * 128, on, lead);
+            }
+          }
+          if (q == NQ - 1) umma_commit(v_free + vs, lead);
+          if (again) {
+            if (q == 0 && !wait(k_full + ks, kph)) break;
+            tc_fence_after();
+            qk(q);
           } else {
-            umma_ts<HI, IDESC_O>(tO, tP + 8 * k, v + k * 128, on, lead);
+            umma_commit(o_full + q, lead);
           }
         }
-        umma_commit(pv_done + q, lead);
-        umma_commit(v_free + vs, lead);
-        if (j + 1 == tiles) umma_commit(o_full + q, lead);
+        if (!ok) break;
         if (++vs == S::VS) vs = 0, vph ^= 1;
-        if (again) {  // P is read before this overwrites it: a thread's MMAs run in order
-          if (S::KS == 1) {
-            if (!wait(k_full + ks, kph)) break;
-            tc_fence_after();
-          }
-          qk(buf);
+        ph_p ^= 1;
+        if (again) {
+          umma_commit(k_free + ks, lead);
+          if (++ks == S::KS) ks = 0, kph ^= 1;
         }
       }
     }
     if (!ok) {  // a wait ran out: see what was issued end before the tensor memory goes
-      umma_commit(drained + 3 * q, lead);
-      mbar_wait(drained + 3 * q, 0, P.status);
+      umma_commit(drained, lead);
+      mbar_wait(drained, 0, P.status);
     }
-    } else if (warp == S::SOFT + 8 + NQ) {
-      // ============================================================== pages
-      constexpr Int4Layout L = int4_layout(D, G);
-      constexpr int CODES = kBlockTokens * D / 2, PAIRS = kBlockTokens * G * 4;
-      uint32_t ph = 1;  // a fresh barrier passes a wait for the phase before its first
-      int rs = 0;
-      bool flying = false;
-      ChunkPart u;
-      while (ok && next(u)) {
-        const int seq = P.rows ? __ldg(P.rows + u.i) : u.i;  // in range: it has tiles
-        const int32_t* table = P.c.table + seq * P.c.table_stride;
-        const int pages = (u.len + kBlockTokens - 1) / kBlockTokens;
-        auto page_of = [&](int tile) -> int {  // a page for each of the first lanes; -1: none
-          const int b = tile * S::PAGES + lane;
-          return lane < S::PAGES && b < pages ? __ldg(table + b) : -1;
-        };
-        int p = page_of(u.t0);
-        for (int j = u.t0; j < u.t1; ++j) {
-          const int b = j * S::PAGES + lane;
-          const bool on = lane < S::PAGES && b < pages;
-          if (on && (p < 0 || p >= P.c.n_pages)) {
-            set_status(P.status, AKV_ERR_SHAPE);
-            p = 0;
-          }
-          const uint8_t* rec = P.c.pool + p * P.c.page_stride + u.h * P.c.head_stride;
-          const uint32_t bytes = __popc(__ballot_sync(~0u, on)) * (CODES + PAIRS);
-          const int ahead = j + 1 < u.t1 ? page_of(j + 1) : 0;
-#pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            const int at = v * S::RS + rs;
-            if (!wait(raw_free + at, ph)) break;
-            unsigned char* raw = smem + S::OFF_RAW + at * S::RAW;
-            if (lane == 0) mbar_arrive_expect_tx(raw_full + at, bytes);
-            __syncwarp();
-            if (on) {
-              tma_load_1d(raw + lane * CODES, rec + (v ? L.vc : L.kc), CODES, raw_full + at);
-              tma_load_1d(raw + S::RAW_CODES + lane * PAIRS, rec + (v ? L.vp : L.kp), PAIRS, raw_full + at);
-            }
-            flying = true;
-          }
-          if (!ok) break;
-          if (++rs == S::RS) rs = 0, ph ^= 1;
-          p = ahead;
-        }
-      }
-      if (!ok && flying)  // a wait ran out: see the copies in flight land
-        for (int v = 0; v < 2 * S::RS; ++v) {
-          mbar_wait(raw_full + v, ph, P.status);
-          mbar_wait(raw_full + v, ph ^ 1, P.status);
-        }
     }
   }
   tc_fence_before();

@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
   if (warp < 8) {
     // ================================================================ weights
     auto wait = [&](uint64_t* bar, uint32_t phase) {
-      if (ok) ok = __all_sync(~0u, mbar_wait(bar, phase, P.status));
+      if (ok) ok = mbar_wait_warp(bar, phase, P.status);
       return ok;
     };
     constexpr Int4Layout L = int4_layout(D, G);
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
     // ================================================================ MMA
     const uint32_t lead = elect_one();
     auto wait = [&](uint64_t* bar, uint32_t phase) {
-      if (ok) ok = __all_sync(~0u, mbar_wait(bar, phase, P.status));
+      if (ok) ok = mbar_wait_warp(bar, phase, P.status);
       return ok;
     };
     constexpr uint32_t IDESC = instr_desc(128, N, 0);
