@@ -6,15 +6,18 @@
 // and the k largest logits, the lowest index first among equal ones.  One pass:
 // a thread keeps the running maximum of what it has seen, Z and sum(e^u u)
 // relative to it (in log2 units), and rescales both when the maximum moves.
-// All sums are fp32; u is clamped to -160 in log2 units, where e^u is 0 in fp32,
-// so that -inf logits add 0 and not 0 * -inf.
+// All sums are fp32.  In a batch where some u is -inf, u is clamped to -160 in
+// log2 units, where e^u is 0 in fp32, so that it adds 0 and not 0 * -inf; a NaN
+// stays one and shows in Z.
 //
 // Top alternatives: a warp holds the best 32 it has met, one a lane in
 // descending order, as 64-bit keys (value's order << 32 | ~index): they decide
-// ties, so the result depends on the inputs alone.  A batch of 32 elements a
-// lane is looked through only if its maximum reaches the k-th key.  The lists
-// of warps and CTAs are merged pairwise (maximum of one and the other reversed
-// is the bitonic top half).
+// ties, so the result depends on the inputs alone.  The lanes' maxima of the
+// first batch, sorted, start the list; from then on a batch of up to 32 elements
+// a lane is looked through only if its maximum reaches the k-th key, and of it the
+// elements that do, a bit each, are read again and inserted.  The lists of warps
+// and CTAs are merged pairwise (maximum of one and the other reversed is the
+// bitonic top half).
 //
 // Bound by memory: every logit is read once.  Few rows are split over clusters
 // of up to 8 CTAs.
@@ -75,10 +78,43 @@ struct LogitElem {  // two 16-bit logits a word
       asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
   }
+  AKV_DEV static uint32_t min_word(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (DT == AKV_BF16)
+      asm("min.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+      asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
   AKV_DEV static float max_of(uint32_t w) {
     float x[2];
     unpack(w, x);
     return fmaxf(x[0], x[1]);
+  }
+  AKV_DEV static float min_of(uint32_t w) {
+    float x[2];
+    unpack(w, x);
+    return fminf(x[0], x[1]);
+  }
+  // ones for the logits of a batch above x, which is a logit itself; counts up to 256 are exact
+  AKV_DEV static int count_above(const uint32_t* w, int n, float x) {
+    float c[2];
+    if constexpr (DT == AKV_BF16) {
+      const __nv_bfloat162 x2 = __float2bfloat162_rn(x);
+      __nv_bfloat162 sum = __float2bfloat162_rn(0.f);
+#pragma unroll
+      for (int i = 0; i < n; ++i) sum = __hadd2(sum, __hgt2(*reinterpret_cast<const __nv_bfloat162*>(w + i), x2));
+      const float2 f = __bfloat1622float2(sum);
+      c[0] = f.x, c[1] = f.y;
+    } else {
+      const __half2 x2 = __float2half2_rn(x);
+      __half2 sum = __float2half2_rn(0.f);
+#pragma unroll
+      for (int i = 0; i < n; ++i) sum = __hadd2(sum, __hgt2(u32_as_h2(w[i]), x2));
+      const float2 f = __half22float2(sum);
+      c[0] = f.x, c[1] = f.y;
+    }
+    return static_cast<int>(c[0] + c[1]);
   }
 };
 template <>
@@ -90,7 +126,17 @@ struct LogitElem<AKV_FP32> {
   AKV_DEV static uint32_t max_word(uint32_t a, uint32_t b) {
     return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
   }
+  AKV_DEV static uint32_t min_word(uint32_t a, uint32_t b) {
+    return __float_as_uint(fminf(__uint_as_float(a), __uint_as_float(b)));
+  }
   AKV_DEV static float max_of(uint32_t w) { return __uint_as_float(w); }
+  AKV_DEV static float min_of(uint32_t w) { return __uint_as_float(w); }
+  AKV_DEV static int count_above(const uint32_t* w, int n, float x) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < n; ++i) c += __uint_as_float(w[i]) > x;
+    return c;
+  }
 };
 
 // 32-bit order of a logit (-0 as +0); never called for NaN
@@ -119,6 +165,20 @@ AKV_DEV LogpSums join(LogpSums a, LogpSums b) {
   r.s = fa * a.s + fb * b.s;
   r.t = fa * fmaf(da, a.s, a.t) + fb * fmaf(db, b.s, b.t);
   return r;
+}
+
+// descending order over the lanes of any keys
+AKV_DEV uint64_t bitonic_sort(uint64_t k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int o = size / 2; o; o >>= 1) {
+      const uint64_t y = __shfl_xor_sync(~0u, k, o);
+      const bool small = ((lane & o) != 0) != (size < 32 && (lane & size) != 0);
+      k = small ? (k < y ? k : y) : (k > y ? k : y);
+    }
+  return k;
 }
 
 // descending order over the lanes of a bitonic sequence of keys
@@ -198,40 +258,75 @@ __global__ void __launch_bounds__(kLogpThreads, 4) token_logprobs_kernel(const L
       const uint4 q = at < v1 ? ldg_nc_v4(xv + at) : make_uint4(E::kNone, E::kNone, E::kNone, E::kNone);
       w[4 * j] = q.x, w[4 * j + 1] = q.y, w[4 * j + 2] = q.z, w[4 * j + 3] = q.w;
     }
-    uint32_t top = w[0];
+    uint32_t top = w[0], low = w[0];
 #pragma unroll
-    for (int i = 1; i < W; ++i) top = E::max_word(top, w[i]);
+    for (int i = 1; i < W; ++i) {
+      top = E::max_word(top, w[i]);
+      low = E::min_word(low, w[i]);
+    }
     const float m = E::max_of(top);
     if (!(m <= a.m)) raise(m);
-    const bool count = m > mine;
+    const bool vanish = (E::min_of(low) - base) * kLog2E == -INFINITY;
+    const uint64_t back = f2_make(-base, -base), unit = f2_make(kLog2E, kLog2E);
+    uint64_t s2 = 0, t2 = 0;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
+    for (int i = 0; i < W; i += 2 / PER) {
+      float x[2];
       if constexpr (PER == 2) {
-        float x[2];
         E::unpack(w[i], x);
-        add(x[0]);
-        add(x[1]);
-        if (count) above += (x[0] > mine) + (x[1] > mine);
       } else {
-        add(__uint_as_float(w[i]));
-        if (count) above += __uint_as_float(w[i]) > mine;
+        x[0] = __uint_as_float(w[i]), x[1] = __uint_as_float(w[i + 1]);
       }
+      uint64_t u2 = f2_mul(f2_add(f2_make(x[0], x[1]), back), unit);
+      float2 u = f2_split(u2);
+      if (vanish) {
+        u.x = max_nan(u.x, -160.f), u.y = max_nan(u.y, -160.f);
+        u2 = f2_make(u.x, u.y);
+      }
+      const uint64_t e2 = f2_make(fast_exp2(u.x), fast_exp2(u.y));
+      s2 = f2_add(s2, e2);
+      t2 = f2_fma(e2, u2, t2);
     }
+    const float2 s = f2_split(s2), t_ = f2_split(t2);
+    a.s += s.x + s.y;
+    a.t += t_.x + t_.y;
+    if (m > mine) above += E::count_above(w, W, mine);
     if constexpr (TOP) {
-      const bool look = m == m && logit_order(m) >= static_cast<uint32_t>(least >> 32);
-      if (__any_sync(~0u, look)) {
+      // the elements that reach `bar`, a bit each: word i's from PER * i on
+      auto reach = [&](float bar) -> uint32_t {
+        uint32_t bits = 0u;
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-          const int at = v + (i / 4) * kLogpThreads + t;
-          const int c = head + at * E::N + (i % 4) * PER;
+          if (v + (i / 4) * kLogpThreads + t >= v1) continue;
           if constexpr (PER == 2) {
             float x[2];
             E::unpack(w[i], x);
-            offer(look && at < v1 ? logit_key(x[0], c) : 0);
-            offer(look && at < v1 ? logit_key(x[1], c + 1) : 0);
+            if (x[0] >= bar) bits |= 1u << (2 * i);
+            if (x[1] >= bar) bits |= 2u << (2 * i);
           } else {
-            offer(look && at < v1 ? logit_key(__uint_as_float(w[i]), c) : 0);
+            if (__uint_as_float(w[i]) >= bar) bits |= 1u << i;
           }
+        }
+        return bits;
+      };
+      auto key_of = [&](int bit) -> uint64_t {
+        const int i = bit / PER;
+        const int c = head + (v + (i / 4) * kLogpThreads + t) * E::N + (i % 4) * PER + bit % PER;
+        return logit_key(E::get(__ldg(x0 + c)), c);
+      };
+      uint32_t done = 0u;
+      if (v == v0) {
+        const uint32_t bits = reach(m);
+        done = bits & -bits;
+        best = bitonic_sort(bits ? key_of(__ffs(bits) - 1) : 0);
+        least = __shfl_sync(~0u, best, P.top - 1);
+      }
+      const bool look = m == m && logit_order(m) >= static_cast<uint32_t>(least >> 32);
+      if (__any_sync(~0u, look)) {
+        uint32_t bits = look ? reach(least ? order_logit(static_cast<uint32_t>(least >> 32)) : -INFINITY) & ~done : 0u;
+        while (__any_sync(~0u, bits != 0u)) {
+          offer(bits ? key_of(__ffs(bits) - 1) : 0);
+          bits &= bits - 1;
         }
       }
     }
@@ -259,10 +354,10 @@ __global__ void __launch_bounds__(kLogpThreads, 4) token_logprobs_kernel(const L
     s_sums[warp] = a;
     s_above[warp] = above;
   }
-  if constexpr (TOP) {
+  // the lists of the first n warps become the first one's
+  auto merge_lists = [&](int n) {
     s_keys[warp][lane] = best;
-#pragma unroll
-    for (int o = 1; o < kLogpWarps; o *= 2) {
+    for (int o = 1; o < n; o *= 2) {
       __syncthreads();
       if (warp % (2 * o) == 0) {
         const uint64_t other = s_keys[warp + o][31 - lane];
@@ -270,7 +365,8 @@ __global__ void __launch_bounds__(kLogpThreads, 4) token_logprobs_kernel(const L
         s_keys[warp][lane] = best;
       }
     }
-  }
+  };
+  if constexpr (TOP) merge_lists(kLogpWarps);
   __syncthreads();
   if (t == 0) {
     for (int i = 1; i < kLogpWarps; ++i) {
@@ -281,19 +377,27 @@ __global__ void __launch_bounds__(kLogpThreads, 4) token_logprobs_kernel(const L
     s_above[0] = above;
   }
   cluster.sync();
+  if constexpr (TOP) {
+    if (rank == 0 && C > 1) {
+      // warp i brings in CTA i's list: one at a time would be as many trips through the cluster
+      if (warp > 0) best = warp < C ? cluster.map_shared_rank(&s_keys[0][0], warp)[lane] : 0;
+      merge_lists(C);
+    }
+  }
   if (rank == 0 && warp == 0) {
-    for (int i = 1; i < C; ++i) {
-      a = join(i == 1 ? s_sums[0] : a, *cluster.map_shared_rank(&s_sums[0], i));
-      above = (i == 1 ? s_above[0] : above) + *cluster.map_shared_rank(&s_above[0], i);
-      if constexpr (TOP) {
-        const uint64_t other = cluster.map_shared_rank(&s_keys[0][0], i)[31 - lane];
-        best = bitonic_merge(best > other ? best : other);
-      }
+    a = LogpSums{-INFINITY, 0.f, 0.f};
+    above = 0;
+    if (lane < C) {
+      a = *cluster.map_shared_rank(&s_sums[0], lane);
+      above = *cluster.map_shared_rank(&s_above[0], lane);
     }
-    if (C == 1) {
-      a = s_sums[0];
-      above = s_above[0];
+#pragma unroll
+    for (int o = 1; o < kLogpMaxCluster; o *= 2) {
+      const LogpSums b{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.t, o)};
+      a = (lane & o) ? join(b, a) : join(a, b);
     }
+    a = LogpSums{__shfl_sync(~0u, a.m, 0), __shfl_sync(~0u, a.s, 0), __shfl_sync(~0u, a.t, 0)};
+    above = __reduce_add_sync(~0u, above);
     // no distribution: NaN or +inf among the logits, or all of them -inf
     const bool bad = !(fabsf(a.m) < INFINITY) || a.s != a.s;
     const float logz = logf(a.s);
