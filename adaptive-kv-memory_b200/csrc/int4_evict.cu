@@ -7,24 +7,22 @@
 // every layer and head.
 //
 // Five steps, each a launch: scores; the keep-th largest score by a radix
-// select and the list of the kept tokens, a CTA a row; pages for those that are
-// shared and would be written (their other holders keep them), in the order of
-// the rows; the moves; tables, lengths and reference counts.
+// select, the list of the kept tokens and the pages that are shared and would be
+// written, a CTA a row; new pages for those (their other holders keep the old
+// ones), in the order of the rows; the moves; tables, lengths and reference counts.
 //
 // Moves in place.  The kept tokens of page j come from pages >= j, so taking
 // the pages in ascending order a CTA may read ahead freely; it only has to have
-// read all of a page's sources before it writes that page.  A CTA owns one
-// (row, layer, head) and its four pages at a time stand in registers between
-// read and write; rows x layers x heads run side by side.  Pages before the
-// first token that goes are left alone.
+// read all of a page's sources before it writes that page.  A CTA owns the K or
+// the V of one (row, layer, head), and four 16-byte pieces a thread stand in
+// registers between read and write.  Pages before the first token that goes are
+// left alone.
 #include "int4.cuh"
 
 namespace akv {
 
 constexpr int kSelectThreads = 1024;
-constexpr int kMoveThreads = 256;
-constexpr int kMovePages = 4;
-constexpr int kMoveTokens = kMovePages * kBlockTokens;
+constexpr int kMovePieces = 4;  // 16-byte pieces of a thread between read and write
 
 // What a step of the eviction knows of a call row.
 struct EvictRow {
@@ -52,7 +50,7 @@ struct EvictParams {
   EvictRow* info;
   uint32_t* score;   // [n][max_blocks * 32] order of the scores
   int32_t* list;     // new pages
-  int32_t* to;       // [n][max_blocks] page each page of the row becomes
+  int32_t* to;       // [n][max_blocks] what each page of the row becomes: new_page()
   int* status;
 };
 
@@ -132,8 +130,9 @@ AKV_DEV int select_scan(int x, int* warp_sums, int& total) {
 // ---------------------------------------------------------------- selection
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams P) {
   __shared__ int s_hist[256], s_warp[32];
-  __shared__ int s_bin, s_above, s_first, s_need;
+  __shared__ int s_bin, s_above, s_first;
   const int i = blockIdx.x, t = threadIdx.x;
+  if (t == 0) s_first = INT32_MAX;
   const int2 row = evict_row(P, i);
   const int seq = row.x, len = row.y;
   const int left = len < P.keep ? len : P.keep;
@@ -169,33 +168,61 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     want -= s_above;
     __syncthreads();
   }
-  // in order: the keys above it, and the first `want` equal to it
-  if (t == 0) s_first = len, s_need = 0;
-  int out = 0, equal = 0;
-  for (int j0 = 0; j0 < len; j0 += kSelectThreads) {
-    const int j = j0 + t;
-    const uint32_t k = j < len ? key[j] : 0u;
-    const bool eq = j < len && k == prefix, gt = j < len && k > prefix;
-    int n_eq, n_on;
-    const int before = select_scan(eq, s_warp, n_eq) - eq + equal;
-    const bool on = gt || (eq && before < want);
-    const int at = select_scan(on, s_warp, n_on) - on + out;
-    if (on) kept[at] = j;
-    else if (j < len) atomicMin(&s_first, j);
-    out += n_on;
-    equal += n_eq;
+  // in order: the keys above it, and the first `want` equal to it; a thread takes a run of keys
+  const int run = (len + 4 * kSelectThreads - 1) / (4 * kSelectThreads) * 4;
+  const int j0 = t * run, j1 = min(len, j0 + run);
+  int n_eq = 0, n_gt = 0;
+  for (int j = j0; j < j1; j += 4) {
+    const uint4 q = *reinterpret_cast<const uint4*>(key + j);
+    const uint32_t k[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      n_eq += j + e < j1 && k[e] == prefix;
+      n_gt += j + e < j1 && k[e] > prefix;
+    }
+  }
+  int total;
+  int equal = select_scan(n_eq, s_warp, total) - n_eq;  // before this run
+  const int on = n_gt + max(0, min(n_eq, want - equal));
+  int at = select_scan(on, s_warp, total) - on;
+  for (int j = j0; j < j1; j += 4) {
+    const uint4 q = *reinterpret_cast<const uint4*>(key + j);
+    const uint32_t k[4] = {q.x, q.y, q.z, q.w};
+    int gone = len;
+#pragma unroll
+    for (int e = 3; e >= 0; --e)
+      if (j + e < j1 && k[e] < prefix) gone = j + e;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (j + e >= j1) continue;
+      const bool stays = k[e] > prefix || (k[e] == prefix && equal < want);
+      if (k[e] == prefix && ++equal > want) gone = min(gone, j + e);
+      if (stays) kept[at++] = j + e;
+    }
+    if (gone < s_first) atomicMin(&s_first, gone);
   }
   __syncthreads();
   const int end = (left + kBlockTokens - 1) / kBlockTokens;
   const int start = s_first < left ? s_first / kBlockTokens : end;  // past the kept tokens: none moves
   int need = 0;
-  for (int b = start + t; b < end; b += kSelectThreads) {
-    const int p = P.T.table[seq * P.T.table_stride + b];
-    if (p >= 0 && p < P.T.n_pages) need += P.T.refs[p] > 1;
+  for (int b0 = start; b0 < end; b0 += kSelectThreads) {
+    const int b = b0 + t;
+    const int p = b < end ? P.T.table[seq * P.T.table_stride + b] : -1;
+    const bool ok = p >= 0 && p < P.T.n_pages, shared = ok && P.T.refs[p] > 1;
+    if (b < end && !ok) set_status(P.status, AKV_ERR_SHAPE);
+    int n;
+    const int rank = need + select_scan(shared, s_warp, n) - shared;
+    if (b < end) P.to[static_cast<int64_t>(i) * P.T.max_blocks + b] = shared ? -2 - rank : ok ? p : -1;
+    need += n;
   }
-  if (need) atomicAdd(&s_need, need);
-  __syncthreads();
-  if (t == 0) P.info[i] = EvictRow{seq, len, left, start, end, s_need, 0, 0};
+  if (t == 0) P.info[i] = EvictRow{seq, len, left, start, end, need, 0, 0};
+}
+
+// Page that page b of call row i becomes: its own, or where that is shared one from
+// the list, the row's -2 - to[b]-th; -1 for one that is no page.
+AKV_DEV int new_page(const EvictParams& P, const EvictRow& r, int i, int b) {
+  const int p = P.to[static_cast<int64_t>(i) * P.T.max_blocks + b];
+  return p < -1 ? P.list[r.off - 2 - p] : p;
 }
 
 // ---------------------------------------------------------------- new pages
@@ -251,110 +278,107 @@ __global__ void __launch_bounds__(kSelectThreads) evict_plan_kernel(const EvictP
 }
 
 // ---------------------------------------------------------------- moves
-// Page that page b of the row becomes: its own, or a new one where it is shared.
-__global__ void __launch_bounds__(kSelectThreads) evict_target_kernel(const EvictParams P) {
-  __shared__ int s_warp[32];
-  const int i = blockIdx.x, t = threadIdx.x;
-  const EvictRow r = P.info[i];
-  if (r.seq < 0) {
-    for (int j = t; j < P.keep; j += kSelectThreads) P.kept[static_cast<int64_t>(i) * P.keep + j] = -1;
-    return;
-  }
-  int taken = r.off;
-  for (int b0 = r.start; b0 < r.end; b0 += kSelectThreads) {
-    const int b = b0 + t;
-    const int p = b < r.end ? P.T.table[r.seq * P.T.table_stride + b] : -1;
-    const bool ok = p >= 0 && p < P.T.n_pages, shared = ok && r.need > 0 && P.T.refs[p] > 1;
-    if (b < r.end && !ok) set_status(P.status, AKV_ERR_SHAPE);
-    int total;
-    const int rank = select_scan(shared, s_warp, total) - shared;
-    if (b < r.end) P.to[static_cast<int64_t>(i) * P.T.max_blocks + b] = shared ? P.list[taken + rank] : (ok ? p : -1);
-    taken += total;
-  }
-}
+template <int B>
+struct MoveWord;
+template <>
+struct MoveWord<4> { using type = uint32_t; };
+template <>
+struct MoveWord<8> { using type = uint2; };
+template <>
+struct MoveWord<16> { using type = uint4; };
 
-template <int D, int G>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams P) {
+// Block x: K (even) or V of head x / 2; the last one the weights.
+template <int D, int G, int NT>
+__global__ void __launch_bounds__(NT) evict_move_kernel(const EvictParams P) {
   constexpr Int4Layout L = int4_layout(D, G);
-  constexpr int CH = D / 32;                 // 16-byte pieces of a token's K (V) codes
-  constexpr int PIECES = kMoveTokens * CH / kMoveThreads * 2;
-  constexpr int PAIRS = kMoveTokens * G * 2; // 4-byte (scale, zero) pairs, K then V
-  constexpr int PW = (PAIRS + kMoveThreads - 1) / kMoveThreads;
+  constexpr int CH = D / 32;                    // 16-byte pieces of a token's codes
+  constexpr int TOK = NT * kMovePieces / CH;    // tokens of a step
+  constexpr int PER = (TOK + NT - 1) / NT;      // tokens whose place and (scale, zero) pairs a thread takes
+  using Pairs = typename MoveWord<G * 4>::type;
+  __shared__ int2 s_from[2][TOK];               // page and slot of the step's sources
+  __shared__ int s_to[2][TOK / kBlockTokens];
   const int t = threadIdx.x;
-  const int h = blockIdx.x, layer = blockIdx.y, i = blockIdx.z;
+  const int layer = blockIdx.y, i = blockIdx.z;
   const EvictRow r = P.info[i];
   if (r.seq < 0 || r.start >= r.end) return;
   const int32_t* kept = P.kept + static_cast<int64_t>(i) * P.keep;
-  if (h == P.kv_heads) {  // the weights move like a head
+  const int first = r.start * kBlockTokens;
+  if (blockIdx.x == 2 * P.kv_heads) {  // the weights move like a head
     float* w = P.weights + layer * P.w_layer + r.seq * P.w_row;
-    for (int j0 = r.start * kBlockTokens; j0 < r.left; j0 += 4 * kMoveThreads) {
+    for (int j0 = first; j0 < r.left; j0 += 4 * NT) {
       float v[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int j = j0 + k * kMoveThreads + t;
+        const int j = j0 + k * NT + t;
         v[k] = j < r.left ? w[kept[j]] : 0.f;
       }
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int j = j0 + k * kMoveThreads + t;
+        const int j = j0 + k * NT + t;
         if (j < r.left) w[j] = v[k];
       }
     }
     return;
   }
   const int32_t* table = P.T.table + r.seq * P.T.table_stride;
-  const int32_t* to = P.to + static_cast<int64_t>(i) * P.T.max_blocks;
-  uint8_t* pool = P.pool + layer * P.layer_stride + h * static_cast<int64_t>(L.bytes);
-  auto record = [&](const int32_t* pages, int tok) -> uint8_t* {
-    const int p = pages[tok / kBlockTokens];
-    return p >= 0 && p < P.T.n_pages ? pool + p * P.page_bytes : nullptr;
-  };
-  for (int j0 = r.start * kBlockTokens; j0 < r.left; j0 += kMoveTokens) {
-    uint4 c[PIECES];
-    uint32_t z[PW];
-    // thread t: piece t % CH of token t / CH and every (kMoveThreads / CH)-th on
+  const bool is_v = blockIdx.x & 1;
+  uint8_t* pool = P.pool + layer * P.layer_stride + (blockIdx.x >> 1) * static_cast<int64_t>(L.bytes);
+  uint8_t* codes = pool + (is_v ? L.vc : L.kc);
+  uint8_t* pairs = pool + (is_v ? L.vp : L.kp);
+  // where the tokens of a step come from and go to; page -1: nowhere
+  auto places = [&](int j0, int buf) {
 #pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
-      const int v = k >= PIECES / 2, x = (v ? k - PIECES / 2 : k) * kMoveThreads + t;
-      const int j = j0 + x / CH;
+    for (int k = 0; k < PER; ++k) {
+      const int x = k * NT + t, j = j0 + x;
+      if (x >= TOK) break;
+      int2 from = make_int2(-1, 0);
       if (j < r.left) {
-        const int src = kept[j];
-        const uint8_t* rec = record(table, src);
-        if (rec) c[k] = *reinterpret_cast<const uint4*>(rec + (v ? L.vc : L.kc) + src % kBlockTokens * (D / 2) + x % CH * 16);
+        const int src = kept[j], p = table[src / kBlockTokens];
+        if (p >= 0 && p < P.T.n_pages) from = make_int2(p, src % kBlockTokens);
         else set_status(P.status, AKV_ERR_SHAPE);
       }
+      s_from[buf][x] = from;
+    }
+    if (t < TOK / kBlockTokens) {
+      const int b = j0 / kBlockTokens + t;
+      s_to[buf][t] = b < r.end ? new_page(P, r, i, b) : -1;
+    }
+  };
+  places(first, 0);
+  int buf = 0;
+  for (int j0 = first; j0 < r.left; j0 += TOK, buf ^= 1) {
+    __syncthreads();  // the places stand; the last step's writes are behind its reads
+    uint4 c[kMovePieces];
+    Pairs z[PER];
+#pragma unroll
+    for (int k = 0; k < kMovePieces; ++k) {
+      const int x = k * NT + t;
+      const int2 from = s_from[buf][x / CH];
+      if (from.x >= 0) c[k] = *reinterpret_cast<const uint4*>(codes + from.x * P.page_bytes + from.y * (D / 2) + x % CH * 16);
     }
 #pragma unroll
-    for (int k = 0; k < PW; ++k) {
-      const int x = k * kMoveThreads + t, v = x >= PAIRS / 2, y = v ? x - PAIRS / 2 : x;
-      const int j = j0 + y / G;
-      if (x < PAIRS && j < r.left) {
-        const int src = kept[j];
-        const uint8_t* rec = record(table, src);
-        if (rec) z[k] = *reinterpret_cast<const uint32_t*>(rec + (v ? L.vp : L.kp) + (src % kBlockTokens * G + y % G) * 4);
-      }
+    for (int k = 0; k < PER; ++k) {
+      const int x = k * NT + t;
+      if (x >= TOK) break;
+      const int2 from = s_from[buf][x];
+      if (from.x >= 0) z[k] = *reinterpret_cast<const Pairs*>(pairs + from.x * P.page_bytes + from.y * (G * 4));
     }
+    if (j0 + TOK < r.left) places(j0 + TOK, buf ^ 1);
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
-      const int v = k >= PIECES / 2, x = (v ? k - PIECES / 2 : k) * kMoveThreads + t;
-      const int j = j0 + x / CH;
-      if (j < r.left) {
-        uint8_t* rec = record(to, j);
-        if (rec && record(table, kept[j]))
-          *reinterpret_cast<uint4*>(rec + (v ? L.vc : L.kc) + j % kBlockTokens * (D / 2) + x % CH * 16) = c[k];
-      }
+    for (int k = 0; k < kMovePieces; ++k) {
+      const int x = k * NT + t, y = x / CH, p = s_to[buf][y / kBlockTokens];
+      if (p >= 0 && s_from[buf][y].x >= 0)
+        *reinterpret_cast<uint4*>(codes + p * P.page_bytes + y % kBlockTokens * (D / 2) + x % CH * 16) = c[k];
     }
 #pragma unroll
-    for (int k = 0; k < PW; ++k) {
-      const int x = k * kMoveThreads + t, v = x >= PAIRS / 2, y = v ? x - PAIRS / 2 : x;
-      const int j = j0 + y / G;
-      if (x < PAIRS && j < r.left) {
-        uint8_t* rec = record(to, j);
-        if (rec && record(table, kept[j]))
-          *reinterpret_cast<uint32_t*>(rec + (v ? L.vp : L.kp) + (j % kBlockTokens * G + y % G) * 4) = z[k];
-      }
+    for (int k = 0; k < PER; ++k) {
+      const int x = k * NT + t;
+      if (x >= TOK) break;
+      const int p = s_to[buf][x / kBlockTokens];
+      if (p >= 0 && s_from[buf][x].x >= 0)
+        *reinterpret_cast<Pairs*>(pairs + p * P.page_bytes + x % kBlockTokens * (G * 4)) = z[k];
     }
   }
 }
@@ -363,11 +387,15 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
 __global__ void __launch_bounds__(256) evict_finish_kernel(const EvictParams P) {
   const int i = blockIdx.x, t = threadIdx.x;
   const EvictRow r = P.info[i];
-  if (r.seq < 0 || r.left == r.len) return;
+  if (r.seq < 0) {
+    for (int j = t; j < P.keep; j += 256) P.kept[static_cast<int64_t>(i) * P.keep + j] = -1;
+    return;
+  }
+  if (r.left == r.len) return;
   int32_t* table = P.T.table + r.seq * P.T.table_stride;
   const int pages = (r.len + kBlockTokens - 1) / kBlockTokens;
   for (int b = r.start + t; b < pages; b += 256) {
-    const int old = table[b], now = b < r.end ? P.to[static_cast<int64_t>(i) * P.T.max_blocks + b] : -1;
+    const int old = table[b], now = b < r.end ? new_page(P, r, i, b) : -1;
     if (old == now) continue;
     table[b] = now;
     if (old < 0 || old >= P.T.n_pages) {
@@ -410,13 +438,13 @@ __global__ void __launch_bounds__(128) weights_fork_kernel(float* weights, int64
 
 static int evict_launched() { return cudaGetLastError() == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH; }
 
-template <int D>
+template <int D, int NT>
 static void launch_move(const EvictParams& P, cudaStream_t st) {
-  const dim3 grid(P.kv_heads + 1, P.n_layers, P.n);
+  const dim3 grid(2 * P.kv_heads + 1, P.n_layers, P.n);
   switch (P.n_groups) {
-    case 1: evict_move_kernel<D, 1><<<grid, kMoveThreads, 0, st>>>(P); break;
-    case 2: evict_move_kernel<D, 2><<<grid, kMoveThreads, 0, st>>>(P); break;
-    default: evict_move_kernel<D, 4><<<grid, kMoveThreads, 0, st>>>(P); break;
+    case 1: evict_move_kernel<D, 1, NT><<<grid, NT, 0, st>>>(P); break;
+    case 2: evict_move_kernel<D, 2, NT><<<grid, NT, 0, st>>>(P); break;
+    default: evict_move_kernel<D, 4, NT><<<grid, NT, 0, st>>>(P); break;
   }
 }
 
@@ -498,11 +526,12 @@ extern "C" int akv_int4_evict(const akv_int4_evict_args* a, void* stream) {
   evict_score_kernel<<<dim3(most < 256 ? most : 256, a->n), 256, 0, st>>>(p);
   evict_select_kernel<<<a->n, kSelectThreads, 0, st>>>(p);
   evict_plan_kernel<<<1, kSelectThreads, 0, st>>>(p);
-  evict_target_kernel<<<a->n, kSelectThreads, 0, st>>>(p);
+  // few blocks: more threads each, so that a block's steps, one after the other, are fewer
+  const bool few = static_cast<int64_t>(a->n) * a->n_layers * a->kv_heads * 2 <= 148 * 2;
   switch (a->head_dim) {
-    case 64: launch_move<64>(p, st); break;
-    case 128: launch_move<128>(p, st); break;
-    default: launch_move<256>(p, st); break;
+    case 64: few ? launch_move<64, 1024>(p, st) : launch_move<64, 256>(p, st); break;
+    case 128: few ? launch_move<128, 1024>(p, st) : launch_move<128, 256>(p, st); break;
+    default: few ? launch_move<256, 1024>(p, st) : launch_move<256, 256>(p, st); break;
   }
   evict_finish_kernel<<<a->n, 256, 0, st>>>(p);
   return evict_launched();
