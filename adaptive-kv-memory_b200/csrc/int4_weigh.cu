@@ -5,9 +5,12 @@
 // with the log-sum-exp that attention returned, so each query's weights sum to
 // 1 and nothing has to be normalised in a second pass.  Only the K half of the
 // records is read.  With K_t = c s_tg + z_tg in channel group g,
-//   q.K_t = sum_g s_tg (q_g . (c_tg - 8)) + (z_tg + 8 s_tg) sum(q_g)
-// the contraction runs on codes, exact in fp16, and its accumulators, scales
-// and sums are fp32: the only rounding before the exponential is fp32's.
+//   q.K_t = sum_g s_tg (q_g . c_tg) + z_tg sum(q_g)
+// the contraction runs on codes, and its accumulators, scales and sums are fp32:
+// the only rounding before the exponential is fp32's.  A code's four bits, masked
+// where they lie in a 16-bit word, are an fp16 subnormal, c 2^-24 in bits 0..3 and
+// 16 c 2^-24 in bits 4..7, which the MMA multiplies exactly: one AND makes two
+// operands.  The 16 is taken out of those channels' queries, the 2^24 goes into s.
 // (Queries enter fp16 scaled per row by a power of two, exact unless 2^-24 of
 // the row's largest.)
 //
@@ -17,7 +20,8 @@
 // Few queries: the pages of all rows form one list that is cut into equal
 // shares, one per resident CTA, from the lengths on the device.  A warp takes
 // every fourth page of its share and streams the page's heads through its own
-// ring of bulk copies; tokens are the MMA's rows, queries its columns.  The
+// ring of asynchronous copies (of threads: a bulk copy's barrier and issue cost a
+// record of 2 KB more than its arithmetic); tokens are the MMA's rows, queries its columns.  The
 // queries of up to kWeighUnits (head, 8 or 16 columns) units stand in shared
 // memory as MMA fragments; more of them take the pages again.
 #include <type_traits>
@@ -47,27 +51,12 @@ struct WeighShape {
   static constexpr int OFF_CQ = OFF_QS + kWeighUnits * ROWS * G * 4;
   static constexpr int OFF_L2 = OFF_CQ + kWeighUnits * ROWS * 4;
   static constexpr int OFF_SEE = OFF_L2 + kWeighUnits * ROWS * 4;
-  static constexpr int OFF_BAR = OFF_SEE + kWeighUnits * ROWS * 4;
-  static constexpr int OFF_PREF = OFF_BAR + kWeighWarps * STAGES * 8;
+  static constexpr int OFF_PREF = OFF_SEE + kWeighUnits * ROWS * 4;
   static constexpr int smem(int rows) { return OFF_PREF + (3 * rows + 1) * 4; }
 };
 
 // token of tile row g: see the attention kernel's bank note
 AKV_DEV int weigh_token(int g) { return g ^ ((g >> 2) & 1); }
-
-// the codes in bits 0..3 (4..7) of both halves, as the fp16 pair c - 8
-AKV_DEV uint32_t code8_low(uint32_t w) {
-  uint32_t r;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(lop_magic<0x000F000Fu>(w)), "r"(0xE408E408u));  // - 1032
-  return r;
-}
-AKV_DEV uint32_t code8_high(uint32_t w) {
-  uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;"  // (1024 + 16 c) / 16 - 72
-      : "=r"(r)
-      : "r"(lop_magic<0x00F000F0u>(w)), "r"(0x2C002C00u), "r"(0xD480D480u));
-  return r;
-}
 
 template <int BYTES>
 AKV_DEV void weigh_lds(const uint8_t* p, uint32_t (&w)[BYTES < 4 ? 1 : BYTES / 4]) {
@@ -128,7 +117,6 @@ __global__ void __launch_bounds__(kWeighThreads, D == 256 ? 2 : 3) weigh_few_ker
   float* s_cq = reinterpret_cast<float*>(smem + S::OFF_CQ);
   float* s_l2 = reinterpret_cast<float*>(smem + S::OFF_L2);
   int* s_see = reinterpret_cast<int*>(smem + S::OFF_SEE);
-  uint64_t* s_bar = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
   int* s_pref = reinterpret_cast<int*>(smem + S::OFF_PREF);
   int* s_len = s_pref + P.R + 1;
   int* s_new = s_len + P.R;
@@ -138,8 +126,6 @@ __global__ void __launch_bounds__(kWeighThreads, D == 256 ? 2 : 3) weigh_few_ker
   const int g = lane >> 2, q4 = lane & 3;
   const int H = P.c.kv_heads, rep = P.Hq / H;
 
-  if (lane < S::STAGES) mbar_init(s_bar + warp * S::STAGES + lane, 1);
-  fence_mbar_init();
   weigh_rows(P, s_pref, s_len, s_new, s_scan);
 
   const int total = s_pref[P.R];
@@ -153,9 +139,7 @@ __global__ void __launch_bounds__(kWeighThreads, D == 256 ? 2 : 3) weigh_few_ker
   }
 
   uint8_t* ring = smem + warp * S::STAGES * S::REC;
-  uint64_t* bars = s_bar + warp * S::STAGES;
-  uint32_t stage = 0, phase = 0;
-  bool alive = true;
+  uint32_t stage = 0;
 
   while (pos < end) {
     while (s_pref[e + 1] <= pos) ++e;
@@ -171,107 +155,122 @@ __global__ void __launch_bounds__(kWeighThreads, D == 256 ? 2 : 3) weigh_few_ker
     for (int u0 = 0; u0 < units; u0 += kWeighUnits) {
       const int u1 = min(units, u0 + kWeighUnits);
       const int h0 = u0 / tiles, heads = (u1 - 1) / tiles - h0 + 1;
-      const int items = mine * heads;  // (page, head) records of this warp
 
-      // a page's number, checked; pages are looked up one ahead of their copies
-      auto page_of = [&](int k) -> int {
-        if (k >= mine) return -1;
-        const int p = __ldg(table + warp + k * kWeighWarps);
+      // a page's number, read one page ahead of its copies, checked when they start
+      auto look = [&](int k) -> int { return k < mine ? __ldg(table + warp + k * kWeighWarps) : 0; };
+      auto check = [&](int p) -> int {
         if (p >= 0 && p < P.c.n_pages) return p;
         set_status(P.status, AKV_ERR_SHAPE);
-        return -1;
+        return 0;  // a bad page is read as page 0; nothing of it is added
       };
-      int next_k = 0, next_h = 0, next_p = page_of(0);  // the next record to copy
+      int next_k = 0, next_h = 0, next_p = check(look(0)), ahead = look(1);  // the next record to copy
       auto issue = [&](uint32_t st) {
         if (next_k < mine) {
-          if (lane == 0) {
-            // a bad page is read as page 0; nothing of it is added
-            const uint8_t* rec = P.c.pool + (next_p < 0 ? 0 : next_p) * P.c.page_stride + (h0 + next_h) * P.c.head_stride;
-            mbar_arrive_expect_tx(bars + st, S::REC);
-            tma_load_1d(ring + st * S::REC, rec + int4_layout(D, G).kc, S::CODES, bars + st);
-            tma_load_1d(ring + st * S::REC + S::CODES, rec + int4_layout(D, G).kp, S::PAIRS, bars + st);
-          }
+          const uint8_t* rec = P.c.pool + next_p * P.c.page_stride + (h0 + next_h) * P.c.head_stride;
+          uint8_t* to = ring + st * S::REC;
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k)
+            cp_async16(to + (k * 32 + lane) * 16, rec + int4_layout(D, G).kc + (k * 32 + lane) * 16);
+          if (lane < G * 8) cp_async16(to + S::CODES + lane * 16, rec + int4_layout(D, G).kp + lane * 16);
           if (++next_h == heads) {
             next_h = 0;
-            next_p = page_of(++next_k);
+            next_p = check(ahead);
+            ahead = look(++next_k + 1);
           }
         }
+        cp_async_commit();
       };
-#pragma unroll
-      for (int k = 0; k < S::STAGES; ++k)
-        if (alive) issue((stage + k) % S::STAGES);
+      for (int k = 0; k < S::STAGES; ++k) issue((stage + k) % S::STAGES);
 
       // ---- queries of the units as MMA operands
       __syncthreads();  // the previous units' are done with
       constexpr int PER = D / 32;
-      for (int n = warp; n < (u1 - u0) * S::ROWS; n += kWeighWarps) {
-        const int unit = n / S::ROWS, col = n % S::ROWS;
-        const int h = (u0 + unit) / tiles, rr = (u0 + unit) % tiles * S::ROWS + col, m = rr / rep;
+      static_assert(kWeighUnits * S::ROWS <= 32 * kWeighWarps, "a lane a column");
+      const int columns = (u1 - u0) * S::ROWS;
+      int64_t where = -1;  // lane c: the warp's c-th column's query
+      {
+        const int n = warp + lane * kWeighWarps, unit = n / S::ROWS;
+        const int h = (u0 + unit) / tiles, rr = (u0 + unit) % tiles * S::ROWS + n % S::ROWS, m = rr / rep;
         const int hq = h * rep + rr - m * rep;
-        const bool on = m < n_new;
-        const uint16_t* src = P.q + i * P.q_sr + hq * P.q_sh + m * P.q_sm + lane * PER;
-        float x[PER];
-        uint32_t top = 0u;
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-          const uint16_t raw = on ? src[k] : 0;
-          x[k] = P.bf16 ? elem_to_float<true>(raw) : elem_to_float<false>(raw);
-          top = max(top, __float_as_uint(x[k]) & 0x7FFFFFFFu);
-        }
-        top = __reduce_max_sync(~0u, top);
-        const bool bad = top >= 0x7F800000u;
-        int ex = 0;  // 2^ex brings the largest into [2^9, 2^10)
-        if (top && !bad) ex = 9 - (static_cast<int>(top >> 23) - 127);
-        ex = ex > 120 ? 120 : (ex < -120 ? -120 : ex);
-        const float up = exp2f(static_cast<float>(ex));
-        uint16_t* frag = reinterpret_cast<uint16_t*>(smem + S::OFF_FRAG + unit * S::FRAG);
-        float sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-          const int c = lane * PER + k;
-          const __half hv = __float2half_rn(bad ? 0.f : x[k] * up);
-          sum += __half2float(hv);
-          const int gi = c / S::GS, r = c % S::GS, cc = r / (S::GS / 4), r2 = r % (S::GS / 4);
-          int ks, half;
-          if constexpr (S::BK >= 4) {
-            ks = gi * (S::GS / 16) + (r2 / 8) * 2 + ((r2 >> 1) & 1);
-            half = (r2 >> 2) & 1;
-          } else {
-            ks = gi;
-            half = r2 >> 1;
+        if (n < columns) {
+          float lse = -INFINITY;
+          if (m < n_new) {
+            where = i * P.q_sr + hq * P.q_sh + m * P.q_sm;
+            lse = __ldg(P.lse + (static_cast<int64_t>(i) * P.Hq + hq) * P.M + m);
           }
-          const int reg = c & 1 ? 0 : 1;
-          frag[(((ks * NT + col / 8) * 32 + (col % 8) * 4 + cc) * 2 + reg) * 2 + half] = __half_as_ushort(hv);
+          const bool counts = fabsf(lse) < INFINITY;
+          s_l2[n] = counts ? -lse * 1.4426950408889634f : -INFINITY;
+          s_see[n] = counts ? len - n_new + m + 1 : 0;
         }
-        constexpr int GL = 32 / G;  // lanes of a group
+      }
+      __syncwarp();
+      constexpr int BATCH = 4;  // columns whose loads fly together
+      for (int n0 = 0; warp + n0 * kWeighWarps < columns; n0 += BATCH) {
+        uint16_t raw[BATCH][PER];
 #pragma unroll
-        for (int o = 1; o < GL; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        if (lane % GL == 0) s_qs[(unit * G + lane / GL) * S::ROWS + col] = sum;
-        if (lane == 0) {
-          const float lse = on ? __ldg(P.lse + (static_cast<int64_t>(i) * P.Hq + hq) * P.M + m) : -INFINITY;
-          const bool counts = on && !bad && fabsf(lse) < INFINITY;
-          s_cq[unit * S::ROWS + col] = ldexpf(P.scale * 1.4426950408889634f, -ex);
-          s_l2[unit * S::ROWS + col] = counts ? -lse * 1.4426950408889634f : -INFINITY;
-          s_see[unit * S::ROWS + col] = counts ? len - n_new + m + 1 : 0;
+        for (int b = 0; b < BATCH; ++b) {
+          const int64_t at = __shfl_sync(~0u, where, n0 + b);
+#pragma unroll
+          for (int k = 0; k < PER; ++k) raw[b][k] = at >= 0 ? P.q[at + lane * PER + k] : 0;
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+          const int n = warp + (n0 + b) * kWeighWarps, unit = n / S::ROWS, col = n % S::ROWS;
+          if (n >= columns) break;
+          float x[PER];
+          uint32_t top = 0u;
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            x[k] = P.bf16 ? elem_to_float<true>(raw[b][k]) : elem_to_float<false>(raw[b][k]);
+            top = max(top, __float_as_uint(x[k]) & 0x7FFFFFFFu);
+          }
+          top = __reduce_max_sync(~0u, top);
+          const bool bad = top >= 0x7F800000u;
+          int ex = 0;  // 2^ex brings the largest into [2^13, 2^14)
+          if (top && !bad) ex = 13 - (static_cast<int>(top >> 23) - 127);
+          ex = ex > 120 ? 120 : (ex < -120 ? -120 : ex);
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+          uint16_t* frag = reinterpret_cast<uint16_t*>(smem + S::OFF_FRAG + unit * S::FRAG);
+          float sum = 0.f;
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            const int c = lane * PER + k;
+            const float part = k & 1 ? 1.f : 16.f;  // even channels' codes are the high four bits
+            const __half hv = __float2half_rn(bad ? 0.f : x[k] * up / part);
+            sum += __half2float(hv) * part;
+            const int gi = c / S::GS, r = c % S::GS, cc = r / (S::GS / 4), r2 = r % (S::GS / 4);
+            int ks, half;
+            if constexpr (S::BK >= 4) {
+              ks = gi * (S::GS / 16) + (r2 / 8) * 2 + ((r2 >> 1) & 1);
+              half = (r2 >> 2) & 1;
+            } else {
+              ks = gi;
+              half = r2 >> 1;
+            }
+            const int reg = c & 1 ? 0 : 1;
+            frag[(((ks * NT + col / 8) * 32 + (col % 8) * 4 + cc) * 2 + reg) * 2 + half] = __half_as_ushort(hv);
+          }
+          constexpr int GL = 32 / G;  // lanes of a group
+#pragma unroll
+          for (int o = 1; o < GL; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
+          if (lane % GL == 0) s_qs[(unit * G + lane / GL) * S::ROWS + col] = sum;
+          if (lane == 0) {
+            s_cq[n] = P.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+            if (bad) s_l2[n] = -INFINITY, s_see[n] = 0;
+          }
         }
       }
       __syncthreads();
 
       // ---- this warp's pages: all heads of the units, then the next page
-      for (int k = 0, item = 0; k < mine && alive; ++k) {
+      for (int k = 0; k < mine; ++k) {
         const int tok0 = (page0 + warp + k * kWeighWarps) * kBlockTokens;
-        const int p = __ldg(table + warp + k * kWeighWarps);
+        const int p = __ldg(table + warp + k * kWeighWarps), tok = tok0 + q4 * 8 + weigh_token(g);
+        const float old = tok < len ? w_row[tok] : 0.f;
         float w[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int hh = 0; hh < heads; ++hh, ++item) {
-          if (!__all_sync(~0u, mbar_wait(bars + stage, phase, P.status))) {
-            // a copy never came: take no more, but see the ones in flight land
-            for (int r = 1; r < S::STAGES && item + r < items; ++r) {
-              const uint32_t st = stage + r;
-              mbar_wait(bars + st % S::STAGES, st >= S::STAGES ? phase ^ 1 : phase, P.status);
-            }
-            alive = false;
-            break;
-          }
+        for (int hh = 0; hh < heads; ++hh) {
+          cp_async_wait<S::STAGES - 1>();
+          __syncwarp();
           const uint8_t* rec = ring + stage * S::REC;
           uint32_t kp[4][G];
 #pragma unroll
@@ -311,8 +310,8 @@ __global__ void __launch_bounds__(kWeighThreads, D == 256 ? 2 : 3) weigh_few_ker
                     uint32_t v;
                     if constexpr (S::BK >= 4) v = s & 1 ? kw[2 * mt + r][s / 2] >> 8 : kw[2 * mt + r][s / 2];
                     else v = prmt(kw[2 * mt + r][0], 0u, 0x4140);
-                    a[r] = code8_low(v);
-                    a[2 + r] = code8_high(v);
+                    a[r] = v & 0x000F000Fu;
+                    a[2 + r] = v & 0x00F000F0u;
                   }
 #pragma unroll
                   for (int nt = 0; nt < NT; ++nt) mma_16816(acc[mt][nt], a[0], a[1], a[2], a[3], b[nt].x, b[nt].y);
@@ -321,8 +320,8 @@ __global__ void __launch_bounds__(kWeighThreads, D == 256 ? 2 : 3) weigh_few_ker
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 const float2 sz = __half22float2(u32_as_h2(kp[r][gi]));
-                const float mid = fmaf(8.f, sz.x, sz.y);
-                const uint64_t s2 = f2_make(sz.x, sz.x), z2 = f2_make(mid, mid);
+                const float up = sz.x * 16777216.f;
+                const uint64_t s2 = f2_make(up, up), z2 = f2_make(sz.y, sz.y);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                   const uint64_t q2 = qs2[(gi * S::ROWS + nt * 8) / 2];
@@ -351,17 +350,15 @@ __global__ void __launch_bounds__(kWeighThreads, D == 256 ? 2 : 3) weigh_few_ker
             }
           }
           __syncwarp();
-          if (++stage == S::STAGES) stage = 0, phase ^= 1;
-          issue((stage + S::STAGES - 1) % S::STAGES);
+          issue(stage);
+          if (++stage == S::STAGES) stage = 0;
         }
-        if (!alive) break;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          w[r] += __shfl_xor_sync(~0u, w[r], 1);
-          w[r] += __shfl_xor_sync(~0u, w[r], 2);
-        }
-        const int tok = tok0 + q4 * 8 + weigh_token(g);
-        if (tok < len && p >= 0 && p < P.c.n_pages) w_row[tok] += q4 < 2 ? (q4 == 0 ? w[0] : w[1]) : (q4 == 2 ? w[2] : w[3]);
+        // lane q4 keeps row q4's sum
+        const bool odd = q4 & 1, high = q4 & 2;
+        const float a = (odd ? w[1] : w[0]) + __shfl_xor_sync(~0u, odd ? w[0] : w[1], 1);
+        const float b = (odd ? w[3] : w[2]) + __shfl_xor_sync(~0u, odd ? w[2] : w[3], 1);
+        const float sum = (high ? b : a) + __shfl_xor_sync(~0u, high ? a : b, 2);
+        if (tok < len && p >= 0 && p < P.c.n_pages) w_row[tok] = old + sum;
       }
     }
     pos += n_pages;
