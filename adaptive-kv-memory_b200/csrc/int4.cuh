@@ -9,6 +9,13 @@
 
 namespace akv {
 
+AKV_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all but this thread's newest N groups have landed
+template <int N>
+AKV_DEV void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Byte offsets of one (page, KV head) record; akv_int4_layout_init and the
 // kernels' compile-time offsets both come from here.
 struct Int4Layout {

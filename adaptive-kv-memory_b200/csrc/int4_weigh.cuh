@@ -5,13 +5,6 @@
 
 namespace akv {
 
-AKV_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// all but this thread's newest N groups have landed
-template <int N>
-AKV_DEV void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 constexpr int kWeighRows = 1024;   // call rows of one launch
 
 struct WeighParams {

@@ -15,7 +15,7 @@
 // ties, so the result depends on the inputs alone.  The lanes' maxima of the
 // first batch, sorted, start the list; from then on a batch of up to 32 elements
 // a lane is looked through only if its maximum reaches the k-th key, and of it the
-// elements that do, a bit each, are read again and inserted.  The lists of warps
+// elements that do, a bit each, are inserted.  The lists of warps
 // and CTAs are merged pairwise (maximum of one and the other reversed is the
 // bitonic top half).
 //
@@ -31,7 +31,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kLogpThreads = 256;
 constexpr int kLogpWarps = kLogpThreads / 32;
-constexpr int kLogpVecs = 4;         // 16-byte loads of a thread in flight
+constexpr int kLogpVecs = 4;         // 16-byte pieces of a thread's batch
+constexpr int kLogpStages = 3;       // batches of the ring
 constexpr int kLogpMaxTop = 32;
 constexpr int kLogpMaxCluster = 8;
 constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -250,12 +251,31 @@ __global__ void __launch_bounds__(kLogpThreads, 4) token_logprobs_kernel(const L
     }
   };
 
+  // a thread copies what it reads itself, two batches ahead: nobody waits for anybody
+  extern __shared__ uint4 ring[];  // [stage][piece][thread]
+  int ahead = v0, into = 0;
+  auto fetch = [&] {
+#pragma unroll
+    for (int j = 0; j < kLogpVecs; ++j) {
+      const int at = ahead + j * kLogpThreads + t;
+      if (at < v1) cp_async16(ring + (into * kLogpVecs + j) * kLogpThreads + t, xv + at);
+    }
+    cp_async_commit();
+    ahead += kLogpVecs * kLogpThreads;
+    into = into + 1 == kLogpStages ? 0 : into + 1;
+  };
+  for (int k = 1; k < kLogpStages; ++k) fetch();
+  int stage = 0;
   for (int v = v0; v < v1; v += kLogpVecs * kLogpThreads) {
+    fetch();
+    cp_async_wait<kLogpStages - 1>();
+    const uint4* mine4 = ring + stage * kLogpVecs * kLogpThreads + t;
+    stage = stage + 1 == kLogpStages ? 0 : stage + 1;
     uint32_t w[W];
 #pragma unroll
     for (int j = 0; j < kLogpVecs; ++j) {
       const int at = v + j * kLogpThreads + t;
-      const uint4 q = at < v1 ? ldg_nc_v4(xv + at) : make_uint4(E::kNone, E::kNone, E::kNone, E::kNone);
+      const uint4 q = at < v1 ? mine4[j * kLogpThreads] : make_uint4(E::kNone, E::kNone, E::kNone, E::kNone);
       w[4 * j] = q.x, w[4 * j + 1] = q.y, w[4 * j + 2] = q.z, w[4 * j + 3] = q.w;
     }
     uint32_t top = w[0], low = w[0];
@@ -312,7 +332,8 @@ __global__ void __launch_bounds__(kLogpThreads, 4) token_logprobs_kernel(const L
       auto key_of = [&](int bit) -> uint64_t {
         const int i = bit / PER;
         const int c = head + (v + (i / 4) * kLogpThreads + t) * E::N + (i % 4) * PER + bit % PER;
-        return logit_key(E::get(__ldg(x0 + c)), c);
+        const T x = reinterpret_cast<const T*>(mine4 + (i / 4) * kLogpThreads)[(i % 4) * PER + bit % PER];
+        return logit_key(E::get(x), c);
       };
       uint32_t done = 0u;
       if (v == v0) {
@@ -419,6 +440,9 @@ __global__ void __launch_bounds__(kLogpThreads, 4) token_logprobs_kernel(const L
 
 template <int DT, bool TOP>
 static int launch_logprobs(const LogpParams& p, int n, int cluster, cudaStream_t st) {
+  constexpr int smem = kLogpStages * kLogpVecs * kLogpThreads * 16;
+  // with the static arrays on top it is past the 48 KB that need no asking
+  if (!ensure_dynamic_smem<token_logprobs_kernel<DT, TOP>>(smem + 1024)) return AKV_ERR_LAUNCH;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = cluster;
@@ -426,6 +450,7 @@ static int launch_logprobs(const LogpParams& p, int n, int cluster, cudaStream_t
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(n) * cluster);
   cfg.blockDim = dim3(kLogpThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = at;
   cfg.numAttrs = 1;
