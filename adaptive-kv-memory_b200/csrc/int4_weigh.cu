@@ -395,9 +395,17 @@ static int weigh_few(const WeighParams& P, cudaStream_t st) {
   }
 }
 
-// From this many query columns (new tokens x query heads of a group) on the
-// tensor-memory kernel takes the call.
-constexpr int kWeighMany = 64;
+// Query columns (new tokens x query heads of a group) that still go to the kernel
+// above; more go to the tensor-memory kernel, whose tiles of 128 / n_groups
+// columns cost the same half empty.  Measured, us, this one : that one, for
+// 1 row x 4,096 tokens, 32 / 8 heads | 16 x 8,192, 32 / 8 | 4 x 16,384, 16 / 2:
+//   one group    16 columns  20 : 21 |  53 : 98 | 16 : 28
+//                32          32 : 20 |  89 : 99 | 23 : 29
+//                64          56 : 21 | 163 : 99 | 36 : 30
+//   four groups  16          22 : 21 |  84 : 81 | 24 : 27
+//                32          34 : 20 | 136 : 81 | 34 : 27
+//                64          59 : 21 | 247 : 109 | 54 : 31
+static int weigh_few_columns(int n_groups) { return n_groups == 1 ? 32 : 16; }
 
 }  // namespace akv
 
@@ -405,7 +413,7 @@ using namespace akv;
 
 extern "C" size_t akv_int4_weigh_workspace_bytes(int R, int M, int Hq, int kv_heads, int head_dim, int group) {
   if (R < 0 || M < 0 || Hq <= 0 || kv_heads <= 0 || Hq % kv_heads || !int4_shape_ok(head_dim, group)) return 0;
-  if (R == 0 || static_cast<int64_t>(M) * (Hq / kv_heads) < kWeighMany) return 16;
+  if (R == 0 || static_cast<int64_t>(M) * (Hq / kv_heads) <= weigh_few_columns(head_dim / group)) return 16;
   if (static_cast<int64_t>(M) * Hq > INT32_MAX / 2) return 0;
   return weigh_many_workspace(R, M, Hq, kv_heads, head_dim, head_dim / group);
 }
@@ -425,7 +433,7 @@ extern "C" int akv_int4_weigh(const akv_int4_weigh_args* a, void* stream) {
     return AKV_ERR_ALIGN;
   // columns and pages of a launch are counted in 32 bits
   if (static_cast<int64_t>(a->M) * a->Hq > INT32_MAX / 2) return AKV_ERR_UNSUPPORTED;
-  const bool many = a->M * (a->Hq / c->kv_heads) >= kWeighMany;
+  const bool many = a->M * (a->Hq / c->kv_heads) > weigh_few_columns(c->head_dim / c->group);
   if (many) {
     if (!a->workspace) return AKV_ERR_NULL;
     if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return AKV_ERR_ALIGN;

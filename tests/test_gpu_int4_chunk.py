@@ -341,3 +341,41 @@ def test_refusals():
         with pytest.raises(err):
             call()
     assert c.attend_chunk(0, q[:0]).shape == (0, 4, 30, 128) and c.attend_chunk(0, q[:, :, :0]).shape == (2, 4, 0, 128)
+
+
+@pytest.mark.parametrize("R,heads,rep,M", [(1100, 1, 1, 3), (700, 8, 1, 2)])
+def test_more_rows_than_a_launch_lists(R, heads, rep, M):
+    c = _cache(pages=R, heads=heads, dim=64, group=64, seqs=R, blocks=2)
+    lens = [3 + i % 30 for i in range(R)]
+    _fill(c, lens, seed=R)
+    q = _query((R, heads * rep, M, 64), 3, torch.float16)
+    out, lse = c.attend_chunk(0, q, return_lse=True)
+    c.check()
+    for i in (0, 511, 512, 513, 699, R - 1):
+        r = torch.tensor([i], dtype=torch.int32, device=DEV)
+        one, one_lse = c.attend_chunk(0, q[i:i + 1], r, return_lse=True)
+        _check(c, q[i:i + 1], out[i:i + 1], lse[i:i + 1], [i], [M])
+        assert torch.equal(one[0], out[i]) and torch.equal(one_lse[0], lse[i])
+
+
+def test_long_chunk():
+    """20,001 new tokens: a few of their queries against the formula."""
+    n = 20001
+    c = _cache(pages=640, heads=1, dim=64, group=64, seqs=1, blocks=640)
+    _fill(c, [n], seed=5)
+    q = _query((1, 2, n, 64), 6, torch.bfloat16)
+    out, lse = c.attend_chunk(0, q, return_lse=True)
+    c.check()
+    for m in (0, 1, 127, 128, 9999, n - 2, n - 1):
+        c.lens[0] = m + 1  # the query as the last of a row that ends with it
+        _check(c, q[:, :, m:m + 1], out[:, :, m:m + 1], lse[:, :, m:m + 1], [0], [1])
+
+
+def test_nothing_to_do():
+    c = _cache(pages=8, blocks=4)
+    _fill(c, [40, 5], seed=1)
+    for shape in ((0, 4, 5, 128), (2, 4, 0, 128)):
+        out, lse = c.attend_chunk(0, _query(shape, 1, torch.float16), torch.arange(shape[0], dtype=torch.int32, device=DEV),
+                                  return_lse=True)
+        assert out.shape == shape and lse.shape == shape[:3]
+    c.check()

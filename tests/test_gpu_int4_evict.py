@@ -313,3 +313,23 @@ def test_refusals():
             c.evict(rows, 10)
     assert c.evict(_i(), 10).shape == (0, 10)
     c.check()
+
+
+@pytest.mark.parametrize("dim,group", [(64, 64), (64, 32), (64, 16), (128, 128), (128, 64), (128, 32), (256, 256),
+                                       (256, 128), (256, 64)])
+def test_many_blocks(dim, group):
+    """Enough rows, layers and heads for the moves' smaller blocks, rows of several of their steps."""
+    c = _cache(layers=8, pages=150, heads=4, dim=dim, group=group, blocks=20)
+    _fill(c, [600, 1, 333, 640, 64, 97], seed=dim + group)
+    c.fork([3], [6])
+    c.check()
+    _run(c, [3, 0, 4, 2, 1], 300, first=3, recent=11)
+
+
+def test_no_rows():
+    c = _cache()
+    _fill(c, [100])
+    buf, table = c.buf.clone(), c.table.clone()
+    assert c.evict(torch.empty(0, dtype=torch.int32, device=DEV), 5).shape == (0, 5)
+    assert torch.equal(c.buf, buf) and torch.equal(c.table, table) and c.lens.tolist()[0] == 100
+    c.check()

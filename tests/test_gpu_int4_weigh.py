@@ -331,3 +331,46 @@ def test_refusals():
         c.weigh(0, q, lse)
     with pytest.raises(ValueError):
         c.reserve(None, 1)
+
+
+@pytest.mark.parametrize("M,group", [(2, 64), (40, 64), (40, 16)])
+def test_more_rows_than_a_launch_lists(M, group):
+    R = 1100
+    c = _cache(pages=2 * R, heads=1, dim=64, group=group, seqs=R, blocks=2)
+    lens = [M + i % 20 for i in range(R)]
+    _fill(c, lens, seed=R)
+    q = _query((R, 1, M, 64), 3, torch.float16)
+    lse = torch.randn(R, 1, M, device=DEV) + 5
+    c.weigh(0, q, lse)
+    c.check()
+    all_of_it = c.weights.clone()
+    for i in (0, 1023, 1024, R - 1):
+        w, tol = _expected(c, 0, q[i:i + 1], lse[i:i + 1], [i], [M])[i]
+        assert ((all_of_it[0, i, :lens[i]].double() - w).abs() <= tol).all()
+        assert (all_of_it[0, i, lens[i]:] == 0).all()
+
+
+def test_nothing_to_do():
+    c = _cache(pages=8, blocks=4)
+    _fill(c, [40, 5], seed=1)
+    for shape in ((0, 4, 5, 128), (2, 4, 0, 128)):
+        c.weigh(0, _query(shape, 1, torch.float16), torch.zeros(shape[:3], device=DEV),
+                torch.arange(shape[0], dtype=torch.int32, device=DEV))
+    c.check()
+    assert not c.weights.any()
+
+
+@pytest.mark.parametrize("group", [128, 64, 32])
+@pytest.mark.parametrize("columns", [15, 16, 17, 31, 32, 33, 48])
+def test_both_kernels_at_their_boundary(group, columns):
+    c = _cache(heads=2, group=group)
+    _fill(c, [200, 33, 64], seed=columns)
+    q = _query((3, 2, columns, 128), 4, torch.bfloat16)
+    new = [columns, min(33, columns), columns]
+    n = torch.tensor(new, dtype=torch.int32, device=DEV)
+    rows = torch.arange(3, dtype=torch.int32, device=DEV)
+    lse = torch.randn(3, 2, columns, device=DEV) + 6
+    before = c.weights.clone()
+    c.weigh(0, q, lse, rows, n)
+    c.check()
+    _check(c, before, _expected(c, 0, q, lse, [0, 1, 2], new))
