@@ -396,15 +396,16 @@ static int weigh_few(const WeighParams& P, cudaStream_t st) {
 }
 
 // Query columns (new tokens x query heads of a group) that still go to the kernel
-// above; more go to the tensor-memory kernel, whose tiles of 128 / n_groups
-// columns cost the same half empty.  Measured, us, this one : that one, for
-// 1 row x 4,096 tokens, 32 / 8 heads | 16 x 8,192, 32 / 8 | 4 x 16,384, 16 / 2:
-//   one group    16 columns  20 : 21 |  53 : 98 | 16 : 28
-//                32          32 : 20 |  89 : 99 | 23 : 29
-//                64          56 : 21 | 163 : 99 | 36 : 30
-//   four groups  16          22 : 21 |  84 : 81 | 24 : 27
-//                32          34 : 20 | 136 : 81 | 34 : 27
-//                64          59 : 21 | 247 : 109 | 54 : 31
+// above; more go to the fifth-generation tensor cores, whose tiles of 64 (four
+// groups) or 128 columns cost the same half empty.  Measured, us, this kernel :
+// that one, for 1 row x 4,096 tokens, 32 / 8 heads | 16 x 8,192, 32 / 8 |
+// 4 x 16,384, 16 / 2:
+//   one group    16 columns  20 : 22 |  53 : 107 | 16 : 29
+//                32          32 : 22 |  89 : 107 | 23 : 29
+//                64          56 : 22 | 163 : 107 | 36 : 29
+//   four groups  16          21 : 25 |  84 : 105 | 24 : 28
+//                32          34 : 25 | 136 : 105 | 34 : 28
+//                64          59 : 26 | 247 : 106 | 54 : 30
 static int weigh_few_columns(int n_groups) { return n_groups == 1 ? 32 : 16; }
 
 }  // namespace akv

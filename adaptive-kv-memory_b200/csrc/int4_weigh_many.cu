@@ -14,7 +14,7 @@
 // two fp32 steps a group and column, an exponential, an addition.
 //
 // A unit is one (call row, 256 tokens): a warpgroup for each 128, whose codes
-// stand in tensor memory as the MMA's A, head after head.  The units'
+// stand in shared (D = 256: tensor) memory as the MMA's A, head after head.  The units'
 // (head, query tile) pairs form one list that is cut into equal shares, one per
 // CTA, from the lengths on the device; parts of a cut unit are joined in order
 // by a third kernel.  While one warpgroup's exponentials run, the other's MMAs
@@ -29,19 +29,29 @@ constexpr int kManyTokens = 256;      // of a unit
 constexpr int kManyThreads = 256 + 64;
 constexpr float kManyLog2e = 1.4426950408889634f;
 
+// Query columns of a tile: an MMA of up to 64 columns takes as long as one of 64
+// (45 cycles; 32 columns are worth 16), so as many as the scores of all groups
+// find room for in the tensor memory, the codes moved to shared memory for it:
+// 1,000 tokens of 32 / 8 heads over 16K, groups of 32, 416 -> 357 us, of 64, 262
+// -> 229.  With D = 256 the codes in shared memory would leave no ring.
+constexpr int many_columns(int D, int G) { return D == 256 ? 128 / G : (G < 4 ? 128 : 64); }
+
 template <int D, int G>
 struct ManyShape {
-  static constexpr int N = 128 / G;              // query columns of a tile
+  static constexpr bool SS = D <= 128;           // codes in shared memory
+  static constexpr int N = many_columns(D, G);
   static constexpr int QB = N * D * 2;           // its operand
   static constexpr int META = N * (G + 1) * 4;   // per column pair: -lse, group sums
   static constexpr int REC = QB + META + 16;     // and the exponent's unit
   static constexpr int STAGES = REC > 48 * 1024 ? 3 : 4;
   static constexpr int KG = D / G / 16;          // MMA steps of a group
-  static constexpr int OFF_BAR = STAGES * REC;
+  static constexpr int AB = SS ? 128 * D * 2 : 0;  // codes of a warpgroup
+  static constexpr int OFF_A = STAGES * REC;
+  static constexpr int OFF_BAR = OFF_A + 2 * AB;
   static constexpr int OFF_ROWS = OFF_BAR + 128;
   static constexpr int smem(int rows) { return OFF_ROWS + (2 * rows + 2) * 4 + (rows + 1) * 8; }
   // tensor memory of a warpgroup: codes, then scores
-  static constexpr int T_A = 0, T_S = D / 2, T_WG = D / 2 + 128;
+  static constexpr int T_A = 0, T_S = SS ? 0 : D / 2, T_WG = T_S + G * N;
   static_assert(2 * T_WG <= 512, "tensor memory");
   static_assert(REC % 16 == 0 && smem(kWeighRows) <= 227 * 1024, "shared memory");
 };
@@ -300,6 +310,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tA = tmem + lanes + wg * S::T_WG + S::T_A, tS = tmem + lanes + wg * S::T_WG + S::T_S;
     uint32_t kw[NW], kp[G];
+    unsigned char* sA = smem + S::OFF_A + wg * S::AB + (t & 127) * 16;
     bool have = false;  // the thread's token is there, on a page
     auto fetch = [&](const ManyPart& x) {
       const int tok = x.tile * kManyTokens + t;
@@ -325,13 +336,22 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
     bool more = walk.next(u);
     if (more) fetch(u);
     while (more && ok) {
-      // ---- this head's codes into tensor memory: every S of the last part is out
+      // ---- this head's codes as the MMA's A: every S of the last part is out
+      if constexpr (S::SS) {
 #pragma unroll
-      for (int k = 0; k < NW / 8; ++k) {
-        uint32_t c[32];
+        for (int k = 0; k < NW; ++k) {
+          uint32_t c[4];
+          centred_codes(kw[k], c);
+          *reinterpret_cast<uint4*>(sA + k * (128 * 16)) = make_uint4(c[0], c[1], c[2], c[3]);
+        }
+      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) centred_codes(kw[8 * k + j], c + 4 * j);
-        tmem_st32u(tA + 32 * k, c);
+        for (int k = 0; k < NW / 8; ++k) {
+          uint32_t c[32];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) centred_codes(kw[8 * k + j], c + 4 * j);
+          tmem_st32u(tA + 32 * k, c);
+        }
       }
       float s[G], mid[G];
 #pragma unroll
@@ -341,7 +361,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
         mid[g] = fmaf(8.f, sz.x, sz.y);
       }
       const bool mine = have;
-      tmem_wait_st();
+      if constexpr (S::SS) fence_proxy_async_shared();
+      else tmem_wait_st();
       tc_fence_before();
       mbar_arrive(a_ready + wg);
       ManyPart nx;
@@ -454,7 +475,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
       return ok;
     };
     constexpr uint32_t IDESC = instr_desc(128, N, 0);
-    const uint32_t base = smem_u32(smem);
+    const uint32_t base = smem_u32(smem), codes = desc_lo(base + S::OFF_A, 128 * 16);
     int st = 0;
     uint32_t ph_q = 0, ph_a = 0, ph_s = 1;
     while (ok && walk.next(u)) {
@@ -473,7 +494,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
 #pragma unroll
             for (int k = 0; k < S::KG; ++k) {
               const int step = g * S::KG + k;
-              umma_ts<desc_hi(128), IDESC>(tS + g * N, tA + 8 * step, tile + step * 2 * N, k > 0 ? 1u : 0u, lead);
+              if constexpr (S::SS)
+                umma_ss<desc_hi(128), desc_hi(128), IDESC>(tS + g * N, codes + wg * (S::AB / 16) + step * 256,
+                                                           tile + step * 2 * N, k > 0 ? 1u : 0u, lead);
+              else umma_ts<desc_hi(128), IDESC>(tS + g * N, tA + 8 * step, tile + step * 2 * N, k > 0 ? 1u : 0u, lead);
             }
           umma_commit(s_full + wg, lead);
         }
@@ -511,7 +535,7 @@ __global__ void __launch_bounds__(kManyTokens) weigh_join_kernel(const WeighPara
 namespace {
 
 int64_t many_row_bytes(int M, int Hq, int kv_heads, int D, int G) {
-  const int64_t N = 128 / G, tiles = (static_cast<int64_t>(M) * (Hq / kv_heads) + N - 1) / N;
+  const int64_t N = many_columns(D, G), tiles = (static_cast<int64_t>(M) * (Hq / kv_heads) + N - 1) / N;
   return tiles * kv_heads * (N * D * 2 + N * (G + 1) * 4 + 16);
 }
 constexpr int64_t kManyRoom = 128 << 20;  // of prepared tiles of a launch, at least one row's
