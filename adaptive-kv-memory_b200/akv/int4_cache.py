@@ -20,8 +20,8 @@ tracks weights holds long sequences within a budget:
     out, lse = cache.attend(layer, q, rows, granted, return_lse=True)
     cache.weigh(layer, q, lse, rows, granted)   # what each token received
     kept = cache.evict(rows, budget, first=4, recent=128)
-  Page tables,
-lengths and reference counts live on the device and every call is a few
+
+Page tables, lengths and reference counts live on the device and every call is a few
 launches on the current stream: nothing waits for the host, so accepted
 counts that only the device knows drive the next step, and a step can be
 captured in a CUDA graph.  A call runs on the cache's GPU, whichever is current,
@@ -313,10 +313,12 @@ class Int4PagedCache:
     def attend_chunk(self, layer: int, query: torch.Tensor, rows=None, n_new=None, sm_scale: Optional[float] = None,
                      out: Optional[torch.Tensor] = None, return_lse: bool = False):
         """``attend`` for a chunk of new tokens a row (a prompt's, tens to thousands): the same arguments and
-        results, on the tensor cores' tiles of 128 query rows.  query (R, Hq, M, head_dim).
+        results, on the tensor cores' tiles of 128 query rows.  query (R, Hq, M, head_dim), M * Hq / kv_heads up to
+        2^20 (head_dim 256: 2^19).
 
         With a bf16 query K, V and the softmax's weights are rounded to fp16 (an eighth of the output's own
-        rounding each; the lse is off by some 1e-4); with an fp16 query K and the weights keep 22 bits."""
+        rounding each; the lse is off by some 1e-4); with an fp16 query V is, K is within 2^-20 of its group's
+        largest value and the weights keep 22 bits."""
         if _C.current_device() != self._dev_index:
             with torch.cuda.device(self._dev_index):
                 return self.attend_chunk(layer, query, rows, n_new, sm_scale, out, return_lse)
@@ -378,7 +380,8 @@ class Int4PagedCache:
 
         query, rows and n_new as in ``attend``; lse (R, Hq, M), or (R, Hq, 1) with a query of one token, fp32, as it
         returned it.  Queries past n_new[i] add nothing, nor do those that are not finite or whose lse is not.  A row
-        named twice counts once."""
+        named twice counts once.  Calls on one layer's weights have to follow one another (streams that both do need
+        an event between them)."""
         if _C.current_device() != self._dev_index:
             with torch.cuda.device(self._dev_index):
                 return self.weigh(layer, query, lse, rows, n_new, sm_scale)

@@ -17,6 +17,12 @@
 // the V of one (row, layer, head), and four 16-byte pieces a thread stand in
 // registers between read and write.  Pages before the first token that goes are
 // left alone.
+//
+// Bound by the moves: 16 rows of 1K to 7K tokens brought to 2,000 in 16 layers of
+// 8 heads of 128, 1.1 GB read and written, 204 us of the call's 247 (170 at the
+// memory's rate); by five launches in a chain where they are few: one row of
+// 4,352 to 4,096 in 28 layers of 2 heads 46 us (scores 6, selection 13, pages 4,
+// moves 17, tables 4).
 #include "int4.cuh"
 
 namespace akv {
@@ -526,7 +532,8 @@ extern "C" int akv_int4_evict(const akv_int4_evict_args* a, void* stream) {
   evict_score_kernel<<<dim3(most < 256 ? most : 256, a->n), 256, 0, st>>>(p);
   evict_select_kernel<<<a->n, kSelectThreads, 0, st>>>(p);
   evict_plan_kernel<<<1, kSelectThreads, 0, st>>>(p);
-  // few blocks: more threads each, so that a block's steps, one after the other, are fewer
+  // few blocks: more threads each, so that a block's steps, one after the other,
+  // are fewer: 112 blocks 54 -> 45 us; 4,096 blocks 247 -> 259 us
   const bool few = static_cast<int64_t>(a->n) * a->n_layers * a->kv_heads * 2 <= 148 * 2;
   switch (a->head_dim) {
     case 64: few ? launch_move<64, 1024>(p, st) : launch_move<64, 256>(p, st); break;

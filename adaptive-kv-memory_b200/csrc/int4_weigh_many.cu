@@ -14,11 +14,17 @@
 // two fp32 steps a group and column, an exponential, an addition.
 //
 // A unit is one (call row, 256 tokens): a warpgroup for each 128, whose codes
-// stand in shared (D = 256: tensor) memory as the MMA's A, head after head.  The units'
-// (head, query tile) pairs form one list that is cut into equal shares, one per
-// CTA, from the lengths on the device; parts of a cut unit are joined in order
-// by a third kernel.  While one warpgroup's exponentials run, the other's MMAs
-// do.
+// stand in shared (D = 256: tensor) memory as the MMA's A, head after head.  The
+// units' (head, query tile) pairs form one list that is cut into equal shares,
+// one per CTA, from the lengths on the device; parts of a cut unit are joined in
+// order by a third kernel.  While one warpgroup's exponentials run, the other's
+// MMAs do.
+//
+// Bound by the chain of a tile (scores out of tensor memory, sums, exponentials,
+// two barriers) with two warps a scheduler: 1,000 tokens of 32 / 8 heads of 128
+// over 16K, 5e8 exponentials that alone would take 110 us, take 192 us with one
+// group, 229 with two, 357 with four.  Sums of a column pair read as 16 bytes
+// instead of 8 gave the same (362): the registers they pair up spill.
 #include "int4_weigh.cuh"
 #include "umma.cuh"
 

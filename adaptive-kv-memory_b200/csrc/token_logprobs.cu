@@ -19,8 +19,13 @@
 // and CTAs are merged pairwise (maximum of one and the other reversed is the
 // bitonic top half).
 //
-// Bound by memory: every logit is read once.  Few rows are split over clusters
-// of up to 8 CTAs.
+// Few rows are split over clusters of up to 8 CTAs.
+//
+// Bound by memory with fp32 logits (1,000 rows of 151,936: 99 us, 6.1 TB/s) and
+// by the exponentials and some 6 instructions a logit with 16-bit ones: 4,093
+// rows 243 us, 5.1 TB/s, with the best alternative 310 us (the first batch's
+// sort, and new candidates of every warp).  One row of 151,936 takes 5 us, with
+// five alternatives 9.7; 64 rows of 32,003 4.8 and 8.3.
 #include <cooperative_groups.h>
 
 #include "int4.cuh"
