@@ -291,30 +291,39 @@ __global__ void __launch_bounds__(kLogpThreads, 4) token_logprobs_kernel(const L
     }
     const float m = E::max_of(top);
     if (!(m <= a.m)) raise(m);
-    const bool vanish = (E::min_of(low) - base) * kLog2E == -INFINITY;
-    const uint64_t back = f2_make(-base, -base), unit = f2_make(kLog2E, kLog2E);
-    uint64_t s2 = 0, t2 = 0;
+    if (__any_sync(~0u, (E::min_of(low) - base) * kLog2E == -INFINITY)) {
 #pragma unroll
-    for (int i = 0; i < W; i += 2 / PER) {
-      float x[2];
-      if constexpr (PER == 2) {
-        E::unpack(w[i], x);
-      } else {
-        x[0] = __uint_as_float(w[i]), x[1] = __uint_as_float(w[i + 1]);
+      for (int i = 0; i < W; ++i) {
+        if constexpr (PER == 2) {
+          float x[2];
+          E::unpack(w[i], x);
+          add(x[0]);
+          add(x[1]);
+        } else {
+          add(__uint_as_float(w[i]));
+        }
       }
-      uint64_t u2 = f2_mul(f2_add(f2_make(x[0], x[1]), back), unit);
-      float2 u = f2_split(u2);
-      if (vanish) {
-        u.x = max_nan(u.x, -160.f), u.y = max_nan(u.y, -160.f);
-        u2 = f2_make(u.x, u.y);
+    } else {
+      const uint64_t back = f2_make(-base, -base), unit = f2_make(kLog2E, kLog2E);
+      uint64_t s2 = 0, t2 = 0;
+#pragma unroll
+      for (int i = 0; i < W; i += 2 / PER) {
+        float x[2];
+        if constexpr (PER == 2) {
+          E::unpack(w[i], x);
+        } else {
+          x[0] = __uint_as_float(w[i]), x[1] = __uint_as_float(w[i + 1]);
+        }
+        const uint64_t u2 = f2_mul(f2_add(f2_make(x[0], x[1]), back), unit);
+        const float2 u = f2_split(u2);
+        const uint64_t e2 = f2_make(fast_exp2(u.x), fast_exp2(u.y));
+        s2 = f2_add(s2, e2);
+        t2 = f2_fma(e2, u2, t2);
       }
-      const uint64_t e2 = f2_make(fast_exp2(u.x), fast_exp2(u.y));
-      s2 = f2_add(s2, e2);
-      t2 = f2_fma(e2, u2, t2);
+      const float2 s = f2_split(s2), t2s = f2_split(t2);
+      a.s += s.x + s.y;
+      a.t += t2s.x + t2s.y;
     }
-    const float2 s = f2_split(s2), t_ = f2_split(t2);
-    a.s += s.x + s.y;
-    a.t += t_.x + t_.y;
     if (m > mine) above += E::count_above(w, W, mine);
     if constexpr (TOP) {
       // the elements that reach `bar`, a bit each: word i's from PER * i on
