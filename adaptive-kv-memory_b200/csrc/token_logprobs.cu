@@ -21,11 +21,11 @@
 //
 // Few rows are split over clusters of up to 8 CTAs.
 //
-// Bound by memory with fp32 logits (1,000 rows of 151,936: 99 us, 6.1 TB/s) and
-// by the exponentials and some 6 instructions a logit with 16-bit ones: 4,093
-// rows 243 us, 5.1 TB/s, with the best alternative 310 us (the first batch's
-// sort, and new candidates of every warp).  One row of 151,936 takes 5 us, with
-// five alternatives 9.7; 64 rows of 32,003 4.8 and 8.3.
+// Bound by memory with fp32 logits (1,000 rows of 151,936: 100 us, 6.1 TB/s); with
+// 16-bit ones, by the exponentials and some 6 instructions a logit between the
+// loads: 4,093 rows 220 us, 5.6 TB/s, with the best alternative 270 us (the first
+// batch's sort, new candidates of every warp, fewer CTAs).  One row of 151,936
+// takes 5 us, with five alternatives 9.4; 64 rows of 32,003 5 and 8.
 #include <cooperative_groups.h>
 
 #include "int4.cuh"
@@ -198,8 +198,14 @@ AKV_DEV uint64_t bitonic_merge(uint64_t k) {
   return k;
 }
 
+// CTAs an SM.  With 16-bit logits and lists four leave too few registers (298 us
+// for 4,093 x 151,936, three 270); with fp32 logits four fit (1,000 rows 100 us,
+// three 108).
 template <int DT, bool TOP>
-__global__ void __launch_bounds__(kLogpThreads, 4) token_logprobs_kernel(const LogpParams P) {
+constexpr int kLogpPerSm = TOP && DT != AKV_FP32 ? 3 : 4;
+
+template <int DT, bool TOP>
+__global__ void __launch_bounds__(kLogpThreads, kLogpPerSm<DT, TOP>) token_logprobs_kernel(const LogpParams P) {
   using E = LogitElem<DT>;
   using T = typename E::type;
   constexpr int W = kLogpVecs * 4;                 // words of a batch
