@@ -72,3 +72,41 @@ def test_example_runs():
     assert cache.lens.tolist() == [96, 70, 96]
     used = cache.table[cache.table >= 0]
     assert torch.equal(torch.bincount(used.long(), minlength=cache.n_pages).int(), cache.refs)
+
+
+def test_calls_on_several_streams_at_once():
+    """Chunks, weights, evictions and log probabilities of three caches side by side: the results of one after another."""
+    import akv
+
+    def work(seed):
+        c = akv.Int4PagedCache(2, 80, 2, 64, group_size=32, max_seqs=4, max_blocks=20, device=DEV, track_weights=True)
+        weigh._fill(c, [600, 333, 500], seed)
+        rows = evict._i(0, 1, 2)
+        q = weigh._query((3, 8, 300, 64), seed, torch.bfloat16)
+        logits = weigh._query((300, 30001), seed, torch.bfloat16)
+        torch.cuda.synchronize()
+        out = []
+
+        def run():
+            for _ in range(5):
+                o, lse = c.attend_chunk(0, q, rows, return_lse=True)
+                c.weigh(0, q, lse, rows)
+                c.weigh(1, q[:, :, -2:], lse[:, :, -2:], rows)
+                out.append((o, c.weights.clone(), akv.token_logprobs(logits, torch.zeros(300, dtype=torch.int64, device=DEV),
+                                                                     top=4).top_logprobs))
+            out.append((c.evict(rows, 200, 4, 50), c.weights, c.lens, c.table, c.buf))
+        return run, out, c
+    alone = [work(s) for s in range(3)]
+    for run, _, c in alone:
+        run()
+        c.check()
+    beside = [work(s) for s in range(3)]
+    streams = [torch.cuda.Stream() for _ in beside]
+    for (run, _, _), s in zip(beside, streams):
+        with torch.cuda.stream(s):
+            run()
+    torch.cuda.synchronize()
+    for (_, a, _), (_, b, c) in zip(alone, beside):
+        c.check()
+        for x, y in zip(a, b):
+            assert all(torch.equal(p, q) for p, q in zip(x, y))

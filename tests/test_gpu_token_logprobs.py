@@ -172,3 +172,27 @@ def test_refusals():
             akv.token_logprobs(x, tok, top=top)
     with pytest.raises(ValueError):
         akv.token_logprobs(x[:, :10], tok, top=11)
+
+
+@pytest.mark.parametrize("v", [8192, 8200, 16384, 24581, 32767, 4099])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_around_the_rings_batches(v, dtype):
+    """Rows of whole and ragged batches, one CTA a row and several; logits of -inf in the middle and at the ends."""
+    import akv
+    for n in (600, 3):
+        x, tok = _logits(n, v, v, dtype), _tokens(n, v, n)
+        x[:, v // 2:v // 2 + 40] = -float("inf")
+        x[0, :17] = x[1, -17:] = -float("inf")
+        _check(x, tok, akv.token_logprobs(x, tok, top=6), 6)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_further_apart_than_the_type_reaches(dtype):
+    """u overflows to -inf for all but the largest logit: weight 0, not NaN."""
+    import akv
+    x = torch.full((2, 9000), -3e38, device=DEV).to(dtype)
+    x[0, 8999] = x[1, 4] = 3e38
+    tok = torch.tensor([8999, 4], device=DEV)
+    r = akv.token_logprobs(x, tok, top=2)
+    assert (r.logprob == 0).all() and (r.entropy == 0).all() and (r.rank == 1).all()
+    assert r.top_tokens.tolist() == [[8999, 0], [4, 0]]
