@@ -845,7 +845,8 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
 // Block (c, k): 32 query rows of the unit whose first part CTA c holds; its
 // parts lie in the slots 2c + 1, 2 (c + 1), ..., 2 last.
 template <int D, int ROWS>
-__global__ void __launch_bounds__(128) int4_chunk_join_kernel(const ChunkParams P) {
+__global__ void __launch_bounds__(D * 4) int4_chunk_join_kernel(const ChunkParams P) {
+  __shared__ float2 s_ml[kChunkSMs][32];
   const int4 meta = P.meta[blockIdx.x];
   if (!meta.w) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -855,40 +856,42 @@ __global__ void __launch_bounds__(128) int4_chunk_join_kernel(const ChunkParams 
   const int rr = e % P.tiles * ROWS + n, m = rr / rep, hq = meta.y * rep + rr - m * rep;
   const int c0 = blockIdx.x, parts = meta.z - c0 + 1;
   auto slot = [&](int s) -> int64_t { return s == 0 ? 2 * c0 + 1 : 2 * (c0 + s); };
+  for (int s = warp; s < parts; s += D / 8) s_ml[s][lane] = __ldcg(&P.ml[slot(s) * ROWS + n]);
+  __syncthreads();
   float top = -INFINITY;
-  for (int s = 0; s < parts; ++s) top = fmaxf(top, __ldcg(&P.ml[slot(s) * ROWS + n].x));
+  for (int s = 0; s < parts; ++s) top = fmaxf(top, s_ml[s][lane].x);
   float L = 0.f;
   for (int s = 0; s < parts; ++s) {
-    const float2 x = __ldcg(&P.ml[slot(s) * ROWS + n]);
+    const float2 x = s_ml[s][lane];
     L += x.x == -INFINITY ? x.y : exp2f(x.x - top) * x.y;
   }
   const bool dead = L == 0.f, in = m < P.M;
   const float inv = 1.f / L;
-  for (int b = warp; b < D / 8; b += 4) {
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < parts; ++s) {
-      const float x = __ldcg(&P.ml[slot(s) * ROWS + n].x);
-      const float f = x == -INFINITY ? 0.f : exp2f(x - top);
-      const float4* at = reinterpret_cast<const float4*>(P.part) + slot(s) * ROWS * (D / 4) + n;
-      const float4 a = __ldcg(at + static_cast<int64_t>(2 * b) * ROWS), c = __ldcg(at + static_cast<int64_t>(2 * b + 1) * ROWS);
-      // channels 0..3 and 4..7 of the block
-      v[0] = fmaf(f, a.x, v[0]), v[1] = fmaf(f, a.y, v[1]), v[2] = fmaf(f, a.z, v[2]), v[3] = fmaf(f, a.w, v[3]);
-      v[4] = fmaf(f, c.x, v[4]), v[5] = fmaf(f, c.y, v[5]), v[6] = fmaf(f, c.z, v[6]), v[7] = fmaf(f, c.w, v[7]);
-    }
-    if (!in) continue;
-    uint32_t w[4];
+  const int b = warp;  // the warp's 8 channels
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float x = s_ml[s][lane].x;
+    const float f = x == -INFINITY ? 0.f : exp2f(x - top);
+    const float4* at = reinterpret_cast<const float4*>(P.part) + slot(s) * ROWS * (D / 4) + n;
+    const float4 a = __ldcg(at + static_cast<int64_t>(2 * b) * ROWS), c = __ldcg(at + static_cast<int64_t>(2 * b + 1) * ROWS);
+    // channels 0..3 and 4..7 of the block
+    v[0] = fmaf(f, a.x, v[0]), v[1] = fmaf(f, a.y, v[1]), v[2] = fmaf(f, a.z, v[2]), v[3] = fmaf(f, a.w, v[3]);
+    v[4] = fmaf(f, c.x, v[4]), v[5] = fmaf(f, c.y, v[5]), v[6] = fmaf(f, c.z, v[6]), v[7] = fmaf(f, c.w, v[7]);
+  }
+  if (!in) return;
+  uint32_t w[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float a = dead ? 0.f : v[2 * k] * inv, c = dead ? 0.f : v[2 * k + 1] * inv;
-      w[k] = P.bf16 ? pack_elems<true>(a, c) : pack_elems<false>(a, c);
-    }
-    uint16_t* dst = P.out + i * P.o_sr + hq * P.o_sh + m * P.o_sm + b * 8;
-    if (P.o16) {
-      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
+  for (int k = 0; k < 4; ++k) {
+    const float a = dead ? 0.f : v[2 * k] * inv, c = dead ? 0.f : v[2 * k + 1] * inv;
+    w[k] = P.bf16 ? pack_elems<true>(a, c) : pack_elems<false>(a, c);
+  }
+  uint16_t* dst = P.out + i * P.o_sr + hq * P.o_sh + m * P.o_sm + b * 8;
+  if (P.o16) {
+    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) dst[k] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
-    }
+    for (int k = 0; k < 8; ++k) dst[k] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
   }
   if (in && P.lse && warp == 0)
     P.lse[(static_cast<int64_t>(i) * P.Hq + hq) * P.M + m] = dead ? -INFINITY : (top + log2f(L)) * 0.6931471805599453f;
@@ -900,7 +903,7 @@ static int chunk_launch(const ChunkParams& P, cudaStream_t st) {
   const int smem = S::smem(P.R, P.R * P.tiles);
   if (!ensure_dynamic_smem<int4_chunk_kernel<D, G, LO>>(smem)) return AKV_ERR_LAUNCH;
   int4_chunk_kernel<D, G, LO><<<kChunkSMs, S::THREADS, smem, st>>>(P);
-  int4_chunk_join_kernel<D, S::ROWS><<<dim3(kChunkSMs, S::ROWS / 32), 128, 0, st>>>(P);
+  int4_chunk_join_kernel<D, S::ROWS><<<dim3(kChunkSMs, S::ROWS / 32), D * 4, 0, st>>>(P);
   return cudaGetLastError() == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH;
 }
 
