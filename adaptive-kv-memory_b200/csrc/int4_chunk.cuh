@@ -60,7 +60,11 @@ constexpr int kChunkEntries = 4096; // (row, tile) pairs of one launch
 constexpr int kChunkRowsMax = 1024; // call rows of one launch
 constexpr int kChunkRep = 4096;     // query heads of a group, at most (the division below)
 constexpr int kChunkSetup = 4;      // token tiles that a unit's set-up counts for
-constexpr int kChunkShare = 4;      // of a CTA's share, at least
+// A CTA's share is this many tiles at least, or as few as leave a unit kChunkParts
+// parts: more of them take the join longer than their CTAs save (64 new tokens
+// after 1,100, 2 heads of 128: shares of 4 32 us, 2 29.4, 1 27.9; one token of 12
+// heads over 4,096: 4 31 us, 2 29.5).
+constexpr int kChunkShare = 4, kChunkParts = 32;
 // A row's maximum stands at 2^7 when its unit is set, and a tile's weights sum up
 // to 2^15 at most before it moves: fp16 holds them down to 2^-21 of the maximum
 // with all their bits.  A sum says so without the tile's maximum: that is formed
@@ -380,7 +384,8 @@ __global__ void __launch_bounds__(ChunkShape<D, G, LO>::THREADS, 1) int4_chunk_k
       s_pref[0] = 0;
       const int total = base * H;
       int share = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-      if (share < kChunkShare) share = kChunkShare;
+      const int each = (total + entries * H - 1) / (entries * H);  // tiles of a unit
+      share = max(share, max(1, min(kChunkShare, (each + kChunkParts - 1) / kChunkParts)));
       const int begin = static_cast<int>(min(static_cast<int64_t>(share) * blockIdx.x, static_cast<int64_t>(total)));
       s_list = ChunkList{s_len, s_new, s_pref, share, total - begin > share ? begin + share : total};
       s_begin = chunk_at(P, s_list, begin);
