@@ -314,7 +314,8 @@ class Int4PagedCache:
                      out: Optional[torch.Tensor] = None, return_lse: bool = False):
         """``attend`` for a chunk of new tokens a row (a prompt's, tens to thousands): the same arguments and
         results, on the tensor cores' tiles of 128 query rows.  query (R, Hq, M, head_dim), M * Hq / kv_heads up to
-        2^20 (head_dim 256: 2^19).
+        2^20 (head_dim 256: 2^19).  ``attend`` is the faster one up to some 64 of these query rows a KV head, over a
+        single row of 4K tokens up to 300.
 
         With a bf16 query K, V and the softmax's weights are rounded to fp16 (an eighth of the output's own
         rounding each; the lse is off by some 1e-4); with an fp16 query V is, K is within 2^-20 of its group's
