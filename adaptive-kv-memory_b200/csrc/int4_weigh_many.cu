@@ -11,7 +11,12 @@
 // -lse, both in units of the exponent.  The main kernel copies a tile at a time
 // into a ring.  With S_g = q_g . (c_g - 8) from the tensor cores,
 //   w += 2^(sum_g s'_g S_g + (z_g + 8 s_g) qs_g - lse),  s' = s * unit:
-// two fp32 steps a group and column, an exponential, an addition.
+// two fp32 steps a group and column, an exponential, an addition.  A tile whose
+// queries' largest elements lie further apart than 2^kManySpread scales each
+// column by itself (its largest element to the same place), sums without lse and
+// unit, and takes one step a column more: 2^(unit_column * sum - lse).  The case
+// below with queries of such sizes takes 259, 293 and 431 us (one, two, four
+// groups); units by column for every tile would take 211, 254 and 404.
 //
 // A unit is one (call row, 256 tokens): a warpgroup for each 128, whose codes
 // stand in shared (D = 256: tensor) memory as the MMA's A, head after head.  The
@@ -22,9 +27,11 @@
 //
 // Bound by the chain of a tile (scores out of tensor memory, sums, exponentials,
 // two barriers) with two warps a scheduler: 1,000 tokens of 32 / 8 heads of 128
-// over 16K, 5e8 exponentials that alone would take 110 us, take 192 us with one
-// group, 229 with two, 357 with four.  Sums of a column pair read as 16 bytes
+// over 16K, 5e8 exponentials that alone would take 110 us, take 202 us with one
+// group, 242 with two, 358 with four.  Sums of a column pair read as 16 bytes
 // instead of 8 gave the same (362): the registers they pair up spill.
+#include <type_traits>
+
 #include "int4_weigh.cuh"
 #include "umma.cuh"
 
@@ -34,6 +41,7 @@ constexpr int kManySMs = 148;
 constexpr int kManyTokens = 256;      // of a unit
 constexpr int kManyThreads = 256 + 64;
 constexpr float kManyLog2e = 1.4426950408889634f;
+constexpr int kManySpread = 14;       // the smallest query of a tile keeps 2^-24 of its largest element
 
 // Query columns of a tile: an MMA of up to 64 columns takes as long as one of 64
 // (45 cycles; 32 columns are worth 16), so as many as the scores of all groups
@@ -48,7 +56,8 @@ struct ManyShape {
   static constexpr int N = many_columns(D, G);
   static constexpr int QB = N * D * 2;           // its operand
   static constexpr int META = N * (G + 1) * 4;   // per column pair: -lse, group sums
-  static constexpr int REC = QB + META + 16;     // and the exponent's unit
+  static constexpr int OWN = QB + META + 16;     // the tile's unit; whether its columns have their own
+  static constexpr int REC = OWN + N * 8;        // those, and -lse: per column pair
   static constexpr int STAGES = REC > 48 * 1024 ? 3 : 4;
   static constexpr int KG = D / G / 16;          // MMA steps of a group
   static constexpr int AB = SS ? 128 * D * 2 : 0;  // codes of a warpgroup
@@ -70,7 +79,7 @@ template <int D, int G>
 __global__ void __launch_bounds__(128) weigh_prepare_kernel(const WeighParams P) {
   using S = ManyShape<D, G>;
   constexpr int N = S::N;
-  __shared__ uint32_t s_top[128 / N];
+  __shared__ uint32_t s_top[128 / N], s_low[128 / N];
   const int t = threadIdx.x, n = t % N, sub = t / N;
   const int H = P.c.kv_heads, rep = P.Hq / H, h = blockIdx.y, e = blockIdx.z, i = P.row0 + e;
   const int all = (P.M * rep + N - 1) / N;           // tiles that a row has room for
@@ -88,7 +97,7 @@ __global__ void __launch_bounds__(128) weigh_prepare_kernel(const WeighParams P)
     for (int k = 0; k < 4; ++k) w[k] = src[8 * c + 2 * k] | static_cast<uint32_t>(src[8 * c + 2 * k + 1]) << 16;
     return make_uint4(w[0], w[1], w[2], w[3]);
   };
-  if (t < 128 / N) s_top[t] = 0u;
+  if (t < 128 / N) s_top[t] = 0u, s_low[t] = 0x7FFFu;
   __syncthreads();
   uint32_t top = 0u;  // largest magnitude, as the 15 bits of the type
 #pragma unroll 8
@@ -98,11 +107,17 @@ __global__ void __launch_bounds__(128) weigh_prepare_kernel(const WeighParams P)
 #pragma unroll
     for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7FFFu, w[k] >> 16 & 0x7FFFu));
   }
-  const bool bad = top >= (P.bf16 ? 0x7F80u : 0x7C00u);  // counts for nothing
-  if (P.bf16 && !bad) atomicMax(&s_top[sub], top);
+  const float lse = on ? __ldg(P.lse + (static_cast<int64_t>(i) * P.Hq + hq) * P.M + m) : -INFINITY;
+  const bool counts = on && top < (P.bf16 ? 0x7F80u : 0x7C00u) && fabsf(lse) < INFINITY;
+  if (P.bf16 && counts && top) {
+    atomicMax(&s_top[sub], top);
+    atomicMin(&s_low[sub], top);
+  }
   __syncthreads();
+  const bool own = static_cast<int>(s_top[sub] >> 7) - static_cast<int>(s_low[sub] >> 7) > kManySpread;
+  const uint32_t most = own ? (counts ? top : 0u) : s_top[sub];
   int ex = 0;
-  if (P.bf16 && s_top[sub]) ex = 13 - (static_cast<int>(s_top[sub] >> 7) - 127);
+  if (P.bf16 && most) ex = 13 - (static_cast<int>(most >> 7) - 127);
   ex = ex > 120 ? 120 : (ex < -120 ? -120 : ex);
   const float up = exp2f(static_cast<float>(ex));
   const float unit = ldexpf(P.scale * kManyLog2e, -ex);
@@ -121,7 +136,7 @@ __global__ void __launch_bounds__(128) weigh_prepare_kernel(const WeighParams P)
         for (int k = 0; k < 4; ++k)
           w[k] = pack_h2(__uint_as_float(w[k] << 16) * up, __uint_as_float(w[k] & 0xFFFF0000u) * up);
       }
-      if (bad) w[0] = w[1] = w[2] = w[3] = 0u;
+      if (!counts) w[0] = w[1] = w[2] = w[3] = 0u;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float2 f = __half22float2(u32_as_h2(w[k]));
@@ -133,13 +148,15 @@ __global__ void __launch_bounds__(128) weigh_prepare_kernel(const WeighParams P)
                      prmt(w[1], w[3], 0x7632));
     }
   }
-  const float lse = on ? __ldg(P.lse + (static_cast<int64_t>(i) * P.Hq + hq) * P.M + m) : -INFINITY;
-  const bool counts = on && !bad && fabsf(lse) < INFINITY;
+  const float less = counts ? -lse * kManyLog2e : -INFINITY;
   float* meta = reinterpret_cast<float*>(rec + S::QB) + (n / 2) * 2 * (G + 1) + (n & 1);
-  meta[0] = counts ? -lse * kManyLog2e : -INFINITY;
+  meta[0] = own ? 0.f : less;
 #pragma unroll
-  for (int g = 0; g < G; ++g) meta[2 + 2 * g] = counts ? sum[g] * unit : 0.f;
-  if (n == 0) *reinterpret_cast<float*>(rec + S::QB + S::META) = unit;
+  for (int g = 0; g < G; ++g) meta[2 + 2 * g] = own ? sum[g] : sum[g] * unit;
+  float* mine = reinterpret_cast<float*>(rec + S::OWN) + (n / 2) * 4 + (n & 1);
+  mine[0] = less;
+  mine[2] = unit;
+  if (n == 0) *reinterpret_cast<float2*>(rec + S::QB + S::META) = make_float2(own ? 1.f : unit, own ? 1.f : 0.f);
 }
 
 // ------------------------------------------------------------------ the list
@@ -382,7 +399,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
       for (int q = u.q0; q < u.q1; ++q) {
         if (!wait(q_full + st, ph_q)) break;
         const unsigned char* rec = smem + st * S::REC;
-        const float unit = *reinterpret_cast<const float*>(rec + S::QB + S::META);
+        const float2 tile = *reinterpret_cast<const float2*>(rec + S::QB + S::META);
+        const float unit = tile.x;
         uint64_t s2[G], m2[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -395,45 +413,55 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
         const int hide = static_cast<int>(see - static_cast<int64_t>(q) * N > N ? N : see - static_cast<int64_t>(q) * N);
         const bool full = __all_sync(~0u, hide <= 0);
         uint64_t sum = 0;
+        // with or without the columns' own units: a form for each, so that the usual one keeps its registers
+        auto add = [&](auto own) {
 #pragma unroll
-        for (int c = 0; c < N / 32; ++c) {
-          uint64_t y[16];
-          const uint64_t* meta = reinterpret_cast<const uint64_t*>(rec + S::QB) + c * 16 * (G + 1);
+          for (int c = 0; c < N / 32; ++c) {
+            uint64_t y[16];
+            const uint64_t* meta = reinterpret_cast<const uint64_t*>(rec + S::QB) + c * 16 * (G + 1);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            if constexpr (G == 1) {
-              const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(meta + 2 * k);
-              y[k] = f2_fma(m2[0], v.y, v.x);
-            } else {
-              y[k] = meta[k * (G + 1)];
+            for (int k = 0; k < 16; ++k) {
+              if constexpr (G == 1) {
+                const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(meta + 2 * k);
+                y[k] = f2_fma(m2[0], v.y, v.x);
+              } else {
+                y[k] = meta[k * (G + 1)];
 #pragma unroll
-              for (int g = 0; g < G; ++g) y[k] = f2_fma(m2[g], meta[k * (G + 1) + 1 + g], y[k]);
+                for (int g = 0; g < G; ++g) y[k] = f2_fma(m2[g], meta[k * (G + 1) + 1 + g], y[k]);
+              }
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              float x[32];
+              tmem_ld32(tS + g * N + c * 32, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) y[k] = f2_fma(f2_make(x[2 * k], x[2 * k + 1]), s2[g], y[k]);
+            }
+            if constexpr (decltype(own)::value) {
+              const ulonglong2* mine = reinterpret_cast<const ulonglong2*>(rec + S::OWN) + c * 16;
+#pragma unroll
+              for (int k = 0; k < 16; ++k) y[k] = f2_fma(y[k], mine[k].y, mine[k].x);
+            }
+            if (c == N / 32 - 1) {  // S is out
+              tc_fence_before();
+              mbar_arrive(s_free + wg);
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float2 v = f2_split(y[k]);
+              v.x = fast_exp2(v.x);
+              v.y = fast_exp2(v.y);
+              if (!full) {
+                if (c * 32 + 2 * k < hide) v.x = 0.f;
+                if (c * 32 + 2 * k + 1 < hide) v.y = 0.f;
+              }
+              sum = f2_add(sum, f2_make(v.x, v.y));
             }
           }
-#pragma unroll
-          for (int g = 0; g < G; ++g) {
-            float x[32];
-            tmem_ld32(tS + g * N + c * 32, x);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 16; ++k) y[k] = f2_fma(f2_make(x[2 * k], x[2 * k + 1]), s2[g], y[k]);
-          }
-          if (c == N / 32 - 1) {  // S is out
-            tc_fence_before();
-            mbar_arrive(s_free + wg);
-          }
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float2 v = f2_split(y[k]);
-            v.x = fast_exp2(v.x);
-            v.y = fast_exp2(v.y);
-            if (!full) {
-              if (c * 32 + 2 * k < hide) v.x = 0.f;
-              if (c * 32 + 2 * k + 1 < hide) v.y = 0.f;
-            }
-            sum = f2_add(sum, f2_make(v.x, v.y));
-          }
-        }
+        };
+        if (__any_sync(~0u, tile.y != 0.f)) add(std::true_type{});
+        else add(std::false_type{});
         const float2 two = f2_split(sum);
         total += two.x + two.y;
         __syncwarp();
@@ -542,7 +570,7 @@ namespace {
 
 int64_t many_row_bytes(int M, int Hq, int kv_heads, int D, int G) {
   const int64_t N = many_columns(D, G), tiles = (static_cast<int64_t>(M) * (Hq / kv_heads) + N - 1) / N;
-  return tiles * kv_heads * (N * D * 2 + N * (G + 1) * 4 + 16);
+  return tiles * kv_heads * (N * D * 2 + N * (G + 3) * 4 + 16);
 }
 constexpr int64_t kManyRoom = 128 << 20;  // of prepared tiles of a launch, at least one row's
 constexpr size_t kManyFixed = kManySMs * sizeof(int4) + 2 * kManySMs * kManyTokens * sizeof(float);
