@@ -15,7 +15,7 @@
 // queries' largest elements lie further apart than 2^kManySpread scales each
 // column by itself (its largest element to the same place), sums without lse and
 // unit, and takes one step a column more: 2^(unit_column * sum - lse).  The case
-// below with queries of such sizes takes 259, 293 and 431 us (one, two, four
+// below with queries of such sizes takes 255, 294 and 426 us (one, two, four
 // groups); units by column for every tile would take 211, 254 and 404.
 //
 // A unit is one (call row, 256 tokens): a warpgroup for each 128, whose codes
@@ -27,8 +27,8 @@
 //
 // Bound by the chain of a tile (scores out of tensor memory, sums, exponentials,
 // two barriers) with two warps a scheduler: 1,000 tokens of 32 / 8 heads of 128
-// over 16K, 5e8 exponentials that alone would take 110 us, take 202 us with one
-// group, 242 with two, 358 with four.  Sums of a column pair read as 16 bytes
+// over 16K, 5e8 exponentials that alone would take 110 us, take 193 us with one
+// group, 235 with two, 353 with four.  Sums of a column pair read as 16 bytes
 // instead of 8 gave the same (362): the registers they pair up spill.
 #include <type_traits>
 
@@ -393,10 +393,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
       if (more) fetch(nx);
 
       const int tok = u.tile * kManyTokens + t;
-      // columns from here on see the token
-      const int64_t see = static_cast<int64_t>(tok - (u.len - u.n_new)) * rep;
+      // Columns of the part's first tile that do not see the token, N fewer of each next one.  An
+      // old token's difference passes 32 bits with many heads; the columns themselves are 2^30 at most.
+      const int64_t see = static_cast<int64_t>(tok - (u.len - u.n_new)) * rep - static_cast<int64_t>(u.q0) * N;
+      int hide = static_cast<int>(max(int64_t{0}, min(int64_t{1} << 30, see)));
       if (u.first) total = 0.f;
-      for (int q = u.q0; q < u.q1; ++q) {
+      for (int q = u.q0; q < u.q1; ++q, hide -= N) {
         if (!wait(q_full + st, ph_q)) break;
         const unsigned char* rec = smem + st * S::REC;
         const float2 tile = *reinterpret_cast<const float2*>(rec + S::QB + S::META);
@@ -410,7 +412,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
         if (!wait(s_full + wg, ph_s)) break;
         ph_s ^= 1;
         tc_fence_after();
-        const int hide = static_cast<int>(see - static_cast<int64_t>(q) * N > N ? N : see - static_cast<int64_t>(q) * N);
         const bool full = __all_sync(~0u, hide <= 0);
         uint64_t sum = 0;
         // with or without the columns' own units: a form for each, so that the usual one keeps its registers
