@@ -17,9 +17,11 @@ AKV_DEV bool mbar_test(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// ... by a whole warp, whose lanes all learn the same.
+// ... by a whole warp, whose lanes all learn the same.  Each lane has to have
+// seen the phase end itself: a vote orders no memory, so another lane's test lets
+// it read nothing of what the barrier protects.
 AKV_DEV bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status) {
-  if (__any_sync(~0u, mbar_test(bar, parity))) return true;
+  if (__all_sync(~0u, mbar_test(bar, parity))) return true;
   return __all_sync(~0u, mbar_wait(bar, parity, status));
 }
 
