@@ -227,6 +227,7 @@ class Int4PagedCache:
             n_new = 0
         if n > self._most_requests:
             raise ValueError(f"{n} requests for {self.max_seqs} sequences")
+        weights = None if self.weights is None else self._weight_args()  # refused before any room is taken
         granted = torch.empty_strided((n,), (1,), dtype=torch.int32, device=self._dev)
         rc = self._lib.akv_pages_reserve_many(
             self._pt_ref, _C.ptr(rows), _C.ptr(counts), n_new, n, granted.data_ptr(), self._pool_ptr, self.n_layers,
@@ -234,8 +235,8 @@ class Int4PagedCache:
             _C.raw_stream(self._dev_index))
         if rc:
             _C.check(rc, "akv_pages_reserve_many")
-        if self.weights is not None:
-            rc = self._lib.akv_int4_weights_clear(self._pt_ref, *self._weight_args(), _C.ptr(rows),
+        if weights is not None:
+            rc = self._lib.akv_int4_weights_clear(self._pt_ref, *weights, _C.ptr(rows),
                                                   granted.data_ptr(), n, _C.raw_stream(self._dev_index))
             if rc:
                 _C.check(rc, "akv_int4_weights_clear")
