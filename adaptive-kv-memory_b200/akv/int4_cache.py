@@ -373,7 +373,8 @@ class Int4PagedCache:
                 w.device != self._dev or not w.is_contiguous():
             raise ValueError(f"weights must be contiguous fp32 ({self.n_layers}, {self.max_seqs}, "
                              f"{self.max_blocks * BLOCK}) on {self._dev}")
-        return w.data_ptr(), w.stride(0), w.stride(1), self.n_layers
+        row = self.max_blocks * BLOCK  # a dim of one may have any stride
+        return w.data_ptr(), self.max_seqs * row, row, self.n_layers
 
     def weigh(self, layer: int, query: torch.Tensor, lse: torch.Tensor, rows=None, n_new=None,
               sm_scale: Optional[float] = None) -> None:
