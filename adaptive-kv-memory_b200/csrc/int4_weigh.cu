@@ -58,6 +58,7 @@ struct WeighShape {
   static constexpr int OFF_SEE = OFF_L2 + kWeighUnits * ROWS * 4;
   static constexpr int OFF_PREF = OFF_SEE + kWeighUnits * ROWS * 4;
   static constexpr int smem(int rows) { return OFF_PREF + (3 * rows + 1) * 4; }
+  static_assert(OFF_FRAG >= kNameBytes, "the rows' names stand where the ring will");
 };
 
 // token of tile row g: see the attention kernel's bank note
@@ -83,13 +84,9 @@ AKV_DEV void weigh_lds(const uint8_t* p, uint32_t (&w)[BYTES < 4 ? 1 : BYTES / 4
 
 // Lengths of the call rows [row0, row0 + R) and their pages' prefix sums; a row
 // without new tokens has none, nor has one that an earlier call row names.
-AKV_DEV void weigh_rows(const WeighParams& P, int* s_pref, int* s_len, int* s_new, int* s_scan) {
+AKV_DEV void weigh_rows(const WeighParams& P, uint32_t* names, int* s_pref, int* s_len, int* s_new, int* s_scan) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, n_warps = blockDim.x >> 5;
-  for (int e = t; e < P.R; e += blockDim.x) {
-    const Int4Row r = int4_row(P.c, P.rows, P.n_new, P.row0 + e, P.M, P.status);
-    s_new[e] = weigh_new(P, e, r);
-    s_len[e] = r.len;
-  }
+  weigh_lengths(P, names, s_len, s_new);
   int base = 0;
   for (int e0 = 0; e0 < P.R; e0 += blockDim.x) {
     __syncthreads();
@@ -131,7 +128,7 @@ __global__ void __launch_bounds__(kWeighThreads, D == 256 ? 2 : 3) weigh_few_ker
   const int g = lane >> 2, q4 = lane & 3;
   const int H = P.c.kv_heads, rep = P.Hq / H;
 
-  weigh_rows(P, s_pref, s_len, s_new, s_scan);
+  weigh_rows(P, reinterpret_cast<uint32_t*>(smem), s_pref, s_len, s_new, s_scan);
 
   const int total = s_pref[P.R];
   const int share = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);

@@ -68,7 +68,7 @@ struct ManyShape {
   // tensor memory of a warpgroup: codes, then scores
   static constexpr int T_A = 0, T_S = SS ? 0 : D / 2, T_WG = T_S + G * N;
   static_assert(2 * T_WG <= 512, "tensor memory");
-  static_assert(REC % 16 == 0 && smem(kWeighRows) <= 227 * 1024, "shared memory");
+  static_assert(OFF_BAR >= kNameBytes && REC % 16 == 0 && smem(kWeighRows) <= 227 * 1024, "shared memory");
 };
 
 // tiles of a call row's query columns
@@ -290,12 +290,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) weigh_many_kernel(const Weigh
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  for (int e = t; e < P.R; e += kManyThreads) {
-    const Int4Row row = int4_row(P.c, P.rows, P.n_new, P.row0 + e, P.M, P.status);
-    s_len[e] = row.len;
-    s_new[e] = weigh_new(P, e, row);
-    s_pref[e + 1] = ManyWalk<N>::weight(s_len[e], s_new[e], rep);
-  }
+  weigh_lengths(P, reinterpret_cast<uint32_t*>(smem), s_len, s_new);
+  fence_proxy_async_shared();  // bulk copies follow where the rows' names stood
+  for (int e = t; e < P.R; e += kManyThreads) s_pref[e + 1] = ManyWalk<N>::weight(s_len[e], s_new[e], rep);
   __syncthreads();
   if (warp == 0) {  // prefix sums
     int64_t base = 0;
