@@ -18,7 +18,7 @@
 // queries), so a call repeated gives the same bits.
 //
 // Few queries: the pages of all rows form one list that is cut into equal
-// shares, one per resident CTA, from the lengths on the device.  A warp takes
+// shares, one per CTA that fits the SMs at once, from the lengths on the device.  A warp takes
 // every fourth page of its share and streams the page's heads through its own
 // ring of asynchronous copies (of threads: a bulk copy's barrier and issue cost a
 // record of 2 KB more than its arithmetic); tokens are the MMA's rows, queries its columns.  The
@@ -38,6 +38,8 @@ namespace akv {
 constexpr int kWeighWarps = 4;
 constexpr int kWeighThreads = kWeighWarps * 32;
 constexpr int kWeighUnits = 8;     // (head, column tile) units prepared at a time
+template <int D>
+constexpr int kWeighPerSm = D == 256 ? 2 : 3;  // CTAs an SM that the registers leave room for
 
 template <int D, int G, int NT>
 struct WeighShape {
@@ -58,6 +60,7 @@ struct WeighShape {
   static constexpr int OFF_SEE = OFF_L2 + kWeighUnits * ROWS * 4;
   static constexpr int OFF_PREF = OFF_SEE + kWeighUnits * ROWS * 4;
   static constexpr int smem(int rows) { return OFF_PREF + (3 * rows + 1) * 4; }
+  static_assert(smem(kWeighRows) <= 227 * 1024, "shared memory");
   static_assert(OFF_FRAG >= kNameBytes, "the rows' names stand where the ring will");
 };
 
@@ -112,7 +115,7 @@ AKV_DEV void weigh_rows(const WeighParams& P, uint32_t* names, int* s_pref, int*
 }
 
 template <int D, int G, int NT>
-__global__ void __launch_bounds__(kWeighThreads, D == 256 ? 2 : 3) weigh_few_kernel(const WeighParams P) {
+__global__ void __launch_bounds__(kWeighThreads, kWeighPerSm<D>) weigh_few_kernel(const WeighParams P) {
   using S = WeighShape<D, G, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
   float* s_qs = reinterpret_cast<float*>(smem + S::OFF_QS);   // [unit][G][ROWS]
@@ -372,9 +375,14 @@ static int launch_few(const WeighParams& P, cudaStream_t st) {
   using S = WeighShape<D, G, NT>;
   const int smem = S::smem(P.R);
   if (!ensure_dynamic_smem<weigh_few_kernel<D, G, NT>>(smem)) return AKV_ERR_LAUNCH;
-  constexpr int kPerSm = D == 256 ? 2 : 3;
+  // CTAs that an SM holds: what its registers allow, and its 228 KB of shared memory, of which each takes 1 KB
+  // more than it asks for.  Shares for those that registers alone allow ran in two waves where the fragments of 16
+  // columns are large, us: 16 rows x 8,192, 32 / 8 heads of 256 112, so 92; 4 x 16,384, 16 / 2 of 128 in four
+  // groups 24, so 18.
+  constexpr int kSmem = 228 * 1024, kSmemOfCta = 1024 + kWeighWarps * 32;
+  const int fit = kSmem / (smem + kSmemOfCta), per_sm = fit < kWeighPerSm<D> ? fit : kWeighPerSm<D>;
   const int64_t pages = static_cast<int64_t>(P.R) * P.c.max_blocks;
-  const int64_t most = 148 * kPerSm, want = (pages + kWeighWarps - 1) / kWeighWarps;
+  const int64_t most = 148 * per_sm, want = (pages + kWeighWarps - 1) / kWeighWarps;
   weigh_few_kernel<D, G, NT><<<static_cast<int>(want < most ? want : most), kWeighThreads, smem, st>>>(P);
   return cudaGetLastError() == cudaSuccess ? AKV_OK : AKV_ERR_LAUNCH;
 }
@@ -402,12 +410,16 @@ static int weigh_few(const WeighParams& P, cudaStream_t st) {
 // groups) or 128 columns cost the same half empty.  Measured, us, this kernel :
 // that one, for 1 row x 4,096 tokens, 32 / 8 heads | 16 x 8,192, 32 / 8 |
 // 4 x 16,384, 16 / 2:
-//   one group    16 columns  20 : 22 |  53 : 107 | 16 : 29
-//                32          32 : 22 |  89 : 107 | 23 : 29
-//                64          56 : 22 | 163 : 107 | 36 : 29
-//   four groups  16          21 : 25 |  84 : 105 | 24 : 28
-//                32          34 : 25 | 136 : 105 | 34 : 28
-//                64          59 : 26 | 247 : 106 | 54 : 30
+//   one group    16 columns  20 : 21 |  51 : 103 | 16 : 29
+//                32          32 : 21 |  87 : 103 | 22 : 30
+//                64          57 : 22 | 159 : 103 | 36 : 29
+//   two groups   16          20 : 23 |  55 : 117 | 16 : 31
+//                32          32 : 23 |  92 : 118 | 24 : 32
+//                64          57 : 23 | 166 : 118 | 36 : 31
+//   four groups  16          20 : 22 |  60 : 105 | 18 : 29
+//                32          33 : 21 |  97 : 105 | 26 : 29
+//                64          59 : 22 | 173 : 105 | 40 : 29
+// (heads of 64 and 256 alike: one group, 32 columns 28 : 18 | 71 : 88 | 20 : 25, 42 : 25 | 146 : 168 | 32 : 37).
 static int weigh_few_columns(int n_groups) { return n_groups == 1 ? 32 : 16; }
 
 }  // namespace akv
