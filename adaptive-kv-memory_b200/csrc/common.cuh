@@ -12,6 +12,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <mutex>
 
 #include "akv_b200.h"
 
@@ -92,7 +93,8 @@ constexpr uint32_t kSuspendHintNs = 1000000u;     // 1 ms
 // Dynamic shared memory above 48 KB needs a per-function attribute; setting
 // it costs a driver call, so each kernel instance (template argument) keeps
 // the largest size it has been given per device and sets it only when a
-// larger one is asked for.
+// larger one is asked for, one thread at a time: a smaller size set late would
+// undo a larger one.
 template <auto Kern>
 inline bool ensure_dynamic_smem(size_t smem) {
   if (smem <= 48 * 1024) return true;
@@ -103,12 +105,13 @@ inline bool ensure_dynamic_smem(size_t smem) {
   if (dev < 0 || dev >= kDevices)
     return cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) ==
            cudaSuccess;
-  int cur = have[dev].load(std::memory_order_acquire);
-  if (cur >= static_cast<int>(smem)) return true;
+  if (have[dev].load(std::memory_order_acquire) >= static_cast<int>(smem)) return true;
+  static std::mutex setting;
+  std::lock_guard<std::mutex> lock(setting);
+  if (have[dev].load(std::memory_order_relaxed) >= static_cast<int>(smem)) return true;
   if (cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
     return false;
-  while (cur < static_cast<int>(smem) && !have[dev].compare_exchange_weak(cur, static_cast<int>(smem))) {
-  }
+  have[dev].store(static_cast<int>(smem), std::memory_order_release);
   return true;
 }
 
