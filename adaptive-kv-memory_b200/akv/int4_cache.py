@@ -40,6 +40,7 @@ from . import _C
 
 BLOCK = _C.BLOCK_TOKENS
 _REQUESTS = 1024  # requests that a call may hold however few the sequences
+_EVICT_ROWS = 65535  # rows of an eviction: a grid dim's blocks
 
 
 _HALF = {torch.float16: 0, torch.bfloat16: 1}
@@ -430,7 +431,7 @@ class Int4PagedCache:
 
         Returns the old positions of the tokens that stay, int32 (rows, keep), -1 past a row's end.  A row that needs
         new pages for shared ones when the pool has none is refused, as are all after it: they stay as they are, -1
-        everywhere.  So is a row named twice, the second time."""
+        everywhere.  So is a row named twice, the second time.  At most 65,535 rows a call."""
         if _C.current_device() != self._dev_index:
             with torch.cuda.device(self._dev_index):
                 return self.evict(rows, keep, first, recent)
@@ -440,6 +441,8 @@ class Int4PagedCache:
             raise ValueError(f"keep must be positive and first + recent at most that (got {keep}, {first}, {recent})")
         rows = self._ints(rows, "rows")
         n = self.max_seqs if rows is None else rows.shape[0]
+        if n > _EVICT_ROWS:
+            raise ValueError(f"at most {_EVICT_ROWS} rows a call (got {n})")
         kept = torch.empty_strided((n, keep), (keep, 1), dtype=torch.int32, device=self._dev)
         need = int(self._lib.akv_int4_evict_workspace_bytes(n, self.max_blocks, self.n_pages)) if n else 0
         ws = torch.empty(need, dtype=torch.uint8, device=self._dev)
