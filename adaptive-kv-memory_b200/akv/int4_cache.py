@@ -60,7 +60,7 @@ class Int4PagedCache:
     head_dim / 2 or head_dim / 4; head_dim 64, 128 or 256.  ``track_weights``: ``weights`` (n_layers, max_seqs,
     max_blocks * 32) fp32 holds the attention weight that each token of each row has received (``weigh``), 0 for a
     token when ``reserve`` makes room for it; ``fork`` and ``evict`` take it along.  It may be read, scaled or
-    replaced between calls."""
+    replaced between calls; a captured graph keeps the tensor that it was captured with."""
 
     def __init__(self, n_layers: int, n_pages: int, kv_heads: int, head_dim: int, group_size: Optional[int] = None,
                  max_seqs: int = 64, max_blocks: int = 1024, device="cuda", track_weights: bool = False):
@@ -314,14 +314,15 @@ class Int4PagedCache:
     # ------------------------------------------------------------------ chunks
     def attend_chunk(self, layer: int, query: torch.Tensor, rows=None, n_new=None, sm_scale: Optional[float] = None,
                      out: Optional[torch.Tensor] = None, return_lse: bool = False):
-        """``attend`` for a chunk of new tokens a row (a prompt's, tens to thousands): the same arguments and
-        results, on the tensor cores' tiles of 128 query rows.  query (R, Hq, M, head_dim), M * Hq / kv_heads up to
-        2^20 (head_dim 256: 2^19).  ``attend`` is the faster one up to some 64 of these query rows a KV head, over a
-        single row of 4K tokens up to 300.
+        """``attend`` for a chunk of new tokens a row (a prompt's, tens to thousands): the same arguments, but for a
+        query of one token without its dim, and the same results, on the tensor cores' tiles of 128 query rows.
+        query (R, Hq, M, head_dim), M * Hq / kv_heads up to 2^20 (head_dim 256: 2^19), Hq / kv_heads up to 4,096.
+        ``attend`` is the faster one up to some 64 of these query rows a KV head, over a single row of 4K tokens up to
+        300.
 
         With a bf16 query K, V and the softmax's weights are rounded to fp16 (an eighth of the output's own
-        rounding each; the lse is off by some 1e-4); with an fp16 query V is, K is within 2^-20 of its group's
-        largest value and the weights keep 22 bits."""
+        rounding each; the lse is off by some 1e-4, more where scores are large); with an fp16 query V is, K is within
+        2^-20 of its group's largest value and the weights keep 22 bits."""
         if _C.current_device() != self._dev_index:
             with torch.cuda.device(self._dev_index):
                 return self.attend_chunk(layer, query, rows, n_new, sm_scale, out, return_lse)
@@ -382,10 +383,11 @@ class Int4PagedCache:
         """Add the attention weight that the rows' newest tokens give to every token they see to
         ``weights[layer]``: over all query heads and new tokens, exp(q . K_t * sm_scale - lse).
 
-        query, rows and n_new as in ``attend``; lse (R, Hq, M), or (R, Hq, 1) with a query of one token, fp32, as it
-        returned it.  Queries past n_new[i] add nothing, nor do those that are not finite or whose lse is not.  A row
-        named twice counts once.  Calls on one layer's weights have to follow one another (streams that both do need
-        an event between them)."""
+        query, rows and n_new as in ``attend``; lse (R, Hq, M), or (R, Hq, 1) with a query of one token, fp32, as
+        ``attend`` or ``attend_chunk`` returned it: one that is off by d makes its query's weights off by d of
+        themselves (some 1e-4 after a bf16 chunk).  Queries past n_new[i] add nothing, nor do those that are not finite
+        or whose lse is not.  A row named twice counts once.  Calls on one layer's weights have to follow one another
+        (streams that both do need an event between them)."""
         if _C.current_device() != self._dev_index:
             with torch.cuda.device(self._dev_index):
                 return self.weigh(layer, query, lse, rows, n_new, sm_scale)

@@ -40,9 +40,11 @@
 // Within a block of 8 channels they stand as the codes come out of a word,
 // 0 4 1 5 2 6 3 7, in Q and K alike; V's order is undone when O is stored.
 //
-// Measured.  2 x 2,048 tokens over 32K, 32 / 8 heads of 128, bf16: 1.95 ms, 1.09
-// PFLOP/s of the 1.68 that a matrix product reaches; D = 256 3.5 ms, fp16 (three
-// products for two, tiles of half the size) 3.4 ms.  A tile of 128 tokens takes
+// Measured.  2 x 2,048 tokens over 32K, 32 / 8 heads of 128, bf16: 1.93 ms in a
+// short burst, 1.10 PFLOP/s of the 1.68 that a matrix product reaches, 2.2 ms (970
+// TFLOP/s of its 1.40) in steady repetition, where power holds the clock.  Bursts:
+// heads of 64 1.73 ms, of 256 7.5 ms (half the TFLOP/s: one query tile a CTA),
+// fp16 (three products for two, tiles of half the size) 3.3 ms.  A tile of 128 tokens takes
 // the two query tiles some 3,850 cycles, their MMAs 2,048: what remains is the
 // chain from a score to its weight and back to the tensor cores, and the value
 // warpgroup's unpacking, 128 tokens in about the tile's time.  Tried and slower:

@@ -19,8 +19,8 @@
 // left alone.
 //
 // Bound by the moves: 16 rows of 1K to 7K tokens brought to 2,000 in 16 layers of
-// 8 heads of 128, 1.1 GB read and written, 204 us of the call's 247 (170 at the
-// memory's rate); by five launches in a chain where they are few: one row of
+// 8 heads of 128, 1.1 GB read and written, 204 us of the call's 225 to 260, by the
+// lengths drawn (170 at the memory's rate); by five launches in a chain where they are few: one row of
 // 4,352 to 4,096 in 28 layers of 2 heads 46 us (scores 6, selection 13, pages 4,
 // moves 17, tables 4).
 #include "int4.cuh"

@@ -21,10 +21,11 @@
 //
 // Few rows are split over clusters of up to 8 CTAs.
 //
-// Bound by memory with fp32 logits (1,000 rows of 151,936: 100 us, 6.1 TB/s); with
+// Bound by memory with fp32 logits (1,000 rows of 151,936: 102 us, 6.0 TB/s); with
 // 16-bit ones, by the exponentials and some 6 instructions a logit between the
-// loads: 4,093 rows 220 us, 5.6 TB/s, with the best alternative 270 us (the first
-// batch's sort, new candidates of every warp, fewer CTAs).  One row of 151,936
+// loads: 4,093 rows 225 us, 5.5 TB/s, with the best alternative 276 us (the first
+// batch's sort, new candidates of every warp, fewer CTAs); 248 and 290 to 303 in
+// steady repetition.  One row of 151,936
 // takes 5 us, with five alternatives 9.4; 64 rows of 32,003 5 and 8.
 #include <cooperative_groups.h>
 
@@ -198,9 +199,9 @@ AKV_DEV uint64_t bitonic_merge(uint64_t k) {
   return k;
 }
 
-// CTAs an SM.  With 16-bit logits and lists four leave too few registers (298 us
-// for 4,093 x 151,936, three 270); with fp32 logits four fit (1,000 rows 100 us,
-// three 108).
+// CTAs an SM.  With 16-bit logits and lists four leave too few registers (305 us
+// for 4,093 x 151,936, three 276); with fp32 logits four fit (1,000 rows 102 us,
+// three 110).
 template <int DT, bool TOP>
 constexpr int kLogpPerSm = TOP && DT != AKV_FP32 ? 3 : 4;
 

@@ -719,7 +719,9 @@ int akv_int4_attention(const akv_int4_attention_args* a, void* stream);
 
 /* The same for a chunk of new tokens (tens to thousands a row), on the fifth-
  * generation tensor cores: arguments and results as akv_int4_attention, but for
- * a bf16 query K, V and the softmax's weights are rounded to fp16 once each.
+ * a bf16 query K, V and the softmax's weights are rounded to fp16 once each, for
+ * an fp16 one V is.  M * Hq / kv_heads <= 2^20 (head_dim 256: 2^19), Hq / kv_heads
+ * <= 4096 (AKV_ERR_UNSUPPORTED).
  * Workspace: akv_int4_chunk_workspace_bytes(...), 16-byte aligned, with any
  * content; calls in order on one stream may share it. */
 size_t akv_int4_chunk_workspace_bytes(int head_dim);
@@ -827,7 +829,7 @@ int akv_pages_copy(uint8_t* pool, int n_layers, int64_t layer_stride, int64_t pa
  * row and all after it are refused and stay as they are (AKV_ERR_EXHAUSTED);
  * so is a bad or repeated row (AKV_ERR_SHAPE).  kept int32 [n][keep]: the old
  * positions of the tokens that stay, ascending, then -1 (all -1 for a refused
- * row).  keep >= 1, first + recent <= keep.
+ * row).  keep >= 1, first + recent <= keep, n <= 65535.
  * Workspace: akv_int4_evict_workspace_bytes(...), 16-byte aligned.
  * ---------------------------------------------------------------------- */
 typedef struct {
