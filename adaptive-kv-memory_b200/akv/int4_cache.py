@@ -126,7 +126,8 @@ class Int4PagedCache:
         return self._state.clone()
 
     def set_page_state(self, state: torch.Tensor) -> None:
-        """The bookkeeping put back as ``page_state`` returned it (the pages' bytes are not touched)."""
+        """The bookkeeping put back as ``page_state`` returned it (the pages' bytes and tracked weights are not
+        touched)."""
         if state.shape != self._state.shape or state.dtype is not torch.int32:
             raise ValueError("the state does not match the cache")
         self._state.copy_(state)

@@ -60,7 +60,7 @@ struct WeighShape {
   static constexpr int OFF_SEE = OFF_L2 + kWeighUnits * ROWS * 4;
   static constexpr int OFF_PREF = OFF_SEE + kWeighUnits * ROWS * 4;
   static constexpr int smem(int rows) { return OFF_PREF + (3 * rows + 1) * 4; }
-  static_assert(smem(kWeighRows) <= 227 * 1024, "shared memory");
+  static_assert(smem(kWeighRows) <= 226 * 1024, "shared memory");
   static_assert(OFF_FRAG >= kNameBytes, "the rows' names stand where the ring will");
 };
 
